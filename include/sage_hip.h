@@ -205,6 +205,62 @@ int sage_train_embeddings(sage_ctx* ctx, int32_t dim, int32_t window, int32_t ne
                           int32_t epochs, double sample, int32_t min_count, uint64_t seed, int64_t vsize,
                           double* out_vectors /*[vsize*dim]*/, int64_t* out_counts /*[vsize]*/);
 
+/*
+ * Softmax over the whole vocabulary (no counterpart in the reference, whose gensim model stands for it with negative samples
+ * and whose compute_losses scores with log-sigmoids, utils.py:125-138): with logits s_nv = x_n . weight_v + bias_v,
+ *   logprob[n] = s_n,target(n) - lse[n],   lse[n] = log sum_v exp s_nv,   entropy[n] = lse[n] - sum_v p_nv s_nv,
+ * and the `alternatives` largest logits of a row, as ids in descending order (ties: the lower id) and log probabilities.
+ * The [n][vocab] matrix of logits is never stored.
+ *   d_x [n][dim], d_weight [vocab][dim]   both SAGE_F32 or both SAGE_BF16, rows ldx / ldw elements apart (>= dim); any alignment
+ *                    of rows.  Products and sums are float32 (float32 inputs at float32 accuracy); the softmax's too.
+ *   d_bias [vocab]   float32 or NULL; -inf, or any value of -1e30 or less, takes an id out (so does a logit of -6e29).  A row that has nothing left gets lse -inf, logprob -inf, entropy 0,
+ *                    alternatives -1.  x and weight are finite: a logit that is NaN or +inf makes its row NaN, alternatives -1.
+ *   d_targets [n]    int64, or NULL (then no d_logprob).  A negative target means none: logprob 0, no gradient.  The host cannot
+ *                    see a target of `vocab` or more: its logprob is NaN, and so are the gradients it reaches.
+ *   d_logprob, d_entropy, d_lse [n] float32 (d_logprob and d_entropy may be NULL); d_alt_ids int32 and d_alt_logprobs float32
+ *                    [n][alternatives]: -1 and -inf where fewer ids than that are left.
+ * Limits (SAGE_E_LIMIT): dim <= 512, vocab <= 2^20, n <= 2^22, alternatives <= 32.  n == 0 is allowed.
+ *
+ * This family and sage_clip_grad_norm_device only enqueue: all pointers are DEVICE pointers, the work goes to `stream` (a
+ * hipStream_t of the context's device; NULL is the default stream), nothing is allocated, nothing waits, and the caller's
+ * current device is left as it is.  They may be captured into a graph.  The workspace (at least what the matching
+ * `_workspace` call returns, aligned to 256 bytes, its contents never read) is the caller's: calls that may overlap in time
+ * need one each, two captured graphs among them.  Results do not depend on timing: no atomic decides an order.
+ */
+enum { SAGE_F32 = 0, SAGE_BF16 = 1 };
+int64_t sage_token_logprobs_workspace(sage_ctx* ctx, int32_t dtype, int64_t n, int64_t vocab, int32_t dim, int32_t alternatives);
+int sage_token_logprobs_device(sage_ctx* ctx, int32_t dtype, int64_t n, int64_t vocab, int32_t dim, const void* d_x, int64_t ldx,
+                               const void* d_weight, int64_t ldw, const float* d_bias, const int64_t* d_targets, int32_t alternatives,
+                               float* d_logprob, float* d_entropy, float* d_lse, int32_t* d_alt_ids, float* d_alt_logprobs,
+                               void* d_workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Its gradient: with G_nv = g_n ([v == target(n)] - p_nv) - h_n p_nv (log p_nv + entropy_n), g = d_grad_logprob and
+ * h = d_grad_entropy (float32 [n]; either may be NULL, not both),
+ *   d_dx [n][dim] = G weight,   d_dweight [vocab][dim] = G^T x  (the inputs' type, rows lddx / lddw apart),   d_dbias[v] = sum_n G_nv
+ * (float32).  d_dx or d_dweight may be NULL; d_dbias needs d_dweight.  d_lse and d_entropy (needed with d_grad_entropy) are
+ * what the forward call returned for the same inputs.  The logits are formed again; sums are float32.  With n == 0 the
+ * weight's and bias's gradients are zeros.  Results are overwritten, not accumulated.
+ */
+int64_t sage_token_logprobs_backward_workspace(sage_ctx* ctx, int32_t dtype, int64_t n, int64_t vocab, int32_t dim);
+int sage_token_logprobs_backward_device(sage_ctx* ctx, int32_t dtype, int64_t n, int64_t vocab, int32_t dim, const void* d_x, int64_t ldx,
+                                        const void* d_weight, int64_t ldw, const float* d_bias, const int64_t* d_targets,
+                                        const float* d_lse, const float* d_entropy, const float* d_grad_logprob,
+                                        const float* d_grad_entropy, void* d_dx, int64_t lddx, void* d_dweight, int64_t lddw,
+                                        float* d_dbias, void* d_workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Clips gradients by their global norm N = sqrt(sum of all squares): d_out[i] = d_grads[i] * (max_norm / N) where N > max_norm,
+ * else d_out[i] = d_grads[i]; *d_norm = N (float32, device).  d_out[i] may be d_grads[i] itself (in place); no other overlap
+ * is allowed.  sizes[i] elements of dtypes[i] (SAGE_F32 / SAGE_BF16), back to back; the four lists are HOST arrays, read
+ * during the call only.  Squares are summed in float64.  A norm that is not finite leaves every gradient as it is: the
+ * caller sees it in *d_norm.  Enqueues only, as described above.
+ */
+int64_t sage_clip_grad_norm_workspace(sage_ctx* ctx, int64_t n_tensors, const int64_t* sizes);
+int sage_clip_grad_norm_device(sage_ctx* ctx, int64_t n_tensors, const void* const* d_grads, void* const* d_out, const int64_t* sizes,
+                               const int32_t* dtypes, double max_norm, float* d_norm, void* d_workspace, int64_t workspace_bytes,
+                               void* stream);
+
 /* Workload statistics of the last step, for the roofline's algorithmic bytes:
  * out[0]=tokens, out[1]=corpus bytes, out[2]=ablated occurrences, out[3]=embedding rows touched (ablated windows +
  * base spans), out[4]=signed pair records, out[5]=unordered position pairs (= records / 2: what the distinct count

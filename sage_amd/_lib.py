@@ -90,6 +90,19 @@ def load():
     lib.sage_measure_unique_rows.argtypes = [vp, C.c_int32, pi64]
     lib.sage_debug_scan_total.restype = C.c_int
     lib.sage_debug_scan_total.argtypes = [vp, C.c_uint32, i64, C.POINTER(C.c_uint64), C.POINTER(C.c_uint32)]
+    lib.sage_token_logprobs_workspace.restype = i64
+    lib.sage_token_logprobs_workspace.argtypes = [vp, i32, i64, i64, i32, i32]
+    lib.sage_token_logprobs_device.restype = C.c_int
+    lib.sage_token_logprobs_device.argtypes = [vp, i32, i64, i64, i32, vp, i64, vp, i64, vp, vp, i32, vp, vp, vp, vp, vp, vp, i64, vp]
+    lib.sage_token_logprobs_backward_workspace.restype = i64
+    lib.sage_token_logprobs_backward_workspace.argtypes = [vp, i32, i64, i64, i32]
+    lib.sage_token_logprobs_backward_device.restype = C.c_int
+    lib.sage_token_logprobs_backward_device.argtypes = [vp, i32, i64, i64, i32, vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, vp, i64,
+                                                        vp, vp, i64, vp]
+    lib.sage_clip_grad_norm_workspace.restype = i64
+    lib.sage_clip_grad_norm_workspace.argtypes = [vp, i64, vp]
+    lib.sage_clip_grad_norm_device.restype = C.c_int
+    lib.sage_clip_grad_norm_device.argtypes = [vp, i64, vp, vp, vp, vp, C.c_double, vp, vp, i64, vp]
     _lib = lib
     return lib
 
@@ -97,7 +110,9 @@ def load():
 EXPORTED = ["sage_version", "sage_create", "sage_destroy", "sage_last_error", "sage_set_vocab", "sage_set_vocab_pruned", "sage_set_corpus",
             "sage_set_embeddings", "sage_tokenize", "sage_tokenize_noalloc", "sage_ablation_step", "sage_ablation_step_device",
             "sage_set_profiling", "sage_reset_kernel_times", "sage_get_kernel_times", "sage_set_batch_bytes",
-            "sage_set_match_mode", "sage_invalidate_matches", "sage_set_count_mode", "sage_set_score_mode", "sage_set_deterministic", "sage_train_embeddings", "sage_get_step_stats", "sage_debug_scan_total", "sage_measure_unique_rows"]
+            "sage_set_match_mode", "sage_invalidate_matches", "sage_set_count_mode", "sage_set_score_mode", "sage_set_deterministic", "sage_train_embeddings", "sage_get_step_stats", "sage_debug_scan_total", "sage_measure_unique_rows",
+            "sage_token_logprobs_workspace", "sage_token_logprobs_device", "sage_token_logprobs_backward_workspace",
+            "sage_token_logprobs_backward_device", "sage_clip_grad_norm_workspace", "sage_clip_grad_norm_device"]
 
 
 class HipSage:
@@ -241,6 +256,47 @@ class HipSage:
         self._check(self._lib.sage_ablation_step_device(self._h, _ptr(b, C.c_int64), len(b) - 1, int(pad),
                                                         C.c_void_p(loss_ptr), C.c_void_p(d_occ), int(vsize),
                                                         C.c_void_p(d_totals), C.c_void_p(hist_ptr), int(hist_len)))
+
+    # ---- vocabulary softmax, gradient clipping (device addresses; sage_amd.vocab_softmax takes torch tensors) ----------
+    F32, BF16 = 0, 1
+    MAX_ALTERNATIVES = 32
+
+    def _size(self, bytes_or_code: int) -> int:
+        if bytes_or_code < 0:
+            self._check(bytes_or_code)
+        return bytes_or_code
+
+    def token_logprobs_workspace(self, dtype: int, n: int, vocab: int, dim: int, alternatives: int = 0) -> int:
+        return self._size(self._lib.sage_token_logprobs_workspace(self._h, dtype, n, vocab, dim, alternatives))
+
+    def token_logprobs_device(self, dtype: int, n: int, vocab: int, dim: int, d_x: int, ldx: int, d_weight: int, ldw: int, d_bias: int,
+                              d_targets: int, alternatives: int, d_logprob: int, d_entropy: int, d_lse: int, d_alt_ids: int,
+                              d_alt_logprobs: int, d_workspace: int, workspace_bytes: int, stream: int):
+        """sage_token_logprobs_device: enqueues on `stream`; addresses of 0 stand for NULL."""
+        self._check(self._lib.sage_token_logprobs_device(self._h, dtype, n, vocab, dim, d_x, ldx, d_weight, ldw, d_bias, d_targets,
+                                                         alternatives, d_logprob, d_entropy, d_lse, d_alt_ids, d_alt_logprobs,
+                                                         d_workspace, workspace_bytes, stream))
+
+    def token_logprobs_backward_workspace(self, dtype: int, n: int, vocab: int, dim: int) -> int:
+        return self._size(self._lib.sage_token_logprobs_backward_workspace(self._h, dtype, n, vocab, dim))
+
+    def token_logprobs_backward_device(self, dtype: int, n: int, vocab: int, dim: int, d_x: int, ldx: int, d_weight: int, ldw: int,
+                                       d_bias: int, d_targets: int, d_lse: int, d_entropy: int, d_grad_logprob: int, d_grad_entropy: int,
+                                       d_dx: int, lddx: int, d_dweight: int, lddw: int, d_dbias: int, d_workspace: int,
+                                       workspace_bytes: int, stream: int):
+        """sage_token_logprobs_backward_device: enqueues on `stream`; addresses of 0 stand for NULL."""
+        self._check(self._lib.sage_token_logprobs_backward_device(self._h, dtype, n, vocab, dim, d_x, ldx, d_weight, ldw, d_bias, d_targets,
+                                                                  d_lse, d_entropy, d_grad_logprob, d_grad_entropy, d_dx, lddx, d_dweight,
+                                                                  lddw, d_dbias, d_workspace, workspace_bytes, stream))
+
+    def clip_grad_norm_workspace(self, sizes: np.ndarray) -> int:
+        return self._size(self._lib.sage_clip_grad_norm_workspace(self._h, len(sizes), sizes.ctypes.data))
+
+    def clip_grad_norm_device(self, d_grads: np.ndarray, d_out: np.ndarray, sizes: np.ndarray, dtypes: np.ndarray, max_norm: float,
+                              d_norm: int, d_workspace: int, workspace_bytes: int, stream: int):
+        """sage_clip_grad_norm_device: the four lists are host arrays (uint64 addresses, int64 sizes, int32 types)."""
+        self._check(self._lib.sage_clip_grad_norm_device(self._h, len(sizes), d_grads.ctypes.data, d_out.ctypes.data, sizes.ctypes.data,
+                                                         dtypes.ctypes.data, float(max_norm), d_norm, d_workspace, workspace_bytes, stream))
 
     # ---- measurement ------------------------------------------------------------------------------------
     def set_profiling(self, on: bool):

@@ -13,7 +13,7 @@
 #include <atomic>
 #include <vector>
 
-#include "../../include/sage_hip.h"
+#include "sage_internal.h"
 #include "sage_common.h"
 #include "sage_kernels.h"
 #include "sage_kernels2.h"
@@ -915,6 +915,13 @@ int step_impl(sage_ctx* c, const int64_t* bounds, int64_t n_seg, int32_t pad, in
 }
 
 }  // namespace
+
+int sage_ctx_device(const sage_ctx* c) { return c->device; }
+int sage_ctx_compute_units(const sage_ctx* c) { return c->n_cu; }
+int sage_ctx_fail(sage_ctx* c, int code, const char* msg) noexcept {
+    try { c->err = msg; } catch (...) { }
+    return code;
+}
 
 extern "C" {
 

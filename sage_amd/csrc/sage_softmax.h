@@ -1,0 +1,667 @@
+// Softmax over a whole vocabulary: log probabilities of given tokens with entropy and the most likely alternatives, and
+// the gradient of both, without ever storing the [tokens][vocabulary] matrix of logits.
+//
+//   s_nv = x_n . w_v + b_v                 lse_n = log sum_v exp s_nv          p_nv = exp(s_nv - lse_n)
+//   logprob_n = s_n,t(n) - lse_n           H_n = lse_n - sum_v p_nv s_nv
+//   G_nv = g_n (1[v = t(n)] - p_nv) - h_n p_nv (log p_nv + H_n)     (g, h: the gradients of logprob and H)
+//   dx = G w      dw = G^T x      db_v = sum_n G_nv
+//
+// Matrix layout.  Every product runs on v_mfma_f32_16x16x32_bf16.  A "stationary" operand (tokens in the forward pass and
+// for dx, ids for dw) stays in a wave's registers, the other one "streams" past it 32 rows at a time.  The product is taken
+// with the streaming rows as matrix rows and the stationary ones as columns: lane l then holds, of column l % 16, the
+// rows 4 (l / 16) .. + 3, so maxima and sums over the streaming axis need no lane to talk to another one until the end,
+// and the eight weights of two 16-row tiles are, as they lie in the registers, the second operand of the next product
+// (its 32 summation slots are the 32 streaming rows in the order 16 (j / 4) + 4 (l / 16) + j % 4; the transposed
+// fragments are laid out in that order).
+//
+// bf16 inputs are multiplied as they are (products of two bf16 are exact in float32).  float32 inputs are taken as the sum
+// of three bf16 (8 + 8 + 8 bits: exact), and six of the nine products are formed -- the other three are below 2^-24 of
+// |x||w| --, which costs 6 bf16 MFMAs where the float32 MFMA costs 16 (256 against 4,096 operations per clock and CU).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+typedef __bf16 vs_bf8 __attribute__((ext_vector_type(8)));
+typedef float vs_f4 __attribute__((ext_vector_type(4)));
+typedef float vs_f8 __attribute__((ext_vector_type(8)));
+
+#define VS_LOG2E 1.4426950408889634f
+#define VS_LN2 0.6931471805599453f
+#define VS_CHUNK 64            // ids per stored maximum (the unit in which alternatives are looked for)
+#define VS_ROWS 32             // streaming rows per step
+#define VS_NOTHING (-1.0e30f)  // reference of a row that has seen no finite logit yet; a bias this low masks its id
+#define VS_SLACK 20.0f         // the running reference lags the maximum by at most this (in powers of two)
+#define VS_TMIN (-200.0f)      // 2^-200 is 0 in float32: what a logit of -inf is raised to, so that 0 * log p is 0
+
+struct VsSrc {                 // a row-major matrix of float32 or bf16
+    const void* p;
+    int64_t ld;                // elements from one row to the next
+    int32_t rows, dim;
+    int32_t is_bf16;
+};
+
+__device__ __forceinline__ float vs_load(const VsSrc& s, int64_t row, int d) {
+    return s.is_bf16 ? __uint_as_float((uint32_t)((const uint16_t*)s.p)[row * s.ld + d] << 16) : ((const float*)s.p)[row * s.ld + d];
+}
+
+// max(a, b) that keeps a NaN (fmaxf would turn a NaN logit into a masked one)
+__device__ __forceinline__ float vs_at_least(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+__device__ __forceinline__ vs_f4 vs_mfma(vs_bf8 a, vs_bf8 b, vs_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// a . b summed into c, both in PL parts (largest first); small products first
+template <int PL>
+__device__ __forceinline__ vs_f4 vs_mfma_parts(const vs_bf8* a, const vs_bf8* b, vs_f4 c) {
+    if constexpr (PL == 3) {
+        c = vs_mfma(a[1], b[1], c);
+        c = vs_mfma(a[2], b[0], c);
+        c = vs_mfma(a[0], b[2], c);
+        c = vs_mfma(a[1], b[0], c);
+        c = vs_mfma(a[0], b[1], c);
+    }
+    return vs_mfma(a[0], b[0], c);
+}
+
+// v as the sum of PL bf16 (each rounding to nearest; exact for PL = 3, within 2^-9 |v| for PL = 1)
+template <int PL>
+__device__ __forceinline__ void vs_split(vs_f8 v, vs_bf8* out) {
+#pragma unroll
+    for (int p = 0; p < PL; ++p) {
+        out[p] = __builtin_convertvector(v, vs_bf8);
+        if (p + 1 < PL) v -= __builtin_convertvector(out[p], vs_f8);
+    }
+}
+
+// ---- fragments ----------------------------------------------------------------------------------------------------
+// S fragments (16 rows x 32 elements): [row / 16][KS][PL][lane] of 8 bf16, lane l holding row l % 16, elements 8 (l / 16)..
+// T fragments (16 elements x 32 rows): [row / 32][2 KS][PL][lane], lane l holding element l % 16 and the rows in the order
+// 16 (j / 4) + 4 (l / 16) + j % 4.  Rows past the end and elements past `dim` are zero.  One workgroup packs 32 rows.
+// A fragment is one coalesced 1 KiB load of a wave, whatever the caller's row length, stride and alignment are.
+template <int KS, int PL>
+__global__ __launch_bounds__(256) void k_vs_pack(VsSrc src, uint4* __restrict__ S, uint4* __restrict__ T, float* __restrict__ group_max) {
+    constexpr int DP = KS * 32, LD = DP + 4;
+    __shared__ float tile[32 * LD];
+    __shared__ float wmax[4];
+    const int64_t row0 = (int64_t)blockIdx.x * 32;
+    float big = 0.0f;
+    for (int i = threadIdx.x; i < 32 * DP; i += 256) {
+        const int r = i / DP, d = i % DP;
+        const float v = (row0 + r < src.rows && d < src.dim) ? vs_load(src, row0 + r, d) : 0.0f;
+        tile[r * LD + d] = v;
+        big = fmaxf(big, fabsf(v));
+    }
+    for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o));
+    if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = big;
+    __syncthreads();
+    if (group_max && threadIdx.x == 0) group_max[blockIdx.x] = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+    for (int i = threadIdx.x; i < 2 * KS * 64; i += 256) {
+        const int lane = i & 63, f = i >> 6, rb = f / KS, ks = f % KS;
+        const float* at = tile + (rb * 16 + (lane & 15)) * LD + ks * 32 + (lane >> 4) * 8;
+        vs_f8 v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = at[j];
+        vs_bf8 part[PL];
+        vs_split<PL>(v, part);
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+            *(vs_bf8*)&S[((((int64_t)blockIdx.x * 2 + rb) * KS + ks) * PL + p) * 64 + lane] = part[p];
+    }
+    if (!T) return;
+    for (int i = threadIdx.x; i < 2 * KS * 64; i += 256) {
+        const int lane = i & 63, db = i >> 6;
+        vs_f8 v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = tile[((j >> 2) * 16 + (lane >> 4) * 4 + (j & 3)) * LD + db * 16 + (lane & 15)];
+        vs_bf8 part[PL];
+        vs_split<PL>(v, part);
+#pragma unroll
+        for (int p = 0; p < PL; ++p) *(vs_bf8*)&T[(((int64_t)blockIdx.x * 2 * KS + db) * PL + p) * 64 + lane] = part[p];
+    }
+}
+
+// The bias of every id, padded to whole chunks: 0 where the caller gives none, -inf past the end (p = 0 there).  A mask of
+// the type's lowest value becomes -inf too: next to it no logit keeps a bit, and float32 could not hold it in powers of two.
+__global__ __launch_bounds__(256) void k_vs_bias(const float* __restrict__ bias, int32_t vocab, int32_t padded, float* __restrict__ out) {
+    const int v = blockIdx.x * 256 + threadIdx.x;
+    if (v < padded) out[v] = v >= vocab ? -INFINITY : !bias ? 0.0f : bias[v] <= VS_NOTHING ? -INFINITY : bias[v];
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------
+struct VsFwd {
+    const uint4 *xS, *wS;
+    const float* bias;         // [padded vocabulary]
+    int32_t has_bias;          // the caller gave one: -inf may stand anywhere (else only past `vocab`)
+    int32_t vocab;
+    int32_t n_tiles;           // token tiles of 16 TB rows
+    int32_t splits;            // ranges of the vocabulary
+    int32_t chunks;            // chunks of VS_CHUNK ids
+    int64_t n_pad;             // row length of the partials
+    float4* part;              // [splits][n_pad]: reference (in powers of two), sum of exps, sum of exp * exponent
+    float* chunk_max;          // [n_pad][chunks] or null
+};
+
+// One unit of work is a wave: a tile of 16 TB tokens against one range of the vocabulary.  A softmax in one pass: sums are
+// kept relative to a reference that follows the running maximum in steps of at least 2^VS_SLACK (so that it is moved a few
+// times per row and the common step has no rescaling), the entropy's sum relative to the same reference.
+template <int KS, int PL, int TB>
+__global__ __launch_bounds__(256) void k_vs_forward(VsFwd a) {
+    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    const int unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= a.n_tiles * a.splits) return;
+    const int tile = unit % a.n_tiles, split = unit / a.n_tiles;
+    const int c0 = (int)((int64_t)a.chunks * split / a.splits), c1 = (int)((int64_t)a.chunks * (split + 1) / a.splits);
+    vs_bf8 x[TB][KS][PL];
+#pragma unroll
+    for (int t = 0; t < TB; ++t)
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int p = 0; p < PL; ++p)
+                x[t][k][p] = *(const vs_bf8*)&a.xS[((((int64_t)tile * TB + t) * KS + k) * PL + p) * 64 + lane];
+    float ref[TB], sum[TB], ent[TB], top[TB];
+#pragma unroll
+    for (int t = 0; t < TB; ++t) { ref[t] = VS_NOTHING; sum[t] = 0.0f; ent[t] = 0.0f; top[t] = -INFINITY; }
+    for (int c = c0; c < c1; ++c) {
+#pragma unroll 1
+        for (int h = 0; h < VS_CHUNK / VS_ROWS; ++h) {
+            const int row0 = c * VS_CHUNK + h * VS_ROWS;
+            const bool biased = a.has_bias || row0 + VS_ROWS > a.vocab;      // the same in the whole grid
+            vs_f4 s[2][TB];
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb) {
+                vs_f4 b = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (biased) b = *(const vs_f4*)&a.bias[row0 + rb * 16 + quad * 4];
+#pragma unroll
+                for (int t = 0; t < TB; ++t) s[rb][t] = b;
+            }
+            const uint4* w = a.wS + (int64_t)row0 / 16 * KS * PL * 64 + lane;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int rb = 0; rb < 2; ++rb) {
+                    vs_bf8 wf[PL];
+#pragma unroll
+                    for (int p = 0; p < PL; ++p) wf[p] = *(const vs_bf8*)&w[((rb * KS + k) * PL + p) * 64];
+#pragma unroll
+                    for (int t = 0; t < TB; ++t) s[rb][t] = vs_mfma_parts<PL>(wf, x[t][k], s[rb][t]);
+                }
+#pragma unroll
+            for (int t = 0; t < TB; ++t) {
+                float mx = fmaxf(fmaxf(fmaxf(s[0][t][0], s[0][t][1]), fmaxf(s[0][t][2], s[0][t][3])),
+                                 fmaxf(fmaxf(s[1][t][0], s[1][t][1]), fmaxf(s[1][t][2], s[1][t][3])));
+                top[t] = fmaxf(top[t], mx);
+                mx *= VS_LOG2E;
+                if (__any(mx > ref[t] + VS_SLACK)) {
+                    const float now = mx > ref[t] + VS_SLACK ? mx : ref[t];
+                    const float f = exp2f(ref[t] - now);
+                    ent[t] = f * fmaf(ref[t] - now, sum[t], ent[t]);
+                    sum[t] *= f;
+                    ref[t] = now;
+                }
+#pragma unroll
+                for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float e = fmaf(s[rb][t][i], VS_LOG2E, -ref[t]);
+                        if (biased) e = vs_at_least(e, VS_TMIN);
+                        const float p = __builtin_amdgcn_exp2f(e);
+                        sum[t] += p;
+                        ent[t] = fmaf(p, e, ent[t]);
+                    }
+            }
+        }
+        if (a.chunk_max) {
+#pragma unroll
+            for (int t = 0; t < TB; ++t) {
+                float m = fmaxf(top[t], __shfl_xor(top[t], 16));
+                m = fmaxf(m, __shfl_xor(m, 32));
+                if (quad == 0) a.chunk_max[((int64_t)tile * TB * 16 + t * 16 + col) * a.chunks + c] = m;
+                top[t] = -INFINITY;
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+#pragma unroll
+        for (int o = 16; o <= 32; o <<= 1) {
+            const float r2 = __shfl_xor(ref[t], o), s2 = __shfl_xor(sum[t], o), e2 = __shfl_xor(ent[t], o);
+            const float now = fmaxf(ref[t], r2), f1 = exp2f(ref[t] - now), f2 = exp2f(r2 - now);
+            ent[t] = f1 * fmaf(ref[t] - now, sum[t], ent[t]) + f2 * fmaf(r2 - now, s2, e2);
+            sum[t] = f1 * sum[t] + f2 * s2;
+            ref[t] = now;
+        }
+        if (quad == 0) a.part[(int64_t)split * a.n_pad + ((int64_t)tile * TB + t) * 16 + col] = make_float4(ref[t], sum[t], ent[t], 0.0f);
+    }
+}
+
+// Joins the ranges of a row and takes the given token's log probability: a wave per row.  The token's own logit is summed
+// in float64 (its rounding would otherwise show where the probability is near 1).
+struct VsJoin {
+    VsSrc x, w;
+    const float* bias;         // padded
+    const int64_t* targets;    // or null
+    const float4* part;
+    int32_t n, splits;
+    int64_t n_pad;
+    float *logprob, *entropy, *lse;
+};
+__global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= a.n) return;
+    float r = VS_NOTHING, s = 0.0f, e = 0.0f;
+    for (int i = lane; i < a.splits; i += 64) {
+        const float4 q = a.part[(int64_t)i * a.n_pad + row];
+        const float now = fmaxf(r, q.x), f1 = exp2f(r - now), f2 = exp2f(q.x - now);
+        e = f1 * fmaf(r - now, s, e) + f2 * fmaf(q.x - now, q.y, q.z);
+        s = f1 * s + f2 * q.y;
+        r = now;
+    }
+    for (int o = 1; o < 64; o <<= 1) {
+        const float r2 = __shfl_xor(r, o), s2 = __shfl_xor(s, o), e2 = __shfl_xor(e, o);
+        const float now = fmaxf(r, r2), f1 = exp2f(r - now), f2 = exp2f(r2 - now);
+        e = f1 * fmaf(r - now, s, e) + f2 * fmaf(r2 - now, s2, e2);
+        s = f1 * s + f2 * s2;
+        r = now;
+    }
+    const bool empty = s == 0.0f;                   // nothing but -inf
+    const double lse = empty ? -INFINITY : ((double)r + (double)log2f(s)) * 0.6931471805599453;
+    const int64_t t = a.targets ? a.targets[row] : -1;
+    double dot = 0.0;
+    if (t >= 0 && t < a.w.rows)
+        for (int d = lane; d < a.w.dim; d += 64) dot += (double)vs_load(a.x, row, d) * (double)vs_load(a.w, t, d);
+    for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
+    if (lane) return;
+    if (a.lse) a.lse[row] = (float)lse;
+    if (a.entropy) {
+        const float h = VS_LN2 * (log2f(s) - e / s);
+        a.entropy[row] = empty || h < 0.0f ? 0.0f : h;
+    }
+    if (a.logprob) {
+        float lp = 0.0f;
+        if (t >= a.w.rows) lp = NAN;
+        else if (t >= 0) {
+            dot += (double)a.bias[t];
+            lp = empty ? -INFINITY : (float)(dot - lse);
+            if (lp > 0.0f) lp = 0.0f;
+        }
+        a.logprob[row] = lp;
+    }
+}
+
+// ---- alternatives -------------------------------------------------------------------------------------------------
+// The k largest logits of a row, ties to the lower id, in the order of the logits as float64 sums them.  The forward pass
+// left each chunk's largest float32 logit m; its float32 sums are within d = 4 (D + 16) 2^-24 (|m| + 2 |x|_1 max |w|) of the
+// true ones.  The k-th largest m - d is a lower bound of the k-th logit, so only chunks with m + d at or above it can hold
+// one: a dozen or two, whose logits are formed again in float64.  A workgroup per row.
+#define VS_MAX_K 32
+#define VS_CAND 1024
+struct VsTop {
+    VsSrc x, w;
+    const float* bias;         // padded
+    const float* chunk_max;    // [rows][chunks]
+    const float* group_max;    // [padded vocabulary / 32] largest |w|
+    int32_t n, chunks, k;
+    const float* lse;
+    int32_t* ids;              // [n][k]
+    float* logprobs;           // [n][k]
+};
+
+__device__ __forceinline__ uint32_t vs_order(float f) {   // unsigned order = float order
+    const uint32_t u = __float_as_uint(f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ bool vs_before(double v, int i, double w, int j) { return v > w || (v == w && i < j); }
+
+__global__ __launch_bounds__(256) void k_vs_top(VsTop a) {
+    __shared__ float xs[512];
+    __shared__ uint32_t hist[256];
+    __shared__ double cv[VS_CAND], cw[VS_MAX_K];
+    __shared__ int ci[VS_CAND], cj[VS_MAX_K];
+    __shared__ int n_cand, sel, need_s, n_list;
+    __shared__ float red[4];
+    __shared__ int list[256];
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const float* cm = a.chunk_max + row * a.chunks;
+    float l1 = 0.0f;
+    for (int d = tid; d < a.x.dim; d += 256) { const float v = vs_load(a.x, row, d); xs[d] = v; l1 += fabsf(v); }
+    for (int o = 1; o < 64; o <<= 1) l1 += __shfl_xor(l1, o);
+    if (lane == 0) red[tid >> 6] = l1;
+    if (tid == 0) n_cand = 0;
+    __syncthreads();
+    l1 = red[0] + red[1] + red[2] + red[3];
+    const float eps = 4.0f * (float)(a.x.dim + 16) * 5.9604645e-8f;
+    auto off = [&](int c, float m) {
+        float g = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VS_CHUNK / 32; ++i) g = fmaxf(g, a.group_max[c * (VS_CHUNK / 32) + i]);
+        return eps * (fabsf(m) + 2.0f * l1 * g);
+    };
+    // the k-th largest lower bound, by its bits, eight at a time
+    uint32_t prefix = 0;
+    bool all = a.chunks <= a.k;
+    int need = a.k;
+    if (!all) {
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            hist[tid] = 0;
+            __syncthreads();
+            for (int c = tid; c < a.chunks; c += 256) {
+                const float m = cm[c];
+                const uint32_t u = vs_order(m - off(c, m));
+                if (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(u >> shift) & 255u], 1u);
+            }
+            __syncthreads();
+            if (tid == 0) {
+                int left = need, b = 255;
+                while (b > 0 && left > (int)hist[b]) left -= (int)hist[b--];
+                sel = b; need_s = left;
+            }
+            __syncthreads();
+            prefix |= (uint32_t)sel << shift;
+            need = need_s;
+            __syncthreads();
+        }
+    }
+    const uint32_t tu = prefix;
+    const float bound = all ? -INFINITY : __uint_as_float(tu & 0x80000000u ? tu & 0x7FFFFFFFu : ~tu);
+    double least = -INFINITY;       // the k-th best so far once k are known: what comes later must beat it
+    bool full = false;
+    auto compact = [&]() {          // keeps the best k of the candidates, in order
+        __syncthreads();
+        const int n = n_cand;
+        for (int i = tid; i < n; i += 256) {
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += vs_before(cv[j], ci[j], cv[i], ci[i]);
+            if (rank < a.k) { cw[rank] = cv[i]; cj[rank] = ci[i]; }
+        }
+        __syncthreads();
+        const int m = min(n, a.k);
+        if (tid < m) { cv[tid] = cw[tid]; ci[tid] = cj[tid]; }
+        if (tid == 0) n_cand = m;
+        __syncthreads();
+        if (m == a.k) { full = true; least = cv[m - 1]; }
+        __syncthreads();
+    };
+    constexpr int PER = 256 / VS_CHUNK;      // chunks that are looked at together
+    for (int c0 = 0; c0 < a.chunks; c0 += 256) {
+        // the next 256 chunks' candidates, in ascending order
+        if (tid == 0) n_list = 0;
+        __syncthreads();
+        const int c = c0 + tid;
+        bool want = false;
+        if (c < a.chunks) {
+            const float m = cm[c];
+            const float up = m + off(c, m);
+            want = up >= bound && m > -INFINITY && !(full && (double)up <= least);
+        }
+        const unsigned long long bal = __ballot(want);
+        for (int wv = 0; wv < 4; ++wv) {
+            if ((tid >> 6) == wv) {
+                if (want) list[n_list + __popcll(bal & ((1ull << lane) - 1ull))] = c;
+            }
+            __syncthreads();
+            if ((tid >> 6) == wv && lane == 0) n_list += __popcll(bal);
+            __syncthreads();
+        }
+        const int nl = n_list;
+        for (int i0 = 0; i0 < nl; i0 += PER) {
+            const int i = i0 + tid / VS_CHUNK;
+            if (i < nl) {
+                const int v = list[i] * VS_CHUNK + tid % VS_CHUNK;
+                if (v < a.w.rows) {
+                    double s = 0.0;
+                    for (int d = 0; d < a.w.dim; ++d) s = fma((double)xs[d], (double)vs_load(a.w, v, d), s);
+                    s += (double)a.bias[v];
+                    // (a double below every candidate chunk's lower bound is none of the k)
+                    if (s >= (double)bound && s > -INFINITY && !(full && s <= least)) {
+                        const int at = atomicAdd(&n_cand, 1);
+                        cv[at] = s; ci[at] = v;
+                    }
+                }
+            }
+            __syncthreads();
+            if (n_cand > VS_CAND - 256) compact();
+            __syncthreads();
+        }
+        __syncthreads();
+    }
+    compact();
+    if (tid < a.k) {
+        const float lse = a.lse[row];
+        const bool have = tid < n_cand && lse == lse;
+        a.ids[row * a.k + tid] = have ? ci[tid] : -1;
+        a.logprobs[row * a.k + tid] = have ? fminf((float)(cv[tid] - (double)lse), 0.0f) : lse == lse ? -INFINITY : lse;
+    }
+}
+
+// ---- backward -----------------------------------------------------------------------------------------------------
+// What the gradient kernels read of a row: lse in powers of two, and G = p (A + B e) + gl [v = target], e = log2 p.
+struct VsRow {
+    float* lse2;               // [n_pad]
+    float* A;
+    float* B;
+    float* gl;
+    int32_t* target;
+};
+__global__ __launch_bounds__(256) void k_vs_rows(const float* __restrict__ lse, const float* __restrict__ entropy, const int64_t* __restrict__ targets,
+                                                 const float* __restrict__ g, const float* __restrict__ h, int32_t n, int64_t n_pad, int32_t vocab, VsRow r) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n_pad) return;
+    // rows past the end and rows whose every id is masked: an lse that makes every p 0, whatever the bias is
+    float l2 = -VS_NOTHING, A = 0.0f, B = 0.0f, gl = 0.0f;
+    int32_t t = -1;
+    if (i < n) {
+        const float l = lse[i];
+        const int64_t tt = targets ? targets[i] : -1;
+        const bool empty = l == -INFINITY;
+        float fix = 1.0f;                         // p is short of 2^-(rounding of l2); A and B make up for it
+        if (!empty) {
+            const double exact = (double)l * 1.4426950408889634;
+            l2 = (float)exact;
+            fix = exp2f((float)((double)l2 - exact));
+        }
+        if (tt >= 0 && g) gl = g[i];
+        if (tt >= vocab) gl = NAN;
+        t = tt >= 0 && tt < vocab ? (int32_t)tt : -1;
+        A = -gl;
+        if (h && !empty) { A -= h[i] * entropy[i]; B = -h[i] * VS_LN2; }
+        A *= fix; B *= fix;
+    }
+    r.lse2[i] = l2; r.A[i] = A; r.B[i] = B; r.gl[i] = gl; r.target[i] = t;
+}
+
+struct VsBwd {
+    const uint4 *stayS;        // stationary rows (columns of the product)
+    const uint4 *flowS, *flowT;// streaming rows, and transposed
+    const float* bias;         // padded, by id
+    int32_t has_bias, has_entropy;
+    int32_t vocab;
+    VsRow row;                 // by token
+    int32_t n_tiles, splits, groups;   // groups of 32 streaming rows
+    int64_t stay_pad;          // rows of a partial
+    float* part;               // [splits][stay_pad][32 KS]
+    float* bias_part;          // [splits][stay_pad] (OF_IDS with a bias gradient)
+};
+
+// One wave: a tile of 16 TB stationary rows against one range of the streaming ones.  OF_IDS = false: the stationary rows
+// are tokens, the result sum_v p' w_v with p' = p (A + B e), or p alone when there is no entropy gradient (A is then a
+// factor of the whole row, applied at the end); the target's own term is added at the end too, so that the largest
+// coefficient is never rounded to bf16.  OF_IDS = true: the stationary rows are ids, the result sum_n G_nv x_n; the few
+// steps in which a token's target lies in the tile add the rounded-off part of G in a second product.
+template <int KS, int PL, int TB, bool OF_IDS>
+__global__ __launch_bounds__(256) void k_vs_backward(VsBwd a) {
+    constexpr int DP = KS * 32;
+    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    const int unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= a.n_tiles * a.splits) return;
+    const int tile = unit % a.n_tiles, split = unit / a.n_tiles;
+    const int g0 = (int)((int64_t)a.groups * split / a.splits), g1 = (int)((int64_t)a.groups * (split + 1) / a.splits);
+    const int64_t stay0 = (int64_t)tile * TB * 16;
+    vs_bf8 y[TB][KS][PL];
+#pragma unroll
+    for (int t = 0; t < TB; ++t)
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int p = 0; p < PL; ++p)
+                y[t][k][p] = *(const vs_bf8*)&a.stayS[((((int64_t)tile * TB + t) * KS + k) * PL + p) * 64 + lane];
+    float lse2[TB], A[TB], B[TB], b0[TB], db[TB];
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+        const int64_t r = stay0 + t * 16 + col;
+        if constexpr (OF_IDS) { b0[t] = a.bias[r]; db[t] = 0.0f; }
+        else { lse2[t] = a.row.lse2[r]; A[t] = a.row.A[r]; B[t] = a.row.B[r]; }
+    }
+    vs_f4 acc[2 * KS][TB];
+#pragma unroll
+    for (int d = 0; d < 2 * KS; ++d)
+#pragma unroll
+        for (int t = 0; t < TB; ++t) acc[d][t] = vs_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int g = g0; g < g1; ++g) {
+        const int row0 = g * 32;
+        vs_f4 s[2][TB];
+        const bool biased = a.has_bias || (OF_IDS ? stay0 + TB * 16 > a.vocab : row0 + 32 > a.vocab);
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+            vs_f4 b = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (!OF_IDS && biased) b = *(const vs_f4*)&a.bias[row0 + rb * 16 + quad * 4];
+#pragma unroll
+            for (int t = 0; t < TB; ++t) {
+                if constexpr (OF_IDS) s[rb][t] = vs_f4{b0[t], b0[t], b0[t], b0[t]};
+                else s[rb][t] = b;
+            }
+        }
+        const uint4* f = a.flowS + (int64_t)g * 2 * KS * PL * 64 + lane;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb) {
+                vs_bf8 wf[PL];
+#pragma unroll
+                for (int p = 0; p < PL; ++p) wf[p] = *(const vs_bf8*)&f[((rb * KS + k) * PL + p) * 64];
+#pragma unroll
+                for (int t = 0; t < TB; ++t) s[rb][t] = vs_mfma_parts<PL>(wf, y[t][k], s[rb][t]);
+            }
+        vs_f4 L[2], rA[2], rB[2];
+        bool hit = false;
+        if constexpr (OF_IDS) {
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb) {
+                L[rb] = *(const vs_f4*)&a.row.lse2[row0 + rb * 16 + quad * 4];
+                rA[rb] = *(const vs_f4*)&a.row.A[row0 + rb * 16 + quad * 4];
+                if (a.has_entropy) rB[rb] = *(const vs_f4*)&a.row.B[row0 + rb * 16 + quad * 4];
+            }
+            const int64_t t = a.row.target[row0 + (lane & 31)];
+            hit = __any(t >= stay0 && t < stay0 + TB * 16);
+        }
+        vs_bf8 P[TB][PL], R[TB];
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
+            vs_f8 G;
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float e = fmaf(s[rb][t][i], VS_LOG2E, OF_IDS ? -L[rb][i] : -lse2[t]);
+                    if (biased) e = vs_at_least(e, VS_TMIN);
+                    float q = __builtin_amdgcn_exp2f(e);
+                    if constexpr (OF_IDS) q *= a.has_entropy ? fmaf(rB[rb][i], e, rA[rb][i]) : rA[rb][i];
+                    else if (a.has_entropy) q *= fmaf(B[t], e, A[t]);
+                    G[rb * 4 + i] = q;
+                }
+            if constexpr (OF_IDS) {
+                if (hit) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int at = row0 + (j >> 2) * 16 + quad * 4 + (j & 3);
+                        if (a.row.target[at] == (int32_t)(stay0 + t * 16 + col)) G[j] += a.row.gl[at];
+                    }
+                }
+                if (a.bias_part)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) db[t] += G[j];
+            }
+            vs_split<PL>(G, P[t]);
+            if (OF_IDS && PL == 1) R[t] = __builtin_convertvector(G - __builtin_convertvector(P[t][0], vs_f8), vs_bf8);
+        }
+        const uint4* ft = a.flowT + (int64_t)g * 2 * KS * PL * 64 + lane;
+#pragma unroll
+        for (int d = 0; d < 2 * KS; ++d) {
+            vs_bf8 wf[PL];
+#pragma unroll
+            for (int p = 0; p < PL; ++p) wf[p] = *(const vs_bf8*)&ft[(d * PL + p) * 64];
+#pragma unroll
+            for (int t = 0; t < TB; ++t) acc[d][t] = vs_mfma_parts<PL>(wf, P[t], acc[d][t]);
+        }
+        if (OF_IDS && PL == 1 && hit) {
+#pragma unroll
+            for (int d = 0; d < 2 * KS; ++d) {
+                const vs_bf8 wf = *(const vs_bf8*)&ft[d * 64];
+#pragma unroll
+                for (int t = 0; t < TB; ++t) acc[d][t] = vs_mfma(wf, R[t], acc[d][t]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+        const int64_t r = stay0 + t * 16 + col;
+        float* out = a.part + ((int64_t)split * a.stay_pad + r) * DP;
+#pragma unroll
+        for (int d = 0; d < 2 * KS; ++d) *(vs_f4*)&out[d * 16 + quad * 4] = acc[d][t];
+        if constexpr (OF_IDS) {
+            if (a.bias_part) {
+                float v = db[t] + __shfl_xor(db[t], 16);
+                v += __shfl_xor(v, 32);
+                if (quad == 0) a.bias_part[(int64_t)split * a.stay_pad + r] = v;
+            }
+        }
+    }
+}
+
+// Sums the partials of a row in a fixed order and writes it: dx = A sum p w + gl w_t (without an entropy gradient; with
+// one the partials hold p (A + B e) already), dw as it is, db beside it.
+struct VsSum {
+    const float* part;
+    const float* bias_part;
+    int32_t rows, dim, dp, splits;
+    int64_t pad;
+    VsRow row;                 // of tokens: null pointers for dw
+    int32_t has_entropy;
+    VsSrc w;
+    void* out;
+    int64_t ldo;
+    int32_t out_bf16;
+    float* db;
+};
+__device__ __forceinline__ void vs_store(void* p, int64_t at, float v, int bf16) {
+    if (bf16) ((__bf16*)p)[at] = (__bf16)v;
+    else ((float*)p)[at] = v;
+}
+__global__ __launch_bounds__(256) void k_vs_sum(VsSum a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (a.db && i < a.rows) {
+        float v = 0.0f;
+        for (int s = 0; s < a.splits; ++s) v += a.bias_part[(int64_t)s * a.pad + i];
+        a.db[i] = v;
+    }
+    if (i >= (int64_t)a.rows * a.dim) return;
+    const int64_t r = i / a.dim;
+    const int d = (int)(i % a.dim);
+    float v = 0.0f;
+    for (int s = 0; s < a.splits; ++s) v += a.part[((int64_t)s * a.pad + r) * a.dp + d];
+    if (a.row.A) {
+        if (!a.has_entropy) v *= a.row.A[r];
+        const int32_t t = a.row.target[r];
+        if (t >= 0) v = fmaf(a.row.gl[r], vs_load(a.w, t, d), v);
+        else if (a.row.gl[r] != a.row.gl[r]) v = a.row.gl[r];
+    }
+    vs_store(a.out, r * a.ldo + d, v, a.out_bf16);
+}
+
+// no tokens: dw = 0, db = 0
+__global__ __launch_bounds__(256) void k_vs_zero(void* out, int64_t ldo, int32_t rows, int32_t dim, int32_t out_bf16, float* db) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (db && i < rows) db[i] = 0.0f;
+    if (i < (int64_t)rows * dim) vs_store(out, i / dim * ldo + i % dim, 0.0f, out_bf16);
+}

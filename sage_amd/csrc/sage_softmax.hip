@@ -1,0 +1,418 @@
+// Host side of the vocabulary softmax and of gradient clipping (include/sage_hip.h).  gfx950 (MI355X) only.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+#include <utility>
+#include <vector>
+
+#include "sage_internal.h"
+#include "sage_softmax.h"
+#include "sage_clip.h"
+
+namespace {
+
+constexpr int64_t VS_PAD = 128;                 // rows and ids are padded to this
+constexpr int64_t VS_ROWS_MAX = 16384;          // tokens of one pass of the forward kernels
+constexpr size_t VS_ALIGN = 256;
+
+inline int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+inline uint32_t cdiv(int64_t a, int64_t b) { return (uint32_t)((a + b - 1) / b); }
+
+// Makes the context's device current for a call and puts the caller's back.
+struct OnDevice {
+    int before = -1;
+    bool ok = false;
+    explicit OnDevice(int device) {
+        if (hipGetDevice(&before) != hipSuccess) before = -1;
+        ok = before == device || hipSetDevice(device) == hipSuccess;
+        if (before == device) before = -1;
+    }
+    ~OnDevice() { if (before >= 0) (void)hipSetDevice(before); }
+};
+
+struct Arena {                                   // offsets first (base null), pointers later
+    char* base = nullptr;
+    int64_t used = 0;
+    template <class T> T* take(int64_t n) {
+        T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+        used += up(n * (int64_t)sizeof(T), VS_ALIGN);
+        return p;
+    }
+};
+
+int launched(sage_ctx* c, const char* what) {
+    const hipError_t e = hipGetLastError();
+    if (e == hipSuccess) return SAGE_OK;
+    char msg[256];
+    std::snprintf(msg, sizeof msg, "%s: %s", what, hipGetErrorString(e));
+    return sage_ctx_fail(c, SAGE_E_HIP, msg);
+}
+
+// 32-element steps of the padded row width: the instantiations there are
+int vs_steps(int dim) {
+    const int opts[] = {2, 4, 8, 10, 16};
+    for (int o : opts) if (dim <= o * 32) return o;
+    return 0;
+}
+
+// 16-row blocks of stationary rows a wave holds
+constexpr int vs_fwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 4 ? 4 : 2) : (ks <= 4 ? 2 : 1); }
+constexpr int vs_bwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 2 ? 4 : ks <= 8 ? 2 : 1) : (ks <= 4 ? 2 : 1); }
+
+#define VS_BY_WIDTH(ks, pl, F)                                                        \
+    do {                                                                              \
+        if ((pl) == 1) {                                                              \
+            switch (ks) {                                                             \
+            case 2: { F(2, 1); break; }                                               \
+            case 4: { F(4, 1); break; }                                               \
+            case 8: { F(8, 1); break; }                                               \
+            case 10: { F(10, 1); break; }                                             \
+            default: { F(16, 1); break; }                                             \
+            }                                                                         \
+        } else {                                                                      \
+            switch (ks) {                                                             \
+            case 2: { F(2, 3); break; }                                               \
+            case 4: { F(4, 3); break; }                                               \
+            case 8: { F(8, 3); break; }                                               \
+            case 10: { F(10, 3); break; }                                             \
+            default: { F(16, 3); break; }                                             \
+            }                                                                         \
+        }                                                                             \
+    } while (0)
+
+struct Shape {
+    int64_t n, vocab, vp;        // tokens, ids, padded ids
+    int dim, ks, pl, k, cus;
+};
+
+int vs_block_rows(const Shape& s, bool fwd) {
+    int tb = 1;
+#define VS_F(KS, PL) tb = fwd ? vs_fwd_blocks(KS, PL) : vs_bwd_blocks(KS, PL)
+    VS_BY_WIDTH(s.ks, s.pl, VS_F);
+#undef VS_F
+    return tb * 16;
+}
+
+// ranges that `flow` streaming units are cut into so that tiles x ranges fill the chip: 4 waves a workgroup, two
+// workgroups a CU
+int vs_splits(const Shape& s, int64_t tiles, int64_t flow, int64_t most) {
+    const int64_t want = cdiv((int64_t)s.cus * 8, tiles);
+    return (int)std::max<int64_t>(1, std::min(std::min(want, flow), most));
+}
+
+struct FwdPlan {
+    int64_t rows, n_pad, tiles, chunks;
+    int splits;
+    uint4 *xS, *wS;
+    float *bias, *group_max, *chunk_max;
+    float4* part;
+    int64_t bytes;
+};
+FwdPlan plan_fwd(const Shape& s, void* ws) {
+    FwdPlan p{};
+    Arena a{(char*)ws};
+    const int br = vs_block_rows(s, true);
+    p.rows = std::min(s.n, VS_ROWS_MAX);
+    p.n_pad = up(p.rows, VS_PAD);
+    p.tiles = cdiv(p.rows, br);
+    p.chunks = s.vp / VS_CHUNK;
+    p.splits = vs_splits(s, p.tiles, p.chunks, 1 << 20);
+    const int64_t frag = (int64_t)s.ks * s.pl * 64;          // uint4 of a 16-row block
+    p.wS = a.take<uint4>(s.vp / 16 * frag);
+    p.xS = a.take<uint4>(p.n_pad / 16 * frag);
+    p.bias = a.take<float>(s.vp);
+    p.group_max = a.take<float>(s.vp / 32);
+    p.part = a.take<float4>(p.splits * p.n_pad);
+    p.chunk_max = a.take<float>(s.k ? p.n_pad * p.chunks : 0);
+    p.bytes = a.used;
+    return p;
+}
+
+struct BwdPlan {
+    int64_t np, tiles_x, tiles_w;
+    int splits_x, splits_w;
+    uint4 *xS, *xT, *wS, *wT;
+    float *bias, *part, *bias_part;
+    VsRow row;
+    int64_t bytes;
+};
+BwdPlan plan_bwd(const Shape& s, bool with_bias, void* ws) {
+    BwdPlan p{};
+    Arena a{(char*)ws};
+    const int br = vs_block_rows(s, false);
+    p.np = up(s.n, VS_PAD);
+    p.tiles_x = cdiv(s.n, br);
+    p.tiles_w = cdiv(s.vocab, br);
+    p.splits_x = vs_splits(s, p.tiles_x, s.vp / 32, 1 << 20);
+    p.splits_w = vs_splits(s, p.tiles_w, p.np / 32, 1 << 20);
+    const int64_t frag = (int64_t)s.ks * s.pl * 64;
+    p.wS = a.take<uint4>(s.vp / 16 * frag);
+    p.wT = a.take<uint4>(s.vp / 16 * frag);
+    p.xS = a.take<uint4>(p.np / 16 * frag);
+    p.xT = a.take<uint4>(p.np / 16 * frag);
+    p.bias = a.take<float>(s.vp);
+    p.row.lse2 = a.take<float>(p.np);
+    p.row.A = a.take<float>(p.np);
+    p.row.B = a.take<float>(p.np);
+    p.row.gl = a.take<float>(p.np);
+    p.row.target = a.take<int32_t>(p.np);
+    // dx and dw are formed one after the other: their partials share the space
+    p.part = a.take<float>(std::max(p.splits_x * p.np, p.splits_w * s.vp) * s.ks * 32);
+    p.bias_part = with_bias ? a.take<float>(p.splits_w * s.vp) : nullptr;
+    p.bytes = a.used;
+    return p;
+}
+
+int vs_shape(sage_ctx* c, int32_t dtype, int64_t n, int64_t vocab, int32_t dim, int32_t k, Shape* s) {
+    if (dtype != SAGE_F32 && dtype != SAGE_BF16) return sage_ctx_fail(c, SAGE_E_ARG, "dtype must be SAGE_F32 or SAGE_BF16");
+    if (n < 0 || vocab < 1 || dim < 1) return sage_ctx_fail(c, SAGE_E_ARG, "need n >= 0, vocab >= 1 and dim >= 1");
+    if (k < 0 || k > VS_MAX_K) return sage_ctx_fail(c, SAGE_E_LIMIT, "at most 32 alternatives");
+    if (dim > 512) return sage_ctx_fail(c, SAGE_E_LIMIT, "embedding dimension above 512 is not supported");
+    if (vocab > (1 << 20)) return sage_ctx_fail(c, SAGE_E_LIMIT, "a vocabulary of more than 2^20 ids is not supported");
+    if (n > (1 << 22)) return sage_ctx_fail(c, SAGE_E_LIMIT, "more than 2^22 tokens in one call are not supported");
+    *s = Shape{n, vocab, up(vocab, VS_PAD), dim, vs_steps(dim), dtype == SAGE_BF16 ? 1 : 3, k, sage_ctx_compute_units(c)};
+    return SAGE_OK;
+}
+
+int check_matrix(sage_ctx* c, const char* what, const void* p, int64_t ld, int32_t dim, int32_t dtype) {
+    char msg[128];
+    const int size = dtype == SAGE_BF16 ? 2 : 4;
+    if (!p) std::snprintf(msg, sizeof msg, "%s is null", what);
+    else if (ld < dim) std::snprintf(msg, sizeof msg, "%s: rows overlap (stride %lld, dimension %d)", what, (long long)ld, (int)dim);
+    else if ((uintptr_t)p % size) std::snprintf(msg, sizeof msg, "%s is not aligned to its elements", what);
+    else return SAGE_OK;
+    return sage_ctx_fail(c, SAGE_E_ARG, msg);
+}
+
+int check_workspace(sage_ctx* c, const void* p, int64_t have, int64_t need) {
+    char msg[128];
+    if (!p || (uintptr_t)p % VS_ALIGN) std::snprintf(msg, sizeof msg, "the workspace must be aligned to 256 bytes");
+    else if (have < need) std::snprintf(msg, sizeof msg, "the workspace holds %lld bytes, %lld are needed", (long long)have, (long long)need);
+    else return SAGE_OK;
+    return sage_ctx_fail(c, SAGE_E_ARG, msg);
+}
+
+void pack(const Shape& s, const VsSrc& src, int64_t padded, uint4* S, uint4* T, float* group_max, hipStream_t st) {
+#define VS_F(KS, PL) k_vs_pack<KS, PL><<<(uint32_t)(padded / 32), 256, 0, st>>>(src, S, T, group_max)
+    VS_BY_WIDTH(s.ks, s.pl, VS_F);
+#undef VS_F
+}
+
+VsSrc rows_from(const VsSrc& m, int64_t row, int64_t rows) {
+    VsSrc r = m;
+    r.p = (const char*)m.p + row * m.ld * (m.is_bf16 ? 2 : 4);
+    r.rows = (int32_t)rows;
+    return r;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t sage_token_logprobs_workspace(sage_ctx* c, int32_t dtype, int64_t n, int64_t vocab, int32_t dim, int32_t alternatives) {
+    if (!c) return SAGE_E_ARG;
+    Shape s;
+    const int rc = vs_shape(c, dtype, n, vocab, dim, alternatives, &s);
+    if (rc) return rc;
+    return n ? plan_fwd(s, nullptr).bytes : 0;
+}
+
+int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vocab, int32_t dim, const void* d_x, int64_t ldx,
+                               const void* d_weight, int64_t ldw, const float* d_bias, const int64_t* d_targets, int32_t alternatives,
+                               float* d_logprob, float* d_entropy, float* d_lse, int32_t* d_alt_ids, float* d_alt_logprobs,
+                               void* d_workspace, int64_t workspace_bytes, void* stream) {
+    if (!c) return SAGE_E_ARG;
+    Shape s;
+    int rc = vs_shape(c, dtype, n, vocab, dim, alternatives, &s);
+    if (rc) return rc;
+    if (!d_lse && n) return sage_ctx_fail(c, SAGE_E_ARG, "d_lse is null");
+    if (alternatives && n && (!d_alt_ids || !d_alt_logprobs)) return sage_ctx_fail(c, SAGE_E_ARG, "alternatives need d_alt_ids and d_alt_logprobs");
+    if (d_logprob && n && !d_targets) return sage_ctx_fail(c, SAGE_E_ARG, "d_logprob needs d_targets");
+    if (n && (rc = check_matrix(c, "d_x", d_x, ldx, dim, dtype))) return rc;
+    if ((rc = check_matrix(c, "d_weight", d_weight, ldw, dim, dtype))) return rc;
+    if (n == 0) return SAGE_OK;
+    const FwdPlan p = plan_fwd(s, d_workspace);
+    if ((rc = check_workspace(c, d_workspace, workspace_bytes, p.bytes))) return rc;
+    OnDevice dev(sage_ctx_device(c));
+    if (!dev.ok) return sage_ctx_fail(c, SAGE_E_HIP, "the context's device cannot be made current");
+    const hipStream_t st = (hipStream_t)stream;
+    const VsSrc w{d_weight, ldw, (int32_t)vocab, dim, dtype == SAGE_BF16}, x{d_x, ldx, (int32_t)n, dim, dtype == SAGE_BF16};
+    pack(s, w, s.vp, p.wS, nullptr, alternatives ? p.group_max : nullptr, st);
+    k_vs_bias<<<cdiv(s.vp, 256), 256, 0, st>>>(d_bias, (int32_t)vocab, (int32_t)s.vp, p.bias);
+    for (int64_t r0 = 0; r0 < n; r0 += p.rows) {
+        const int64_t rows = std::min(p.rows, n - r0);
+        const VsSrc xr = rows_from(x, r0, rows);
+        pack(s, xr, p.n_pad, p.xS, nullptr, nullptr, st);
+        const VsFwd f{p.xS, p.wS, p.bias, d_bias != nullptr, (int32_t)vocab, (int32_t)p.tiles, p.splits, (int32_t)p.chunks, p.n_pad, p.part,
+                      alternatives ? p.chunk_max : nullptr};
+        const uint32_t grid = cdiv(p.tiles * p.splits, 4);
+#define VS_F(KS, PL) k_vs_forward<KS, PL, vs_fwd_blocks(KS, PL)><<<grid, 256, 0, st>>>(f)
+        VS_BY_WIDTH(s.ks, s.pl, VS_F);
+#undef VS_F
+        const VsJoin j{xr, w, p.bias, d_targets ? d_targets + r0 : nullptr, p.part, (int32_t)rows, p.splits, p.n_pad,
+                       d_logprob ? d_logprob + r0 : nullptr, d_entropy ? d_entropy + r0 : nullptr, d_lse + r0};
+        k_vs_join<<<cdiv(rows, 4), 256, 0, st>>>(j);
+        if (alternatives) {
+            const VsTop t{xr, w, p.bias, p.chunk_max, p.group_max, (int32_t)rows, (int32_t)p.chunks, alternatives, d_lse + r0,
+                          d_alt_ids + r0 * alternatives, d_alt_logprobs + r0 * alternatives};
+            k_vs_top<<<(uint32_t)rows, 256, 0, st>>>(t);
+        }
+    }
+    return launched(c, "sage_token_logprobs_device");
+}
+
+int64_t sage_token_logprobs_backward_workspace(sage_ctx* c, int32_t dtype, int64_t n, int64_t vocab, int32_t dim) {
+    if (!c) return SAGE_E_ARG;
+    Shape s;
+    const int rc = vs_shape(c, dtype, n, vocab, dim, 0, &s);
+    if (rc) return rc;
+    return n ? plan_bwd(s, true, nullptr).bytes : 0;
+}
+
+int sage_token_logprobs_backward_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vocab, int32_t dim, const void* d_x, int64_t ldx,
+                                        const void* d_weight, int64_t ldw, const float* d_bias, const int64_t* d_targets,
+                                        const float* d_lse, const float* d_entropy, const float* d_grad_logprob, const float* d_grad_entropy,
+                                        void* d_dx, int64_t lddx, void* d_dweight, int64_t lddw, float* d_dbias, void* d_workspace,
+                                        int64_t workspace_bytes, void* stream) {
+    if (!c) return SAGE_E_ARG;
+    Shape s;
+    int rc = vs_shape(c, dtype, n, vocab, dim, 0, &s);
+    if (rc) return rc;
+    if (n && !d_lse) return sage_ctx_fail(c, SAGE_E_ARG, "d_lse is null");
+    if (n && !d_grad_logprob && !d_grad_entropy) return sage_ctx_fail(c, SAGE_E_ARG, "no gradient is given");
+    if (n && d_grad_logprob && !d_targets) return sage_ctx_fail(c, SAGE_E_ARG, "d_grad_logprob needs d_targets");
+    if (n && d_grad_entropy && !d_entropy) return sage_ctx_fail(c, SAGE_E_ARG, "d_grad_entropy needs d_entropy");
+    if (!d_dx && !d_dweight && !d_dbias) return sage_ctx_fail(c, SAGE_E_ARG, "no result is asked for");
+    if (d_dbias && !d_dweight) return sage_ctx_fail(c, SAGE_E_ARG, "d_dbias comes with d_dweight");
+    if (n && (rc = check_matrix(c, "d_x", d_x, ldx, dim, dtype))) return rc;
+    if ((rc = check_matrix(c, "d_weight", d_weight, ldw, dim, dtype))) return rc;
+    if (n && d_dx && (rc = check_matrix(c, "d_dx", d_dx, lddx, dim, dtype))) return rc;
+    if (d_dweight && (rc = check_matrix(c, "d_dweight", d_dweight, lddw, dim, dtype))) return rc;
+    OnDevice dev(sage_ctx_device(c));
+    if (!dev.ok) return sage_ctx_fail(c, SAGE_E_HIP, "the context's device cannot be made current");
+    const hipStream_t st = (hipStream_t)stream;
+    const int bf16 = dtype == SAGE_BF16;
+    if (n == 0) {
+        if (d_dweight) k_vs_zero<<<cdiv(vocab * dim, 256), 256, 0, st>>>(d_dweight, lddw, (int32_t)vocab, dim, bf16, d_dbias);
+        return launched(c, "sage_token_logprobs_backward_device");
+    }
+    const BwdPlan p = plan_bwd(s, true, d_workspace);
+    if ((rc = check_workspace(c, d_workspace, workspace_bytes, p.bytes))) return rc;
+    const VsSrc w{d_weight, ldw, (int32_t)vocab, dim, bf16}, x{d_x, ldx, (int32_t)n, dim, bf16};
+    pack(s, w, s.vp, p.wS, d_dx ? p.wT : nullptr, nullptr, st);
+    pack(s, x, p.np, p.xS, d_dweight ? p.xT : nullptr, nullptr, st);
+    k_vs_bias<<<cdiv(s.vp, 256), 256, 0, st>>>(d_bias, (int32_t)vocab, (int32_t)s.vp, p.bias);
+    k_vs_rows<<<cdiv(p.np, 256), 256, 0, st>>>(d_lse, d_entropy, d_targets, d_grad_logprob, d_grad_entropy, (int32_t)n, p.np, (int32_t)vocab, p.row);
+    VsBwd b{};
+    b.bias = p.bias; b.has_bias = d_bias != nullptr; b.has_entropy = d_grad_entropy != nullptr; b.vocab = (int32_t)vocab; b.row = p.row; b.part = p.part;
+    if (d_dx) {
+        b.stayS = p.xS; b.flowS = p.wS; b.flowT = p.wT;
+        b.n_tiles = (int32_t)p.tiles_x; b.splits = p.splits_x; b.groups = (int32_t)(s.vp / 32); b.stay_pad = p.np; b.bias_part = nullptr;
+        const uint32_t grid = cdiv(p.tiles_x * p.splits_x, 4);
+#define VS_F(KS, PL) k_vs_backward<KS, PL, vs_bwd_blocks(KS, PL), false><<<grid, 256, 0, st>>>(b)
+        VS_BY_WIDTH(s.ks, s.pl, VS_F);
+#undef VS_F
+        const VsSum r{p.part, nullptr, (int32_t)n, dim, s.ks * 32, p.splits_x, p.np, p.row, b.has_entropy, w, d_dx, lddx, bf16, nullptr};
+        k_vs_sum<<<cdiv(n * dim, 256), 256, 0, st>>>(r);
+    }
+    if (d_dweight) {
+        b.stayS = p.wS; b.flowS = p.xS; b.flowT = p.xT;
+        b.n_tiles = (int32_t)p.tiles_w; b.splits = p.splits_w; b.groups = (int32_t)(p.np / 32); b.stay_pad = s.vp;
+        b.bias_part = d_dbias ? p.bias_part : nullptr;
+        const uint32_t grid = cdiv(p.tiles_w * p.splits_w, 4);
+#define VS_F(KS, PL) k_vs_backward<KS, PL, vs_bwd_blocks(KS, PL), true><<<grid, 256, 0, st>>>(b)
+        VS_BY_WIDTH(s.ks, s.pl, VS_F);
+#undef VS_F
+        const VsSum r{p.part, p.bias_part, (int32_t)vocab, dim, s.ks * 32, p.splits_w, s.vp, VsRow{}, 0, w, d_dweight, lddw, bf16, d_dbias};
+        k_vs_sum<<<cdiv(vocab * dim, 256), 256, 0, st>>>(r);
+    }
+    return launched(c, "sage_token_logprobs_backward_device");
+}
+
+int64_t sage_clip_grad_norm_workspace(sage_ctx* c, int64_t n_tensors, const int64_t* sizes) {
+    if (!c) return SAGE_E_ARG;
+    if (n_tensors < 0 || (n_tensors && !sizes)) return sage_ctx_fail(c, SAGE_E_ARG, "need n_tensors >= 0 and their sizes");
+    int64_t blocks = 0;
+    for (int64_t i = 0; i < n_tensors; ++i) {
+        if (sizes[i] < 0) return sage_ctx_fail(c, SAGE_E_ARG, "a tensor has a negative size");
+        if (sizes[i] > (int64_t)1 << 40) return sage_ctx_fail(c, SAGE_E_LIMIT, "a tensor of more than 2^40 elements is not supported");
+        blocks += (sizes[i] + CLIP_BLOCK - 1) / CLIP_BLOCK;
+        if (blocks > 1 << 30) return sage_ctx_fail(c, SAGE_E_LIMIT, "more than 2^45 elements are not supported");
+    }
+    return up(blocks * 8, VS_ALIGN) + (int64_t)VS_ALIGN;
+}
+
+int sage_clip_grad_norm_device(sage_ctx* c, int64_t n_tensors, const void* const* d_grads, void* const* d_out, const int64_t* sizes,
+                               const int32_t* dtypes, double max_norm, float* d_norm, void* d_workspace, int64_t workspace_bytes,
+                               void* stream) {
+    if (!c) return SAGE_E_ARG;
+    const int64_t need = sage_clip_grad_norm_workspace(c, n_tensors, sizes);
+    if (need < 0) return (int)need;
+    if (!d_norm) return sage_ctx_fail(c, SAGE_E_ARG, "d_norm is null");
+    if (!(max_norm >= 0.0) || std::isinf(max_norm)) return sage_ctx_fail(c, SAGE_E_ARG, "max_norm must be finite and not negative");
+    if (n_tensors && (!d_grads || !d_out || !dtypes)) return sage_ctx_fail(c, SAGE_E_ARG, "need the tensors' addresses and types");
+    int rc;
+    if ((rc = check_workspace(c, d_workspace, workspace_bytes, need))) return rc;
+    try {
+        std::vector<std::pair<uintptr_t, int64_t>> written;      // address, bytes
+        written.reserve((size_t)n_tensors);
+        for (int64_t i = 0; i < n_tensors; ++i) {
+            if (dtypes[i] != SAGE_F32 && dtypes[i] != SAGE_BF16) return sage_ctx_fail(c, SAGE_E_ARG, "a tensor's type must be SAGE_F32 or SAGE_BF16");
+            if (sizes[i] == 0) continue;
+            const int w = dtypes[i] == SAGE_BF16 ? 2 : 4;
+            if (!d_grads[i] || !d_out[i]) return sage_ctx_fail(c, SAGE_E_ARG, "a tensor's address is null");
+            if ((uintptr_t)d_grads[i] % w || (uintptr_t)d_out[i] % w) return sage_ctx_fail(c, SAGE_E_ARG, "a tensor is not aligned to its elements");
+            written.emplace_back((uintptr_t)d_out[i], sizes[i] * w);
+        }
+        std::sort(written.begin(), written.end());
+        for (size_t i = 1; i < written.size(); ++i)
+            if (written[i - 1].first + (uintptr_t)written[i - 1].second > written[i].first)
+                return sage_ctx_fail(c, SAGE_E_ARG, "two of the written tensors overlap");
+        for (int64_t i = 0; i < n_tensors; ++i) {                // a gradient may be written in place, and no other way over one
+            if (sizes[i] == 0) continue;
+            const uintptr_t lo = (uintptr_t)d_grads[i], hi = lo + (uintptr_t)sizes[i] * (dtypes[i] == SAGE_BF16 ? 2 : 4);
+            auto it = std::lower_bound(written.begin(), written.end(), std::make_pair(lo, (int64_t)0));
+            if (it != written.begin() && std::prev(it)->first + (uintptr_t)std::prev(it)->second > lo) --it;
+            for (; it != written.end() && it->first < hi; ++it)
+                if (it->first + (uintptr_t)it->second > lo && !((uintptr_t)d_out[i] == lo && it->first == lo))
+                    return sage_ctx_fail(c, SAGE_E_ARG, "a written tensor overlaps a gradient other than its own");
+        }
+    } catch (...) {
+        return sage_ctx_fail(c, SAGE_E_HIP, "out of host memory");
+    }
+    OnDevice dev(sage_ctx_device(c));
+    if (!dev.ok) return sage_ctx_fail(c, SAGE_E_HIP, "the context's device cannot be made current");
+    const hipStream_t st = (hipStream_t)stream;
+    double* part = (double*)d_workspace;
+    float* factor = (float*)((char*)d_workspace + need - VS_ALIGN);
+    ClipTable t;
+    uint32_t total = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        uint32_t block0 = 0;
+        int64_t i = 0;
+        while (i < n_tensors) {
+            t.n = 0; t.block0 = block0; t.first[0] = 0;
+            for (; i < n_tensors && t.n < CLIP_TENSORS; ++i) {
+                if (sizes[i] == 0) continue;
+                t.in[t.n] = d_grads[i]; t.out[t.n] = d_out[i];
+                t.size[t.n] = dtypes[i] == SAGE_BF16 ? -sizes[i] : sizes[i];
+                t.first[t.n + 1] = t.first[t.n] + cdiv(sizes[i], CLIP_BLOCK);
+                ++t.n;
+            }
+            const uint32_t blocks = t.first[t.n];
+            if (!blocks) continue;
+            if (pass == 0) k_clip_squares<<<blocks, 256, 0, st>>>(t, part);
+            else k_clip_scale<<<blocks, 256, 0, st>>>(t, factor);
+            block0 += blocks;
+        }
+        if (pass == 0) {
+            total = block0;
+            k_clip_norm<<<1, 1024, 0, st>>>(part, total, max_norm, d_norm, factor);
+        }
+    }
+    return launched(c, "sage_clip_grad_norm_device");
+}
+
+}  // extern "C"
