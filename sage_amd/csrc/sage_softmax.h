@@ -28,7 +28,7 @@ typedef float vs_f8 __attribute__((ext_vector_type(8)));
 #define VS_LOG2E 1.4426950408889634f
 #define VS_LN2 0.6931471805599453f
 #define VS_CHUNK 64            // ids per stored maximum (the unit in which alternatives are looked for)
-#define VS_ROWS 32             // streaming rows per step
+#define VS_BLOCK 256           // ids are dealt out in blocks of this many
 #define VS_NOTHING (-1.0e30f)  // reference of a row that has seen no finite logit yet; a bias this low masks its id
 #define VS_SLACK 20.0f         // the running reference lags the maximum by at most this (in powers of two)
 #define VS_TMIN (-200.0f)      // 2^-200 is 0 in float32: what a logit of -inf is raised to, so that 0 * log p is 0
@@ -44,22 +44,22 @@ __device__ __forceinline__ float vs_load(const VsSrc& s, int64_t row, int d) {
     return s.is_bf16 ? __uint_as_float((uint32_t)((const uint16_t*)s.p)[row * s.ld + d] << 16) : ((const float*)s.p)[row * s.ld + d];
 }
 
-// max(a, b) that keeps a NaN (fmaxf would turn a NaN logit into a masked one)
-__device__ __forceinline__ float vs_at_least(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+// max(a, b) that keeps a NaN (fmaxf would turn a NaN logit into a masked one, and takes an instruction more to do it)
+__device__ __forceinline__ float vs_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 __device__ __forceinline__ vs_f4 vs_mfma(vs_bf8 a, vs_bf8 b, vs_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// a . b summed into c, both in PL parts (largest first); small products first
-template <int PL>
-__device__ __forceinline__ vs_f4 vs_mfma_parts(const vs_bf8* a, const vs_bf8* b, vs_f4 c) {
-    if constexpr (PL == 3) {
-        c = vs_mfma(a[1], b[1], c);
-        c = vs_mfma(a[2], b[0], c);
-        c = vs_mfma(a[0], b[2], c);
-        c = vs_mfma(a[1], b[0], c);
-        c = vs_mfma(a[0], b[1], c);
-    }
-    return vs_mfma(a[0], b[0], c);
+// c[r][t] += a[r] . b[t] for R x TB independent accumulators, both operands in PL parts (largest first): the parts are the
+// outer loop, small products first, so that an accumulator is not needed again right after it was written.
+template <int PL, int R, int TB, class B>
+__device__ __forceinline__ void vs_mfma_parts(const vs_bf8 (&a)[R][PL], const B& b, vs_f4 (&c)[R][TB]) {
+    constexpr int pa[6] = {1, 2, 0, 1, 0, 0}, pb[6] = {1, 0, 2, 0, 1, 0};
+#pragma unroll
+    for (int q = PL == 3 ? 0 : 5; q < 6; ++q)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < TB; ++t) c[r][t] = vs_mfma(a[r][pa[q]], b(t, pb[q]), c[r][t]);
 }
 
 // v as the sum of PL bf16 (each rounding to nearest; exact for PL = 3, within 2^-9 |v| for PL = 1)
@@ -134,104 +134,232 @@ struct VsFwd {
     int32_t vocab;
     int32_t n_tiles;           // token tiles of 16 TB rows
     int32_t splits;            // ranges of the vocabulary
+    int32_t blocks;            // blocks of VS_BLOCK ids
     int32_t chunks;            // chunks of VS_CHUNK ids
     int64_t n_pad;             // row length of the partials
     float4* part;              // [splits][n_pad]: reference (in powers of two), sum of exps, sum of exp * exponent
     float* chunk_max;          // [n_pad][chunks] or null
 };
 
-// One unit of work is a wave: a tile of 16 TB tokens against one range of the vocabulary.  A softmax in one pass: sums are
-// kept relative to a reference that follows the running maximum in steps of at least 2^VS_SLACK (so that it is moved a few
-// times per row and the common step has no rescaling), the entropy's sum relative to the same reference.
+// Sums of a row, relative to 2^ref: s of exp, e of exp * exponent (the entropy's).  A softmax in one pass: the reference
+// follows the running maximum in steps of at least 2^VS_SLACK, so it moves a few times per row and the common step has no
+// rescaling.  Eight terms are summed first, then up to VS_BLOCK / 4 of those, then these: sums of 262,144 terms keep
+// their last bits.
+struct VsStat {
+    float ref, s, e, S, E;
+    __device__ __forceinline__ void clear() { ref = VS_NOTHING; s = e = S = E = 0.0f; }
+    __device__ __forceinline__ void flush() { S += s; E += e; s = e = 0.0f; }
+    __device__ __forceinline__ void move(float now) {      // (a sum that vanishes takes its exponents with it: 0 * inf)
+        const float d = ref - now, f = exp2f(d);
+        e = f == 0.0f ? 0.0f : f * fmaf(d, s, e);
+        E = f == 0.0f ? 0.0f : f * fmaf(d, S, E);
+        s *= f; S *= f;
+        ref = now;
+    }
+    __device__ __forceinline__ void join(float r2, float s2, float e2) {     // S and E with another range's
+        const float now = fmaxf(ref, r2);
+        if (now > ref) move(now);
+        const float d = r2 - now, f = exp2f(d);
+        E += f == 0.0f ? 0.0f : f * fmaf(d, s2, e2);
+        S += s2 != s2 ? s2 : f * s2;
+    }
+};
+
+// 32 streaming rows against the stationary ones: s[rb][t] += w . x
 template <int KS, int PL, int TB>
-__global__ __launch_bounds__(256) void k_vs_forward(VsFwd a) {
-    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-    const int unit = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (unit >= a.n_tiles * a.splits) return;
-    const int tile = unit % a.n_tiles, split = unit / a.n_tiles;
-    const int c0 = (int)((int64_t)a.chunks * split / a.splits), c1 = (int)((int64_t)a.chunks * (split + 1) / a.splits);
-    vs_bf8 x[TB][KS][PL];
+__device__ __forceinline__ void vs_product(const uint4* w, const vs_bf8 (&x)[TB][KS][PL], vs_f4 (&s)[2][TB]) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+        vs_bf8 wf[2][PL];
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+            for (int p = 0; p < PL; ++p) wf[rb][p] = *(const vs_bf8*)&w[((rb * KS + k) * PL + p) * 64];
+        vs_mfma_parts<PL, 2, TB>(wf, [&](int t, int p) { return x[t][k][p]; }, s);
+    }
+}
+
+template <int KS, int PL, int TB>
+__device__ __forceinline__ void vs_stationary(const uint4* S, int64_t tile, int lane, vs_bf8 (&x)[TB][KS][PL]) {
 #pragma unroll
     for (int t = 0; t < TB; ++t)
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int p = 0; p < PL; ++p)
-                x[t][k][p] = *(const vs_bf8*)&a.xS[((((int64_t)tile * TB + t) * KS + k) * PL + p) * 64 + lane];
-    float ref[TB], sum[TB], ent[TB], top[TB];
+            for (int p = 0; p < PL; ++p) x[t][k][p] = *(const vs_bf8*)&S[(((tile * TB + t) * KS + k) * PL + p) * 64 + lane];
+}
+
+template <int TB>
+struct VsRowsOfTile {
+    VsStat st[TB];
+    float top[TB], keep[TB];
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int t = 0; t < TB; ++t) { ref[t] = VS_NOTHING; sum[t] = 0.0f; ent[t] = 0.0f; top[t] = -INFINITY; }
-    for (int c = c0; c < c1; ++c) {
-#pragma unroll 1
-        for (int h = 0; h < VS_CHUNK / VS_ROWS; ++h) {
-            const int row0 = c * VS_CHUNK + h * VS_ROWS;
-            const bool biased = a.has_bias || row0 + VS_ROWS > a.vocab;      // the same in the whole grid
-            vs_f4 s[2][TB];
+        for (int t = 0; t < TB; ++t) { st[t].clear(); top[t] = -INFINITY; keep[t] = -INFINITY; }
+    }
+    // the logits of 32 ids; MASKED: some may be -inf
+    template <bool MASKED>
+    __device__ __forceinline__ void add(const vs_f4 (&s)[2][TB]) {
 #pragma unroll
-            for (int rb = 0; rb < 2; ++rb) {
-                vs_f4 b = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (biased) b = *(const vs_f4*)&a.bias[row0 + rb * 16 + quad * 4];
+        for (int t = 0; t < TB; ++t) {
+            float mx = vs_max(vs_max(vs_max(s[0][t][0], s[0][t][1]), s[0][t][2]), vs_max(vs_max(s[0][t][3], s[1][t][0]), s[1][t][1]));
+            mx = vs_max(vs_max(mx, s[1][t][2]), s[1][t][3]);
+            top[t] = vs_max(top[t], mx);
+            mx *= VS_LOG2E;
+            const bool up = mx > st[t].ref + VS_SLACK;
+            if (__any(up)) st[t].move(up ? mx : st[t].ref);
+            float ls, le;
 #pragma unroll
-                for (int t = 0; t < TB; ++t) s[rb][t] = b;
+            for (int j = 0; j < 8; ++j) {
+                float e = fmaf(s[j >> 2][t][j & 3], VS_LOG2E, -st[t].ref);
+                if (MASKED) e = vs_max(e, VS_TMIN);
+                const float p = __builtin_amdgcn_exp2f(e);
+                ls = j ? ls + p : p;
+                le = j ? fmaf(p, e, le) : p * e;
             }
-            const uint4* w = a.wS + (int64_t)row0 / 16 * KS * PL * 64 + lane;
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-                for (int rb = 0; rb < 2; ++rb) {
-                    vs_bf8 wf[PL];
-#pragma unroll
-                    for (int p = 0; p < PL; ++p) wf[p] = *(const vs_bf8*)&w[((rb * KS + k) * PL + p) * 64];
-#pragma unroll
-                    for (int t = 0; t < TB; ++t) s[rb][t] = vs_mfma_parts<PL>(wf, x[t][k], s[rb][t]);
-                }
-#pragma unroll
-            for (int t = 0; t < TB; ++t) {
-                float mx = fmaxf(fmaxf(fmaxf(s[0][t][0], s[0][t][1]), fmaxf(s[0][t][2], s[0][t][3])),
-                                 fmaxf(fmaxf(s[1][t][0], s[1][t][1]), fmaxf(s[1][t][2], s[1][t][3])));
-                top[t] = fmaxf(top[t], mx);
-                mx *= VS_LOG2E;
-                if (__any(mx > ref[t] + VS_SLACK)) {
-                    const float now = mx > ref[t] + VS_SLACK ? mx : ref[t];
-                    const float f = exp2f(ref[t] - now);
-                    ent[t] = f * fmaf(ref[t] - now, sum[t], ent[t]);
-                    sum[t] *= f;
-                    ref[t] = now;
-                }
-#pragma unroll
-                for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float e = fmaf(s[rb][t][i], VS_LOG2E, -ref[t]);
-                        if (biased) e = vs_at_least(e, VS_TMIN);
-                        const float p = __builtin_amdgcn_exp2f(e);
-                        sum[t] += p;
-                        ent[t] = fmaf(p, e, ent[t]);
-                    }
-            }
+            st[t].s += ls;
+            st[t].e += le;
         }
+    }
+    // chunk c is done; the largest logits of four chunks are stored together, sixteen bytes a row
+    __device__ __forceinline__ void chunk(const VsFwd& a, int64_t tile, int c, int lane, bool live) {
         if (a.chunk_max) {
 #pragma unroll
             for (int t = 0; t < TB; ++t) {
-                float m = fmaxf(top[t], __shfl_xor(top[t], 16));
-                m = fmaxf(m, __shfl_xor(m, 32));
-                if (quad == 0) a.chunk_max[((int64_t)tile * TB * 16 + t * 16 + col) * a.chunks + c] = m;
+                float m = vs_max(top[t], __shfl_xor(top[t], 16));
+                m = vs_max(m, __shfl_xor(m, 32));
+                if ((c & 3) == (lane >> 4)) keep[t] = m;
                 top[t] = -INFINITY;
+                if ((c & 3) == 3 && live) a.chunk_max[((tile * TB + t) * 16 + (lane & 15)) * a.chunks + (c & ~3) + (lane >> 4)] = keep[t];
             }
         }
     }
+    __device__ __forceinline__ void flush() {
 #pragma unroll
-    for (int t = 0; t < TB; ++t) {
-#pragma unroll
-        for (int o = 16; o <= 32; o <<= 1) {
-            const float r2 = __shfl_xor(ref[t], o), s2 = __shfl_xor(sum[t], o), e2 = __shfl_xor(ent[t], o);
-            const float now = fmaxf(ref[t], r2), f1 = exp2f(ref[t] - now), f2 = exp2f(r2 - now);
-            ent[t] = f1 * fmaf(ref[t] - now, sum[t], ent[t]) + f2 * fmaf(r2 - now, s2, e2);
-            sum[t] = f1 * sum[t] + f2 * s2;
-            ref[t] = now;
-        }
-        if (quad == 0) a.part[(int64_t)split * a.n_pad + ((int64_t)tile * TB + t) * 16 + col] = make_float4(ref[t], sum[t], ent[t], 0.0f);
+        for (int t = 0; t < TB; ++t) st[t].flush();
     }
+    __device__ __forceinline__ void store(const VsFwd& a, int64_t tile, int split, int lane) {
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
+            st[t].flush();
+#pragma unroll
+            for (int o = 16; o <= 32; o <<= 1) {
+                const float r2 = __shfl_xor(st[t].ref, o), s2 = __shfl_xor(st[t].S, o), e2 = __shfl_xor(st[t].E, o);
+                st[t].join(r2, s2, e2);
+            }
+            if (lane < 16) a.part[(int64_t)split * a.n_pad + (tile * TB + t) * 16 + lane] = make_float4(st[t].ref, st[t].S, st[t].E, 0.0f);
+        }
+    }
+};
+
+template <int TB>
+__device__ __forceinline__ void vs_bias_init(const float* bias, int lane, vs_f4 (&s)[2][TB]) {
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {
+        const vs_f4 b = *(const vs_f4*)&bias[rb * 16 + (lane >> 4) * 4];
+#pragma unroll
+        for (int t = 0; t < TB; ++t) s[rb][t] = b;
+    }
+}
+
+// Few tokens: a wave is a tile of 16 TB tokens against one range of the vocabulary and reads its fragments itself.
+template <int KS, int PL, int TB>
+__global__ __launch_bounds__(256, 2) void k_vs_forward(VsFwd a) {
+    const int lane = threadIdx.x & 63;
+    const int unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (unit >= a.n_tiles * a.splits) return;
+    const int tile = unit % a.n_tiles, split = unit / a.n_tiles;
+    const int b0 = (int)((int64_t)a.blocks * split / a.splits), b1 = (int)((int64_t)a.blocks * (split + 1) / a.splits);
+    vs_bf8 x[TB][KS][PL];
+    vs_stationary<KS, PL, TB>(a.xS, tile, lane, x);
+    VsRowsOfTile<TB> rows;
+    rows.clear();
+    for (int b = b0; b < b1; ++b) {
+        for (int c = b * (VS_BLOCK / VS_CHUNK); c < (b + 1) * (VS_BLOCK / VS_CHUNK); ++c) {
+#pragma unroll 1
+            for (int row0 = c * VS_CHUNK; row0 < (c + 1) * VS_CHUNK; row0 += 32) {
+                vs_f4 s[2][TB];
+                vs_bias_init<TB>(a.bias + row0, lane, s);
+                vs_product<KS, PL, TB>(a.wS + (int64_t)row0 / 16 * KS * PL * 64 + lane, x, s);
+                if (a.has_bias || row0 + 32 > a.vocab) rows.template add<true>(s);      // the same in the whole grid
+                else rows.template add<false>(s);
+            }
+            rows.chunk(a, tile, c, lane, true);
+        }
+        rows.flush();
+    }
+    rows.store(a, tile, split, lane);
+}
+
+// Many tokens: four waves, a tile each, share the streaming rows through LDS.  SR rows at a time are copied straight into
+// LDS (they are packed in the order of the copy) while the SR before them are worked on: one barrier a step.
+typedef const __attribute__((address_space(1))) void* vs_global_ptr;
+typedef __attribute__((address_space(3))) void* vs_lds_ptr;
+template <int N>               // 16-byte pieces, a multiple of 256
+__device__ __forceinline__ void vs_stage(const uint4* from, uint4* to) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < N; i += 256)
+        __builtin_amdgcn_global_load_lds((vs_global_ptr)(from + i + wave * 64 + lane), (vs_lds_ptr)(to + i + wave * 64), 16, 0, 0);
+}
+
+// This wave's copies into LDS have arrived: vmcnt 0, the other counters as they are.
+__device__ __forceinline__ void vs_copies_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
+// A stage: SR rows of fragments and their SR biases.  `to` and `from` are different stages, and the compiler has to know it
+// (__restrict__ through an inlined function): else it waits for the copy under way before each read of LDS.
+template <int KS, int PL, int SR>
+struct VsStage {
+    static constexpr int N = SR * KS * PL * 4, SIZE = N + SR / 4;
+    static __device__ __forceinline__ void fetch(const uint4* w, const float* bias, uint4* to) {
+        vs_stage<N>(w, to);
+        if (threadIdx.x < SR)
+            __builtin_amdgcn_global_load_lds((vs_global_ptr)(bias + threadIdx.x), (vs_lds_ptr)(to + N + (threadIdx.x & ~63) / 4), 4, 0, 0);
+    }
+    template <int TB>
+    static __device__ __forceinline__ void step(const VsFwd& a, int base, bool more, const uint4* __restrict__ next, const float* __restrict__ next_bias,
+                                                uint4* __restrict__ to, const uint4* __restrict__ from, const vs_bf8 (&x)[TB][KS][PL], VsRowsOfTile<TB>& rows, int64_t tile, bool live) {
+        const int lane = threadIdx.x & 63;
+        vs_copies_done();                  // (a barrier alone does not wait for them)
+        __syncthreads();                   // `from` has arrived, and nobody reads `to` any more
+        if (more) fetch(next, next_bias, to);
+#pragma unroll 1
+        for (int r = 0; r < SR; r += 32) {
+            const int row0 = base + r;
+            vs_f4 s[2][TB];
+            vs_bias_init<TB>((const float*)(from + N) + r, lane, s);
+            vs_product<KS, PL, TB>(from + r * KS * PL * 4 + lane, x, s);
+            if (a.has_bias || row0 + 32 > a.vocab) rows.template add<true>(s);
+            else rows.template add<false>(s);
+            if ((row0 & (VS_CHUNK - 1)) == VS_CHUNK - 32) rows.chunk(a, tile, row0 / VS_CHUNK, lane, live);
+        }
+        if (((base + SR) & (VS_BLOCK - 1)) == 0) rows.flush();
+    }
+};
+
+template <int KS, int PL, int TB, int SR>
+__global__ __launch_bounds__(256, 2) void k_vs_forward_staged(VsFwd a) {
+    using Stage = VsStage<KS, PL, SR>;
+    __shared__ uint4 buf0[Stage::SIZE], buf1[Stage::SIZE];
+    const int lane = threadIdx.x & 63;
+    const int split = blockIdx.x % a.splits;
+    const int tile = (blockIdx.x / a.splits) * 4 + (threadIdx.x >> 6);
+    const bool live = tile < a.n_tiles;
+    const int row_begin = (int)((int64_t)a.blocks * split / a.splits) * VS_BLOCK, row_end = (int)((int64_t)a.blocks * (split + 1) / a.splits) * VS_BLOCK;
+    vs_bf8 x[TB][KS][PL];
+    vs_stationary<KS, PL, TB>(a.xS, live ? tile : 0, lane, x);
+    VsRowsOfTile<TB> rows;
+    rows.clear();
+    const uint4* w = a.wS + (int64_t)row_begin * KS * PL * 4;
+    const float* bias = a.bias + row_begin;
+    Stage::fetch(w, bias, buf0);
+    for (int base = row_begin; base < row_end; base += 2 * SR) {
+        w += SR * KS * PL * 4; bias += SR;
+        Stage::template step<TB>(a, base, true, w, bias, buf1, buf0, x, rows, tile, live);
+        w += SR * KS * PL * 4; bias += SR;
+        Stage::template step<TB>(a, base + SR, base + 2 * SR < row_end, w, bias, buf0, buf1, x, rows, tile, live);
+    }
+    if (live) rows.store(a, tile, split, lane);
 }
 
 // Joins the ranges of a row and takes the given token's log probability: a wave per row.  The token's own logit is summed
@@ -249,21 +377,17 @@ __global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= a.n) return;
-    float r = VS_NOTHING, s = 0.0f, e = 0.0f;
+    VsStat st;
+    st.clear();
     for (int i = lane; i < a.splits; i += 64) {
         const float4 q = a.part[(int64_t)i * a.n_pad + row];
-        const float now = fmaxf(r, q.x), f1 = exp2f(r - now), f2 = exp2f(q.x - now);
-        e = f1 * fmaf(r - now, s, e) + f2 * fmaf(q.x - now, q.y, q.z);
-        s = f1 * s + f2 * q.y;
-        r = now;
+        st.join(q.x, q.y, q.z);
     }
     for (int o = 1; o < 64; o <<= 1) {
-        const float r2 = __shfl_xor(r, o), s2 = __shfl_xor(s, o), e2 = __shfl_xor(e, o);
-        const float now = fmaxf(r, r2), f1 = exp2f(r - now), f2 = exp2f(r2 - now);
-        e = f1 * fmaf(r - now, s, e) + f2 * fmaf(r2 - now, s2, e2);
-        s = f1 * s + f2 * s2;
-        r = now;
+        const float r2 = __shfl_xor(st.ref, o), s2 = __shfl_xor(st.S, o), e2 = __shfl_xor(st.E, o);
+        st.join(r2, s2, e2);
     }
+    const float r = st.ref, s = st.S, e = st.E;
     const bool empty = s == 0.0f;                   // nothing but -inf
     const double lse = empty ? -INFINITY : ((double)r + (double)log2f(s)) * 0.6931471805599453;
     const int64_t t = a.targets ? a.targets[row] : -1;
@@ -324,6 +448,10 @@ __global__ __launch_bounds__(256) void k_vs_top(VsTop a) {
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63;
     const float* cm = a.chunk_max + row * a.chunks;
+    if (a.lse[row] != a.lse[row]) {         // no order among the logits
+        if (tid < a.k) { a.ids[row * a.k + tid] = -1; a.logprobs[row * a.k + tid] = NAN; }
+        return;
+    }
     float l1 = 0.0f;
     for (int d = tid; d < a.x.dim; d += 256) { const float v = vs_load(a.x, row, d); xs[d] = v; l1 += fabsf(v); }
     for (int o = 1; o < 64; o <<= 1) l1 += __shfl_xor(l1, o);
@@ -499,13 +627,7 @@ __global__ __launch_bounds__(256) void k_vs_backward(VsBwd a) {
     const int g0 = (int)((int64_t)a.groups * split / a.splits), g1 = (int)((int64_t)a.groups * (split + 1) / a.splits);
     const int64_t stay0 = (int64_t)tile * TB * 16;
     vs_bf8 y[TB][KS][PL];
-#pragma unroll
-    for (int t = 0; t < TB; ++t)
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int p = 0; p < PL; ++p)
-                y[t][k][p] = *(const vs_bf8*)&a.stayS[((((int64_t)tile * TB + t) * KS + k) * PL + p) * 64 + lane];
+    vs_stationary<KS, PL, TB>(a.stayS, tile, lane, y);
     float lse2[TB], A[TB], B[TB], b0[TB], db[TB];
 #pragma unroll
     for (int t = 0; t < TB; ++t) {
@@ -532,17 +654,7 @@ __global__ __launch_bounds__(256) void k_vs_backward(VsBwd a) {
                 else s[rb][t] = b;
             }
         }
-        const uint4* f = a.flowS + (int64_t)g * 2 * KS * PL * 64 + lane;
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int rb = 0; rb < 2; ++rb) {
-                vs_bf8 wf[PL];
-#pragma unroll
-                for (int p = 0; p < PL; ++p) wf[p] = *(const vs_bf8*)&f[((rb * KS + k) * PL + p) * 64];
-#pragma unroll
-                for (int t = 0; t < TB; ++t) s[rb][t] = vs_mfma_parts<PL>(wf, y[t][k], s[rb][t]);
-            }
+        vs_product<KS, PL, TB>(a.flowS + (int64_t)g * 2 * KS * PL * 64 + lane, y, s);
         vs_f4 L[2], rA[2], rB[2];
         bool hit = false;
         if constexpr (OF_IDS) {
@@ -564,7 +676,7 @@ __global__ __launch_bounds__(256) void k_vs_backward(VsBwd a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float e = fmaf(s[rb][t][i], VS_LOG2E, OF_IDS ? -L[rb][i] : -lse2[t]);
-                    if (biased) e = vs_at_least(e, VS_TMIN);
+                    if (biased) e = vs_max(e, VS_TMIN);
                     float q = __builtin_amdgcn_exp2f(e);
                     if constexpr (OF_IDS) q *= a.has_entropy ? fmaf(rB[rb][i], e, rA[rb][i]) : rA[rb][i];
                     else if (a.has_entropy) q *= fmaf(B[t], e, A[t]);
@@ -587,12 +699,13 @@ __global__ __launch_bounds__(256) void k_vs_backward(VsBwd a) {
         }
         const uint4* ft = a.flowT + (int64_t)g * 2 * KS * PL * 64 + lane;
 #pragma unroll
-        for (int d = 0; d < 2 * KS; ++d) {
-            vs_bf8 wf[PL];
+        for (int d = 0; d < 2 * KS; d += 2) {
+            vs_bf8 wf[2][PL];
 #pragma unroll
-            for (int p = 0; p < PL; ++p) wf[p] = *(const vs_bf8*)&ft[(d * PL + p) * 64];
+            for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int t = 0; t < TB; ++t) acc[d][t] = vs_mfma_parts<PL>(wf, P[t], acc[d][t]);
+                for (int p = 0; p < PL; ++p) wf[r][p] = *(const vs_bf8*)&ft[((d + r) * PL + p) * 64];
+            vs_mfma_parts<PL, 2, TB>(wf, [&](int t, int p) { return P[t][p]; }, *(vs_f4(*)[2][TB]) & acc[d]);
         }
         if (OF_IDS && PL == 1 && hit) {
 #pragma unroll

@@ -13,7 +13,7 @@
 
 namespace {
 
-constexpr int64_t VS_PAD = 128;                 // rows and ids are padded to this
+constexpr int64_t VS_PAD = 128;                 // rows are padded to this (ids to VS_BLOCK)
 constexpr int64_t VS_ROWS_MAX = 16384;          // tokens of one pass of the forward kernels
 constexpr size_t VS_ALIGN = 256;
 
@@ -61,6 +61,9 @@ int vs_steps(int dim) {
 constexpr int vs_fwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 4 ? 4 : 2) : (ks <= 4 ? 2 : 1); }
 constexpr int vs_bwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 2 ? 4 : ks <= 8 ? 2 : 1) : (ks <= 4 ? 2 : 1); }
 
+// streaming rows of a stage of the forward kernel: two stages of at most 40 KiB (0: too wide, the waves read for themselves)
+constexpr int vs_stage_rows(int ks, int pl) { return ks * pl <= 4 ? 128 : ks * pl <= 8 ? 64 : ks * pl <= 20 ? 32 : 0; }
+
 #define VS_BY_WIDTH(ks, pl, F)                                                        \
     do {                                                                              \
         if ((pl) == 1) {                                                              \
@@ -105,6 +108,7 @@ int vs_splits(const Shape& s, int64_t tiles, int64_t flow, int64_t most) {
 struct FwdPlan {
     int64_t rows, n_pad, tiles, chunks;
     int splits;
+    bool staged;
     uint4 *xS, *wS;
     float *bias, *group_max, *chunk_max;
     float4* part;
@@ -118,7 +122,9 @@ FwdPlan plan_fwd(const Shape& s, void* ws) {
     p.n_pad = up(p.rows, VS_PAD);
     p.tiles = cdiv(p.rows, br);
     p.chunks = s.vp / VS_CHUNK;
-    p.splits = vs_splits(s, p.tiles, p.chunks, 1 << 20);
+    p.staged = p.tiles >= 4 && vs_stage_rows(s.ks, s.pl) > 0;
+    const int64_t blocks = s.vp / VS_BLOCK;
+    p.splits = p.staged ? (int)std::min<int64_t>(blocks, cdiv((int64_t)s.cus * 4, cdiv(p.tiles, 4))) : vs_splits(s, p.tiles, blocks, 1 << 20);
     const int64_t frag = (int64_t)s.ks * s.pl * 64;          // uint4 of a 16-row block
     p.wS = a.take<uint4>(s.vp / 16 * frag);
     p.xS = a.take<uint4>(p.n_pad / 16 * frag);
@@ -172,7 +178,7 @@ int vs_shape(sage_ctx* c, int32_t dtype, int64_t n, int64_t vocab, int32_t dim, 
     if (dim > 512) return sage_ctx_fail(c, SAGE_E_LIMIT, "embedding dimension above 512 is not supported");
     if (vocab > (1 << 20)) return sage_ctx_fail(c, SAGE_E_LIMIT, "a vocabulary of more than 2^20 ids is not supported");
     if (n > (1 << 22)) return sage_ctx_fail(c, SAGE_E_LIMIT, "more than 2^22 tokens in one call are not supported");
-    *s = Shape{n, vocab, up(vocab, VS_PAD), dim, vs_steps(dim), dtype == SAGE_BF16 ? 1 : 3, k, sage_ctx_compute_units(c)};
+    *s = Shape{n, vocab, up(vocab, VS_BLOCK), dim, vs_steps(dim), dtype == SAGE_BF16 ? 1 : 3, k, sage_ctx_compute_units(c)};
     return SAGE_OK;
 }
 
@@ -245,10 +251,13 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
         const int64_t rows = std::min(p.rows, n - r0);
         const VsSrc xr = rows_from(x, r0, rows);
         pack(s, xr, p.n_pad, p.xS, nullptr, nullptr, st);
-        const VsFwd f{p.xS, p.wS, p.bias, d_bias != nullptr, (int32_t)vocab, (int32_t)p.tiles, p.splits, (int32_t)p.chunks, p.n_pad, p.part,
+        const VsFwd f{p.xS, p.wS, p.bias, d_bias != nullptr, (int32_t)vocab, (int32_t)p.tiles, p.splits, (int32_t)(s.vp / VS_BLOCK), (int32_t)p.chunks, p.n_pad, p.part,
                       alternatives ? p.chunk_max : nullptr};
-        const uint32_t grid = cdiv(p.tiles * p.splits, 4);
-#define VS_F(KS, PL) k_vs_forward<KS, PL, vs_fwd_blocks(KS, PL)><<<grid, 256, 0, st>>>(f)
+        const uint32_t grid = cdiv(p.tiles * p.splits, 4), grid_staged = cdiv(p.tiles, 4) * p.splits;
+#define VS_F(KS, PL)                                                                                                          \
+    if constexpr (vs_stage_rows(KS, PL) > 0)                                                                                  \
+        if (p.staged) { k_vs_forward_staged<KS, PL, vs_fwd_blocks(KS, PL), vs_stage_rows(KS, PL)><<<grid_staged, 256, 0, st>>>(f); break; } \
+    k_vs_forward<KS, PL, vs_fwd_blocks(KS, PL)><<<grid, 256, 0, st>>>(f)
         VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
         const VsJoin j{xr, w, p.bias, d_targets ? d_targets + r0 : nullptr, p.part, (int32_t)rows, p.splits, p.n_pad,
