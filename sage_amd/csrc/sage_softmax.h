@@ -238,7 +238,7 @@ struct VsRowsOfTile {
 #pragma unroll
         for (int t = 0; t < TB; ++t) st[t].flush();
     }
-    __device__ __forceinline__ void store(const VsFwd& a, int64_t tile, int split, int lane) {
+    __device__ __forceinline__ void join_lanes() {
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
             st[t].flush();
@@ -247,6 +247,12 @@ struct VsRowsOfTile {
                 const float r2 = __shfl_xor(st[t].ref, o), s2 = __shfl_xor(st[t].S, o), e2 = __shfl_xor(st[t].E, o);
                 st[t].join(r2, s2, e2);
             }
+        }
+    }
+    __device__ __forceinline__ void store(const VsFwd& a, int64_t tile, int split, int lane) {
+        join_lanes();
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
             if (lane < 16) a.part[(int64_t)split * a.n_pad + (tile * TB + t) * 16 + lane] = make_float4(st[t].ref, st[t].S, st[t].E, 0.0f);
         }
     }
@@ -262,7 +268,8 @@ __device__ __forceinline__ void vs_bias_init(const float* bias, int lane, vs_f4 
     }
 }
 
-// Few tokens: a wave is a tile of 16 TB tokens against one range of the vocabulary and reads its fragments itself.
+// The widest float32 rows (a stage would not fit LDS twice): a wave is a tile of 16 TB tokens against one range of the
+// vocabulary and reads its fragments itself.
 template <int KS, int PL, int TB>
 __global__ __launch_bounds__(256, 2) void k_vs_forward(VsFwd a) {
     const int lane = threadIdx.x & 63;
@@ -362,143 +369,361 @@ __global__ __launch_bounds__(256, 2) void k_vs_forward_staged(VsFwd a) {
     if (live) rows.store(a, tile, split, lane);
 }
 
-// Joins the ranges of a row and takes the given token's log probability: a wave per row.  The token's own logit is summed
-// in float64 (its rounding would otherwise show where the probability is near 1).
+// The bias of one id: 0 where the caller gives none, -inf where it masks the id.
+__device__ __forceinline__ float vs_bias_of(const float* bias, int64_t v) {
+    const float b = bias ? bias[v] : 0.0f;
+    return b <= VS_NOTHING ? -INFINITY : b;
+}
+
+// sum over the 16 lanes of a DPP row, in every lane of it
+__device__ __forceinline__ float vs_row_sum(float v) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, true));    // quad_perm [1,0,3,2]
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, true));    // quad_perm [2,3,0,1]
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, true));   // row_half_mirror
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, true));   // row_mirror
+    return v;
+}
+
+// Few tokens: bound by the one reading of the weights, which are taken as they lie (no packing): a lane loads the eight
+// elements of a row that its place in a fragment asks for, at whatever alignment they have.  The last piece of a row that is
+// no whole number of pieces long is taken back from the row's end, with the elements before it weighted 0 in x: no read
+// leaves the row (so there are eight elements at least).  A wave is a tile of 16 TB tokens against one range of the vocabulary; the four of a workgroup join theirs.
+template <int PL> struct VsPiece;
+template <> struct VsPiece<1> {            // of bf16: a fragment as it is
+    vs_bf8 v;
+    __device__ __forceinline__ void load(const VsSrc& s, int64_t row, int at) {
+        struct __attribute__((packed, aligned(2))) Raw { uint32_t v[4]; };
+        v = __builtin_bit_cast(vs_bf8, *(const Raw*)((const uint16_t*)s.p + row * s.ld + at));
+    }
+    __device__ __forceinline__ vs_f8 floats() const { return __builtin_convertvector(v, vs_f8); }
+    __device__ __forceinline__ void parts(vs_bf8 (&out)[1]) const { out[0] = v; }
+    typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+    u16x8 most;                            // running largest size: the bits of a bf16 without its sign are ordered
+    __device__ __forceinline__ void clear() { most = u16x8(0); }
+    __device__ __forceinline__ void measure(const VsPiece& q) { most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x8, q.v) & u16x8(0x7FFF)); }
+    __device__ __forceinline__ float largest() const {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, (unsigned)most[i]);
+        return __uint_as_float(m << 16);
+    }
+};
+template <> struct VsPiece<3> {            // of float32
+    vs_f8 v;
+    __device__ __forceinline__ void load(const VsSrc& s, int64_t row, int at) {
+        struct __attribute__((packed, aligned(4))) Raw { float v[4]; };
+        const Raw r = *(const Raw*)((const float*)s.p + row * s.ld + at), q = *(const Raw*)((const float*)s.p + row * s.ld + at + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[i] = r.v[i]; v[i + 4] = q.v[i]; }
+    }
+    __device__ __forceinline__ vs_f8 floats() const { return v; }
+    __device__ __forceinline__ void parts(vs_bf8 (&out)[3]) const { vs_split<3>(v, out); }
+    __device__ __forceinline__ void clear() { v = vs_f8(0.0f); }
+    __device__ __forceinline__ void measure(const VsPiece& q) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fmaxf(v[i], fabsf(q.v[i]));
+    }
+    __device__ __forceinline__ float largest() const {
+        float m = v[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) m = fmaxf(m, v[i]);
+        return m;
+    }
+};
+
+struct VsRaw {
+    VsSrc x, w;
+    const float* bias;         // as the caller gave it, or null
+    float* group_max;          // [ids / 32] or null
+    VsFwd f;                   // chunks, blocks, n_pad, part, chunk_max; splits: workgroups of a tile
+};
+template <int KS, int PL, int TB>
+__global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(VsRaw a) {
+    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    constexpr int KG = PL == 1 ? (KS < 16 ? KS : 8) : 2;    // 32-element steps whose loads are under way together
+    __shared__ float4 red[4][TB * 16];
+    const int tile = blockIdx.y;
+    int at[KS];
+    vs_bf8 x[TB][KS][PL];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+        const int d = k * 32 + quad * 8;
+        at[k] = min(d, a.w.dim - 8);
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
+            const int row = (tile * TB + t) * 16 + col;
+            VsPiece<PL> q;
+            q.load(a.x, min(row, a.x.rows - 1), at[k]);
+            vs_f8 v = q.floats();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = row < a.x.rows && d < a.w.dim && at[k] + i >= d ? v[i] : 0.0f;
+            vs_split<PL>(v, x[t][k]);
+        }
+    }
+    VsRowsOfTile<TB> rows;
+    rows.clear();
+    const int units = gridDim.x * 4, unit = blockIdx.x * 4 + (threadIdx.x >> 6), quads = a.f.chunks / 4;
+    const int c0 = (int)((int64_t)quads * unit / units) * 4, c1 = (int)((int64_t)quads * (unit + 1) / units) * 4;
+    for (int c = c0; c < c1; ++c) {
+#pragma unroll 1
+        for (int row0 = c * VS_CHUNK; row0 < (c + 1) * VS_CHUNK; row0 += 32) {
+            // (loads first and together; the bias is added last, so that no wait for it stands before the products)
+            VsPiece<PL> raw[2][KG], big;
+            vs_f4 s[2][TB], b[2];
+            big.clear();
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+                for (int t = 0; t < TB; ++t) s[rb][t] = vs_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int g = 0; g < KS; g += KG) {
+#pragma unroll
+                for (int k = 0; k < KG; ++k)
+#pragma unroll
+                    for (int rb = 0; rb < 2; ++rb)
+                        if (g + k < KS) raw[rb][k].load(a.w, min(row0 + rb * 16 + col, a.w.rows - 1), at[g + k]);
+                if (g + KG >= KS && a.bias) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) b[j >> 2][j & 3] = a.bias[min(row0 + (j >> 2) * 16 + quad * 4 + (j & 3), a.w.rows - 1)];
+                }
+#pragma unroll
+                for (int k = 0; k < KG; ++k)
+                    if (g + k < KS) {
+                        vs_bf8 wf[2][PL];
+#pragma unroll
+                        for (int rb = 0; rb < 2; ++rb) {
+                            big.measure(raw[rb][k]);
+                            raw[rb][k].parts(wf[rb]);
+                        }
+                        vs_mfma_parts<PL, 2, TB>(wf, [&](int t, int p) { return x[t][g + k][p]; }, s);
+                    }
+            }
+            if (a.bias || row0 + 32 > a.w.rows) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float q = a.bias ? b[j >> 2][j & 3] : 0.0f;
+                    const bool gone = q <= VS_NOTHING || row0 + (j >> 2) * 16 + quad * 4 + (j & 3) >= a.w.rows;
+#pragma unroll
+                    for (int t = 0; t < TB; ++t) s[j >> 2][t][j & 3] = gone ? -INFINITY : s[j >> 2][t][j & 3] + q;
+                }
+            }
+            if (a.group_max) {
+                float m = big.largest();
+                for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+                if (lane == 0 && tile == 0) a.group_max[row0 / 32] = m;
+            }
+            if (a.bias || row0 + 32 > a.w.rows) rows.template add<true>(s);
+            else rows.template add<false>(s);
+        }
+        rows.chunk(a.f, tile, c, lane, true);
+        if ((c & 3) == 3) rows.flush();
+    }
+    rows.join_lanes();
+#pragma unroll
+    for (int t = 0; t < TB; ++t)
+        if (quad == 0) red[threadIdx.x >> 6][t * 16 + col] = make_float4(rows.st[t].ref, rows.st[t].S, rows.st[t].E, 0.0f);
+    __syncthreads();
+    if (threadIdx.x < TB * 16) {
+        VsStat st;
+        st.clear();
+        for (int i = 0; i < 4; ++i) { const float4 q = red[i][threadIdx.x]; st.join(q.x, q.y, q.z); }
+        a.f.part[(int64_t)blockIdx.x * a.f.n_pad + tile * TB * 16 + threadIdx.x] = make_float4(st.ref, st.S, st.E, 0.0f);
+    }
+}
+
+// Joins the ranges of a row and takes the given token's log probability.  The token's own logit is summed in float64 (its
+// rounding would otherwise show where the probability is near 1).  WAVES waves work on a row; returns its lse to them all.
 struct VsJoin {
     VsSrc x, w;
-    const float* bias;         // padded
+    const float* bias;         // as the caller gave it, or null
     const int64_t* targets;    // or null
     const float4* part;
     int32_t n, splits;
     int64_t n_pad;
     float *logprob, *entropy, *lse;
 };
-__global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.n) return;
+template <int WAVES>
+__device__ __forceinline__ float vs_join_row(const VsJoin& a, int64_t row, int tid, float4* red, double* dred) {
+    const int lane = tid & 63, wave = tid >> 6;
     VsStat st;
     st.clear();
-    for (int i = lane; i < a.splits; i += 64) {
+    for (int i = tid; i < a.splits; i += 64 * WAVES) {
         const float4 q = a.part[(int64_t)i * a.n_pad + row];
         st.join(q.x, q.y, q.z);
     }
-    for (int o = 1; o < 64; o <<= 1) {
-        const float r2 = __shfl_xor(st.ref, o), s2 = __shfl_xor(st.S, o), e2 = __shfl_xor(st.E, o);
-        st.join(r2, s2, e2);
-    }
-    const float r = st.ref, s = st.S, e = st.E;
-    const bool empty = s == 0.0f;                   // nothing but -inf
-    const double lse = empty ? -INFINITY : ((double)r + (double)log2f(s)) * 0.6931471805599453;
     const int64_t t = a.targets ? a.targets[row] : -1;
     double dot = 0.0;
     if (t >= 0 && t < a.w.rows)
-        for (int d = lane; d < a.w.dim; d += 64) dot += (double)vs_load(a.x, row, d) * (double)vs_load(a.w, t, d);
-    for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
-    if (lane) return;
-    if (a.lse) a.lse[row] = (float)lse;
-    if (a.entropy) {
-        const float h = VS_LN2 * (log2f(s) - e / s);
-        a.entropy[row] = empty || h < 0.0f ? 0.0f : h;
+        for (int d = tid; d < a.w.dim; d += 64 * WAVES) dot += (double)vs_load(a.x, row, d) * (double)vs_load(a.w, t, d);
+    for (int o = 1; o < 64; o <<= 1) {
+        const float r2 = __shfl_xor(st.ref, o), s2 = __shfl_xor(st.S, o), e2 = __shfl_xor(st.E, o);
+        st.join(r2, s2, e2);
+        dot += __shfl_xor(dot, o);
     }
-    if (a.logprob) {
-        float lp = 0.0f;
-        if (t >= a.w.rows) lp = NAN;
-        else if (t >= 0) {
-            dot += (double)a.bias[t];
-            lp = empty ? -INFINITY : (float)(dot - lse);
-            if (lp > 0.0f) lp = 0.0f;
+    if constexpr (WAVES > 1) {
+        if (lane == 0) { red[wave] = make_float4(st.ref, st.S, st.E, 0.0f); dred[wave] = dot; }
+        __syncthreads();
+        st.clear();
+        dot = 0.0;
+        for (int i = 0; i < WAVES; ++i) { st.join(red[i].x, red[i].y, red[i].z); dot += dred[i]; }
+    }
+    const bool empty = st.S == 0.0f;                // nothing but -inf
+    const double lse = empty ? -INFINITY : ((double)st.ref + (double)log2f(st.S)) * 0.6931471805599453;
+    if (tid == 0) {
+        a.lse[row] = (float)lse;
+        if (a.entropy) {
+            const float h = VS_LN2 * (log2f(st.S) - st.E / st.S);
+            a.entropy[row] = empty || h < 0.0f ? 0.0f : h;
         }
-        a.logprob[row] = lp;
+        if (a.logprob) {
+            float lp = 0.0f;
+            if (t >= a.w.rows) lp = NAN;
+            else if (t >= 0) {
+                lp = empty ? -INFINITY : (float)(dot + (double)vs_bias_of(a.bias, t) - lse);
+                if (lp > 0.0f) lp = 0.0f;
+            }
+            a.logprob[row] = lp;
+        }
     }
+    return (float)lse;
+}
+template <int WAVES>
+__global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
+    __shared__ float4 red[4];
+    __shared__ double dred[4];
+    const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (row >= a.n) return;
+    (void)vs_join_row<WAVES>(a, row, WAVES == 1 ? threadIdx.x & 63 : threadIdx.x, red, dred);
 }
 
 // ---- alternatives -------------------------------------------------------------------------------------------------
 // The k largest logits of a row, ties to the lower id, in the order of the logits as float64 sums them.  The forward pass
-// left each chunk's largest float32 logit m; its float32 sums are within d = 4 (D + 16) 2^-24 (|m| + 2 |x|_1 max |w|) of the
-// true ones.  The k-th largest m - d is a lower bound of the k-th logit, so only chunks with m + d at or above it can hold
-// one: a dozen or two, whose logits are formed again in float64.  A workgroup per row.
+// left each chunk's largest float32 logit m; a float32 sum is within d = 4 (D + 16) 2^-24 (|m| + 2 |x|_1 max |w|) of the true
+// one.  At least k logits are no less than the k-th largest m - d, so only chunks with m + d at or above that can hold one
+// of the k: a few more than k.  Their logits are formed again in float32, those that reach the bound once more in float64,
+// and the best k of these few are ranked by counting.  A workgroup per row.
+//
+// The bound is taken over 256 groups of chunks (the k-th largest of the groups' largest m - d is a bound too, and rarely a
+// lower one): one pass over the maxima.  Chunks are visited in ascending order, so once k logits are known a chunk that
+// cannot beat the k-th is skipped even when it ties: a row of equal logits (a zero vector) ends after the first few.
 #define VS_MAX_K 32
 #define VS_CAND 1024
+#define VS_LIST 256
 struct VsTop {
-    VsSrc x, w;
-    const float* bias;         // padded
+    VsJoin join;               // the row's ranges are joined first
     const float* chunk_max;    // [rows][chunks]
-    const float* group_max;    // [padded vocabulary / 32] largest |w|
-    int32_t n, chunks, k;
-    const float* lse;
+    const float* group_max;    // [2 chunks] largest |w|
+    int32_t chunks, k;
     int32_t* ids;              // [n][k]
     float* logprobs;           // [n][k]
 };
 
-__device__ __forceinline__ uint32_t vs_order(float f) {   // unsigned order = float order
-    const uint32_t u = __float_as_uint(f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
 __device__ __forceinline__ bool vs_before(double v, int i, double w, int j) { return v > w || (v == w && i < j); }
 
-__global__ __launch_bounds__(256) void k_vs_top(VsTop a) {
+// 16 bytes of a row at whatever alignment its elements have, as floats
+template <bool BF16>
+struct VsVec {
+    static constexpr int E = BF16 ? 8 : 4;
+    struct __attribute__((packed, aligned(2))) Raw { uint32_t v[4]; };
+    float f[E];
+    __device__ __forceinline__ void load(const void* base, int64_t element) {
+        if constexpr (BF16) {
+            const Raw r = *(const Raw*)((const uint16_t*)base + element);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(r.v[i] << 16); f[2 * i + 1] = __uint_as_float(r.v[i] & 0xFFFF0000u); }
+        } else {
+            const Raw r = *(const Raw*)((const float*)base + element);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(r.v[i]);
+        }
+    }
+};
+
+// x . row over 16 lanes (xs: x in LDS); the result is in all of them.  The last piece of a row that is no whole number of
+// pieces long is taken back from the row's end, with the elements before it weighted 0 -- no read leaves the row.
+template <bool BF16>
+__device__ __forceinline__ float vs_dot16(const VsSrc& w, int64_t row, const float* xs, int l16) {
+    constexpr int E = VsVec<BF16>::E;
+    float s = 0.0f;
+    if (w.dim < E) {
+        if (l16 < w.dim) s = xs[l16] * vs_load(w, row, l16);
+    } else {
+        for (int d = l16 * E; d < w.dim; d += 16 * E) {
+            const int at = min(d, w.dim - E);
+            VsVec<BF16> v;
+            v.load(w.p, row * w.ld + at);
+#pragma unroll
+            for (int i = 0; i < E; ++i) s = at + i >= d ? fmaf(xs[at + i], v.f[i], s) : s;
+        }
+    }
+    return vs_row_sum(s);
+}
+
+template <bool BF16, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
+    const VsSrc &x = a.join.x, &w = a.join.w;
     __shared__ float xs[512];
-    __shared__ uint32_t hist[256];
+    __shared__ float best[256];
     __shared__ double cv[VS_CAND], cw[VS_MAX_K];
     __shared__ int ci[VS_CAND], cj[VS_MAX_K];
-    __shared__ int n_cand, sel, need_s, n_list;
-    __shared__ float red[4];
-    __shared__ int list[256];
+    __shared__ float red[THREADS / 64];
+    __shared__ uint32_t found[4];
+    __shared__ uint16_t list[VS_LIST], rows[VS_CAND];
+    __shared__ int n_cand, n_rows, n_list;
     const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = tid & 15, quarter = lane >> 4;
     const float* cm = a.chunk_max + row * a.chunks;
-    if (a.lse[row] != a.lse[row]) {         // no order among the logits
+    const float lse = vs_join_row<THREADS / 64>(a.join, row, tid, (float4*)cv, cw);
+    __syncthreads();
+    if (lse != lse) {                       // no order among the logits
         if (tid < a.k) { a.ids[row * a.k + tid] = -1; a.logprobs[row * a.k + tid] = NAN; }
         return;
     }
     float l1 = 0.0f;
-    for (int d = tid; d < a.x.dim; d += 256) { const float v = vs_load(a.x, row, d); xs[d] = v; l1 += fabsf(v); }
+    for (int d = tid; d < x.dim; d += THREADS) { const float v = vs_load(x, row, d); xs[d] = v; l1 += fabsf(v); }
     for (int o = 1; o < 64; o <<= 1) l1 += __shfl_xor(l1, o);
-    if (lane == 0) red[tid >> 6] = l1;
-    if (tid == 0) n_cand = 0;
+    if (lane == 0) red[wave] = l1;
+    if (tid == 0) n_cand = n_rows = n_list = 0;
     __syncthreads();
-    l1 = red[0] + red[1] + red[2] + red[3];
-    const float eps = 4.0f * (float)(a.x.dim + 16) * 5.9604645e-8f;
+    l1 = 0.0f;
+    for (int i = 0; i < THREADS / 64; ++i) l1 += red[i];
+    __syncthreads();
+    const float eps = 4.0f * (float)(x.dim + 16) * 5.9604645e-8f;
     auto off = [&](int c, float m) {
-        float g = 0.0f;
-#pragma unroll
-        for (int i = 0; i < VS_CHUNK / 32; ++i) g = fmaxf(g, a.group_max[c * (VS_CHUNK / 32) + i]);
-        return eps * (fabsf(m) + 2.0f * l1 * g);
+        const float2 g = *(const float2*)&a.group_max[c * 2];
+        return eps * (fabsf(m) + 2.0f * l1 * fmaxf(g.x, g.y));
     };
-    // the k-th largest lower bound, by its bits, eight at a time
-    uint32_t prefix = 0;
-    bool all = a.chunks <= a.k;
-    int need = a.k;
-    if (!all) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            hist[tid] = 0;
-            __syncthreads();
-            for (int c = tid; c < a.chunks; c += 256) {
-                const float m = cm[c];
-                const uint32_t u = vs_order(m - off(c, m));
-                if (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(u >> shift) & 255u], 1u);
+    float low = -INFINITY;
+#pragma unroll 4
+    for (int c = tid; c < a.chunks; c += THREADS) {
+        const float m = cm[c];
+        low = fmaxf(low, m > -INFINITY ? m - off(c, m) : -INFINITY);
+    }
+    for (int o = 1; o < THREADS / 256; o <<= 1) low = fmaxf(low, __shfl_xor(low, o));
+    if (tid % (THREADS / 256) == 0) best[tid / (THREADS / 256)] = low;
+    __syncthreads();
+    {                                       // the k-th largest of the 256: the largest value with at least k not below it
+        float t = -INFINITY;
+        if (tid < 256) {
+            const float mine = best[tid];
+            int above = 0;
+            for (int j = 0; j < 256; j += 4) {
+                const float4 q = *(const float4*)&best[j];
+                above += (q.x >= mine) + (q.y >= mine) + (q.z >= mine) + (q.w >= mine);
             }
-            __syncthreads();
-            if (tid == 0) {
-                int left = need, b = 255;
-                while (b > 0 && left > (int)hist[b]) left -= (int)hist[b--];
-                sel = b; need_s = left;
-            }
-            __syncthreads();
-            prefix |= (uint32_t)sel << shift;
-            need = need_s;
-            __syncthreads();
+            t = above >= a.k ? mine : -INFINITY;
+            for (int o = 1; o < 64; o <<= 1) t = fmaxf(t, __shfl_xor(t, o));
+            if (lane == 0) red[wave] = t;
         }
     }
-    const uint32_t tu = prefix;
-    const float bound = all ? -INFINITY : __uint_as_float(tu & 0x80000000u ? tu & 0x7FFFFFFFu : ~tu);
-    double least = -INFINITY;       // the k-th best so far once k are known: what comes later must beat it
+    __syncthreads();
+    const float bound = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    double least = -INFINITY;               // the k-th best so far once k are known: what comes later must beat it
     bool full = false;
-    auto compact = [&]() {          // keeps the best k of the candidates, in order
+    auto compact = [&]() {                  // keeps the best k of the candidates, in order
         __syncthreads();
         const int n = n_cand;
-        for (int i = tid; i < n; i += 256) {
+        for (int i = tid; i < n; i += THREADS) {
             int rank = 0;
             for (int j = 0; j < n; ++j) rank += vs_before(cv[j], ci[j], cv[i], ci[i]);
             if (rank < a.k) { cw[rank] = cv[i]; cj[rank] = ci[i]; }
@@ -509,57 +734,88 @@ __global__ __launch_bounds__(256) void k_vs_top(VsTop a) {
         if (tid == 0) n_cand = m;
         __syncthreads();
         if (m == a.k) { full = true; least = cv[m - 1]; }
-        __syncthreads();
     };
-    constexpr int PER = 256 / VS_CHUNK;      // chunks that are looked at together
-    for (int c0 = 0; c0 < a.chunks; c0 += 256) {
-        // the next 256 chunks' candidates, in ascending order
-        if (tid == 0) n_list = 0;
-        __syncthreads();
-        const int c = c0 + tid;
-        bool want = false;
-        if (c < a.chunks) {
-            const float m = cm[c];
-            const float up = m + off(c, m);
-            want = up >= bound && m > -INFINITY && !(full && (double)up <= least);
-        }
-        const unsigned long long bal = __ballot(want);
-        for (int wv = 0; wv < 4; ++wv) {
-            if ((tid >> 6) == wv) {
-                if (want) list[n_list + __popcll(bal & ((1ull << lane) - 1ull))] = c;
+    // the rows of a chunk that reach the bound, four at a time; float64 logits of rows
+    auto look = [&](int c, int r0, int r1, int tag) {
+        const float d = off(c, cm[c]);
+#pragma unroll 4
+        for (int r = r0; r < r1; r += 4) {
+            const int v = c * VS_CHUNK + r + quarter, u = min(v, w.rows - 1);
+            const float s = vs_dot16<BF16>(w, u, xs, l16) + vs_bias_of(a.join.bias, u);
+            if (l16 == 0 && v == u && s > -INFINITY && s + d >= bound) {
+                const int at = atomicAdd(&n_rows, 1);
+                if (at < VS_CAND) rows[at] = (uint16_t)(tag * VS_CHUNK + r + quarter);
             }
-            __syncthreads();
-            if ((tid >> 6) == wv && lane == 0) n_list += __popcll(bal);
-            __syncthreads();
         }
-        const int nl = n_list;
-        for (int i0 = 0; i0 < nl; i0 += PER) {
-            const int i = i0 + tid / VS_CHUNK;
-            if (i < nl) {
-                const int v = list[i] * VS_CHUNK + tid % VS_CHUNK;
-                if (v < a.w.rows) {
-                    double s = 0.0;
-                    for (int d = 0; d < a.w.dim; ++d) s = fma((double)xs[d], (double)vs_load(a.w, v, d), s);
-                    s += (double)a.bias[v];
-                    // (a double below every candidate chunk's lower bound is none of the k)
-                    if (s >= (double)bound && s > -INFINITY && !(full && s <= least)) {
-                        const int at = atomicAdd(&n_cand, 1);
-                        cv[at] = s; ci[at] = v;
-                    }
-                }
-            }
-            __syncthreads();
-            if (n_cand > VS_CAND - 256) compact();
-            __syncthreads();
+    };
+    auto exact = [&](int v) {
+        double s = 0.0;
+        for (int q = lane; q < w.dim; q += 64) s = fma((double)xs[q], (double)vs_load(w, v, q), s);
+        for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
+        s += (double)vs_bias_of(a.join.bias, v);
+        if (lane == 0 && !(full && s <= least)) {
+            const int at = atomicAdd(&n_cand, 1);
+            cv[at] = s; ci[at] = v;
         }
+    };
+    // every chunk that may hold one of the k: usually a few more than k
+#pragma unroll 4
+    for (int c = tid; c < a.chunks; c += THREADS) {
+        const float m = cm[c];
+        if (m > -INFINITY && m + off(c, m) >= bound) {
+            const int at = atomicAdd(&n_list, 1);
+            if (at < VS_LIST) list[at] = (uint16_t)c;
+        }
+    }
+    __syncthreads();
+    bool done = n_list <= VS_LIST;
+    if (done) {                             // all their rows at once, a quarter of a chunk for each wave
+        const int n = n_list;
+        for (int i = wave; i < n * 4; i += THREADS / 64) look(list[i >> 2], (i & 3) * (VS_CHUNK / 4), ((i & 3) + 1) * (VS_CHUNK / 4), i >> 2);
         __syncthreads();
+        done = n_rows <= VS_CAND;
+        if (done) {
+            const int nr = n_rows;
+            for (int i = wave; i < nr; i += THREADS / 64) exact(list[rows[i] / VS_CHUNK] * VS_CHUNK + rows[i] % VS_CHUNK);
+        }
+    }
+    if (!done) {                            // many equal logits: chunk after chunk
+        __syncthreads();
+        for (int c0 = 0; c0 < a.chunks; c0 += 256) {
+            const int c = c0 + tid;
+            bool want = false;
+            if (tid < 256 && c < a.chunks) {
+                const float m = cm[c], up = m + off(c, m);
+                want = m > -INFINITY && up >= bound && !(full && (double)up <= least);
+            }
+            const unsigned long long bal = __ballot(want);
+            if (lane == 0 && wave < 4) found[wave] = __popcll(bal);
+            __syncthreads();
+            int before = 0;
+            for (int i = 0; i < min(wave, 4); ++i) before += found[i];
+            const int nl = found[0] + found[1] + found[2] + found[3];
+            if (want) list[before + __popcll(bal & ((1ull << lane) - 1ull))] = (uint16_t)c;
+            __syncthreads();
+            for (int i0 = 0; i0 < nl; i0 += 4) {
+                if (tid == 0) n_rows = 0;
+                __syncthreads();
+                if (wave < 4 && i0 + wave < nl) look(list[i0 + wave], 0, VS_CHUNK, wave);
+                __syncthreads();
+                const int nr = n_rows;
+                for (int i = wave; i < nr; i += THREADS / 64) exact(list[i0 + rows[i] / VS_CHUNK] * VS_CHUNK + rows[i] % VS_CHUNK);
+                __syncthreads();
+                const bool crowded = n_cand > VS_CAND - 256;
+                if (crowded) compact();
+                __syncthreads();
+            }
+        }
     }
     compact();
+    __syncthreads();
     if (tid < a.k) {
-        const float lse = a.lse[row];
-        const bool have = tid < n_cand && lse == lse;
+        const bool have = tid < n_cand;
         a.ids[row * a.k + tid] = have ? ci[tid] : -1;
-        a.logprobs[row * a.k + tid] = have ? fminf((float)(cv[tid] - (double)lse), 0.0f) : lse == lse ? -INFINITY : lse;
+        a.logprobs[row * a.k + tid] = have ? fminf((float)(cv[tid] - (double)lse), 0.0f) : -INFINITY;
     }
 }
 

@@ -15,6 +15,7 @@ namespace {
 
 constexpr int64_t VS_PAD = 128;                 // rows are padded to this (ids to VS_BLOCK)
 constexpr int64_t VS_ROWS_MAX = 16384;          // tokens of one pass of the forward kernels
+constexpr int64_t VS_RAW = 128;                 // at most this many tokens read the weights as they lie
 constexpr size_t VS_ALIGN = 256;
 
 inline int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -61,8 +62,8 @@ int vs_steps(int dim) {
 constexpr int vs_fwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 4 ? 4 : 2) : (ks <= 4 ? 2 : 1); }
 constexpr int vs_bwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 2 ? 4 : ks <= 8 ? 2 : 1) : (ks <= 4 ? 2 : 1); }
 
-// streaming rows of a stage of the forward kernel: two stages of at most 40 KiB (0: too wide, the waves read for themselves)
-constexpr int vs_stage_rows(int ks, int pl) { return ks * pl <= 4 ? 128 : ks * pl <= 8 ? 64 : ks * pl <= 20 ? 32 : 0; }
+// streaming rows of a stage of the forward kernel: two stages of at most 60 KiB (0: too wide, the waves read for themselves)
+constexpr int vs_stage_rows(int ks, int pl) { return ks * pl <= 4 ? 128 : ks * pl <= 8 ? 64 : ks * pl <= 30 ? 32 : 0; }
 
 #define VS_BY_WIDTH(ks, pl, F)                                                        \
     do {                                                                              \
@@ -90,6 +91,17 @@ struct Shape {
     int dim, ks, pl, k, cus;
 };
 
+// 16-token blocks of a wave that reads the weights as they lie: one, or two where registers allow and tokens are there
+constexpr int vs_raw_most(int ks, int pl) { return ks * pl <= 10 ? 2 : 1; }
+int vs_raw_blocks(const Shape& s) {
+    if (s.n > VS_RAW || s.dim < 8) return 0;
+    int most = 1;
+#define VS_F(KS, PL) most = vs_raw_most(KS, PL)
+    VS_BY_WIDTH(s.ks, s.pl, VS_F);
+#undef VS_F
+    return s.n <= 16 ? 1 : most;
+}
+
 int vs_block_rows(const Shape& s, bool fwd) {
     int tb = 1;
 #define VS_F(KS, PL) tb = fwd ? vs_fwd_blocks(KS, PL) : vs_bwd_blocks(KS, PL)
@@ -108,6 +120,7 @@ int vs_splits(const Shape& s, int64_t tiles, int64_t flow, int64_t most) {
 struct FwdPlan {
     int64_t rows, n_pad, tiles, chunks;
     int splits;
+    int raw;                    // 16-token blocks of a tile of k_vs_forward_raw (0: the weights are packed)
     bool staged;
     uint4 *xS, *wS;
     float *bias, *group_max, *chunk_max;
@@ -118,17 +131,24 @@ FwdPlan plan_fwd(const Shape& s, void* ws) {
     FwdPlan p{};
     Arena a{(char*)ws};
     const int br = vs_block_rows(s, true);
-    p.rows = std::min(s.n, VS_ROWS_MAX);
-    p.n_pad = up(p.rows, VS_PAD);
-    p.tiles = cdiv(p.rows, br);
+    const int64_t blocks = s.vp / VS_BLOCK, frag = (int64_t)s.ks * s.pl * 64;          // uint4 of a 16-row block
     p.chunks = s.vp / VS_CHUNK;
-    p.staged = p.tiles >= 4 && vs_stage_rows(s.ks, s.pl) > 0;
-    const int64_t blocks = s.vp / VS_BLOCK;
-    p.splits = p.staged ? (int)std::min<int64_t>(blocks, cdiv((int64_t)s.cus * 4, cdiv(p.tiles, 4))) : vs_splits(s, p.tiles, blocks, 1 << 20);
-    const int64_t frag = (int64_t)s.ks * s.pl * 64;          // uint4 of a 16-row block
-    p.wS = a.take<uint4>(s.vp / 16 * frag);
-    p.xS = a.take<uint4>(p.n_pad / 16 * frag);
-    p.bias = a.take<float>(s.vp);
+    p.raw = vs_raw_blocks(s);
+    if (p.raw) {
+        p.rows = s.n;
+        p.tiles = cdiv(s.n, p.raw * 16);
+        p.n_pad = p.tiles * p.raw * 16;
+        p.splits = (int)std::min<int64_t>(cdiv(p.chunks, 16), s.cus * 2);
+    } else {
+        p.rows = std::min(s.n, VS_ROWS_MAX);
+        p.n_pad = up(p.rows, VS_PAD);
+        p.tiles = cdiv(p.rows, br);
+        p.staged = vs_stage_rows(s.ks, s.pl) > 0;
+        p.splits = p.staged ? (int)std::min<int64_t>(blocks, cdiv((int64_t)s.cus * 4, cdiv(p.tiles, 4))) : vs_splits(s, p.tiles, blocks, 1 << 20);
+        p.wS = a.take<uint4>(s.vp / 16 * frag);
+        p.xS = a.take<uint4>(p.n_pad / 16 * frag);
+        p.bias = a.take<float>(s.vp);
+    }
     p.group_max = a.take<float>(s.vp / 32);
     p.part = a.take<float4>(p.splits * p.n_pad);
     p.chunk_max = a.take<float>(s.k ? p.n_pad * p.chunks : 0);
@@ -245,29 +265,44 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
     if (!dev.ok) return sage_ctx_fail(c, SAGE_E_HIP, "the context's device cannot be made current");
     const hipStream_t st = (hipStream_t)stream;
     const VsSrc w{d_weight, ldw, (int32_t)vocab, dim, dtype == SAGE_BF16}, x{d_x, ldx, (int32_t)n, dim, dtype == SAGE_BF16};
-    pack(s, w, s.vp, p.wS, nullptr, alternatives ? p.group_max : nullptr, st);
-    k_vs_bias<<<cdiv(s.vp, 256), 256, 0, st>>>(d_bias, (int32_t)vocab, (int32_t)s.vp, p.bias);
+    if (!p.raw) {
+        pack(s, w, s.vp, p.wS, nullptr, alternatives ? p.group_max : nullptr, st);
+        k_vs_bias<<<cdiv(s.vp, 256), 256, 0, st>>>(d_bias, (int32_t)vocab, (int32_t)s.vp, p.bias);
+    }
     for (int64_t r0 = 0; r0 < n; r0 += p.rows) {
         const int64_t rows = std::min(p.rows, n - r0);
         const VsSrc xr = rows_from(x, r0, rows);
-        pack(s, xr, p.n_pad, p.xS, nullptr, nullptr, st);
-        const VsFwd f{p.xS, p.wS, p.bias, d_bias != nullptr, (int32_t)vocab, (int32_t)p.tiles, p.splits, (int32_t)(s.vp / VS_BLOCK), (int32_t)p.chunks, p.n_pad, p.part,
-                      alternatives ? p.chunk_max : nullptr};
-        const uint32_t grid = cdiv(p.tiles * p.splits, 4), grid_staged = cdiv(p.tiles, 4) * p.splits;
-#define VS_F(KS, PL)                                                                                                          \
-    if constexpr (vs_stage_rows(KS, PL) > 0)                                                                                  \
-        if (p.staged) { k_vs_forward_staged<KS, PL, vs_fwd_blocks(KS, PL), vs_stage_rows(KS, PL)><<<grid_staged, 256, 0, st>>>(f); break; } \
-    k_vs_forward<KS, PL, vs_fwd_blocks(KS, PL)><<<grid, 256, 0, st>>>(f)
-        VS_BY_WIDTH(s.ks, s.pl, VS_F);
+        const VsFwd f{p.xS, p.wS, p.bias, d_bias != nullptr, (int32_t)vocab, (int32_t)p.tiles, p.splits, (int32_t)(s.vp / VS_BLOCK), (int32_t)p.chunks,
+                      p.n_pad, p.part, alternatives ? p.chunk_max : nullptr};
+        if (p.raw) {
+            const VsRaw q{xr, w, d_bias, alternatives ? p.group_max : nullptr, f};
+            const dim3 grid(p.splits, (uint32_t)p.tiles);
+#define VS_F(KS, PL)                                                                                                            \
+    if constexpr (vs_raw_most(KS, PL) > 1)                                                                                      \
+        if (p.raw > 1) { k_vs_forward_raw<KS, PL, vs_raw_most(KS, PL)><<<grid, 256, 0, st>>>(q); break; }                       \
+    k_vs_forward_raw<KS, PL, 1><<<grid, 256, 0, st>>>(q)
+            VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
-        const VsJoin j{xr, w, p.bias, d_targets ? d_targets + r0 : nullptr, p.part, (int32_t)rows, p.splits, p.n_pad,
-                       d_logprob ? d_logprob + r0 : nullptr, d_entropy ? d_entropy + r0 : nullptr, d_lse + r0};
-        k_vs_join<<<cdiv(rows, 4), 256, 0, st>>>(j);
-        if (alternatives) {
-            const VsTop t{xr, w, p.bias, p.chunk_max, p.group_max, (int32_t)rows, (int32_t)p.chunks, alternatives, d_lse + r0,
-                          d_alt_ids + r0 * alternatives, d_alt_logprobs + r0 * alternatives};
-            k_vs_top<<<(uint32_t)rows, 256, 0, st>>>(t);
+        } else {
+            pack(s, xr, p.n_pad, p.xS, nullptr, nullptr, st);
+            const uint32_t grid = cdiv(p.tiles * p.splits, 4), grid_staged = cdiv(p.tiles, 4) * p.splits;
+#define VS_F(KS, PL)                                                                                                            \
+    if constexpr (vs_stage_rows(KS, PL) > 0)                                                                                    \
+        k_vs_forward_staged<KS, PL, vs_fwd_blocks(KS, PL), vs_stage_rows(KS, PL)><<<grid_staged, 256, 0, st>>>(f);              \
+    else k_vs_forward<KS, PL, vs_fwd_blocks(KS, PL)><<<grid, 256, 0, st>>>(f)
+            VS_BY_WIDTH(s.ks, s.pl, VS_F);
+#undef VS_F
         }
+        const VsJoin j{xr, w, d_bias, d_targets ? d_targets + r0 : nullptr, p.part, (int32_t)rows, p.splits, p.n_pad,
+                       d_logprob ? d_logprob + r0 : nullptr, d_entropy ? d_entropy + r0 : nullptr, d_lse + r0};
+        if (alternatives) {
+            const VsTop t{j, p.chunk_max, p.group_max, (int32_t)p.chunks, alternatives, d_alt_ids + r0 * alternatives, d_alt_logprobs + r0 * alternatives};
+            // a row alone on a CU is bound by latency: sixteen waves share its chain of loads
+            const bool wide = rows <= s.cus;
+            if (dtype == SAGE_BF16) { if (wide) k_vs_top<true, 1024><<<(uint32_t)rows, 1024, 0, st>>>(t); else k_vs_top<true, 256><<<(uint32_t)rows, 256, 0, st>>>(t); }
+            else { if (wide) k_vs_top<false, 1024><<<(uint32_t)rows, 1024, 0, st>>>(t); else k_vs_top<false, 256><<<(uint32_t)rows, 256, 0, st>>>(t); }
+        } else if (p.splits > 64) k_vs_join<4><<<(uint32_t)rows, 256, 0, st>>>(j);
+        else k_vs_join<1><<<cdiv(rows, 4), 256, 0, st>>>(j);
     }
     return launched(c, "sage_token_logprobs_device");
 }

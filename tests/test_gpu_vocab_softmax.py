@@ -159,6 +159,16 @@ def test_long_vocabulary(n, V, D, dtype):
     check_forward(vs.token_logprobs(x, w, t, bias=b, alternatives=10), e, 10)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [3, 4, 7, 8, 50, 64, 65, 129, 200, 257, 300, 385, 511, 512])
+def test_one_to_seventeen_tokens(D, dtype):
+    """The kernel that reads the weights as they lie takes up to sixteen tokens, 1, 2, 4 or 8 at a time."""
+    from sage_amd import vocab_softmax as vs
+    for n in (1, 2, 3, 4, 5, 8, 9, 13, 16, 17):
+        x, w, b, t = make(n, 300, D, dtype, ("none", "prior", "mask")[n % 3])
+        check_forward(vs.token_logprobs(x, w, t, bias=b, alternatives=n), Exact(x, w, b, t, n), n)
+
+
 def test_many_rows_cross_a_pass():
     """More rows than one pass of the forward kernels takes."""
     from sage_amd import vocab_softmax as vs
