@@ -27,8 +27,13 @@ typedef float vs_f8 __attribute__((ext_vector_type(8)));
 
 #define VS_LOG2E 1.4426950408889634f
 #define VS_LN2 0.6931471805599453f
-#define VS_CHUNK 64            // ids per stored maximum (the unit in which alternatives are looked for)
+#define VS_CHUNK 16            // ids per stored maximum (the unit in which alternatives are looked for)
 #define VS_BLOCK 256           // ids are dealt out in blocks of this many
+// A chunk is what one lane of a fragment sees of 64 ids: 4 (of each of four 16-row tiles), so its maximum needs no other
+// lane.  Chunk c: of block c / 16 the lane quarter c / 4 % 4 of the 64 ids c % 4; a lane stores its four of a block at once.
+__device__ __forceinline__ int vs_chunk_row(int c, int i) {      // the i-th of the 16 ids of a chunk
+    return (c >> 4) * VS_BLOCK + (c & 3) * 64 + (i >> 2) * 16 + ((c >> 2) & 3) * 4 + (i & 3);
+}
 #define VS_NOTHING (-1.0e30f)  // reference of a row that has seen no finite logit yet; a bias this low masks its id
 #define VS_SLACK 20.0f         // the running reference lags the maximum by at most this (in powers of two)
 #define VS_TMIN (-200.0f)      // 2^-200 is 0 in float32: what a logit of -inf is raised to, so that 0 * log p is 0
@@ -62,13 +67,25 @@ __device__ __forceinline__ void vs_mfma_parts(const vs_bf8 (&a)[R][PL], const B&
             for (int t = 0; t < TB; ++t) c[r][t] = vs_mfma(a[r][pa[q]], b(t, pb[q]), c[r][t]);
 }
 
-// v as the sum of PL bf16 (each rounding to nearest; exact for PL = 3, within 2^-9 |v| for PL = 1)
+// v as the sum of PL bf16 (each rounding to nearest; exact for PL = 3, within 2^-9 |v| for PL = 1), two at a time
 template <int PL>
 __device__ __forceinline__ void vs_split(vs_f8 v, vs_bf8* out) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int p = 0; p < PL; ++p) {
-        out[p] = __builtin_convertvector(v, vs_bf8);
-        if (p + 1 < PL) v -= __builtin_convertvector(out[p], vs_f8);
+        u4 bits;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f2 pair = {v[2 * i], v[2 * i + 1]};
+            bits[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, b2));
+            if (p + 1 < PL) {
+                v[2 * i] -= __uint_as_float(bits[i] << 16);
+                v[2 * i + 1] -= __uint_as_float(bits[i] & 0xFFFF0000u);
+            }
+        }
+        out[p] = __builtin_bit_cast(vs_bf8, bits);
     }
 }
 
@@ -135,7 +152,7 @@ struct VsFwd {
     int32_t n_tiles;           // token tiles of 16 TB rows
     int32_t splits;            // ranges of the vocabulary
     int32_t blocks;            // blocks of VS_BLOCK ids
-    int32_t chunks;            // chunks of VS_CHUNK ids
+    int32_t chunks;            // chunks of VS_CHUNK ids: 16 a block
     int64_t n_pad;             // row length of the partials
     float4* part;              // [splits][n_pad]: reference (in powers of two), sum of exps, sum of exp * exponent
     float* chunk_max;          // [n_pad][chunks] or null
@@ -192,10 +209,11 @@ __device__ __forceinline__ void vs_stationary(const uint4* S, int64_t tile, int 
 template <int TB>
 struct VsRowsOfTile {
     VsStat st[TB];
-    float top[TB], keep[TB];
+    float top[TB];
+    vs_f4 keep[TB];
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int t = 0; t < TB; ++t) { st[t].clear(); top[t] = -INFINITY; keep[t] = -INFINITY; }
+        for (int t = 0; t < TB; ++t) { st[t].clear(); top[t] = -INFINITY; }
     }
     // the logits of 32 ids; MASKED: some may be -inf
     template <bool MASKED>
@@ -221,16 +239,21 @@ struct VsRowsOfTile {
             st[t].e += le;
         }
     }
-    // chunk c is done; the largest logits of four chunks are stored together, sixteen bytes a row
-    __device__ __forceinline__ void chunk(const VsFwd& a, int64_t tile, int c, int lane, bool live) {
+    // 64 ids are done, the h-th of their block: their largest logits are stored with those of the rest of the block, sixteen
+    // bytes a lane (WHOLE: the wave sees whole blocks), or at once
+    template <bool WHOLE>
+    __device__ __forceinline__ void chunk(const VsFwd& a, int64_t tile, int block, int h, int lane, bool live) {
         if (a.chunk_max) {
 #pragma unroll
             for (int t = 0; t < TB; ++t) {
-                float m = vs_max(top[t], __shfl_xor(top[t], 16));
-                m = vs_max(m, __shfl_xor(m, 32));
-                if ((c & 3) == (lane >> 4)) keep[t] = m;
+                float* to = a.chunk_max + ((tile * TB + t) * 16 + (lane & 15)) * a.chunks + block * 16 + (lane >> 4) * 4;
+                if (WHOLE) {
+                    if (h == 0) keep[t][0] = top[t];
+                    else if (h == 1) keep[t][1] = top[t];
+                    else if (h == 2) keep[t][2] = top[t];
+                    else if (live) *(vs_f4*)to = vs_f4{keep[t][0], keep[t][1], keep[t][2], top[t]};
+                } else if (live) to[h] = top[t];
                 top[t] = -INFINITY;
-                if ((c & 3) == 3 && live) a.chunk_max[((tile * TB + t) * 16 + (lane & 15)) * a.chunks + (c & ~3) + (lane >> 4)] = keep[t];
             }
         }
     }
@@ -282,16 +305,16 @@ __global__ __launch_bounds__(256, 2) void k_vs_forward(VsFwd a) {
     VsRowsOfTile<TB> rows;
     rows.clear();
     for (int b = b0; b < b1; ++b) {
-        for (int c = b * (VS_BLOCK / VS_CHUNK); c < (b + 1) * (VS_BLOCK / VS_CHUNK); ++c) {
+        for (int h = 0; h < 4; ++h) {
 #pragma unroll 1
-            for (int row0 = c * VS_CHUNK; row0 < (c + 1) * VS_CHUNK; row0 += 32) {
+            for (int row0 = b * VS_BLOCK + h * 64; row0 < b * VS_BLOCK + (h + 1) * 64; row0 += 32) {
                 vs_f4 s[2][TB];
                 vs_bias_init<TB>(a.bias + row0, lane, s);
                 vs_product<KS, PL, TB>(a.wS + (int64_t)row0 / 16 * KS * PL * 64 + lane, x, s);
                 if (a.has_bias || row0 + 32 > a.vocab) rows.template add<true>(s);      // the same in the whole grid
                 else rows.template add<false>(s);
             }
-            rows.chunk(a, tile, c, lane, true);
+            rows.template chunk<true>(a, tile, b, h, lane, true);
         }
         rows.flush();
     }
@@ -338,7 +361,7 @@ struct VsStage {
             vs_product<KS, PL, TB>(from + r * KS * PL * 4 + lane, x, s);
             if (a.has_bias || row0 + 32 > a.vocab) rows.template add<true>(s);
             else rows.template add<false>(s);
-            if ((row0 & (VS_CHUNK - 1)) == VS_CHUNK - 32) rows.chunk(a, tile, row0 / VS_CHUNK, lane, live);
+            if (row0 & 32) rows.template chunk<true>(a, tile, row0 / VS_BLOCK, (row0 >> 6) & 3, lane, live);
         }
         if (((base + SR) & (VS_BLOCK - 1)) == 0) rows.flush();
     }
@@ -440,7 +463,7 @@ struct VsRaw {
 template <int KS, int PL, int TB>
 __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(VsRaw a) {
     const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-    constexpr int KG = PL == 1 ? (KS < 16 ? KS : 8) : 2;    // 32-element steps whose loads are under way together
+    constexpr int KG = PL == 1 ? (KS < 16 ? KS : 8) : KS <= 4 ? KS : 2;    // 32-element steps whose loads are under way together
     __shared__ float4 red[4][TB * 16];
     const int tile = blockIdx.y;
     int at[KS];
@@ -462,11 +485,11 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
     }
     VsRowsOfTile<TB> rows;
     rows.clear();
-    const int units = gridDim.x * 4, unit = blockIdx.x * 4 + (threadIdx.x >> 6), quads = a.f.chunks / 4;
-    const int c0 = (int)((int64_t)quads * unit / units) * 4, c1 = (int)((int64_t)quads * (unit + 1) / units) * 4;
+    const int units = gridDim.x * 4, unit = blockIdx.x * 4 + (threadIdx.x >> 6), pieces = a.f.blocks * 4;
+    const int c0 = (int)((int64_t)pieces * unit / units), c1 = (int)((int64_t)pieces * (unit + 1) / units);
     for (int c = c0; c < c1; ++c) {
 #pragma unroll 1
-        for (int row0 = c * VS_CHUNK; row0 < (c + 1) * VS_CHUNK; row0 += 32) {
+        for (int row0 = c * 64; row0 < (c + 1) * 64; row0 += 32) {
             // (loads first and together; the bias is added last, so that no wait for it stands before the products)
             VsPiece<PL> raw[2][KG], big;
             vs_f4 s[2][TB], b[2];
@@ -497,6 +520,7 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
                         }
                         vs_mfma_parts<PL, 2, TB>(wf, [&](int t, int p) { return x[t][g + k][p]; }, s);
                     }
+                if (KG < KS) __builtin_amdgcn_sched_barrier(0);     // (the loads of all groups at once would spill)
             }
             if (a.bias || row0 + 32 > a.w.rows) {
 #pragma unroll
@@ -515,7 +539,7 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
             if (a.bias || row0 + 32 > a.w.rows) rows.template add<true>(s);
             else rows.template add<false>(s);
         }
-        rows.chunk(a.f, tile, c, lane, true);
+        rows.template chunk<false>(a.f, tile, c >> 2, c & 3, lane, true);
         if ((c & 3) == 3) rows.flush();
     }
     rows.join_lanes();
@@ -600,19 +624,19 @@ __global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
 // The k largest logits of a row, ties to the lower id, in the order of the logits as float64 sums them.  The forward pass
 // left each chunk's largest float32 logit m; a float32 sum is within d = 4 (D + 16) 2^-24 (|m| + 2 |x|_1 max |w|) of the true
 // one.  At least k logits are no less than the k-th largest m - d, so only chunks with m + d at or above that can hold one
-// of the k: a few more than k.  Their logits are formed again in float32, those that reach the bound once more in float64,
+// of the k: a few more than k, of 16 ids each.  Their logits are formed again in float32, those that reach the bound once more in float64,
 // and the best k of these few are ranked by counting.  A workgroup per row.
 //
 // The bound is taken over 256 groups of chunks (the k-th largest of the groups' largest m - d is a bound too, and rarely a
-// lower one): one pass over the maxima.  Chunks are visited in ascending order, so once k logits are known a chunk that
-// cannot beat the k-th is skipped even when it ties: a row of equal logits (a zero vector) ends after the first few.
+// lower one): one pass over the maxima.  Where too many chunks reach it (many equal logits, a zero vector), they are visited
+// in ascending order, and once k logits are known a later one that cannot beat the k-th is skipped even when it ties.
 #define VS_MAX_K 32
 #define VS_CAND 1024
 #define VS_LIST 256
 struct VsTop {
     VsJoin join;               // the row's ranges are joined first
     const float* chunk_max;    // [rows][chunks]
-    const float* group_max;    // [2 chunks] largest |w|
+    const float* group_max;    // [8 blocks] largest |w| of 32 ids
     int32_t chunks, k;
     int32_t* ids;              // [n][k]
     float* logprobs;           // [n][k]
@@ -689,18 +713,29 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
     for (int i = 0; i < THREADS / 64; ++i) l1 += red[i];
     __syncthreads();
     const float eps = 4.0f * (float)(x.dim + 16) * 5.9604645e-8f;
-    auto off = [&](int c, float m) {
-        const float2 g = *(const float2*)&a.group_max[c * 2];
-        return eps * (fabsf(m) + 2.0f * l1 * fmaxf(g.x, g.y));
+    auto widest = [&](int block) {          // eps 2 |x|_1 max |w| of the block
+        const float4 p = *(const float4*)&a.group_max[block * 8], q = *(const float4*)&a.group_max[block * 8 + 4];
+        return eps * 2.0f * l1 * fmaxf(fmaxf(fmaxf(p.x, p.y), fmaxf(p.z, p.w)), fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)));
     };
+    auto off = [&](int c, float m) { return fmaf(eps, fabsf(m), widest(c >> 4)); };
     float low = -INFINITY;
-#pragma unroll 4
-    for (int c = tid; c < a.chunks; c += THREADS) {
-        const float m = cm[c];
-        low = fmaxf(low, m > -INFINITY ? m - off(c, m) : -INFINITY);
+    if (a.chunks <= 256) {
+        if (tid < a.chunks && cm[tid] > -INFINITY) low = cm[tid] - off(tid, cm[tid]);
+    } else
+#pragma unroll 2
+    for (int c = tid * 4; c < a.chunks; c += THREADS * 4) {
+        const float4 m = *(const float4*)&cm[c];
+        const float g = widest(c >> 4);
+        // (m - d is increasing in m; of -inf it is -inf)
+        const float top = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
+        low = fmaxf(low, top - fmaf(eps, fabsf(top), g));
     }
-    for (int o = 1; o < THREADS / 256; o <<= 1) low = fmaxf(low, __shfl_xor(low, o));
-    if (tid % (THREADS / 256) == 0) best[tid / (THREADS / 256)] = low;
+    if (a.chunks <= 256) {
+        if (tid < 256) best[tid] = low;
+    } else {
+        for (int o = 1; o < THREADS / 256; o <<= 1) low = fmaxf(low, __shfl_xor(low, o));
+        if (tid % (THREADS / 256) == 0) best[tid / (THREADS / 256)] = low;
+    }
     __syncthreads();
     {                                       // the k-th largest of the 256: the largest value with at least k not below it
         float t = -INFINITY;
@@ -735,59 +770,65 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
         __syncthreads();
         if (m == a.k) { full = true; least = cv[m - 1]; }
     };
-    // the rows of a chunk that reach the bound, four at a time; float64 logits of rows
-    auto look = [&](int c, int r0, int r1, int tag) {
+    // the ids of a chunk that reach the bound, four at a time; the float64 logit of an id
+    auto look = [&](int c, int i0, int i1, int tag) {
         const float d = off(c, cm[c]);
 #pragma unroll 4
-        for (int r = r0; r < r1; r += 4) {
-            const int v = c * VS_CHUNK + r + quarter, u = min(v, w.rows - 1);
+        for (int i = i0; i < i1; i += 4) {
+            const int v = vs_chunk_row(c, i + quarter), u = min(v, w.rows - 1);
             const float s = vs_dot16<BF16>(w, u, xs, l16) + vs_bias_of(a.join.bias, u);
             if (l16 == 0 && v == u && s > -INFINITY && s + d >= bound) {
                 const int at = atomicAdd(&n_rows, 1);
-                if (at < VS_CAND) rows[at] = (uint16_t)(tag * VS_CHUNK + r + quarter);
+                if (at < VS_CAND) rows[at] = (uint16_t)(tag * VS_CHUNK + i + quarter);
             }
         }
     };
+    int least_end = 0;                      // ids from here on had no part in `least`: equal ones come after it
+    auto beaten = [&](double s, int v) { return full && (s < least || (s == least && v >= least_end)); };
     auto exact = [&](int v) {
         double s = 0.0;
         for (int q = lane; q < w.dim; q += 64) s = fma((double)xs[q], (double)vs_load(w, v, q), s);
         for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
         s += (double)vs_bias_of(a.join.bias, v);
-        if (lane == 0 && !(full && s <= least)) {
+        if (lane == 0 && !beaten(s, v)) {
             const int at = atomicAdd(&n_cand, 1);
             cv[at] = s; ci[at] = v;
         }
     };
+    auto may = [&](int c, float m) {
+        const float up = m + off(c, m);
+        return m > -INFINITY && up >= bound && !beaten((double)up, (c >> 4) * VS_BLOCK);
+    };
     // every chunk that may hold one of the k: usually a few more than k
-#pragma unroll 4
-    for (int c = tid; c < a.chunks; c += THREADS) {
-        const float m = cm[c];
-        if (m > -INFINITY && m + off(c, m) >= bound) {
-            const int at = atomicAdd(&n_list, 1);
-            if (at < VS_LIST) list[at] = (uint16_t)c;
-        }
+#pragma unroll 2
+    for (int c = tid * 4; c < a.chunks; c += THREADS * 4) {
+        const float4 m = *(const float4*)&cm[c];
+        const float g = widest(c >> 4);
+        const float v[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (v[i] > -INFINITY && v[i] + fmaf(eps, fabsf(v[i]), g) >= bound) {
+                const int at = atomicAdd(&n_list, 1);
+                if (at < VS_LIST) list[at] = (uint16_t)(c + i);
+            }
     }
     __syncthreads();
     bool done = n_list <= VS_LIST;
-    if (done) {                             // all their rows at once, a quarter of a chunk for each wave
+    if (done) {                             // all their ids at once, a chunk for each wave
         const int n = n_list;
-        for (int i = wave; i < n * 4; i += THREADS / 64) look(list[i >> 2], (i & 3) * (VS_CHUNK / 4), ((i & 3) + 1) * (VS_CHUNK / 4), i >> 2);
+        for (int i = wave; i < n; i += THREADS / 64) look(list[i], 0, VS_CHUNK, i);
         __syncthreads();
         done = n_rows <= VS_CAND;
         if (done) {
             const int nr = n_rows;
-            for (int i = wave; i < nr; i += THREADS / 64) exact(list[rows[i] / VS_CHUNK] * VS_CHUNK + rows[i] % VS_CHUNK);
+            for (int i = wave; i < nr; i += THREADS / 64) exact(vs_chunk_row(list[rows[i] / VS_CHUNK], rows[i] % VS_CHUNK));
         }
     }
-    if (!done) {                            // many equal logits: chunk after chunk
+    if (!done) {                            // many equal logits: block after block
         __syncthreads();
         for (int c0 = 0; c0 < a.chunks; c0 += 256) {
             const int c = c0 + tid;
-            bool want = false;
-            if (tid < 256 && c < a.chunks) {
-                const float m = cm[c], up = m + off(c, m);
-                want = m > -INFINITY && up >= bound && !(full && (double)up <= least);
-            }
+            const bool want = tid < 256 && c < a.chunks && may(c, cm[c]);
             const unsigned long long bal = __ballot(want);
             if (lane == 0 && wave < 4) found[wave] = __popcll(bal);
             __syncthreads();
@@ -796,16 +837,17 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
             const int nl = found[0] + found[1] + found[2] + found[3];
             if (want) list[before + __popcll(bal & ((1ull << lane) - 1ull))] = (uint16_t)c;
             __syncthreads();
-            for (int i0 = 0; i0 < nl; i0 += 4) {
+            for (int i0 = 0; i0 < nl; i0 += 16) {
                 if (tid == 0) n_rows = 0;
                 __syncthreads();
-                if (wave < 4 && i0 + wave < nl) look(list[i0 + wave], 0, VS_CHUNK, wave);
+                for (int i = i0 + wave; i < min(i0 + 16, nl); i += THREADS / 64)
+                    if (may(list[i], cm[list[i]])) look(list[i], 0, VS_CHUNK, i - i0);
                 __syncthreads();
                 const int nr = n_rows;
-                for (int i = wave; i < nr; i += THREADS / 64) exact(list[i0 + rows[i] / VS_CHUNK] * VS_CHUNK + rows[i] % VS_CHUNK);
+                for (int i = wave; i < nr; i += THREADS / 64) exact(vs_chunk_row(list[i0 + rows[i] / VS_CHUNK], rows[i] % VS_CHUNK));
                 __syncthreads();
                 const bool crowded = n_cand > VS_CAND - 256;
-                if (crowded) compact();
+                if (crowded) { compact(); least_end = ((list[min(i0 + 15, nl - 1)] >> 4) + 1) * VS_BLOCK; }
                 __syncthreads();
             }
         }

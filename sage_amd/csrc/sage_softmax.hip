@@ -138,7 +138,7 @@ FwdPlan plan_fwd(const Shape& s, void* ws) {
         p.rows = s.n;
         p.tiles = cdiv(s.n, p.raw * 16);
         p.n_pad = p.tiles * p.raw * 16;
-        p.splits = (int)std::min<int64_t>(cdiv(p.chunks, 16), s.cus * 2);
+        p.splits = (int)std::min<int64_t>(blocks, s.cus * 4);     // a wave has 64 ids at least
     } else {
         p.rows = std::min(s.n, VS_ROWS_MAX);
         p.n_pad = up(p.rows, VS_PAD);
