@@ -14,9 +14,13 @@
 // (its 32 summation slots are the 32 streaming rows in the order 16 (j / 4) + 4 (l / 16) + j % 4; the transposed
 // fragments are laid out in that order).
 //
-// bf16 inputs are multiplied as they are (products of two bf16 are exact in float32).  float32 inputs are taken as the sum
-// of three bf16 (8 + 8 + 8 bits: exact), and six of the nine products are formed -- the other three are below 2^-24 of
-// |x||w| --, which costs 6 bf16 MFMAs where the float32 MFMA costs 16 (256 against 4,096 operations per clock and CU).
+// bf16 inputs are multiplied as they are (products of two bf16 are exact in float32).  float32 inputs are taken as the sum of
+// two float16 (11 + 11 bits) and three of the four products are formed; what is left out is 2^-22 of |x||w|, the size of
+// float32's own rounding in a sum of a few terms, and it costs 3 MFMAs where three bf16 parts cost 6 and the float32 MFMA 16
+// (256 against 4,096 operations per clock and CU).  float16's narrow range is met by powers of two, exact in both
+// directions: 32 rows share one that brings their largest element to 2^13, and the weights of a column share one that
+// follows their largest (both below).  Where the weights are read only once (few tokens), the three bf16 parts are formed on
+// the way instead: they need no scale.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -52,101 +56,169 @@ __device__ __forceinline__ float vs_load(const VsSrc& s, int64_t row, int d) {
 // max(a, b) that keeps a NaN (fmaxf would turn a NaN logit into a masked one, and takes an instruction more to do it)
 __device__ __forceinline__ float vs_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-__device__ __forceinline__ vs_f4 vs_mfma(vs_bf8 a, vs_bf8 b, vs_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+// eight 16-bit elements of a fragment: bf16, or float16 where values are in two parts
+typedef uint32_t vs_bits __attribute__((ext_vector_type(4)));
+typedef _Float16 vs_h8 __attribute__((ext_vector_type(8)));
 
-// c[r][t] += a[r] . b[t] for R x TB independent accumulators, both operands in PL parts (largest first): the parts are the
-// outer loop, small products first, so that an accumulator is not needed again right after it was written.
+template <int PL>
+__device__ __forceinline__ vs_f4 vs_mfma(vs_bits a, vs_bits b, vs_f4 c) {
+    if constexpr (PL == 2) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vs_h8, a), __builtin_bit_cast(vs_h8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vs_bf8, a), __builtin_bit_cast(vs_bf8, b), c, 0, 0, 0);
+}
+
+// c[r][t] += a[r] . b[t] for R x TB independent accumulators, both operands in PL parts (largest first): the products are the
+// outer loop, small ones first, so that an accumulator is not needed again right after it was written.
 template <int PL, int R, int TB, class B>
-__device__ __forceinline__ void vs_mfma_parts(const vs_bf8 (&a)[R][PL], const B& b, vs_f4 (&c)[R][TB]) {
+__device__ __forceinline__ void vs_mfma_parts(const vs_bits (&a)[R][PL], const B& b, vs_f4 (&c)[R][TB]) {
     constexpr int pa[6] = {1, 2, 0, 1, 0, 0}, pb[6] = {1, 0, 2, 0, 1, 0};
 #pragma unroll
-    for (int q = PL == 3 ? 0 : 5; q < 6; ++q)
+    for (int q = PL == 3 ? 0 : PL == 2 ? 3 : 5; q < 6; ++q)
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int t = 0; t < TB; ++t) c[r][t] = vs_mfma(a[r][pa[q]], b(t, pb[q]), c[r][t]);
+            for (int t = 0; t < TB; ++t) c[r][t] = vs_mfma<PL>(a[r][pa[q]], b(t, pb[q]), c[r][t]);
 }
 
-// v as the sum of PL bf16 (each rounding to nearest; exact for PL = 3, within 2^-9 |v| for PL = 1), two at a time
+// v as the sum of PL parts, each rounded to nearest: one bf16 (within 2^-9 |v|), two float16 (within 2^-23 |v| if |v| is between
+// 2^-3 and 2^15), three bf16 (exact).  Two elements at a time.
 template <int PL>
-__device__ __forceinline__ void vs_split(vs_f8 v, vs_bf8* out) {
+__device__ __forceinline__ void vs_split(vs_f8 v, vs_bits* out) {
     typedef float f2 __attribute__((ext_vector_type(2)));
     typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int p = 0; p < PL; ++p) {
-        u4 bits;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const f2 pair = {v[2 * i], v[2 * i + 1]};
-            bits[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, b2));
-            if (p + 1 < PL) {
-                v[2 * i] -= __uint_as_float(bits[i] << 16);
-                v[2 * i + 1] -= __uint_as_float(bits[i] & 0xFFFF0000u);
+            if constexpr (PL == 2) {
+                const h2 h = __builtin_convertvector(pair, h2);
+                out[p][i] = __builtin_bit_cast(uint32_t, h);
+                if (p + 1 < PL) { v[2 * i] -= (float)h[0]; v[2 * i + 1] -= (float)h[1]; }
+            } else {
+                const uint32_t u = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, b2));
+                out[p][i] = u;
+                if (p + 1 < PL) { v[2 * i] -= __uint_as_float(u << 16); v[2 * i + 1] -= __uint_as_float(u & 0xFFFF0000u); }
             }
         }
-        out[p] = __builtin_bit_cast(vs_bf8, bits);
     }
 }
 
 // ---- fragments ----------------------------------------------------------------------------------------------------
-// S fragments (16 rows x 32 elements): [row / 16][KS][PL][lane] of 8 bf16, lane l holding row l % 16, elements 8 (l / 16)..
-// T fragments (16 elements x 32 rows): [row / 32][2 KS][PL][lane], lane l holding element l % 16 and the rows in the order
-// 16 (j / 4) + 4 (l / 16) + j % 4.  Rows past the end and elements past `dim` are zero.  One workgroup packs 32 rows.
-// A fragment is one coalesced 1 KiB load of a wave, whatever the caller's row length, stride and alignment are.
+// S fragments (16 rows x 32 elements): [row / 16][KS][PL][lane] of eight elements, lane l holding row l % 16, elements
+// 8 (l / 16).. .  T fragments (16 elements x 32 rows): [row / 32][2 KS][PL][lane], lane l holding element l % 16 and the rows
+// in the order 16 (j / 4) + 4 (l / 16) + j % 4.  Rows past the end and elements past `dim` are zero.  A fragment is one
+// coalesced 1 KiB load of a wave, whatever the caller's row length, stride and alignment are.  One workgroup packs 32 rows:
+// a lane loads the eight elements that its place in an S fragment asks for; T fragments are read back through LDS.
+// PL = 2: the 32 rows are multiplied by 2^e, e such that the largest finite element comes to just under 2^13.
+
+// eight elements from `d` on; zeros past the end of the row
+template <int PL>
+__device__ __forceinline__ vs_f8 vs_eight(const VsSrc& s, int64_t row, int d) {
+    vs_f8 v;
+    if (d + 8 <= s.dim) {
+        if constexpr (PL == 1) {
+            struct __attribute__((packed, aligned(2))) Raw { uint32_t v[4]; };
+            v = __builtin_convertvector(__builtin_bit_cast(vs_bf8, *(const Raw*)((const uint16_t*)s.p + row * s.ld + d)), vs_f8);
+        } else {
+            struct __attribute__((packed, aligned(4))) Raw { float v[8]; };
+            v = __builtin_bit_cast(vs_f8, *(const Raw*)((const float*)s.p + row * s.ld + d));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = d + i < s.dim ? vs_load(s, row, d + i) : 0.0f;
+    }
+    return v;
+}
+
+struct VsPack {
+    VsSrc src;
+    uint4 *S, *T;              // T may be null
+    float* group_max;          // [rows / 32] largest size, or null
+    float* exps;               // PL = 2: e of group g at exps[g * exps_step]
+    int32_t exps_step;
+};
 template <int KS, int PL>
-__global__ __launch_bounds__(256) void k_vs_pack(VsSrc src, uint4* __restrict__ S, uint4* __restrict__ T, float* __restrict__ group_max) {
-    constexpr int DP = KS * 32, LD = DP + 4;
+__global__ __launch_bounds__(256) void k_vs_pack(VsPack a) {
+    constexpr int DP = KS * 32, LD = DP + 4, N = (KS + 1) / 2;      // fragments of a wave
     __shared__ float tile[32 * LD];
-    __shared__ float wmax[4];
+    __shared__ float wmax[4], wfin[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
     const int64_t row0 = (int64_t)blockIdx.x * 32;
-    float big = 0.0f;
-    for (int i = threadIdx.x; i < 32 * DP; i += 256) {
-        const int r = i / DP, d = i % DP;
-        const float v = (row0 + r < src.rows && d < src.dim) ? vs_load(src, row0 + r, d) : 0.0f;
-        tile[r * LD + d] = v;
-        big = fmaxf(big, fabsf(v));
+    vs_f8 v[N];
+    float big = 0.0f, fin = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int f = i * 4 + wave, rb = f / KS, ks = f % KS;
+        const int64_t row = row0 + rb * 16 + col;
+        v[i] = vs_f8(0.0f);
+        if (f < 2 * KS && row < a.src.rows && ks * 32 + quad * 8 < a.src.dim) v[i] = vs_eight<PL>(a.src, row, ks * 32 + quad * 8);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float q = fabsf(v[i][j]);
+            big = fmaxf(big, q);
+            fin = fmaxf(fin, q < INFINITY ? q : 0.0f);
+        }
     }
-    for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o));
-    if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = big;
+    for (int o = 1; o < 64; o <<= 1) { big = fmaxf(big, __shfl_xor(big, o)); fin = fmaxf(fin, __shfl_xor(fin, o)); }
+    if (lane == 0) { wmax[wave] = big; wfin[wave] = fin; }
     __syncthreads();
-    if (group_max && threadIdx.x == 0) group_max[blockIdx.x] = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-    for (int i = threadIdx.x; i < 2 * KS * 64; i += 256) {
-        const int lane = i & 63, f = i >> 6, rb = f / KS, ks = f % KS;
-        const float* at = tile + (rb * 16 + (lane & 15)) * LD + ks * 32 + (lane >> 4) * 8;
-        vs_f8 v;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = at[j];
-        vs_bf8 part[PL];
-        vs_split<PL>(v, part);
-#pragma unroll
-        for (int p = 0; p < PL; ++p)
-            *(vs_bf8*)&S[((((int64_t)blockIdx.x * 2 + rb) * KS + ks) * PL + p) * 64 + lane] = part[p];
+    big = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+    fin = fmaxf(fmaxf(wfin[0], wfin[1]), fmaxf(wfin[2], wfin[3]));
+    int e = 0;
+    if (PL == 2 && fin > 0.0f) e = 13 - __builtin_amdgcn_frexp_expf(fin);
+    if (threadIdx.x == 0) {
+        if (a.group_max) a.group_max[blockIdx.x] = big;
+        if (PL == 2) a.exps[(int64_t)blockIdx.x * a.exps_step] = (float)e;
     }
-    if (!T) return;
-    for (int i = threadIdx.x; i < 2 * KS * 64; i += 256) {
-        const int lane = i & 63, db = i >> 6;
-        vs_f8 v;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = tile[((j >> 2) * 16 + (lane >> 4) * 4 + (j & 3)) * LD + db * 16 + (lane & 15)];
-        vs_bf8 part[PL];
-        vs_split<PL>(v, part);
+    for (int i = 0; i < N; ++i) {
+        const int f = i * 4 + wave, rb = f / KS, ks = f % KS;
+        if (f >= 2 * KS) continue;
+        if (PL == 2)
 #pragma unroll
-        for (int p = 0; p < PL; ++p) *(vs_bf8*)&T[(((int64_t)blockIdx.x * 2 * KS + db) * PL + p) * 64 + lane] = part[p];
+            for (int j = 0; j < 8; ++j) v[i][j] = ldexpf(v[i][j], e);
+        if (a.T) {
+            float* to = tile + (rb * 16 + col) * LD + ks * 32 + quad * 8;
+            *(vs_f4*)to = vs_f4{v[i][0], v[i][1], v[i][2], v[i][3]};
+            *(vs_f4*)(to + 4) = vs_f4{v[i][4], v[i][5], v[i][6], v[i][7]};
+        }
+        vs_bits part[PL];
+        vs_split<PL>(v[i], part);
+#pragma unroll
+        for (int p = 0; p < PL; ++p) *(vs_bits*)&a.S[((((int64_t)blockIdx.x * 2 + rb) * KS + ks) * PL + p) * 64 + lane] = part[p];
+    }
+    if (!a.T) return;
+    __syncthreads();
+    for (int db = wave; db < 2 * KS; db += 4) {
+        vs_f8 q;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = tile[((j >> 2) * 16 + quad * 4 + (j & 3)) * LD + db * 16 + col];
+        vs_bits part[PL];
+        vs_split<PL>(q, part);
+#pragma unroll
+        for (int p = 0; p < PL; ++p) *(vs_bits*)&a.T[(((int64_t)blockIdx.x * 2 * KS + db) * PL + p) * 64 + lane] = part[p];
     }
 }
 
-// The bias of every id, padded to whole chunks: 0 where the caller gives none, -inf past the end (p = 0 there).  A mask of
-// the type's lowest value becomes -inf too: next to it no logit keeps a bit, and float32 could not hold it in powers of two.
-__global__ __launch_bounds__(256) void k_vs_bias(const float* __restrict__ bias, int32_t vocab, int32_t padded, float* __restrict__ out) {
+// What goes with the fragments of 32 ids: their biases (0 where the caller gives none, -inf past the end: p = 0 there), then
+// the exponent of their scale.  A mask of the type's lowest value becomes -inf too: next to it no logit keeps a bit, and
+// float32 could not hold it in powers of two.  PL = 2 keeps the biases in powers of two.
+#define VS_INFO 36
+#define VS_INFO_EXP 32
+__global__ __launch_bounds__(256) void k_vs_bias(const float* __restrict__ bias, float unit, int32_t vocab, int32_t padded, float* __restrict__ info) {
     const int v = blockIdx.x * 256 + threadIdx.x;
-    if (v < padded) out[v] = v >= vocab ? -INFINITY : !bias ? 0.0f : bias[v] <= VS_NOTHING ? -INFINITY : bias[v];
+    if (v < padded) info[(v >> 5) * VS_INFO + (v & 31)] = v >= vocab ? -INFINITY : !bias ? 0.0f : bias[v] <= VS_NOTHING ? -INFINITY : bias[v] * unit;
 }
+
+// 2^n as a factor of log2(e), kept finite (logits beyond float32 are inf or 0 all the same)
+__device__ __forceinline__ float vs_unit(float n) { return ldexpf(VS_LOG2E, (int)fmaxf(fminf(n, 126.0f), -126.0f)); }
 
 // ---- forward ------------------------------------------------------------------------------------------------------
 struct VsFwd {
     const uint4 *xS, *wS;
-    const float* bias;         // [padded vocabulary]
+    const float* info;         // [ids / 32][VS_INFO]
+    const float* x_exp;        // PL = 2: [tokens / 32]
     int32_t has_bias;          // the caller gave one: -inf may stand anywhere (else only past `vocab`)
     int32_t vocab;
     int32_t n_tiles;           // token tiles of 16 TB rows
@@ -184,26 +256,26 @@ struct VsStat {
 
 // 32 streaming rows against the stationary ones: s[rb][t] += w . x
 template <int KS, int PL, int TB>
-__device__ __forceinline__ void vs_product(const uint4* w, const vs_bf8 (&x)[TB][KS][PL], vs_f4 (&s)[2][TB]) {
+__device__ __forceinline__ void vs_product(const uint4* w, const vs_bits (&x)[TB][KS][PL], vs_f4 (&s)[2][TB]) {
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-        vs_bf8 wf[2][PL];
+        vs_bits wf[2][PL];
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
-            for (int p = 0; p < PL; ++p) wf[rb][p] = *(const vs_bf8*)&w[((rb * KS + k) * PL + p) * 64];
+            for (int p = 0; p < PL; ++p) wf[rb][p] = *(const vs_bits*)&w[((rb * KS + k) * PL + p) * 64];
         vs_mfma_parts<PL, 2, TB>(wf, [&](int t, int p) { return x[t][k][p]; }, s);
     }
 }
 
 template <int KS, int PL, int TB>
-__device__ __forceinline__ void vs_stationary(const uint4* S, int64_t tile, int lane, vs_bf8 (&x)[TB][KS][PL]) {
+__device__ __forceinline__ void vs_stationary(const uint4* S, int64_t tile, int lane, vs_bits (&x)[TB][KS][PL]) {
 #pragma unroll
     for (int t = 0; t < TB; ++t)
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int p = 0; p < PL; ++p) x[t][k][p] = *(const vs_bf8*)&S[(((tile * TB + t) * KS + k) * PL + p) * 64 + lane];
+            for (int p = 0; p < PL; ++p) x[t][k][p] = *(const vs_bits*)&S[(((tile * TB + t) * KS + k) * PL + p) * 64 + lane];
 }
 
 template <int TB>
@@ -215,21 +287,30 @@ struct VsRowsOfTile {
 #pragma unroll
         for (int t = 0; t < TB; ++t) { st[t].clear(); top[t] = -INFINITY; }
     }
-    // the logits of 32 ids; MASKED: some may be -inf
-    template <bool MASKED>
-    __device__ __forceinline__ void add(const vs_f4 (&s)[2][TB]) {
+    // the logits of 32 ids, in powers of two after multiplication by unit[t] (and addition of `bias`, if they are SCALED and
+    // MASKED); MASKED: some may be -inf
+    template <bool MASKED, bool SCALED>
+    __device__ __forceinline__ void add(const vs_f4 (&s)[2][TB], const float (&unit)[TB], const vs_f4 (&bias)[2]) {
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
-            float mx = vs_max(vs_max(vs_max(s[0][t][0], s[0][t][1]), s[0][t][2]), vs_max(vs_max(s[0][t][3], s[1][t][0]), s[1][t][1]));
-            mx = vs_max(vs_max(mx, s[1][t][2]), s[1][t][3]);
-            top[t] = vs_max(top[t], mx);
-            mx *= VS_LOG2E;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = s[j >> 2][t][j & 3];
+                if (SCALED && MASKED) v[j] = fmaf(v[j], unit[t], bias[j >> 2][j & 3]);
+            }
+            float mx = vs_max(vs_max(vs_max(v[0], v[1]), v[2]), vs_max(vs_max(v[3], v[4]), v[5]));
+            mx = vs_max(vs_max(mx, v[6]), v[7]);
+            if (!SCALED) top[t] = vs_max(top[t], mx);
+            if (!SCALED) mx *= VS_LOG2E;
+            else if (!MASKED) mx *= unit[t];
+            if (SCALED) top[t] = vs_max(top[t], mx * VS_LN2);
             const bool up = mx > st[t].ref + VS_SLACK;
             if (__any(up)) st[t].move(up ? mx : st[t].ref);
             float ls, le;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float e = fmaf(s[j >> 2][t][j & 3], VS_LOG2E, -st[t].ref);
+                float e = SCALED && MASKED ? v[j] - st[t].ref : fmaf(v[j], SCALED ? unit[t] : VS_LOG2E, -st[t].ref);
                 if (MASKED) e = vs_max(e, VS_TMIN);
                 const float p = __builtin_amdgcn_exp2f(e);
                 ls = j ? ls + p : p;
@@ -281,48 +362,29 @@ struct VsRowsOfTile {
     }
 };
 
-template <int TB>
-__device__ __forceinline__ void vs_bias_init(const float* bias, int lane, vs_f4 (&s)[2][TB]) {
+// 32 ids against a tile: their logits are formed and counted
+template <int KS, int PL, int TB>
+__device__ __forceinline__ void vs_forward_step(const VsFwd& a, int row0, const uint4* w, const float* info, const vs_bits (&x)[TB][KS][PL],
+                                                const float (&x_exp)[TB], VsRowsOfTile<TB>& rows) {
+    const int lane = threadIdx.x & 63, quad = lane >> 4;
+    vs_f4 s[2][TB], b[2];
+    float unit[TB];
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb) {
-        const vs_f4 b = *(const vs_f4*)&bias[rb * 16 + (lane >> 4) * 4];
+        b[rb] = *(const vs_f4*)&info[rb * 16 + quad * 4];
 #pragma unroll
-        for (int t = 0; t < TB; ++t) s[rb][t] = b;
+        for (int t = 0; t < TB; ++t) s[rb][t] = PL == 1 ? b[rb] : vs_f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    const float e = PL == 2 ? info[VS_INFO_EXP] : 0.0f;
+#pragma unroll
+    for (int t = 0; t < TB; ++t) unit[t] = PL == 2 ? vs_unit(-(e + x_exp[t])) : VS_LOG2E;
+    vs_product<KS, PL, TB>(w, x, s);
+    if (a.has_bias || row0 + 32 > a.vocab) rows.template add<true, PL == 2>(s, unit, b);      // the same in the whole grid
+    else rows.template add<false, PL == 2>(s, unit, b);
 }
 
-// The widest float32 rows (a stage would not fit LDS twice): a wave is a tile of 16 TB tokens against one range of the
-// vocabulary and reads its fragments itself.
-template <int KS, int PL, int TB>
-__global__ __launch_bounds__(256, 2) void k_vs_forward(VsFwd a) {
-    const int lane = threadIdx.x & 63;
-    const int unit = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (unit >= a.n_tiles * a.splits) return;
-    const int tile = unit % a.n_tiles, split = unit / a.n_tiles;
-    const int b0 = (int)((int64_t)a.blocks * split / a.splits), b1 = (int)((int64_t)a.blocks * (split + 1) / a.splits);
-    vs_bf8 x[TB][KS][PL];
-    vs_stationary<KS, PL, TB>(a.xS, tile, lane, x);
-    VsRowsOfTile<TB> rows;
-    rows.clear();
-    for (int b = b0; b < b1; ++b) {
-        for (int h = 0; h < 4; ++h) {
-#pragma unroll 1
-            for (int row0 = b * VS_BLOCK + h * 64; row0 < b * VS_BLOCK + (h + 1) * 64; row0 += 32) {
-                vs_f4 s[2][TB];
-                vs_bias_init<TB>(a.bias + row0, lane, s);
-                vs_product<KS, PL, TB>(a.wS + (int64_t)row0 / 16 * KS * PL * 64 + lane, x, s);
-                if (a.has_bias || row0 + 32 > a.vocab) rows.template add<true>(s);      // the same in the whole grid
-                else rows.template add<false>(s);
-            }
-            rows.template chunk<true>(a, tile, b, h, lane, true);
-        }
-        rows.flush();
-    }
-    rows.store(a, tile, split, lane);
-}
-
-// Many tokens: four waves, a tile each, share the streaming rows through LDS.  SR rows at a time are copied straight into
-// LDS (they are packed in the order of the copy) while the SR before them are worked on: one barrier a step.
+// Four waves, a tile each, share the streaming rows through LDS.  SR rows at a time are copied straight into LDS (they are
+// packed in the order of the copy) while the SR before them are worked on: one barrier a step.
 typedef const __attribute__((address_space(1))) void* vs_global_ptr;
 typedef __attribute__((address_space(3))) void* vs_lds_ptr;
 template <int N>               // 16-byte pieces, a multiple of 256
@@ -332,35 +394,34 @@ __device__ __forceinline__ void vs_stage(const uint4* from, uint4* to) {
     for (int i = 0; i < N; i += 256)
         __builtin_amdgcn_global_load_lds((vs_global_ptr)(from + i + wave * 64 + lane), (vs_lds_ptr)(to + i + wave * 64), 16, 0, 0);
 }
-
+template <int N>               // floats, at most 256
+__device__ __forceinline__ void vs_stage_floats(const float* from, float* to) {
+    if (threadIdx.x < N) __builtin_amdgcn_global_load_lds((vs_global_ptr)(from + threadIdx.x), (vs_lds_ptr)(to + (threadIdx.x & ~63)), 4, 0, 0);
+}
 // This wave's copies into LDS have arrived: vmcnt 0, the other counters as they are.
 __device__ __forceinline__ void vs_copies_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
-// A stage: SR rows of fragments and their SR biases.  `to` and `from` are different stages, and the compiler has to know it
-// (__restrict__ through an inlined function): else it waits for the copy under way before each read of LDS.
+// A stage: SR rows of fragments and what goes with them.  `to` and `from` are different stages, and the compiler has to know
+// it (__restrict__ through an inlined function): else it waits for the copy under way before each read of LDS.
 template <int KS, int PL, int SR>
 struct VsStage {
-    static constexpr int N = SR * KS * PL * 4, SIZE = N + SR / 4;
-    static __device__ __forceinline__ void fetch(const uint4* w, const float* bias, uint4* to) {
+    static constexpr int N = SR * KS * PL * 4, INFO = SR / 32 * VS_INFO, SIZE = N + INFO / 4;
+    static __device__ __forceinline__ void fetch(const uint4* w, const float* info, uint4* to) {
         vs_stage<N>(w, to);
-        if (threadIdx.x < SR)
-            __builtin_amdgcn_global_load_lds((vs_global_ptr)(bias + threadIdx.x), (vs_lds_ptr)(to + N + (threadIdx.x & ~63) / 4), 4, 0, 0);
+        vs_stage_floats<INFO>(info, (float*)(to + N));
     }
     template <int TB>
-    static __device__ __forceinline__ void step(const VsFwd& a, int base, bool more, const uint4* __restrict__ next, const float* __restrict__ next_bias,
-                                                uint4* __restrict__ to, const uint4* __restrict__ from, const vs_bf8 (&x)[TB][KS][PL], VsRowsOfTile<TB>& rows, int64_t tile, bool live) {
+    static __device__ __forceinline__ void step(const VsFwd& a, int base, bool more, const uint4* __restrict__ next, const float* __restrict__ next_info,
+                                                uint4* __restrict__ to, const uint4* __restrict__ from, const vs_bits (&x)[TB][KS][PL],
+                                                const float (&x_exp)[TB], VsRowsOfTile<TB>& rows, int64_t tile, bool live) {
         const int lane = threadIdx.x & 63;
         vs_copies_done();                  // (a barrier alone does not wait for them)
         __syncthreads();                   // `from` has arrived, and nobody reads `to` any more
-        if (more) fetch(next, next_bias, to);
+        if (more) fetch(next, next_info, to);
 #pragma unroll 1
         for (int r = 0; r < SR; r += 32) {
             const int row0 = base + r;
-            vs_f4 s[2][TB];
-            vs_bias_init<TB>((const float*)(from + N) + r, lane, s);
-            vs_product<KS, PL, TB>(from + r * KS * PL * 4 + lane, x, s);
-            if (a.has_bias || row0 + 32 > a.vocab) rows.template add<true>(s);
-            else rows.template add<false>(s);
+            vs_forward_step<KS, PL, TB>(a, row0, from + r * KS * PL * 4 + lane, (const float*)(from + N) + r / 32 * VS_INFO, x, x_exp, rows);
             if (row0 & 32) rows.template chunk<true>(a, tile, row0 / VS_BLOCK, (row0 >> 6) & 3, lane, live);
         }
         if (((base + SR) & (VS_BLOCK - 1)) == 0) rows.flush();
@@ -368,7 +429,7 @@ struct VsStage {
 };
 
 template <int KS, int PL, int TB, int SR>
-__global__ __launch_bounds__(256, 2) void k_vs_forward_staged(VsFwd a) {
+__global__ __launch_bounds__(256, 2) void k_vs_forward(VsFwd a) {
     using Stage = VsStage<KS, PL, SR>;
     __shared__ uint4 buf0[Stage::SIZE], buf1[Stage::SIZE];
     const int lane = threadIdx.x & 63;
@@ -376,18 +437,21 @@ __global__ __launch_bounds__(256, 2) void k_vs_forward_staged(VsFwd a) {
     const int tile = (blockIdx.x / a.splits) * 4 + (threadIdx.x >> 6);
     const bool live = tile < a.n_tiles;
     const int row_begin = (int)((int64_t)a.blocks * split / a.splits) * VS_BLOCK, row_end = (int)((int64_t)a.blocks * (split + 1) / a.splits) * VS_BLOCK;
-    vs_bf8 x[TB][KS][PL];
+    vs_bits x[TB][KS][PL];
     vs_stationary<KS, PL, TB>(a.xS, live ? tile : 0, lane, x);
+    float x_exp[TB];
+#pragma unroll
+    for (int t = 0; t < TB; ++t) x_exp[t] = PL == 2 ? a.x_exp[((live ? tile : 0) * TB + t) / 2] : 0.0f;
     VsRowsOfTile<TB> rows;
     rows.clear();
     const uint4* w = a.wS + (int64_t)row_begin * KS * PL * 4;
-    const float* bias = a.bias + row_begin;
-    Stage::fetch(w, bias, buf0);
+    const float* info = a.info + row_begin / 32 * VS_INFO;
+    Stage::fetch(w, info, buf0);
     for (int base = row_begin; base < row_end; base += 2 * SR) {
-        w += SR * KS * PL * 4; bias += SR;
-        Stage::template step<TB>(a, base, true, w, bias, buf1, buf0, x, rows, tile, live);
-        w += SR * KS * PL * 4; bias += SR;
-        Stage::template step<TB>(a, base + SR, base + 2 * SR < row_end, w, bias, buf0, buf1, x, rows, tile, live);
+        w += SR * KS * PL * 4; info += Stage::INFO;
+        Stage::template step<TB>(a, base, true, w, info, buf1, buf0, x, x_exp, rows, tile, live);
+        w += SR * KS * PL * 4; info += Stage::INFO;
+        Stage::template step<TB>(a, base + SR, base + 2 * SR < row_end, w, info, buf0, buf1, x, x_exp, rows, tile, live);
     }
     if (live) rows.store(a, tile, split, lane);
 }
@@ -396,15 +460,6 @@ __global__ __launch_bounds__(256, 2) void k_vs_forward_staged(VsFwd a) {
 __device__ __forceinline__ float vs_bias_of(const float* bias, int64_t v) {
     const float b = bias ? bias[v] : 0.0f;
     return b <= VS_NOTHING ? -INFINITY : b;
-}
-
-// sum over the 16 lanes of a DPP row, in every lane of it
-__device__ __forceinline__ float vs_row_sum(float v) {
-    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, true));    // quad_perm [1,0,3,2]
-    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, true));    // quad_perm [2,3,0,1]
-    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, true));   // row_half_mirror
-    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, true));   // row_mirror
-    return v;
 }
 
 // Few tokens: bound by the one reading of the weights, which are taken as they lie (no packing): a lane loads the eight
@@ -419,7 +474,7 @@ template <> struct VsPiece<1> {            // of bf16: a fragment as it is
         v = __builtin_bit_cast(vs_bf8, *(const Raw*)((const uint16_t*)s.p + row * s.ld + at));
     }
     __device__ __forceinline__ vs_f8 floats() const { return __builtin_convertvector(v, vs_f8); }
-    __device__ __forceinline__ void parts(vs_bf8 (&out)[1]) const { out[0] = v; }
+    __device__ __forceinline__ void parts(vs_bits (&out)[1]) const { out[0] = __builtin_bit_cast(vs_bits, v); }
     typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
     u16x8 most;                            // running largest size: the bits of a bf16 without its sign are ordered
     __device__ __forceinline__ void clear() { most = u16x8(0); }
@@ -440,7 +495,7 @@ template <> struct VsPiece<3> {            // of float32
         for (int i = 0; i < 4; ++i) { v[i] = r.v[i]; v[i + 4] = q.v[i]; }
     }
     __device__ __forceinline__ vs_f8 floats() const { return v; }
-    __device__ __forceinline__ void parts(vs_bf8 (&out)[3]) const { vs_split<3>(v, out); }
+    __device__ __forceinline__ void parts(vs_bits (&out)[3]) const { vs_split<3>(v, out); }
     __device__ __forceinline__ void clear() { v = vs_f8(0.0f); }
     __device__ __forceinline__ void measure(const VsPiece& q) {
 #pragma unroll
@@ -467,7 +522,7 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
     __shared__ float4 red[4][TB * 16];
     const int tile = blockIdx.y;
     int at[KS];
-    vs_bf8 x[TB][KS][PL];
+    vs_bits x[TB][KS][PL];
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
         const int d = k * 32 + quad * 8;
@@ -485,6 +540,7 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
     }
     VsRowsOfTile<TB> rows;
     rows.clear();
+    const float unscaled[TB] = {};
     const int units = gridDim.x * 4, unit = blockIdx.x * 4 + (threadIdx.x >> 6), pieces = a.f.blocks * 4;
     const int c0 = (int)((int64_t)pieces * unit / units), c1 = (int)((int64_t)pieces * (unit + 1) / units);
     for (int c = c0; c < c1; ++c) {
@@ -512,7 +568,7 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
 #pragma unroll
                 for (int k = 0; k < KG; ++k)
                     if (g + k < KS) {
-                        vs_bf8 wf[2][PL];
+                        vs_bits wf[2][PL];
 #pragma unroll
                         for (int rb = 0; rb < 2; ++rb) {
                             big.measure(raw[rb][k]);
@@ -536,8 +592,8 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
                 for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
                 if (lane == 0 && tile == 0) a.group_max[row0 / 32] = m;
             }
-            if (a.bias || row0 + 32 > a.w.rows) rows.template add<true>(s);
-            else rows.template add<false>(s);
+            if (a.bias || row0 + 32 > a.w.rows) rows.template add<true, false>(s, unscaled, b);
+            else rows.template add<false, false>(s, unscaled, b);
         }
         rows.template chunk<false>(a.f, tile, c >> 2, c & 3, lane, true);
         if ((c & 3) == 3) rows.flush();
@@ -662,6 +718,15 @@ struct VsVec {
         }
     }
 };
+
+// sum over the 16 lanes of a DPP row, in every lane of it
+__device__ __forceinline__ float vs_row_sum(float v) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, true));    // quad_perm [1,0,3,2]
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, true));    // quad_perm [2,3,0,1]
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, true));   // row_half_mirror
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, true));   // row_mirror
+    return v;
+}
 
 // x . row over 16 lanes (xs: x in LDS); the result is in all of them.  The last piece of a row that is no whole number of
 // pieces long is taken back from the row's end, with the elements before it weighted 0 -- no read leaves the row.
@@ -862,16 +927,17 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
-// What the gradient kernels read of a row: lse in powers of two, and G = p (A + B e) + gl [v = target], e = log2 p.
-struct VsRow {
-    float* lse2;               // [n_pad]
-    float* A;
-    float* B;
-    float* gl;
-    int32_t* target;
-};
+// What the gradient kernels read of 32 tokens: lse in powers of two (L), and G = p (A + B e) + gl [v = target], e = log2 p;
+// the exponent of their scale last.
+#define VS_TOKEN 164
+#define VS_TOKEN_A 32
+#define VS_TOKEN_B 64
+#define VS_TOKEN_GL 96
+#define VS_TOKEN_TARGET 128
+#define VS_TOKEN_EXP 160
 __global__ __launch_bounds__(256) void k_vs_rows(const float* __restrict__ lse, const float* __restrict__ entropy, const int64_t* __restrict__ targets,
-                                                 const float* __restrict__ g, const float* __restrict__ h, int32_t n, int64_t n_pad, int32_t vocab, VsRow r) {
+                                                 const float* __restrict__ g, const float* __restrict__ h, int32_t n, int64_t n_pad, int32_t vocab,
+                                                 float* __restrict__ tokens) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n_pad) return;
     // rows past the end and rows whose every id is masked: an lse that makes every p 0, whatever the bias is
@@ -894,140 +960,312 @@ __global__ __launch_bounds__(256) void k_vs_rows(const float* __restrict__ lse, 
         if (h && !empty) { A -= h[i] * entropy[i]; B = -h[i] * VS_LN2; }
         A *= fix; B *= fix;
     }
-    r.lse2[i] = l2; r.A[i] = A; r.B[i] = B; r.gl[i] = gl; r.target[i] = t;
+    float* to = tokens + (i >> 5) * VS_TOKEN + (i & 31);
+    to[0] = l2; to[VS_TOKEN_A] = A; to[VS_TOKEN_B] = B; to[VS_TOKEN_GL] = gl; to[VS_TOKEN_TARGET] = __int_as_float(t);
 }
 
 struct VsBwd {
     const uint4 *stayS;        // stationary rows (columns of the product)
     const uint4 *flowS, *flowT;// streaming rows, and transposed
-    const float* bias;         // padded, by id
-    int32_t has_bias, has_entropy;
+    const float* info;         // of ids: [ids / 32][VS_INFO]
+    const float* tokens;       // of tokens: [tokens / 32][VS_TOKEN]
+    int32_t has_bias, has_entropy, want_db;
     int32_t vocab;
-    VsRow row;                 // by token
     int32_t n_tiles, splits, groups;   // groups of 32 streaming rows
     int64_t stay_pad;          // rows of a partial
     float* part;               // [splits][stay_pad][32 KS]
-    float* bias_part;          // [splits][stay_pad] (OF_IDS with a bias gradient)
+    float* bias_part;          // [splits][stay_pad]
 };
 
-// One wave: a tile of 16 TB stationary rows against one range of the streaming ones.  OF_IDS = false: the stationary rows
+// A wave: a tile of 16 TB stationary rows against one range of the streaming ones.  OF_IDS = false: the stationary rows
 // are tokens, the result sum_v p' w_v with p' = p (A + B e), or p alone when there is no entropy gradient (A is then a
 // factor of the whole row, applied at the end); the target's own term is added at the end too, so that the largest
-// coefficient is never rounded to bf16.  OF_IDS = true: the stationary rows are ids, the result sum_n G_nv x_n; the few
-// steps in which a token's target lies in the tile add the rounded-off part of G in a second product.
+// coefficient is never rounded to bf16.  OF_IDS = true: the stationary rows are ids, the result sum_n G_nv x_n; in the few
+// steps in which a token's target lies in the tile, bf16 adds the rounded-off part of G in a second product.
+//
+// Two float16 parts (PL = 2) of a weight: column t is kept multiplied by 2^sg[t], sg as large as the largest weight of the column
+// so far allows (2^15 after the streaming rows' scale), and the sums with it.  It starts high and falls a few times.
 template <int KS, int PL, int TB, bool OF_IDS>
-__global__ __launch_bounds__(256) void k_vs_backward(VsBwd a) {
-    constexpr int DP = KS * 32;
-    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-    const int unit = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (unit >= a.n_tiles * a.splits) return;
-    const int tile = unit % a.n_tiles, split = unit / a.n_tiles;
-    const int g0 = (int)((int64_t)a.groups * split / a.splits), g1 = (int)((int64_t)a.groups * (split + 1) / a.splits);
-    const int64_t stay0 = (int64_t)tile * TB * 16;
-    vs_bf8 y[TB][KS][PL];
-    vs_stationary<KS, PL, TB>(a.stayS, tile, lane, y);
-    float lse2[TB], A[TB], B[TB], b0[TB], db[TB];
-#pragma unroll
-    for (int t = 0; t < TB; ++t) {
-        const int64_t r = stay0 + t * 16 + col;
-        if constexpr (OF_IDS) { b0[t] = a.bias[r]; db[t] = 0.0f; }
-        else { lse2[t] = a.row.lse2[r]; A[t] = a.row.A[r]; B[t] = a.row.B[r]; }
-    }
+struct VsGrad {
+    static constexpr float MOST = 15.0f, AIM = 13.0f;
+    vs_bits y[TB][KS][PL];
     vs_f4 acc[2 * KS][TB];
+    float L[TB], A[TB], B[TB], db[TB], y_exp[TB], sg[TB], norm[TB];   // (of ids, L is the bias)
+    int64_t stay0;
+
+    __device__ __forceinline__ void start(const VsBwd& a, int64_t tile, int lane) {
+        vs_stationary<KS, PL, TB>(a.stayS, tile, lane, y);
+        stay0 = tile * TB * 16;
 #pragma unroll
-    for (int d = 0; d < 2 * KS; ++d)
-#pragma unroll
-        for (int t = 0; t < TB; ++t) acc[d][t] = vs_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int g = g0; g < g1; ++g) {
-        const int row0 = g * 32;
-        vs_f4 s[2][TB];
-        const bool biased = a.has_bias || (OF_IDS ? stay0 + TB * 16 > a.vocab : row0 + 32 > a.vocab);
-#pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
-            vs_f4 b = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (!OF_IDS && biased) b = *(const vs_f4*)&a.bias[row0 + rb * 16 + quad * 4];
-#pragma unroll
-            for (int t = 0; t < TB; ++t) {
-                if constexpr (OF_IDS) s[rb][t] = vs_f4{b0[t], b0[t], b0[t], b0[t]};
-                else s[rb][t] = b;
+        for (int t = 0; t < TB; ++t) {
+            const int64_t r = stay0 + t * 16 + (lane & 15);
+            db[t] = 0.0f; sg[t] = 300.0f; norm[t] = 0.0f;
+            if constexpr (OF_IDS) {
+                const float* of = a.info + (r >> 5) * VS_INFO;
+                L[t] = of[r & 31];
+                y_exp[t] = PL == 2 ? of[VS_INFO_EXP] : 0.0f;
+            } else {
+                const float* of = a.tokens + (r >> 5) * VS_TOKEN;
+                L[t] = of[r & 31]; A[t] = of[VS_TOKEN_A + (r & 31)]; B[t] = of[VS_TOKEN_B + (r & 31)];
+                y_exp[t] = PL == 2 ? of[VS_TOKEN_EXP] : 0.0f;
+                if (PL == 2 && a.has_entropy) {      // |A + B e| brought below 1
+                    const float size = fabsf(A[t]) + fabsf(B[t]) * 256.0f;
+                    norm[t] = size > 0.0f && size < INFINITY ? (float)__builtin_amdgcn_frexp_expf(size) : 0.0f;
+                    A[t] = ldexpf(A[t], -(int)norm[t]);
+                    B[t] = ldexpf(B[t], -(int)norm[t]);
+                }
             }
         }
-        vs_product<KS, PL, TB>(a.flowS + (int64_t)g * 2 * KS * PL * 64 + lane, y, s);
-        vs_f4 L[2], rA[2], rB[2];
+#pragma unroll
+        for (int d = 0; d < 2 * KS; ++d)
+#pragma unroll
+            for (int t = 0; t < TB; ++t) acc[d][t] = vs_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // column t gives up the powers of two that its lanes ask for (`ask` <= 0: none)
+    __device__ __forceinline__ void lower(int t, float ask) {
+        ask = fmaxf(ask, __shfl_xor(ask, 16));
+        ask = fmaxf(ask, __shfl_xor(ask, 32));
+        if (!(ask > 0.0f)) ask = 0.0f;
+        sg[t] -= ask;
+#pragma unroll
+        for (int d = 0; d < 2 * KS; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[d][t][i] = ldexpf(acc[d][t][i], -(int)ask);
+    }
+
+    // P: the weights of the 32 streaming rows from row0 on, in parts; R: what bf16 rounds off
+    __device__ __forceinline__ bool weights(const VsBwd& a, int row0, const uint4* S, const float* of, vs_bits (&P)[TB][PL], vs_bits (&R)[TB]) {
+        const int lane = threadIdx.x & 63, quad = lane >> 4;
+        const bool masked = a.has_bias || (OF_IDS ? stay0 + TB * 16 > a.vocab : row0 + 32 > a.vocab);
+        vs_f4 s[2][TB], b[2];
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+            if constexpr (!OF_IDS) b[rb] = *(const vs_f4*)&of[rb * 16 + quad * 4];
+#pragma unroll
+            for (int t = 0; t < TB; ++t) {
+                if constexpr (PL == 2) s[rb][t] = vs_f4{0.0f, 0.0f, 0.0f, 0.0f};
+                else if constexpr (OF_IDS) s[rb][t] = vs_f4{L[t], L[t], L[t], L[t]};
+                else s[rb][t] = b[rb];
+            }
+        }
+        const float f_exp = PL == 2 ? of[OF_IDS ? VS_TOKEN_EXP : VS_INFO_EXP] : 0.0f;
+        vs_product<KS, PL, TB>(S, y, s);
         bool hit = false;
+        if constexpr (OF_IDS) {
+            const int target = __float_as_int(of[VS_TOKEN_TARGET + (lane & 31)]);
+            hit = __any(target >= stay0 && target < stay0 + TB * 16);
+        }
+        if (masked) { if (a.has_entropy) form<true, true>(a, row0, of, f_exp, s, b, hit, P, R); else form<true, false>(a, row0, of, f_exp, s, b, hit, P, R); }
+        else { if (a.has_entropy) form<false, true>(a, row0, of, f_exp, s, b, hit, P, R); else form<false, false>(a, row0, of, f_exp, s, b, hit, P, R); }
+        return hit;
+    }
+
+    template <bool MASKED, bool ENTROPY>
+    __device__ __forceinline__ void form(const VsBwd& a, int row0, const float* of, float f_exp, const vs_f4 (&s)[2][TB], const vs_f4 (&b)[2], bool hit,
+                                         vs_bits (&P)[TB][PL], vs_bits (&R)[TB]) {
+        const int lane = threadIdx.x & 63, quad = lane >> 4;
+        vs_f4 rl[2], ra[2], rb_[2];
         if constexpr (OF_IDS) {
 #pragma unroll
             for (int rb = 0; rb < 2; ++rb) {
-                L[rb] = *(const vs_f4*)&a.row.lse2[row0 + rb * 16 + quad * 4];
-                rA[rb] = *(const vs_f4*)&a.row.A[row0 + rb * 16 + quad * 4];
-                if (a.has_entropy) rB[rb] = *(const vs_f4*)&a.row.B[row0 + rb * 16 + quad * 4];
+                rl[rb] = *(const vs_f4*)&of[rb * 16 + quad * 4];
+                ra[rb] = *(const vs_f4*)&of[VS_TOKEN_A + rb * 16 + quad * 4];
+                if (ENTROPY) rb_[rb] = *(const vs_f4*)&of[VS_TOKEN_B + rb * 16 + quad * 4];
             }
-            const int64_t t = a.row.target[row0 + (lane & 31)];
-            hit = __any(t >= stay0 && t < stay0 + TB * 16);
         }
-        vs_bf8 P[TB][PL], R[TB];
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
             vs_f8 G;
-#pragma unroll
-            for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float e = fmaf(s[rb][t][i], VS_LOG2E, OF_IDS ? -L[rb][i] : -lse2[t]);
-                    if (biased) e = vs_max(e, VS_TMIN);
-                    float q = __builtin_amdgcn_exp2f(e);
-                    if constexpr (OF_IDS) q *= a.has_entropy ? fmaf(rB[rb][i], e, rA[rb][i]) : rA[rb][i];
-                    else if (a.has_entropy) q *= fmaf(B[t], e, A[t]);
-                    G[rb * 4 + i] = q;
-                }
+            const float unit = PL == 2 ? vs_unit(-(f_exp + y_exp[t])) : VS_LOG2E;
             if constexpr (OF_IDS) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float e = fmaf(s[j >> 2][t][j & 3], unit, -rl[j >> 2][j & 3]);
+                    if (PL == 2 && MASKED) e += L[t];
+                    if (MASKED) e = vs_max(e, VS_TMIN);
+                    const float p = __builtin_amdgcn_exp2f(e);
+                    G[j] = p * (ENTROPY ? fmaf(rb_[j >> 2][j & 3], e, ra[j >> 2][j & 3]) : ra[j >> 2][j & 3]);
+                }
                 if (hit) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int at = row0 + (j >> 2) * 16 + quad * 4 + (j & 3);
-                        if (a.row.target[at] == (int32_t)(stay0 + t * 16 + col)) G[j] += a.row.gl[at];
+                        const int at = (j >> 2) * 16 + quad * 4 + (j & 3);
+                        if (__float_as_int(of[VS_TOKEN_TARGET + at]) == (int32_t)(stay0 + t * 16 + (lane & 15))) G[j] += of[VS_TOKEN_GL + at];
                     }
                 }
-                if (a.bias_part)
+                if (a.want_db) db[t] += ((G[0] + G[1]) + (G[2] + G[3])) + ((G[4] + G[5]) + (G[6] + G[7]));
+                if constexpr (PL == 2) {
+                    float m = fmaxf(fmaxf(fmaxf(fabsf(G[0]), fabsf(G[1])), fabsf(G[2])), fmaxf(fmaxf(fabsf(G[3]), fabsf(G[4])), fabsf(G[5])));
+                    m = fmaxf(fmaxf(m, fabsf(G[6])), fabsf(G[7]));
+                    const float x = m > 0.0f ? (float)__builtin_amdgcn_frexp_expf(m) + sg[t] - f_exp : 0.0f;
+                    if (__any(x > MOST)) lower(t, x - AIM);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) db[t] += G[j];
+                    for (int j = 0; j < 8; ++j) G[j] = ldexpf(G[j], (int)(sg[t] - f_exp));
+                }
+            } else if constexpr (PL == 2) {
+                float e[8];
+                auto exponents = [&]() {
+                    const float k = (sg[t] - f_exp) - L[t];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        e[j] = fmaf(s[j >> 2][t][j & 3], unit, k);
+                        if (MASKED) e[j] = vs_max(e[j] + b[j >> 2][j & 3], VS_TMIN);
+                    }
+                };
+                exponents();
+                const float m = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
+                if (__any(m > MOST)) { lower(t, ceilf(m - AIM)); exponents(); }
+                const float a2 = ENTROPY ? fmaf(-B[t], sg[t] - f_exp, A[t]) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    G[j] = __builtin_amdgcn_exp2f(e[j]);
+                    if (ENTROPY) G[j] *= fmaf(B[t], e[j], a2);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float e = fmaf(s[j >> 2][t][j & 3], VS_LOG2E, -L[t]);
+                    if (MASKED) e = vs_max(e, VS_TMIN);
+                    G[j] = __builtin_amdgcn_exp2f(e);
+                    if (ENTROPY) G[j] *= fmaf(B[t], e, A[t]);
+                }
             }
             vs_split<PL>(G, P[t]);
-            if (OF_IDS && PL == 1) R[t] = __builtin_convertvector(G - __builtin_convertvector(P[t][0], vs_f8), vs_bf8);
-        }
-        const uint4* ft = a.flowT + (int64_t)g * 2 * KS * PL * 64 + lane;
-#pragma unroll
-        for (int d = 0; d < 2 * KS; d += 2) {
-            vs_bf8 wf[2][PL];
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-                for (int p = 0; p < PL; ++p) wf[r][p] = *(const vs_bf8*)&ft[((d + r) * PL + p) * 64];
-            vs_mfma_parts<PL, 2, TB>(wf, [&](int t, int p) { return P[t][p]; }, *(vs_f4(*)[2][TB]) & acc[d]);
-        }
-        if (OF_IDS && PL == 1 && hit) {
-#pragma unroll
-            for (int d = 0; d < 2 * KS; ++d) {
-                const vs_bf8 wf = *(const vs_bf8*)&ft[d * 64];
-#pragma unroll
-                for (int t = 0; t < TB; ++t) acc[d][t] = vs_mfma(wf, R[t], acc[d][t]);
+            if (OF_IDS && PL == 1 && hit) {
+                const vs_f8 r = G - __builtin_convertvector(__builtin_bit_cast(vs_bf8, P[t][0]), vs_f8);
+                vs_split<1>(r, &R[t]);
             }
         }
     }
+
+    __device__ __forceinline__ void products(const uint4* T, const vs_bits (&P)[TB][PL], const vs_bits (&R)[TB], bool hit) {
 #pragma unroll
-    for (int t = 0; t < TB; ++t) {
-        const int64_t r = stay0 + t * 16 + col;
-        float* out = a.part + ((int64_t)split * a.stay_pad + r) * DP;
+        for (int d = 0; d < 2 * KS; d += 2) {
+            vs_bits f[2][PL];
 #pragma unroll
-        for (int d = 0; d < 2 * KS; ++d) *(vs_f4*)&out[d * 16 + quad * 4] = acc[d][t];
-        if constexpr (OF_IDS) {
-            if (a.bias_part) {
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int p = 0; p < PL; ++p) f[r][p] = *(const vs_bits*)&T[((d + r) * PL + p) * 64];
+            vs_mfma_parts<PL, 2, TB>(f, [&](int t, int p) { return P[t][p]; }, *(vs_f4(*)[2][TB]) & acc[d]);
+            if (OF_IDS && PL == 1)
+                if (hit) vs_mfma_parts<PL, 2, TB>(f, [&](int t, int) { return R[t]; }, *(vs_f4(*)[2][TB]) & acc[d]);
+        }
+    }
+
+    __device__ __forceinline__ void store(const VsBwd& a, int split, int lane) {
+        const int col = lane & 15, quad = lane >> 4;
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
+            const int64_t r = stay0 + t * 16 + col;
+            float* out = a.part + ((int64_t)split * a.stay_pad + r) * (KS * 32);
+#pragma unroll
+            for (int d = 0; d < 2 * KS; ++d) {
+                vs_f4 v = acc[d][t];
+                if (PL == 2)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = ldexpf(v[i], (int)(norm[t] - sg[t]));
+                *(vs_f4*)&out[d * 16 + quad * 4] = v;
+            }
+            if (OF_IDS && a.want_db) {
                 float v = db[t] + __shfl_xor(db[t], 16);
                 v += __shfl_xor(v, 32);
                 if (quad == 0) a.bias_part[(int64_t)split * a.stay_pad + r] = v;
             }
         }
     }
+};
+
+// The stages in LDS.  TURNS = false: SR rows with both their fragments at a time, two stages (one worked on, one under way).
+// TURNS = true (wide rows): 32 rows, their S and their T fragments by turns, each under way while the other is worked on.
+template <int KS, int PL, int SR, bool OF_IDS>
+struct VsGradStage {
+    static constexpr int HALF = SR * KS * PL * 4, INFO = (OF_IDS ? VS_TOKEN : VS_INFO), INFOS = SR / 32 * INFO;
+    static constexpr int SIZE = 2 * HALF + (INFOS + 3) / 4;
+    static __device__ __forceinline__ void fetch(const uint4* S, const uint4* T, const float* info, uint4* to) {
+        vs_stage<HALF>(S, to);
+        vs_stage<HALF>(T, to + HALF);
+#pragma unroll
+        for (int i = 0; i < SR / 32; ++i) vs_stage_floats<INFO>(info + i * INFO, (float*)(to + 2 * HALF) + i * INFO);
+    }
+    template <int TB>
+    static __device__ __forceinline__ void step(const VsBwd& a, int base, bool more, const uint4* __restrict__ S, const uint4* __restrict__ T,
+                                                const float* __restrict__ info, uint4* __restrict__ to, const uint4* __restrict__ from,
+                                                VsGrad<KS, PL, TB, OF_IDS>& g) {
+        const int lane = threadIdx.x & 63;
+        vs_copies_done();
+        __syncthreads();
+        if (more) fetch(S, T, info, to);
+#pragma unroll 1
+        for (int r = 0; r < SR; r += 32) {
+            vs_bits P[TB][PL], R[TB];
+            const bool hit = g.weights(a, base + r, from + r * KS * PL * 4 + lane, (const float*)(from + 2 * HALF) + r / 32 * INFO, P, R);
+            g.products(from + HALF + r * KS * PL * 4 + lane, P, R, hit);
+        }
+    }
+    // by turns
+    static __device__ __forceinline__ void fetch_s(const uint4* S, const float* info, uint4* to) {
+        vs_stage<HALF>(S, to);
+        vs_stage_floats<INFO>(info, (float*)(to + HALF));
+    }
+    template <int TB>
+    static __device__ __forceinline__ bool turn_s(const VsBwd& a, int base, const uint4* __restrict__ T, uint4* __restrict__ to, const uint4* __restrict__ from,
+                                                  VsGrad<KS, PL, TB, OF_IDS>& g, vs_bits (&P)[TB][PL], vs_bits (&R)[TB]) {
+        vs_copies_done();
+        __syncthreads();
+        vs_stage<HALF>(T, to);
+        return g.weights(a, base, from + (threadIdx.x & 63), (const float*)(from + HALF), P, R);
+    }
+    template <int TB>
+    static __device__ __forceinline__ void turn_t(bool more, const uint4* __restrict__ S, const float* __restrict__ info, uint4* __restrict__ to,
+                                                  const uint4* __restrict__ from, VsGrad<KS, PL, TB, OF_IDS>& g, const vs_bits (&P)[TB][PL],
+                                                  const vs_bits (&R)[TB], bool hit) {
+        vs_copies_done();
+        __syncthreads();
+        if (more) fetch_s(S, info, to);
+        g.products(from + (threadIdx.x & 63), P, R, hit);
+    }
+};
+
+template <int KS, int PL, int TB, int SR, bool TURNS, bool OF_IDS>
+__global__ __launch_bounds__(256, TB * KS * (4 * PL + 8) > 170 ? 1 : 2) void k_vs_backward(VsBwd a) {
+    using Stage = VsGradStage<KS, PL, SR, OF_IDS>;
+    constexpr int SIZE0 = TURNS ? Stage::HALF + (Stage::INFO + 3) / 4 : Stage::SIZE, SIZE1 = TURNS ? Stage::HALF : Stage::SIZE;
+    __shared__ uint4 buf0[SIZE0], buf1[SIZE1];
+    constexpr int PIECE = KS * PL * 4;         // 16-byte pieces of a row's fragments
+    const int lane = threadIdx.x & 63;
+    const int split = blockIdx.x % a.splits;
+    const int tile = (blockIdx.x / a.splits) * 4 + (threadIdx.x >> 6);
+    const bool live = tile < a.n_tiles;
+    VsGrad<KS, PL, TB, OF_IDS> g;
+    g.start(a, live ? tile : 0, lane);
+    const float* info = OF_IDS ? a.tokens : a.info;
+    if constexpr (TURNS) {
+        const int row_begin = (int)((int64_t)a.groups * split / a.splits) * 32, row_end = (int)((int64_t)a.groups * (split + 1) / a.splits) * 32;
+        const uint4 *S = a.flowS + (int64_t)row_begin * PIECE, *T = a.flowT + (int64_t)row_begin * PIECE;
+        info += (int64_t)row_begin / 32 * Stage::INFO;
+        Stage::fetch_s(S, info, buf0);
+        for (int base = row_begin; base < row_end; base += 32) {
+            vs_bits P[TB][PL], R[TB];
+            const bool hit = Stage::template turn_s<TB>(a, base, T, buf1, buf0, g, P, R);
+            S += 32 * PIECE; T += 32 * PIECE; info += Stage::INFO;
+            Stage::template turn_t<TB>(base + 32 < row_end, S, info, buf0, buf1, g, P, R, hit);
+        }
+    } else {
+        const int units = a.groups / (SR / 32);
+        const int row_begin = (int)((int64_t)units * split / a.splits) * SR, row_end = (int)((int64_t)units * (split + 1) / a.splits) * SR;
+        const uint4 *S = a.flowS + (int64_t)row_begin * PIECE, *T = a.flowT + (int64_t)row_begin * PIECE;
+        info += (int64_t)row_begin / 32 * Stage::INFO;
+        Stage::fetch(S, T, info, buf0);
+        for (int base = row_begin; base < row_end; base += 2 * SR) {
+            S += SR * PIECE; T += SR * PIECE; info += Stage::INFOS;
+            Stage::template step<TB>(a, base, base + SR < row_end, S, T, info, buf1, buf0, g);
+            if (base + SR >= row_end) break;
+            S += SR * PIECE; T += SR * PIECE; info += Stage::INFOS;
+            Stage::template step<TB>(a, base + SR, base + 2 * SR < row_end, S, T, info, buf0, buf1, g);
+        }
+    }
+    if (live) g.store(a, split, lane);
 }
 
 // Sums the partials of a row in a fixed order and writes it: dx = A sum p w + gl w_t (without an entropy gradient; with
@@ -1037,7 +1275,7 @@ struct VsSum {
     const float* bias_part;
     int32_t rows, dim, dp, splits;
     int64_t pad;
-    VsRow row;                 // of tokens: null pointers for dw
+    const float* tokens;       // of tokens; null for dw
     int32_t has_entropy;
     VsSrc w;
     void* out;
@@ -1061,11 +1299,13 @@ __global__ __launch_bounds__(256) void k_vs_sum(VsSum a) {
     const int d = (int)(i % a.dim);
     float v = 0.0f;
     for (int s = 0; s < a.splits; ++s) v += a.part[((int64_t)s * a.pad + r) * a.dp + d];
-    if (a.row.A) {
-        if (!a.has_entropy) v *= a.row.A[r];
-        const int32_t t = a.row.target[r];
-        if (t >= 0) v = fmaf(a.row.gl[r], vs_load(a.w, t, d), v);
-        else if (a.row.gl[r] != a.row.gl[r]) v = a.row.gl[r];
+    if (a.tokens) {
+        const float* of = a.tokens + (r >> 5) * VS_TOKEN + (r & 31);
+        if (!a.has_entropy) v *= of[VS_TOKEN_A];
+        const int32_t t = __float_as_int(of[VS_TOKEN_TARGET]);
+        const float gl = of[VS_TOKEN_GL];
+        if (t >= 0) v = fmaf(gl, vs_load(a.w, t, d), v);
+        else if (gl != gl) v = gl;
     }
     vs_store(a.out, r * a.ldo + d, v, a.out_bf16);
 }

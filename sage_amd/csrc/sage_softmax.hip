@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <utility>
@@ -58,12 +59,17 @@ int vs_steps(int dim) {
     return 0;
 }
 
-// 16-row blocks of stationary rows a wave holds
-constexpr int vs_fwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 4 ? 4 : 2) : (ks <= 4 ? 2 : 1); }
-constexpr int vs_bwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 2 ? 4 : ks <= 8 ? 2 : 1) : (ks <= 4 ? 2 : 1); }
-
-// streaming rows of a stage of the forward kernel: two stages of at most 60 KiB (0: too wide, the waves read for themselves)
-constexpr int vs_stage_rows(int ks, int pl) { return ks * pl <= 4 ? 128 : ks * pl <= 8 ? 64 : ks * pl <= 30 ? 32 : 0; }
+// How each width runs.  ks: 32-element steps of the padded row; pl: parts of a packed element (1 bf16, 2 float32).
+// 16-row blocks of stationary rows a wave holds: as many as leave two waves to a SIMD
+constexpr int vs_fwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 4 ? 4 : 2) : (ks <= 2 ? 4 : ks <= 8 ? 2 : 1); }
+constexpr int vs_bwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 2 ? 4 : ks <= 8 ? 2 : 1) : (ks <= 2 ? 4 : ks <= 4 ? 2 : 1); }
+// streaming rows of a stage: two stages of 16 to 64 KiB
+constexpr int vs_fwd_rows(int ks, int pl) { return ks * pl <= 2 ? 128 : ks * pl <= 8 ? 64 : 32; }
+constexpr int vs_bwd_rows(int ks, int pl) { return ks * pl <= 4 ? 64 : 32; }
+constexpr bool vs_bwd_turns(int ks, int) { return ks >= 8; }
+// 16-token blocks of a wave that reads the weights as they lie (the three bf16 parts of float32 are formed there)
+constexpr int vs_raw_parts(int pl) { return pl == 1 ? 1 : 3; }
+constexpr int vs_raw_most(int ks, int pl) { return ks * vs_raw_parts(pl) <= 10 ? 2 : 1; }
 
 #define VS_BY_WIDTH(ks, pl, F)                                                        \
     do {                                                                              \
@@ -77,11 +83,11 @@ constexpr int vs_stage_rows(int ks, int pl) { return ks * pl <= 4 ? 128 : ks * p
             }                                                                         \
         } else {                                                                      \
             switch (ks) {                                                             \
-            case 2: { F(2, 3); break; }                                               \
-            case 4: { F(4, 3); break; }                                               \
-            case 8: { F(8, 3); break; }                                               \
-            case 10: { F(10, 3); break; }                                             \
-            default: { F(16, 3); break; }                                             \
+            case 2: { F(2, 2); break; }                                               \
+            case 4: { F(4, 2); break; }                                               \
+            case 8: { F(8, 2); break; }                                               \
+            case 10: { F(10, 2); break; }                                             \
+            default: { F(16, 2); break; }                                             \
             }                                                                         \
         }                                                                             \
     } while (0)
@@ -91,8 +97,37 @@ struct Shape {
     int dim, ks, pl, k, cus;
 };
 
-// 16-token blocks of a wave that reads the weights as they lie: one, or two where registers allow and tokens are there
-constexpr int vs_raw_most(int ks, int pl) { return ks * pl <= 10 ? 2 : 1; }
+template <int KS, int PL> constexpr auto vs_fwd_kernel = &k_vs_forward<KS, PL, vs_fwd_blocks(KS, PL), vs_fwd_rows(KS, PL)>;
+template <int KS, int PL, bool OF_IDS>
+constexpr auto vs_bwd_kernel = &k_vs_backward<KS, PL, vs_bwd_blocks(KS, PL), vs_bwd_rows(KS, PL), vs_bwd_turns(KS, PL), OF_IDS>;
+
+// workgroups of a kernel that a CU holds at once (the same on every gfx950)
+template <auto KERNEL>
+int per_cu() {
+    static std::atomic<int> cached{0};
+    int n = cached.load(std::memory_order_relaxed);
+    if (!n) {
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, 256, 0) != hipSuccess || n < 1) n = 1;
+        cached.store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// Into how many ranges the streaming axis (of `units` pieces) is cut, for `groups` workgroups along the other: the number that
+// ends soonest if the chip works `resident` workgroups off at a time, each as long as its pieces and `cost` more to start
+// and end (the loading of its stationary rows; for the gradients the writing and adding of its sums too).
+int vs_splits(int64_t resident, int64_t groups, int64_t units, double cost) {
+    const int64_t most = std::min(units, std::max<int64_t>(1, 4 * resident / groups));
+    int64_t best = 1;
+    double least = 1e300;
+    for (int64_t s = 1; s <= most; ++s) {
+        const double t = (double)((groups * s + resident - 1) / resident) * ((double)((units + s - 1) / s) + cost);
+        if (t < least) { least = t; best = s; }
+    }
+    return (int)best;
+}
+
+// Token blocks of a wave that reads the weights as they lie: one, or two where registers allow and tokens are there
 int vs_raw_blocks(const Shape& s) {
     if (s.n > VS_RAW || s.dim < 8) return 0;
     int most = 1;
@@ -102,35 +137,18 @@ int vs_raw_blocks(const Shape& s) {
     return s.n <= 16 ? 1 : most;
 }
 
-int vs_block_rows(const Shape& s, bool fwd) {
-    int tb = 1;
-#define VS_F(KS, PL) tb = fwd ? vs_fwd_blocks(KS, PL) : vs_bwd_blocks(KS, PL)
-    VS_BY_WIDTH(s.ks, s.pl, VS_F);
-#undef VS_F
-    return tb * 16;
-}
-
-// ranges that `flow` streaming units are cut into so that tiles x ranges fill the chip: 4 waves a workgroup, two
-// workgroups a CU
-int vs_splits(const Shape& s, int64_t tiles, int64_t flow, int64_t most) {
-    const int64_t want = cdiv((int64_t)s.cus * 8, tiles);
-    return (int)std::max<int64_t>(1, std::min(std::min(want, flow), most));
-}
-
 struct FwdPlan {
     int64_t rows, n_pad, tiles, chunks;
     int splits;
     int raw;                    // 16-token blocks of a tile of k_vs_forward_raw (0: the weights are packed)
-    bool staged;
     uint4 *xS, *wS;
-    float *bias, *group_max, *chunk_max;
+    float *info, *x_exp, *group_max, *chunk_max;
     float4* part;
     int64_t bytes;
 };
 FwdPlan plan_fwd(const Shape& s, void* ws) {
     FwdPlan p{};
     Arena a{(char*)ws};
-    const int br = vs_block_rows(s, true);
     const int64_t blocks = s.vp / VS_BLOCK, frag = (int64_t)s.ks * s.pl * 64;          // uint4 of a 16-row block
     p.chunks = s.vp / VS_CHUNK;
     p.raw = vs_raw_blocks(s);
@@ -142,12 +160,15 @@ FwdPlan plan_fwd(const Shape& s, void* ws) {
     } else {
         p.rows = std::min(s.n, VS_ROWS_MAX);
         p.n_pad = up(p.rows, VS_PAD);
-        p.tiles = cdiv(p.rows, br);
-        p.staged = vs_stage_rows(s.ks, s.pl) > 0;
-        p.splits = p.staged ? (int)std::min<int64_t>(blocks, cdiv((int64_t)s.cus * 4, cdiv(p.tiles, 4))) : vs_splits(s, p.tiles, blocks, 1 << 20);
+        int64_t resident = s.cus;
+#define VS_F(KS, PL) p.tiles = cdiv(p.rows, vs_fwd_blocks(KS, PL) * 16); resident *= per_cu<vs_fwd_kernel<KS, PL>>()
+        VS_BY_WIDTH(s.ks, s.pl, VS_F);
+#undef VS_F
+        p.splits = vs_splits(resident, cdiv(p.tiles, 4), blocks, 1.0);
         p.wS = a.take<uint4>(s.vp / 16 * frag);
         p.xS = a.take<uint4>(p.n_pad / 16 * frag);
-        p.bias = a.take<float>(s.vp);
+        p.info = a.take<float>(s.vp / 32 * VS_INFO);
+        p.x_exp = a.take<float>(p.n_pad / 32);
     }
     p.group_max = a.take<float>(s.vp / 32);
     p.part = a.take<float4>(p.splits * p.n_pad);
@@ -160,33 +181,32 @@ struct BwdPlan {
     int64_t np, tiles_x, tiles_w;
     int splits_x, splits_w;
     uint4 *xS, *xT, *wS, *wT;
-    float *bias, *part, *bias_part;
-    VsRow row;
+    float *info, *tokens, *part, *bias_part;
     int64_t bytes;
 };
-BwdPlan plan_bwd(const Shape& s, bool with_bias, void* ws) {
+BwdPlan plan_bwd(const Shape& s, void* ws) {
     BwdPlan p{};
     Arena a{(char*)ws};
-    const int br = vs_block_rows(s, false);
     p.np = up(s.n, VS_PAD);
-    p.tiles_x = cdiv(s.n, br);
-    p.tiles_w = cdiv(s.vocab, br);
-    p.splits_x = vs_splits(s, p.tiles_x, s.vp / 32, 1 << 20);
-    p.splits_w = vs_splits(s, p.tiles_w, p.np / 32, 1 << 20);
+    int64_t units_w = 1, units_x = 1, resident_x = s.cus, resident_w = s.cus;
+#define VS_F(KS, PL)                                                                            \
+    p.tiles_x = cdiv(s.n, vs_bwd_blocks(KS, PL) * 16); p.tiles_w = cdiv(s.vocab, vs_bwd_blocks(KS, PL) * 16); \
+    units_x = s.vp / vs_bwd_rows(KS, PL); units_w = p.np / vs_bwd_rows(KS, PL);                 \
+    resident_x *= per_cu<vs_bwd_kernel<KS, PL, false>>(); resident_w *= per_cu<vs_bwd_kernel<KS, PL, true>>()
+    VS_BY_WIDTH(s.ks, s.pl, VS_F);
+#undef VS_F
+    p.splits_x = vs_splits(resident_x, cdiv(p.tiles_x, 4), units_x, 8.0);
+    p.splits_w = vs_splits(resident_w, cdiv(p.tiles_w, 4), units_w, 8.0);
     const int64_t frag = (int64_t)s.ks * s.pl * 64;
     p.wS = a.take<uint4>(s.vp / 16 * frag);
     p.wT = a.take<uint4>(s.vp / 16 * frag);
     p.xS = a.take<uint4>(p.np / 16 * frag);
     p.xT = a.take<uint4>(p.np / 16 * frag);
-    p.bias = a.take<float>(s.vp);
-    p.row.lse2 = a.take<float>(p.np);
-    p.row.A = a.take<float>(p.np);
-    p.row.B = a.take<float>(p.np);
-    p.row.gl = a.take<float>(p.np);
-    p.row.target = a.take<int32_t>(p.np);
+    p.info = a.take<float>(s.vp / 32 * VS_INFO);
+    p.tokens = a.take<float>(p.np / 32 * VS_TOKEN);
     // dx and dw are formed one after the other: their partials share the space
     p.part = a.take<float>(std::max(p.splits_x * p.np, p.splits_w * s.vp) * s.ks * 32);
-    p.bias_part = with_bias ? a.take<float>(p.splits_w * s.vp) : nullptr;
+    p.bias_part = a.take<float>(p.splits_w * s.vp);
     p.bytes = a.used;
     return p;
 }
@@ -198,7 +218,7 @@ int vs_shape(sage_ctx* c, int32_t dtype, int64_t n, int64_t vocab, int32_t dim, 
     if (dim > 512) return sage_ctx_fail(c, SAGE_E_LIMIT, "embedding dimension above 512 is not supported");
     if (vocab > (1 << 20)) return sage_ctx_fail(c, SAGE_E_LIMIT, "a vocabulary of more than 2^20 ids is not supported");
     if (n > (1 << 22)) return sage_ctx_fail(c, SAGE_E_LIMIT, "more than 2^22 tokens in one call are not supported");
-    *s = Shape{n, vocab, up(vocab, VS_BLOCK), dim, vs_steps(dim), dtype == SAGE_BF16 ? 1 : 3, k, sage_ctx_compute_units(c)};
+    *s = Shape{n, vocab, up(vocab, VS_BLOCK), dim, vs_steps(dim), dtype == SAGE_BF16 ? 1 : 2, k, sage_ctx_compute_units(c)};
     return SAGE_OK;
 }
 
@@ -220,10 +240,13 @@ int check_workspace(sage_ctx* c, const void* p, int64_t have, int64_t need) {
     return sage_ctx_fail(c, SAGE_E_ARG, msg);
 }
 
-void pack(const Shape& s, const VsSrc& src, int64_t padded, uint4* S, uint4* T, float* group_max, hipStream_t st) {
-#define VS_F(KS, PL) k_vs_pack<KS, PL><<<(uint32_t)(padded / 32), 256, 0, st>>>(src, S, T, group_max)
+void pack(const Shape& s, const VsPack& p, int64_t padded, hipStream_t st) {
+#define VS_F(KS, PL) k_vs_pack<KS, PL><<<(uint32_t)(padded / 32), 256, 0, st>>>(p)
     VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
+}
+void pack_info(const Shape& s, const float* bias, float* info, hipStream_t st) {
+    k_vs_bias<<<cdiv(s.vp, 256), 256, 0, st>>>(bias, s.pl == 2 ? VS_LOG2E : 1.0f, (int32_t)s.vocab, (int32_t)s.vp, info);
 }
 
 VsSrc rows_from(const VsSrc& m, int64_t row, int64_t rows) {
@@ -266,30 +289,27 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
     const hipStream_t st = (hipStream_t)stream;
     const VsSrc w{d_weight, ldw, (int32_t)vocab, dim, dtype == SAGE_BF16}, x{d_x, ldx, (int32_t)n, dim, dtype == SAGE_BF16};
     if (!p.raw) {
-        pack(s, w, s.vp, p.wS, nullptr, alternatives ? p.group_max : nullptr, st);
-        k_vs_bias<<<cdiv(s.vp, 256), 256, 0, st>>>(d_bias, (int32_t)vocab, (int32_t)s.vp, p.bias);
+        pack(s, VsPack{w, p.wS, nullptr, alternatives ? p.group_max : nullptr, p.info + VS_INFO_EXP, VS_INFO}, s.vp, st);
+        pack_info(s, d_bias, p.info, st);
     }
     for (int64_t r0 = 0; r0 < n; r0 += p.rows) {
         const int64_t rows = std::min(p.rows, n - r0);
         const VsSrc xr = rows_from(x, r0, rows);
-        const VsFwd f{p.xS, p.wS, p.bias, d_bias != nullptr, (int32_t)vocab, (int32_t)p.tiles, p.splits, (int32_t)(s.vp / VS_BLOCK), (int32_t)p.chunks,
+        const VsFwd f{p.xS, p.wS, p.info, p.x_exp, d_bias != nullptr, (int32_t)vocab, (int32_t)p.tiles, p.splits, (int32_t)(s.vp / VS_BLOCK), (int32_t)p.chunks,
                       p.n_pad, p.part, alternatives ? p.chunk_max : nullptr};
         if (p.raw) {
             const VsRaw q{xr, w, d_bias, alternatives ? p.group_max : nullptr, f};
             const dim3 grid(p.splits, (uint32_t)p.tiles);
 #define VS_F(KS, PL)                                                                                                            \
     if constexpr (vs_raw_most(KS, PL) > 1)                                                                                      \
-        if (p.raw > 1) { k_vs_forward_raw<KS, PL, vs_raw_most(KS, PL)><<<grid, 256, 0, st>>>(q); break; }                       \
-    k_vs_forward_raw<KS, PL, 1><<<grid, 256, 0, st>>>(q)
+        if (p.raw > 1) { k_vs_forward_raw<KS, vs_raw_parts(PL), vs_raw_most(KS, PL)><<<grid, 256, 0, st>>>(q); break; }         \
+    k_vs_forward_raw<KS, vs_raw_parts(PL), 1><<<grid, 256, 0, st>>>(q)
             VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
         } else {
-            pack(s, xr, p.n_pad, p.xS, nullptr, nullptr, st);
-            const uint32_t grid = cdiv(p.tiles * p.splits, 4), grid_staged = cdiv(p.tiles, 4) * p.splits;
-#define VS_F(KS, PL)                                                                                                            \
-    if constexpr (vs_stage_rows(KS, PL) > 0)                                                                                    \
-        k_vs_forward_staged<KS, PL, vs_fwd_blocks(KS, PL), vs_stage_rows(KS, PL)><<<grid_staged, 256, 0, st>>>(f);              \
-    else k_vs_forward<KS, PL, vs_fwd_blocks(KS, PL)><<<grid, 256, 0, st>>>(f)
+            pack(s, VsPack{xr, p.xS, nullptr, nullptr, p.x_exp, 1}, p.n_pad, st);
+            const uint32_t grid = cdiv(p.tiles, 4) * p.splits;
+#define VS_F(KS, PL) vs_fwd_kernel<KS, PL><<<grid, 256, 0, st>>>(f)
             VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
         }
@@ -312,7 +332,7 @@ int64_t sage_token_logprobs_backward_workspace(sage_ctx* c, int32_t dtype, int64
     Shape s;
     const int rc = vs_shape(c, dtype, n, vocab, dim, 0, &s);
     if (rc) return rc;
-    return n ? plan_bwd(s, true, nullptr).bytes : 0;
+    return n ? plan_bwd(s, nullptr).bytes : 0;
 }
 
 int sage_token_logprobs_backward_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vocab, int32_t dim, const void* d_x, int64_t ldx,
@@ -342,34 +362,35 @@ int sage_token_logprobs_backward_device(sage_ctx* c, int32_t dtype, int64_t n, i
         if (d_dweight) k_vs_zero<<<cdiv(vocab * dim, 256), 256, 0, st>>>(d_dweight, lddw, (int32_t)vocab, dim, bf16, d_dbias);
         return launched(c, "sage_token_logprobs_backward_device");
     }
-    const BwdPlan p = plan_bwd(s, true, d_workspace);
+    const BwdPlan p = plan_bwd(s, d_workspace);
     if ((rc = check_workspace(c, d_workspace, workspace_bytes, p.bytes))) return rc;
     const VsSrc w{d_weight, ldw, (int32_t)vocab, dim, bf16}, x{d_x, ldx, (int32_t)n, dim, bf16};
-    pack(s, w, s.vp, p.wS, d_dx ? p.wT : nullptr, nullptr, st);
-    pack(s, x, p.np, p.xS, d_dweight ? p.xT : nullptr, nullptr, st);
-    k_vs_bias<<<cdiv(s.vp, 256), 256, 0, st>>>(d_bias, (int32_t)vocab, (int32_t)s.vp, p.bias);
-    k_vs_rows<<<cdiv(p.np, 256), 256, 0, st>>>(d_lse, d_entropy, d_targets, d_grad_logprob, d_grad_entropy, (int32_t)n, p.np, (int32_t)vocab, p.row);
+    pack(s, VsPack{w, p.wS, d_dx ? p.wT : nullptr, nullptr, p.info + VS_INFO_EXP, VS_INFO}, s.vp, st);
+    pack(s, VsPack{x, p.xS, d_dweight ? p.xT : nullptr, nullptr, p.tokens + VS_TOKEN_EXP, VS_TOKEN}, p.np, st);
+    pack_info(s, d_bias, p.info, st);
+    k_vs_rows<<<cdiv(p.np, 256), 256, 0, st>>>(d_lse, d_entropy, d_targets, d_grad_logprob, d_grad_entropy, (int32_t)n, p.np, (int32_t)vocab, p.tokens);
     VsBwd b{};
-    b.bias = p.bias; b.has_bias = d_bias != nullptr; b.has_entropy = d_grad_entropy != nullptr; b.vocab = (int32_t)vocab; b.row = p.row; b.part = p.part;
+    b.info = p.info; b.tokens = p.tokens; b.has_bias = d_bias != nullptr; b.has_entropy = d_grad_entropy != nullptr; b.vocab = (int32_t)vocab;
+    b.part = p.part;
     if (d_dx) {
         b.stayS = p.xS; b.flowS = p.wS; b.flowT = p.wT;
-        b.n_tiles = (int32_t)p.tiles_x; b.splits = p.splits_x; b.groups = (int32_t)(s.vp / 32); b.stay_pad = p.np; b.bias_part = nullptr;
-        const uint32_t grid = cdiv(p.tiles_x * p.splits_x, 4);
-#define VS_F(KS, PL) k_vs_backward<KS, PL, vs_bwd_blocks(KS, PL), false><<<grid, 256, 0, st>>>(b)
+        b.n_tiles = (int32_t)p.tiles_x; b.splits = p.splits_x; b.groups = (int32_t)(s.vp / 32); b.stay_pad = p.np;
+        const uint32_t grid = cdiv(p.tiles_x, 4) * p.splits_x;
+#define VS_F(KS, PL) vs_bwd_kernel<KS, PL, false><<<grid, 256, 0, st>>>(b)
         VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
-        const VsSum r{p.part, nullptr, (int32_t)n, dim, s.ks * 32, p.splits_x, p.np, p.row, b.has_entropy, w, d_dx, lddx, bf16, nullptr};
+        const VsSum r{p.part, nullptr, (int32_t)n, dim, s.ks * 32, p.splits_x, p.np, p.tokens, b.has_entropy, w, d_dx, lddx, bf16, nullptr};
         k_vs_sum<<<cdiv(n * dim, 256), 256, 0, st>>>(r);
     }
     if (d_dweight) {
         b.stayS = p.wS; b.flowS = p.xS; b.flowT = p.xT;
         b.n_tiles = (int32_t)p.tiles_w; b.splits = p.splits_w; b.groups = (int32_t)(p.np / 32); b.stay_pad = s.vp;
-        b.bias_part = d_dbias ? p.bias_part : nullptr;
-        const uint32_t grid = cdiv(p.tiles_w * p.splits_w, 4);
-#define VS_F(KS, PL) k_vs_backward<KS, PL, vs_bwd_blocks(KS, PL), true><<<grid, 256, 0, st>>>(b)
+        b.want_db = d_dbias != nullptr; b.bias_part = p.bias_part;
+        const uint32_t grid = cdiv(p.tiles_w, 4) * p.splits_w;
+#define VS_F(KS, PL) vs_bwd_kernel<KS, PL, true><<<grid, 256, 0, st>>>(b)
         VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
-        const VsSum r{p.part, p.bias_part, (int32_t)vocab, dim, s.ks * 32, p.splits_w, s.vp, VsRow{}, 0, w, d_dweight, lddw, bf16, d_dbias};
+        const VsSum r{p.part, p.bias_part, (int32_t)vocab, dim, s.ks * 32, p.splits_w, s.vp, nullptr, 0, w, d_dweight, lddw, bf16, d_dbias};
         k_vs_sum<<<cdiv(vocab * dim, 256), 256, 0, st>>>(r);
     }
     return launched(c, "sage_token_logprobs_backward_device");

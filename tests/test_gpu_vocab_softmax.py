@@ -10,7 +10,14 @@ Tolerances, with u = 2^-24 (half a float32 step) and D, V, n the lengths summed 
   p                the logit's and lse's together, and u times the exponent's size, relative
   entropy          the derivative of H by the logits is p (log p + H): (1 + H) times twice lse's tolerance
   gradients        |G|'s error as an [n, V] matrix, taken through |w| or |x|, plus the sum's, plus half a step of the result's type;
-                   bf16 inputs round G to bf16 before the second product: 2^-8 |G| more"""
+                   bf16 inputs round G to bf16 before the second product: 2^-8 |G| more.
+                   float32 products (of more than 128 tokens, and all gradients) take an element as two float16 of a value
+                   scaled by a power of two, so that the largest of its 32 rows, m, lies in [2^12, 2^13): an element is off by
+                   at most 2^-25 of that scale (half a step of the smallest float16), 2^-25 / 2^12 m = 2^-37 m, beside its
+                   relative 2^-22; a weight likewise by 2^-25 of a scale in which the largest weight of its column times m
+                   has come to at least 2^12: 2^-37 of the largest |G| m, times an element that may be m.  Each of the
+                   N terms of a sum is thus off by at most 2^-36 of the largest |G| times the largest element, absolutely:
+                   N 2^-36 max|G| max|w| more (it shows only where a sum is one term with an element 10^-7 of m)"""
 import math
 
 import numpy as np
@@ -90,7 +97,10 @@ class Exact:
 
         def through(a, size, other, length):
             value = a @ other
-            tol = size @ other.abs() + (8 * math.sqrt(length) + 16) * U * (mass if a is G else mass.t().contiguous()) @ other.abs()
+            m = mass if a is G else mass.t().contiguous()
+            tol = size @ other.abs() + (8 * math.sqrt(length) + 16) * U * m @ other.abs()
+            if dtype == F32:
+                tol = tol + length * 2.0 ** -36 * m.amax(1, keepdim=True) * other.abs().max()
             return value, tol + step * value.abs() * (1 + step) + step * tol + 1e-37
         Gt, et = G.t().contiguous(), err.t().contiguous()
         ones = torch.ones(n, 1, dtype=torch.float64, device=G.device)
@@ -283,6 +293,22 @@ def test_large_and_small_logits():
         dx, dw, db = vs.token_logprobs_backward(x, w, t, f, gl, bias=bias)
         (wx, tx), (ww, tw), (wb, tb) = e.gradient(gl, None, F32)
         close(dx, wx, tx, "dx"), close(dw, ww, tw, "dw")
+
+
+def test_rows_of_very_different_sizes():
+    """float32 rows share a power of two by 32: sizes from 1e-6 to 1e2 side by side, in x and in the weights."""
+    from sage_amd import vocab_softmax as vs
+    x, w, b, t = make(200, 900, 50, F32, "prior")
+    x *= torch.logspace(-6, 2, 200, device="cuda")[torch.randperm(200, generator=torch.Generator().manual_seed(1)).cuda(), None]
+    w *= torch.logspace(-5, 0.5, 900, device="cuda")[torch.randperm(900, generator=torch.Generator().manual_seed(2)).cuda(), None]
+    gl, gh = torch.logspace(-9, 0, 200).cuda(), -torch.logspace(0, -9, 200).cuda()
+    e = Exact(x, w, b, t, 5)
+    f = vs.token_logprobs(x, w, t, bias=b, alternatives=5)
+    check_forward(f, e, 5)
+    for h in (None, gh):
+        dx, dw, db = vs.token_logprobs_backward(x, w, t, f, gl, bias=b, grad_entropy=h)
+        (wx, tx), (ww, tw), (wb, tb) = e.gradient(gl, h, F32)
+        close(dx, wx, tx, "dx"), close(dw, ww, tw, "dw"), close(db, wb, tb, "db")
 
 
 def test_not_a_number_stays_in_its_row():
