@@ -39,8 +39,9 @@ __device__ __forceinline__ int vs_chunk_row(int c, int i) {      // the i-th of 
     return (c >> 4) * VS_BLOCK + (c & 3) * 64 + (i >> 2) * 16 + ((c >> 2) & 3) * 4 + (i & 3);
 }
 #define VS_NOTHING (-1.0e30f)  // reference of a row that has seen no finite logit yet; a bias this low masks its id
-#define VS_SLACK 20.0f         // the running reference lags the maximum by at most this (in powers of two)
-#define VS_TMIN (-200.0f)      // 2^-200 is 0 in float32: what a logit of -inf is raised to, so that 0 * log p is 0
+#define VS_MASKED (-3.0e30f)   // what a masked logit is raised to: p is 0 there, and p times the exponent too
+#define VS_SLACK 4096.0f       // eight terms that sum to more than this move the running reference
+#define VS_TMIN (-200.0f)      // 2^-200 is 0 in float32
 
 struct VsSrc {                 // a row-major matrix of float32 or bf16
     const void* p;
@@ -211,8 +212,16 @@ __global__ __launch_bounds__(256) void k_vs_bias(const float* __restrict__ bias,
     if (v < padded) info[(v >> 5) * VS_INFO + (v & 31)] = v >= vocab ? -INFINITY : !bias ? 0.0f : bias[v] <= VS_NOTHING ? -INFINITY : bias[v] * unit;
 }
 
+// All four are known before any is written back: without this the compiler takes a new register quadruple for what a rarely
+// taken branch changes, and copies the old one into it each time the branch is not taken.
+__device__ __forceinline__ void vs_in_place(vs_f4& v) {
+    float a = v[0], b = v[1], c = v[2], d = v[3];
+    asm volatile("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+    v = vs_f4{a, b, c, d};
+}
+
 // 2^n as a factor of log2(e), kept finite (logits beyond float32 are inf or 0 all the same)
-__device__ __forceinline__ float vs_unit(float n) { return ldexpf(VS_LOG2E, (int)fmaxf(fminf(n, 126.0f), -126.0f)); }
+__device__ __forceinline__ float vs_unit(float n) { return ldexpf(VS_LOG2E, (int)__builtin_amdgcn_fmed3f(n, -126.0f, 126.0f)); }
 
 // ---- forward ------------------------------------------------------------------------------------------------------
 struct VsFwd {
@@ -230,9 +239,9 @@ struct VsFwd {
     float* chunk_max;          // [n_pad][chunks] or null
 };
 
-// Sums of a row, relative to 2^ref: s of exp, e of exp * exponent (the entropy's).  A softmax in one pass: the reference
-// follows the running maximum in steps of at least 2^VS_SLACK, so it moves a few times per row and the common step has no
-// rescaling.  Eight terms are summed first, then up to VS_BLOCK / 4 of those, then these: sums of 262,144 terms keep
+// Sums of a row, relative to 2^ref: s of exp, e of exp * exponent (the entropy's).  A softmax in one pass: the reference is
+// moved to the running maximum only when a step's terms have outgrown it by VS_SLACK, a few times per row; the common step
+// neither rescales nor looks for a maximum.  Eight terms are summed first, then up to VS_BLOCK / 4 of those, then these: sums of 262,144 terms keep
 // their last bits.
 struct VsStat {
     float ref, s, e, S, E;
@@ -287,44 +296,45 @@ struct VsRowsOfTile {
 #pragma unroll
         for (int t = 0; t < TB; ++t) { st[t].clear(); top[t] = -INFINITY; }
     }
-    // the logits of 32 ids, in powers of two after multiplication by unit[t] (and addition of `bias`, if they are SCALED and
-    // MASKED); MASKED: some may be -inf
-    template <bool MASKED, bool SCALED>
-    __device__ __forceinline__ void add(const vs_f4 (&s)[2][TB], const float (&unit)[TB], const vs_f4 (&bias)[2]) {
+    // the logits of 32 ids, in powers of two after multiplication by unit[t]; TOP: their largest is kept
+    template <bool TOP, bool SCALED>
+    __device__ __forceinline__ void add(const vs_f4 (&s)[2][TB], const float (&unit)[TB]) {
+        float ls[TB], le[TB];
+        auto sums = [&]() {
+            float most = 0.0f;
+#pragma unroll
+            for (int t = 0; t < TB; ++t) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float e = fmaf(s[j >> 2][t][j & 3], SCALED ? unit[t] : VS_LOG2E, -st[t].ref), p = __builtin_amdgcn_exp2f(e);
+                    ls[t] = j ? ls[t] + p : p;
+                    le[t] = j ? fmaf(p, e, le[t]) : p * e;
+                }
+                most = fmaxf(most, ls[t]);
+            }
+            return most;
+        };
+        if (__any(sums() > VS_SLACK)) {
+#pragma unroll
+            for (int t = 0; t < TB; ++t) st[t].move(ls[t] > VS_SLACK ? largest(s, t) * (SCALED ? unit[t] : VS_LOG2E) : st[t].ref);
+            sums();
+        }
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = s[j >> 2][t][j & 3];
-                if (SCALED && MASKED) v[j] = fmaf(v[j], unit[t], bias[j >> 2][j & 3]);
-            }
-            float mx = vs_max(vs_max(vs_max(v[0], v[1]), v[2]), vs_max(vs_max(v[3], v[4]), v[5]));
-            mx = vs_max(vs_max(mx, v[6]), v[7]);
-            if (!SCALED) top[t] = vs_max(top[t], mx);
-            if (!SCALED) mx *= VS_LOG2E;
-            else if (!MASKED) mx *= unit[t];
-            if (SCALED) top[t] = vs_max(top[t], mx * VS_LN2);
-            const bool up = mx > st[t].ref + VS_SLACK;
-            if (__any(up)) st[t].move(up ? mx : st[t].ref);
-            float ls, le;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float e = SCALED && MASKED ? v[j] - st[t].ref : fmaf(v[j], SCALED ? unit[t] : VS_LOG2E, -st[t].ref);
-                if (MASKED) e = vs_max(e, VS_TMIN);
-                const float p = __builtin_amdgcn_exp2f(e);
-                ls = j ? ls + p : p;
-                le = j ? fmaf(p, e, le) : p * e;
-            }
-            st[t].s += ls;
-            st[t].e += le;
+            st[t].s += ls[t];
+            st[t].e += le[t];
+            if (TOP) top[t] = vs_max(top[t], SCALED ? largest(s, t) * (unit[t] * VS_LN2) : largest(s, t));
         }
+    }
+    static __device__ __forceinline__ float largest(const vs_f4 (&s)[2][TB], int t) {
+        const float m = vs_max(vs_max(vs_max(s[0][t][0], s[0][t][1]), s[0][t][2]), vs_max(vs_max(s[0][t][3], s[1][t][0]), s[1][t][1]));
+        return vs_max(vs_max(m, s[1][t][2]), s[1][t][3]);
     }
     // 64 ids are done, the h-th of their block: their largest logits are stored with those of the rest of the block, sixteen
     // bytes a lane (WHOLE: the wave sees whole blocks), or at once
     template <bool WHOLE>
     __device__ __forceinline__ void chunk(const VsFwd& a, int64_t tile, int block, int h, int lane, bool live) {
-        if (a.chunk_max) {
+        {
 #pragma unroll
             for (int t = 0; t < TB; ++t) {
                 float* to = a.chunk_max + ((tile * TB + t) * 16 + (lane & 15)) * a.chunks + block * 16 + (lane >> 4) * 4;
@@ -362,8 +372,23 @@ struct VsRowsOfTile {
     }
 };
 
+// Adds the biases where the product did not start from them, and raises masked logits.
+template <int TB, bool SCALED>
+__device__ __forceinline__ void vs_mask(vs_f4 (&s)[2][TB], float (&unit)[TB], const vs_f4 (&b)[2]) {
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float v = s[j >> 2][t][j & 3];
+            if (SCALED) v = fmaf(v, unit[t], b[j >> 2][j & 3]);
+            s[j >> 2][t][j & 3] = vs_max(v, VS_MASKED);
+        }
+        if (SCALED) unit[t] = 1.0f;
+    }
+}
+
 // 32 ids against a tile: their logits are formed and counted
-template <int KS, int PL, int TB>
+template <int KS, int PL, int TB, bool TOP>
 __device__ __forceinline__ void vs_forward_step(const VsFwd& a, int row0, const uint4* w, const float* info, const vs_bits (&x)[TB][KS][PL],
                                                 const float (&x_exp)[TB], VsRowsOfTile<TB>& rows) {
     const int lane = threadIdx.x & 63, quad = lane >> 4;
@@ -379,8 +404,8 @@ __device__ __forceinline__ void vs_forward_step(const VsFwd& a, int row0, const 
 #pragma unroll
     for (int t = 0; t < TB; ++t) unit[t] = PL == 2 ? vs_unit(-(e + x_exp[t])) : VS_LOG2E;
     vs_product<KS, PL, TB>(w, x, s);
-    if (a.has_bias || row0 + 32 > a.vocab) rows.template add<true, PL == 2>(s, unit, b);      // the same in the whole grid
-    else rows.template add<false, PL == 2>(s, unit, b);
+    if (a.has_bias || row0 + 32 > a.vocab) vs_mask<TB, PL == 2>(s, unit, b);      // (the same in the whole grid)
+    rows.template add<TOP, PL == 2>(s, unit);
 }
 
 // Four waves, a tile each, share the streaming rows through LDS.  SR rows at a time are copied straight into LDS (they are
@@ -410,7 +435,7 @@ struct VsStage {
         vs_stage<N>(w, to);
         vs_stage_floats<INFO>(info, (float*)(to + N));
     }
-    template <int TB>
+    template <int TB, bool TOP>
     static __device__ __forceinline__ void step(const VsFwd& a, int base, bool more, const uint4* __restrict__ next, const float* __restrict__ next_info,
                                                 uint4* __restrict__ to, const uint4* __restrict__ from, const vs_bits (&x)[TB][KS][PL],
                                                 const float (&x_exp)[TB], VsRowsOfTile<TB>& rows, int64_t tile, bool live) {
@@ -421,14 +446,14 @@ struct VsStage {
 #pragma unroll 1
         for (int r = 0; r < SR; r += 32) {
             const int row0 = base + r;
-            vs_forward_step<KS, PL, TB>(a, row0, from + r * KS * PL * 4 + lane, (const float*)(from + N) + r / 32 * VS_INFO, x, x_exp, rows);
-            if (row0 & 32) rows.template chunk<true>(a, tile, row0 / VS_BLOCK, (row0 >> 6) & 3, lane, live);
+            vs_forward_step<KS, PL, TB, TOP>(a, row0, from + r * KS * PL * 4 + lane, (const float*)(from + N) + r / 32 * VS_INFO, x, x_exp, rows);
+            if (TOP && (row0 & 32)) rows.template chunk<true>(a, tile, row0 / VS_BLOCK, (row0 >> 6) & 3, lane, live);
         }
         if (((base + SR) & (VS_BLOCK - 1)) == 0) rows.flush();
     }
 };
 
-template <int KS, int PL, int TB, int SR>
+template <int KS, int PL, int TB, int SR, bool TOP>
 __global__ __launch_bounds__(256, 2) void k_vs_forward(VsFwd a) {
     using Stage = VsStage<KS, PL, SR>;
     __shared__ uint4 buf0[Stage::SIZE], buf1[Stage::SIZE];
@@ -449,9 +474,9 @@ __global__ __launch_bounds__(256, 2) void k_vs_forward(VsFwd a) {
     Stage::fetch(w, info, buf0);
     for (int base = row_begin; base < row_end; base += 2 * SR) {
         w += SR * KS * PL * 4; info += Stage::INFO;
-        Stage::template step<TB>(a, base, true, w, info, buf1, buf0, x, x_exp, rows, tile, live);
+        Stage::template step<TB, TOP>(a, base, true, w, info, buf1, buf0, x, x_exp, rows, tile, live);
         w += SR * KS * PL * 4; info += Stage::INFO;
-        Stage::template step<TB>(a, base + SR, base + 2 * SR < row_end, w, info, buf0, buf1, x, x_exp, rows, tile, live);
+        Stage::template step<TB, TOP>(a, base + SR, base + 2 * SR < row_end, w, info, buf0, buf1, x, x_exp, rows, tile, live);
     }
     if (live) rows.store(a, tile, split, lane);
 }
@@ -584,7 +609,7 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
                     const float q = a.bias ? b[j >> 2][j & 3] : 0.0f;
                     const bool gone = q <= VS_NOTHING || row0 + (j >> 2) * 16 + quad * 4 + (j & 3) >= a.w.rows;
 #pragma unroll
-                    for (int t = 0; t < TB; ++t) s[j >> 2][t][j & 3] = gone ? -INFINITY : s[j >> 2][t][j & 3] + q;
+                    for (int t = 0; t < TB; ++t) s[j >> 2][t][j & 3] = gone ? VS_MASKED : s[j >> 2][t][j & 3] + q;
                 }
             }
             if (a.group_max) {
@@ -592,10 +617,9 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
                 for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
                 if (lane == 0 && tile == 0) a.group_max[row0 / 32] = m;
             }
-            if (a.bias || row0 + 32 > a.w.rows) rows.template add<true, false>(s, unscaled, b);
-            else rows.template add<false, false>(s, unscaled, b);
+            rows.template add<true, false>(s, unscaled);
         }
-        rows.template chunk<false>(a.f, tile, c >> 2, c & 3, lane, true);
+        if (a.f.chunk_max) rows.template chunk<false>(a.f, tile, c >> 2, c & 3, lane, true);
         if ((c & 3) == 3) rows.flush();
     }
     rows.join_lanes();
@@ -785,15 +809,14 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
     auto off = [&](int c, float m) { return fmaf(eps, fabsf(m), widest(c >> 4)); };
     float low = -INFINITY;
     if (a.chunks <= 256) {
-        if (tid < a.chunks && cm[tid] > -INFINITY) low = cm[tid] - off(tid, cm[tid]);
+        if (tid < a.chunks && cm[tid] > VS_NOTHING) low = cm[tid] - off(tid, cm[tid]);
     } else
 #pragma unroll 2
     for (int c = tid * 4; c < a.chunks; c += THREADS * 4) {
         const float4 m = *(const float4*)&cm[c];
         const float g = widest(c >> 4);
-        // (m - d is increasing in m; of -inf it is -inf)
-        const float top = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
-        low = fmaxf(low, top - fmaf(eps, fabsf(top), g));
+        const float top = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));      // (m - d is increasing in m)
+        if (top > VS_NOTHING) low = fmaxf(low, top - fmaf(eps, fabsf(top), g));
     }
     if (a.chunks <= 256) {
         if (tid < 256) best[tid] = low;
@@ -862,7 +885,7 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
     };
     auto may = [&](int c, float m) {
         const float up = m + off(c, m);
-        return m > -INFINITY && up >= bound && !beaten((double)up, (c >> 4) * VS_BLOCK);
+        return m > VS_NOTHING && up >= bound && !beaten((double)up, (c >> 4) * VS_BLOCK);
     };
     // every chunk that may hold one of the k: usually a few more than k
 #pragma unroll 2
@@ -872,7 +895,7 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
         const float v[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (v[i] > -INFINITY && v[i] + fmaf(eps, fabsf(v[i]), g) >= bound) {
+            if (v[i] > VS_NOTHING && v[i] + fmaf(eps, fabsf(v[i]), g) >= bound) {
                 const int at = atomicAdd(&n_list, 1);
                 if (at < VS_LIST) list[at] = (uint16_t)(c + i);
             }
@@ -969,7 +992,7 @@ struct VsBwd {
     const uint4 *flowS, *flowT;// streaming rows, and transposed
     const float* info;         // of ids: [ids / 32][VS_INFO]
     const float* tokens;       // of tokens: [tokens / 32][VS_TOKEN]
-    int32_t has_bias, has_entropy, want_db;
+    int32_t has_bias, want_db;
     int32_t vocab;
     int32_t n_tiles, splits, groups;   // groups of 32 streaming rows
     int64_t stay_pad;          // rows of a partial
@@ -980,12 +1003,12 @@ struct VsBwd {
 // A wave: a tile of 16 TB stationary rows against one range of the streaming ones.  OF_IDS = false: the stationary rows
 // are tokens, the result sum_v p' w_v with p' = p (A + B e), or p alone when there is no entropy gradient (A is then a
 // factor of the whole row, applied at the end); the target's own term is added at the end too, so that the largest
-// coefficient is never rounded to bf16.  OF_IDS = true: the stationary rows are ids, the result sum_n G_nv x_n; in the few
-// steps in which a token's target lies in the tile, bf16 adds the rounded-off part of G in a second product.
+// coefficient is never rounded to bf16.  OF_IDS = true: the stationary rows are ids, the result sum_n G_nv x_n; the targets'
+// own terms are products of their own (in two parts, for the same reason) in the few steps in which one lies in the tile.
 //
 // Two float16 parts (PL = 2) of a weight: column t is kept multiplied by 2^sg[t], sg as large as the largest weight of the column
 // so far allows (2^15 after the streaming rows' scale), and the sums with it.  It starts high and falls a few times.
-template <int KS, int PL, int TB, bool OF_IDS>
+template <int KS, int PL, int TB, bool OF_IDS, bool ENTROPY>
 struct VsGrad {
     static constexpr float MOST = 15.0f, AIM = 13.0f;
     vs_bits y[TB][KS][PL];
@@ -1008,7 +1031,7 @@ struct VsGrad {
                 const float* of = a.tokens + (r >> 5) * VS_TOKEN;
                 L[t] = of[r & 31]; A[t] = of[VS_TOKEN_A + (r & 31)]; B[t] = of[VS_TOKEN_B + (r & 31)];
                 y_exp[t] = PL == 2 ? of[VS_TOKEN_EXP] : 0.0f;
-                if (PL == 2 && a.has_entropy) {      // |A + B e| brought below 1
+                if (PL == 2 && ENTROPY) {      // |A + B e| brought below 1
                     const float size = fabsf(A[t]) + fabsf(B[t]) * 256.0f;
                     norm[t] = size > 0.0f && size < INFINITY ? (float)__builtin_amdgcn_frexp_expf(size) : 0.0f;
                     A[t] = ldexpf(A[t], -(int)norm[t]);
@@ -1029,16 +1052,21 @@ struct VsGrad {
         if (!(ask > 0.0f)) ask = 0.0f;
         sg[t] -= ask;
 #pragma unroll
-        for (int d = 0; d < 2 * KS; ++d)
+        for (int d = 0; d < 2 * KS; ++d) {
+            vs_f4 v;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[d][t][i] = ldexpf(acc[d][t][i], -(int)ask);
+            for (int i = 0; i < 4; ++i) v[i] = ldexpf(acc[d][t][i], -(int)ask);
+            vs_in_place(v);
+            acc[d][t] = v;
+        }
     }
 
-    // P: the weights of the 32 streaming rows from row0 on, in parts; R: what bf16 rounds off
-    __device__ __forceinline__ bool weights(const VsBwd& a, int row0, const uint4* S, const float* of, vs_bits (&P)[TB][PL], vs_bits (&R)[TB]) {
-        const int lane = threadIdx.x & 63, quad = lane >> 4;
-        const bool masked = a.has_bias || (OF_IDS ? stay0 + TB * 16 > a.vocab : row0 + 32 > a.vocab);
+    // P: the weights of the 32 streaming rows from row0 on, in parts, without the targets' own terms
+    __device__ __forceinline__ void weights(const VsBwd& a, int row0, const uint4* S, const float* of, vs_bits (&P)[TB][PL]) {
+        const int quad = (threadIdx.x & 63) >> 4;
         vs_f4 s[2][TB], b[2];
+        float unit[TB];
+        const float f_exp = PL == 2 ? of[OF_IDS ? VS_TOKEN_EXP : VS_INFO_EXP] : 0.0f;
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb) {
             if constexpr (!OF_IDS) b[rb] = *(const vs_f4*)&of[rb * 16 + quad * 4];
@@ -1049,97 +1077,87 @@ struct VsGrad {
                 else s[rb][t] = b[rb];
             }
         }
-        const float f_exp = PL == 2 ? of[OF_IDS ? VS_TOKEN_EXP : VS_INFO_EXP] : 0.0f;
+#pragma unroll
+        for (int t = 0; t < TB; ++t) unit[t] = PL == 2 ? vs_unit(-(f_exp + y_exp[t])) : VS_LOG2E;
         vs_product<KS, PL, TB>(S, y, s);
-        bool hit = false;
-        if constexpr (OF_IDS) {
-            const int target = __float_as_int(of[VS_TOKEN_TARGET + (lane & 31)]);
-            hit = __any(target >= stay0 && target < stay0 + TB * 16);
-        }
-        if (masked) { if (a.has_entropy) form<true, true>(a, row0, of, f_exp, s, b, hit, P, R); else form<true, false>(a, row0, of, f_exp, s, b, hit, P, R); }
-        else { if (a.has_entropy) form<false, true>(a, row0, of, f_exp, s, b, hit, P, R); else form<false, false>(a, row0, of, f_exp, s, b, hit, P, R); }
-        return hit;
-    }
-
-    template <bool MASKED, bool ENTROPY>
-    __device__ __forceinline__ void form(const VsBwd& a, int row0, const float* of, float f_exp, const vs_f4 (&s)[2][TB], const vs_f4 (&b)[2], bool hit,
-                                         vs_bits (&P)[TB][PL], vs_bits (&R)[TB]) {
-        const int lane = threadIdx.x & 63, quad = lane >> 4;
-        vs_f4 rl[2], ra[2], rb_[2];
-        if constexpr (OF_IDS) {
-#pragma unroll
-            for (int rb = 0; rb < 2; ++rb) {
-                rl[rb] = *(const vs_f4*)&of[rb * 16 + quad * 4];
-                ra[rb] = *(const vs_f4*)&of[VS_TOKEN_A + rb * 16 + quad * 4];
-                if (ENTROPY) rb_[rb] = *(const vs_f4*)&of[VS_TOKEN_B + rb * 16 + quad * 4];
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < TB; ++t) {
-            vs_f8 G;
-            const float unit = PL == 2 ? vs_unit(-(f_exp + y_exp[t])) : VS_LOG2E;
+        if (a.has_bias || (OF_IDS ? stay0 + TB * 16 > a.vocab : row0 + 32 > a.vocab)) {
             if constexpr (OF_IDS) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float e = fmaf(s[j >> 2][t][j & 3], unit, -rl[j >> 2][j & 3]);
-                    if (PL == 2 && MASKED) e += L[t];
-                    if (MASKED) e = vs_max(e, VS_TMIN);
-                    const float p = __builtin_amdgcn_exp2f(e);
-                    G[j] = p * (ENTROPY ? fmaf(rb_[j >> 2][j & 3], e, ra[j >> 2][j & 3]) : ra[j >> 2][j & 3]);
-                }
-                if (hit) {
+                for (int t = 0; t < TB; ++t) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int at = (j >> 2) * 16 + quad * 4 + (j & 3);
-                        if (__float_as_int(of[VS_TOKEN_TARGET + at]) == (int32_t)(stay0 + t * 16 + (lane & 15))) G[j] += of[VS_TOKEN_GL + at];
+                        float v = s[j >> 2][t][j & 3];
+                        if (PL == 2) v = fmaf(v, unit[t], L[t]);
+                        s[j >> 2][t][j & 3] = vs_max(v, VS_MASKED);
+                    }
+                    if (PL == 2) unit[t] = 1.0f;
+                }
+            } else vs_mask<TB, PL == 2>(s, unit, b);
+        }
+        vs_f8 G[TB];
+        float big[TB];                         // PL = 2: the power of two that a column's largest scaled weight is below
+        auto form = [&]() {
+            vs_f4 rl[2], ra[2], rb_[2];
+            if constexpr (OF_IDS) {
+#pragma unroll
+                for (int rb = 0; rb < 2; ++rb) {
+                    rl[rb] = *(const vs_f4*)&of[rb * 16 + quad * 4];
+                    ra[rb] = *(const vs_f4*)&of[VS_TOKEN_A + rb * 16 + quad * 4];
+                    if (ENTROPY) rb_[rb] = *(const vs_f4*)&of[VS_TOKEN_B + rb * 16 + quad * 4];
+                }
+            }
+            float most = 0.0f;
+#pragma unroll
+            for (int t = 0; t < TB; ++t) {
+                const float shift = PL == 2 ? sg[t] - f_exp : 0.0f;
+                float m = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float v = s[j >> 2][t][j & 3];
+                    if constexpr (OF_IDS) {
+                        float e = fmaf(v, PL == 2 ? unit[t] : VS_LOG2E, -rl[j >> 2][j & 3]);
+                        const float p = __builtin_amdgcn_exp2f(e);
+                        if (ENTROPY) e = vs_max(e, VS_TMIN);
+                        G[t][j] = p * (ENTROPY ? fmaf(rb_[j >> 2][j & 3], e, ra[j >> 2][j & 3]) : ra[j >> 2][j & 3]);
+                        if (PL == 2) m = fmaxf(m, fabsf(G[t][j]));
+                    } else {
+                        float e = fmaf(v, PL == 2 ? unit[t] : VS_LOG2E, shift - L[t]);
+                        if (PL == 2) m = j ? fmaxf(m, e) : e;
+                        G[t][j] = __builtin_amdgcn_exp2f(e);
+                        if (ENTROPY) {
+                            e = vs_max(e, VS_TMIN);
+                            G[t][j] *= fmaf(B[t], e, PL == 2 ? fmaf(-B[t], shift, A[t]) : A[t]);
+                        }
                     }
                 }
-                if (a.want_db) db[t] += ((G[0] + G[1]) + (G[2] + G[3])) + ((G[4] + G[5]) + (G[6] + G[7]));
+                if (PL == 2 && OF_IDS) m = m > 0.0f ? (float)__builtin_amdgcn_frexp_expf(m) + shift : 0.0f;
+                big[t] = m;
+                most = fmaxf(most, m);
+            }
+            return most;
+        };
+        const float most = form();
+        if (PL == 2)
+            if (__any(most > MOST)) {
+#pragma unroll
+                for (int t = 0; t < TB; ++t) lower(t, ceilf(big[t] - AIM));
+                if (!OF_IDS) form();           // (there the scale is in the exponent already)
+            }
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
+            if constexpr (OF_IDS) {
+                if (a.want_db) db[t] += ((G[t][0] + G[t][1]) + (G[t][2] + G[t][3])) + ((G[t][4] + G[t][5]) + (G[t][6] + G[t][7]));
                 if constexpr (PL == 2) {
-                    float m = fmaxf(fmaxf(fmaxf(fabsf(G[0]), fabsf(G[1])), fabsf(G[2])), fmaxf(fmaxf(fabsf(G[3]), fabsf(G[4])), fabsf(G[5])));
-                    m = fmaxf(fmaxf(m, fabsf(G[6])), fabsf(G[7]));
-                    const float x = m > 0.0f ? (float)__builtin_amdgcn_frexp_expf(m) + sg[t] - f_exp : 0.0f;
-                    if (__any(x > MOST)) lower(t, x - AIM);
+                    const int by = (int)(sg[t] - f_exp);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) G[j] = ldexpf(G[j], (int)(sg[t] - f_exp));
-                }
-            } else if constexpr (PL == 2) {
-                float e[8];
-                auto exponents = [&]() {
-                    const float k = (sg[t] - f_exp) - L[t];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        e[j] = fmaf(s[j >> 2][t][j & 3], unit, k);
-                        if (MASKED) e[j] = vs_max(e[j] + b[j >> 2][j & 3], VS_TMIN);
-                    }
-                };
-                exponents();
-                const float m = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
-                if (__any(m > MOST)) { lower(t, ceilf(m - AIM)); exponents(); }
-                const float a2 = ENTROPY ? fmaf(-B[t], sg[t] - f_exp, A[t]) : 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    G[j] = __builtin_amdgcn_exp2f(e[j]);
-                    if (ENTROPY) G[j] *= fmaf(B[t], e[j], a2);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float e = fmaf(s[j >> 2][t][j & 3], VS_LOG2E, -L[t]);
-                    if (MASKED) e = vs_max(e, VS_TMIN);
-                    G[j] = __builtin_amdgcn_exp2f(e);
-                    if (ENTROPY) G[j] *= fmaf(B[t], e, A[t]);
+                    for (int j = 0; j < 8; ++j) G[t][j] = ldexpf(G[t][j], by);
                 }
             }
-            vs_split<PL>(G, P[t]);
-            if (OF_IDS && PL == 1 && hit) {
-                const vs_f8 r = G - __builtin_convertvector(__builtin_bit_cast(vs_bf8, P[t][0]), vs_f8);
-                vs_split<1>(r, &R[t]);
-            }
+            vs_split<PL>(G[t], P[t]);
         }
     }
 
-    __device__ __forceinline__ void products(const uint4* T, const vs_bits (&P)[TB][PL], const vs_bits (&R)[TB], bool hit) {
+    __device__ __forceinline__ void products(const uint4* T, const vs_bits (&P)[TB][PL]) {
 #pragma unroll
         for (int d = 0; d < 2 * KS; d += 2) {
             vs_bits f[2][PL];
@@ -1148,8 +1166,55 @@ struct VsGrad {
 #pragma unroll
                 for (int p = 0; p < PL; ++p) f[r][p] = *(const vs_bits*)&T[((d + r) * PL + p) * 64];
             vs_mfma_parts<PL, 2, TB>(f, [&](int t, int p) { return P[t][p]; }, *(vs_f4(*)[2][TB]) & acc[d]);
-            if (OF_IDS && PL == 1)
-                if (hit) vs_mfma_parts<PL, 2, TB>(f, [&](int t, int) { return R[t]; }, *(vs_f4(*)[2][TB]) & acc[d]);
+        }
+    }
+
+    // OF_IDS: gl of the tokens whose target lies in the tile, in two parts of either type.  Rare: a token has one target.
+    __device__ __forceinline__ void targets(const VsBwd& a, const uint4* T, const float* of) {
+        const int lane = threadIdx.x & 63, quad = lane >> 4;
+        const int target = __float_as_int(of[VS_TOKEN_TARGET + (lane & 31)]);
+        if (!__any(target >= stay0 && target < stay0 + TB * 16)) return;
+#pragma unroll 1
+        for (int t = 0; t < TB; ++t) {
+            vs_f8 G;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int at = (j >> 2) * 16 + quad * 4 + (j & 3);
+                G[j] = __float_as_int(of[VS_TOKEN_TARGET + at]) == (int32_t)(stay0 + t * 16 + (lane & 15)) ? of[VS_TOKEN_GL + at] : 0.0f;
+            }
+            vs_bits part[2];
+#pragma unroll
+            for (int u = 0; u < TB; ++u)       // (registers have no index)
+                if (u == t) {
+                    db[u] += ((G[0] + G[1]) + (G[2] + G[3])) + ((G[4] + G[5]) + (G[6] + G[7]));
+                    if constexpr (PL == 2) {
+                        const float f_exp = of[VS_TOKEN_EXP];
+                        float m = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(G[j]));
+                        lower(u, m > 0.0f ? (float)__builtin_amdgcn_frexp_expf(m) + sg[u] - f_exp - AIM : 0.0f);
+                        const int by = (int)(sg[u] - f_exp);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) G[j] = ldexpf(G[j], by);
+                        vs_split<2>(G, part);
+                    } else {
+                        vs_split<1>(G, &part[0]);
+                        const vs_f8 rest = G - __builtin_convertvector(__builtin_bit_cast(vs_bf8, part[0]), vs_f8);
+                        vs_split<1>(rest, &part[1]);
+                    }
+#pragma unroll
+                    for (int d = 0; d < 2 * KS; ++d) {
+                        vs_f4 v = acc[d][u];
+#pragma unroll
+                        for (int p = 0; p < PL; ++p) {
+                            const vs_bits f = *(const vs_bits*)&T[(d * PL + p) * 64];
+                            v = vs_mfma<PL>(f, part[1], v);
+                            v = vs_mfma<PL>(f, part[0], v);
+                        }
+                        vs_in_place(v);
+                        acc[d][u] = v;
+                    }
+                }
         }
     }
 
@@ -1178,7 +1243,7 @@ struct VsGrad {
 
 // The stages in LDS.  TURNS = false: SR rows with both their fragments at a time, two stages (one worked on, one under way).
 // TURNS = true (wide rows): 32 rows, their S and their T fragments by turns, each under way while the other is worked on.
-template <int KS, int PL, int SR, bool OF_IDS>
+template <int KS, int PL, int SR, bool OF_IDS, bool ENTROPY>
 struct VsGradStage {
     static constexpr int HALF = SR * KS * PL * 4, INFO = (OF_IDS ? VS_TOKEN : VS_INFO), INFOS = SR / 32 * INFO;
     static constexpr int SIZE = 2 * HALF + (INFOS + 3) / 4;
@@ -1191,65 +1256,68 @@ struct VsGradStage {
     template <int TB>
     static __device__ __forceinline__ void step(const VsBwd& a, int base, bool more, const uint4* __restrict__ S, const uint4* __restrict__ T,
                                                 const float* __restrict__ info, uint4* __restrict__ to, const uint4* __restrict__ from,
-                                                VsGrad<KS, PL, TB, OF_IDS>& g) {
+                                                VsGrad<KS, PL, TB, OF_IDS, ENTROPY>& g) {
         const int lane = threadIdx.x & 63;
         vs_copies_done();
         __syncthreads();
         if (more) fetch(S, T, info, to);
 #pragma unroll 1
         for (int r = 0; r < SR; r += 32) {
-            vs_bits P[TB][PL], R[TB];
-            const bool hit = g.weights(a, base + r, from + r * KS * PL * 4 + lane, (const float*)(from + 2 * HALF) + r / 32 * INFO, P, R);
-            g.products(from + HALF + r * KS * PL * 4 + lane, P, R, hit);
+            vs_bits P[TB][PL];
+            const float* of = (const float*)(from + 2 * HALF) + r / 32 * INFO;
+            g.weights(a, base + r, from + r * KS * PL * 4 + lane, of, P);
+            g.products(from + HALF + r * KS * PL * 4 + lane, P);
+            if (OF_IDS) g.targets(a, from + HALF + r * KS * PL * 4 + lane, of);
         }
     }
-    // by turns
-    static __device__ __forceinline__ void fetch_s(const uint4* S, const float* info, uint4* to) {
-        vs_stage<HALF>(S, to);
+    // by turns: each half with its own copy of what goes with it
+    static constexpr int TURN = HALF + (INFO + 3) / 4;
+    static __device__ __forceinline__ void fetch_half(const uint4* half, const float* info, uint4* to) {
+        vs_stage<HALF>(half, to);
         vs_stage_floats<INFO>(info, (float*)(to + HALF));
     }
     template <int TB>
-    static __device__ __forceinline__ bool turn_s(const VsBwd& a, int base, const uint4* __restrict__ T, uint4* __restrict__ to, const uint4* __restrict__ from,
-                                                  VsGrad<KS, PL, TB, OF_IDS>& g, vs_bits (&P)[TB][PL], vs_bits (&R)[TB]) {
+    static __device__ __forceinline__ void turn_s(const VsBwd& a, int base, const uint4* __restrict__ T, const float* __restrict__ info, uint4* __restrict__ to,
+                                                  const uint4* __restrict__ from, VsGrad<KS, PL, TB, OF_IDS, ENTROPY>& g, vs_bits (&P)[TB][PL]) {
         vs_copies_done();
         __syncthreads();
-        vs_stage<HALF>(T, to);
-        return g.weights(a, base, from + (threadIdx.x & 63), (const float*)(from + HALF), P, R);
+        fetch_half(T, info, to);
+        g.weights(a, base, from + (threadIdx.x & 63), (const float*)(from + HALF), P);
     }
     template <int TB>
-    static __device__ __forceinline__ void turn_t(bool more, const uint4* __restrict__ S, const float* __restrict__ info, uint4* __restrict__ to,
-                                                  const uint4* __restrict__ from, VsGrad<KS, PL, TB, OF_IDS>& g, const vs_bits (&P)[TB][PL],
-                                                  const vs_bits (&R)[TB], bool hit) {
+    static __device__ __forceinline__ void turn_t(const VsBwd& a, bool more, const uint4* __restrict__ S, const float* __restrict__ info, uint4* __restrict__ to,
+                                                  const uint4* __restrict__ from, VsGrad<KS, PL, TB, OF_IDS, ENTROPY>& g, const vs_bits (&P)[TB][PL]) {
         vs_copies_done();
         __syncthreads();
-        if (more) fetch_s(S, info, to);
-        g.products(from + (threadIdx.x & 63), P, R, hit);
+        if (more) fetch_half(S, info, to);
+        g.products(from + (threadIdx.x & 63), P);
+        if (OF_IDS) g.targets(a, from + (threadIdx.x & 63), (const float*)(from + HALF));
     }
 };
 
-template <int KS, int PL, int TB, int SR, bool TURNS, bool OF_IDS>
+template <int KS, int PL, int TB, int SR, bool TURNS, bool OF_IDS, bool ENTROPY>
 __global__ __launch_bounds__(256, TB * KS * (4 * PL + 8) > 170 ? 1 : 2) void k_vs_backward(VsBwd a) {
-    using Stage = VsGradStage<KS, PL, SR, OF_IDS>;
-    constexpr int SIZE0 = TURNS ? Stage::HALF + (Stage::INFO + 3) / 4 : Stage::SIZE, SIZE1 = TURNS ? Stage::HALF : Stage::SIZE;
-    __shared__ uint4 buf0[SIZE0], buf1[SIZE1];
+    using Stage = VsGradStage<KS, PL, SR, OF_IDS, ENTROPY>;
+    constexpr int SIZE = TURNS ? Stage::TURN : Stage::SIZE;
+    __shared__ uint4 buf0[SIZE], buf1[SIZE];
     constexpr int PIECE = KS * PL * 4;         // 16-byte pieces of a row's fragments
     const int lane = threadIdx.x & 63;
     const int split = blockIdx.x % a.splits;
     const int tile = (blockIdx.x / a.splits) * 4 + (threadIdx.x >> 6);
     const bool live = tile < a.n_tiles;
-    VsGrad<KS, PL, TB, OF_IDS> g;
+    VsGrad<KS, PL, TB, OF_IDS, ENTROPY> g;
     g.start(a, live ? tile : 0, lane);
     const float* info = OF_IDS ? a.tokens : a.info;
     if constexpr (TURNS) {
         const int row_begin = (int)((int64_t)a.groups * split / a.splits) * 32, row_end = (int)((int64_t)a.groups * (split + 1) / a.splits) * 32;
         const uint4 *S = a.flowS + (int64_t)row_begin * PIECE, *T = a.flowT + (int64_t)row_begin * PIECE;
         info += (int64_t)row_begin / 32 * Stage::INFO;
-        Stage::fetch_s(S, info, buf0);
+        Stage::fetch_half(S, info, buf0);
         for (int base = row_begin; base < row_end; base += 32) {
-            vs_bits P[TB][PL], R[TB];
-            const bool hit = Stage::template turn_s<TB>(a, base, T, buf1, buf0, g, P, R);
+            vs_bits P[TB][PL];
+            Stage::template turn_s<TB>(a, base, T, info, buf1, buf0, g, P);
             S += 32 * PIECE; T += 32 * PIECE; info += Stage::INFO;
-            Stage::template turn_t<TB>(base + 32 < row_end, S, info, buf0, buf1, g, P, R, hit);
+            Stage::template turn_t<TB>(a, base + 32 < row_end, S, info, buf0, buf1, g, P);
         }
     } else {
         const int units = a.groups / (SR / 32);

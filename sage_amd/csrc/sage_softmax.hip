@@ -62,7 +62,7 @@ int vs_steps(int dim) {
 // How each width runs.  ks: 32-element steps of the padded row; pl: parts of a packed element (1 bf16, 2 float32).
 // 16-row blocks of stationary rows a wave holds: as many as leave two waves to a SIMD
 constexpr int vs_fwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 4 ? 4 : 2) : (ks <= 2 ? 4 : ks <= 8 ? 2 : 1); }
-constexpr int vs_bwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 2 ? 4 : ks <= 8 ? 2 : 1) : (ks <= 2 ? 4 : ks <= 4 ? 2 : 1); }
+constexpr int vs_bwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 2 ? 4 : ks <= 8 ? 2 : 1) : (ks <= 2 ? 2 : 1); }
 // streaming rows of a stage: two stages of 16 to 64 KiB
 constexpr int vs_fwd_rows(int ks, int pl) { return ks * pl <= 2 ? 128 : ks * pl <= 8 ? 64 : 32; }
 constexpr int vs_bwd_rows(int ks, int pl) { return ks * pl <= 4 ? 64 : 32; }
@@ -97,9 +97,9 @@ struct Shape {
     int dim, ks, pl, k, cus;
 };
 
-template <int KS, int PL> constexpr auto vs_fwd_kernel = &k_vs_forward<KS, PL, vs_fwd_blocks(KS, PL), vs_fwd_rows(KS, PL)>;
-template <int KS, int PL, bool OF_IDS>
-constexpr auto vs_bwd_kernel = &k_vs_backward<KS, PL, vs_bwd_blocks(KS, PL), vs_bwd_rows(KS, PL), vs_bwd_turns(KS, PL), OF_IDS>;
+template <int KS, int PL, bool TOP> constexpr auto vs_fwd_kernel = &k_vs_forward<KS, PL, vs_fwd_blocks(KS, PL), vs_fwd_rows(KS, PL), TOP>;
+template <int KS, int PL, bool OF_IDS, bool ENTROPY>
+constexpr auto vs_bwd_kernel = &k_vs_backward<KS, PL, vs_bwd_blocks(KS, PL), vs_bwd_rows(KS, PL), vs_bwd_turns(KS, PL), OF_IDS, ENTROPY>;
 
 // workgroups of a kernel that a CU holds at once (the same on every gfx950)
 template <auto KERNEL>
@@ -161,7 +161,7 @@ FwdPlan plan_fwd(const Shape& s, void* ws) {
         p.rows = std::min(s.n, VS_ROWS_MAX);
         p.n_pad = up(p.rows, VS_PAD);
         int64_t resident = s.cus;
-#define VS_F(KS, PL) p.tiles = cdiv(p.rows, vs_fwd_blocks(KS, PL) * 16); resident *= per_cu<vs_fwd_kernel<KS, PL>>()
+#define VS_F(KS, PL) p.tiles = cdiv(p.rows, vs_fwd_blocks(KS, PL) * 16); resident *= per_cu<vs_fwd_kernel<KS, PL, false>>()
         VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
         p.splits = vs_splits(resident, cdiv(p.tiles, 4), blocks, 1.0);
@@ -192,7 +192,7 @@ BwdPlan plan_bwd(const Shape& s, void* ws) {
 #define VS_F(KS, PL)                                                                            \
     p.tiles_x = cdiv(s.n, vs_bwd_blocks(KS, PL) * 16); p.tiles_w = cdiv(s.vocab, vs_bwd_blocks(KS, PL) * 16); \
     units_x = s.vp / vs_bwd_rows(KS, PL); units_w = p.np / vs_bwd_rows(KS, PL);                 \
-    resident_x *= per_cu<vs_bwd_kernel<KS, PL, false>>(); resident_w *= per_cu<vs_bwd_kernel<KS, PL, true>>()
+    resident_x *= per_cu<vs_bwd_kernel<KS, PL, false, false>>(); resident_w *= per_cu<vs_bwd_kernel<KS, PL, true, false>>()
     VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
     p.splits_x = vs_splits(resident_x, cdiv(p.tiles_x, 4), units_x, 8.0);
@@ -309,7 +309,7 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
         } else {
             pack(s, VsPack{xr, p.xS, nullptr, nullptr, p.x_exp, 1}, p.n_pad, st);
             const uint32_t grid = cdiv(p.tiles, 4) * p.splits;
-#define VS_F(KS, PL) vs_fwd_kernel<KS, PL><<<grid, 256, 0, st>>>(f)
+#define VS_F(KS, PL) if (alternatives) vs_fwd_kernel<KS, PL, true><<<grid, 256, 0, st>>>(f); else vs_fwd_kernel<KS, PL, false><<<grid, 256, 0, st>>>(f)
             VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
         }
@@ -369,17 +369,18 @@ int sage_token_logprobs_backward_device(sage_ctx* c, int32_t dtype, int64_t n, i
     pack(s, VsPack{x, p.xS, d_dweight ? p.xT : nullptr, nullptr, p.tokens + VS_TOKEN_EXP, VS_TOKEN}, p.np, st);
     pack_info(s, d_bias, p.info, st);
     k_vs_rows<<<cdiv(p.np, 256), 256, 0, st>>>(d_lse, d_entropy, d_targets, d_grad_logprob, d_grad_entropy, (int32_t)n, p.np, (int32_t)vocab, p.tokens);
+    const bool entropy = d_grad_entropy != nullptr;
     VsBwd b{};
-    b.info = p.info; b.tokens = p.tokens; b.has_bias = d_bias != nullptr; b.has_entropy = d_grad_entropy != nullptr; b.vocab = (int32_t)vocab;
+    b.info = p.info; b.tokens = p.tokens; b.has_bias = d_bias != nullptr; b.vocab = (int32_t)vocab;
     b.part = p.part;
     if (d_dx) {
         b.stayS = p.xS; b.flowS = p.wS; b.flowT = p.wT;
         b.n_tiles = (int32_t)p.tiles_x; b.splits = p.splits_x; b.groups = (int32_t)(s.vp / 32); b.stay_pad = p.np;
         const uint32_t grid = cdiv(p.tiles_x, 4) * p.splits_x;
-#define VS_F(KS, PL) vs_bwd_kernel<KS, PL, false><<<grid, 256, 0, st>>>(b)
+#define VS_F(KS, PL) if (entropy) vs_bwd_kernel<KS, PL, false, true><<<grid, 256, 0, st>>>(b); else vs_bwd_kernel<KS, PL, false, false><<<grid, 256, 0, st>>>(b)
         VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
-        const VsSum r{p.part, nullptr, (int32_t)n, dim, s.ks * 32, p.splits_x, p.np, p.tokens, b.has_entropy, w, d_dx, lddx, bf16, nullptr};
+        const VsSum r{p.part, nullptr, (int32_t)n, dim, s.ks * 32, p.splits_x, p.np, p.tokens, entropy, w, d_dx, lddx, bf16, nullptr};
         k_vs_sum<<<cdiv(n * dim, 256), 256, 0, st>>>(r);
     }
     if (d_dweight) {
@@ -387,7 +388,7 @@ int sage_token_logprobs_backward_device(sage_ctx* c, int32_t dtype, int64_t n, i
         b.n_tiles = (int32_t)p.tiles_w; b.splits = p.splits_w; b.groups = (int32_t)(p.np / 32); b.stay_pad = s.vp;
         b.want_db = d_dbias != nullptr; b.bias_part = p.bias_part;
         const uint32_t grid = cdiv(p.tiles_w, 4) * p.splits_w;
-#define VS_F(KS, PL) vs_bwd_kernel<KS, PL, true><<<grid, 256, 0, st>>>(b)
+#define VS_F(KS, PL) if (entropy) vs_bwd_kernel<KS, PL, true, true><<<grid, 256, 0, st>>>(b); else vs_bwd_kernel<KS, PL, true, false><<<grid, 256, 0, st>>>(b)
         VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
         const VsSum r{p.part, p.bias_part, (int32_t)vocab, dim, s.ks * 32, p.splits_w, s.vp, nullptr, 0, w, d_dweight, lddw, bf16, d_dbias};
