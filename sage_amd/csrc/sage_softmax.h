@@ -6,13 +6,14 @@
 //   G_nv = g_n (1[v = t(n)] - p_nv) - h_n p_nv (log p_nv + H_n)     (g, h: the gradients of logprob and H)
 //   dx = G w      dw = G^T x      db_v = sum_n G_nv
 //
-// Matrix layout.  Every product runs on v_mfma_f32_16x16x32_bf16.  A "stationary" operand (tokens in the forward pass and
-// for dx, ids for dw) stays in a wave's registers, the other one "streams" past it 32 rows at a time.  The product is taken
-// with the streaming rows as matrix rows and the stationary ones as columns: lane l then holds, of column l % 16, the
-// rows 4 (l / 16) .. + 3, so maxima and sums over the streaming axis need no lane to talk to another one until the end,
-// and the eight weights of two 16-row tiles are, as they lie in the registers, the second operand of the next product
-// (its 32 summation slots are the 32 streaming rows in the order 16 (j / 4) + 4 (l / 16) + j % 4; the transposed
-// fragments are laid out in that order).
+// Matrix layout.  A "stationary" operand (tokens in the forward pass and for dx, ids for dw) stays in a wave's registers, the
+// other one "streams" past it 32 rows at a time, on v_mfma_f32_32x32x16 (M = 32) or, where a wave's registers hold no 32 columns
+// (the widest rows, few tokens), v_mfma_f32_16x16x32 (M = 16).  The streaming rows are the matrix's rows and the stationary
+// ones its columns: lane l then holds, of column l % M, the values j = 0 .. M / 2 - 1 of rows RS (j / 4) + 4 (l / M) + j % 4, so
+// maxima and sums over the streaming axis need no lane to talk to another one until the end, and eight of the weights are, as
+// they lie in the registers, an operand of the next product (the transposed fragments list their rows in that order).
+// Vector instructions hide behind the 32x32 MFMA and hardly behind the 16x16 one (4 waves a SIMD, 16 fma and 3 exp
+// beside 131,072 products' MFMAs: 64 ns against 82, the MFMAs alone 55 and 61).
 //
 // bf16 inputs are multiplied as they are (products of two bf16 are exact in float32).  float32 inputs are taken as the sum of
 // two float16 (11 + 11 bits) and three of the four products are formed; what is left out is 2^-22 of |x||w|, the size of
@@ -28,19 +29,33 @@
 typedef __bf16 vs_bf8 __attribute__((ext_vector_type(8)));
 typedef float vs_f4 __attribute__((ext_vector_type(4)));
 typedef float vs_f8 __attribute__((ext_vector_type(8)));
+typedef float vs_f16 __attribute__((ext_vector_type(16)));
+
+template <int M> struct VsTile;
+template <> struct VsTile<16> {
+    using Acc = vs_f4;
+    static constexpr int K = 32, NB = 2, RS = 16;      // summation slots, row tiles of 32 rows
+};
+template <> struct VsTile<32> {
+    using Acc = vs_f16;
+    static constexpr int K = 16, NB = 1, RS = 8;
+};
+template <int M> constexpr int VS_NJ = M / 2;          // values of a lane in 32 rows x M columns
+template <int M> constexpr int VS_HALVES = M / 16;     // operands of the second product they make
+template <int M> __device__ __forceinline__ int vs_row(int j, int lane) { return (j >> 2) * VsTile<M>::RS + (lane / M) * 4 + (j & 3); }
 
 #define VS_LOG2E 1.4426950408889634f
 #define VS_LN2 0.6931471805599453f
 #define VS_CHUNK 16            // ids per stored maximum (the unit in which alternatives are looked for)
 #define VS_BLOCK 256           // ids are dealt out in blocks of this many
-// A chunk is what one lane of a fragment sees of 64 ids: 4 (of each of four 16-row tiles), so its maximum needs no other
-// lane.  Chunk c: of block c / 16 the lane quarter c / 4 % 4 of the 64 ids c % 4; a lane stores its four of a block at once.
+// A chunk is what one lane sees of 32 rows in a 32x32 tile: its maximum needs no other lane.  Chunk c: of block c / 16 the lane
+// half c / 8 % 2 of the 32 ids c % 8.
 __device__ __forceinline__ int vs_chunk_row(int c, int i) {      // the i-th of the 16 ids of a chunk
-    return (c >> 4) * VS_BLOCK + (c & 3) * 64 + (i >> 2) * 16 + ((c >> 2) & 3) * 4 + (i & 3);
+    return (c >> 4) * VS_BLOCK + (c & 7) * 32 + (i >> 2) * 8 + ((c >> 3) & 1) * 4 + (i & 3);
 }
 #define VS_NOTHING (-1.0e30f)  // reference of a row that has seen no finite logit yet; a bias this low masks its id
 #define VS_MASKED (-3.0e30f)   // what a masked logit is raised to: p is 0 there, and p times the exponent too
-#define VS_SLACK 4096.0f       // eight terms that sum to more than this move the running reference
+#define VS_SLACK 4096.0f       // a lane's terms of 32 rows that sum to more than this move the running reference
 #define VS_TMIN (-200.0f)      // 2^-200 is 0 in float32
 
 struct VsSrc {                 // a row-major matrix of float32 or bf16
@@ -61,23 +76,25 @@ __device__ __forceinline__ float vs_max(float a, float b) { return __builtin_ele
 typedef uint32_t vs_bits __attribute__((ext_vector_type(4)));
 typedef _Float16 vs_h8 __attribute__((ext_vector_type(8)));
 
-template <int PL>
-__device__ __forceinline__ vs_f4 vs_mfma(vs_bits a, vs_bits b, vs_f4 c) {
-    if constexpr (PL == 2) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vs_h8, a), __builtin_bit_cast(vs_h8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vs_bf8, a), __builtin_bit_cast(vs_bf8, b), c, 0, 0, 0);
+template <int PL, int M>
+__device__ __forceinline__ typename VsTile<M>::Acc vs_mfma(vs_bits a, vs_bits b, typename VsTile<M>::Acc c) {
+    const vs_h8 ah = __builtin_bit_cast(vs_h8, a), bh = __builtin_bit_cast(vs_h8, b);
+    const vs_bf8 ab = __builtin_bit_cast(vs_bf8, a), bb = __builtin_bit_cast(vs_bf8, b);
+    if constexpr (M == 32) return PL == 2 ? __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, c, 0, 0, 0) : __builtin_amdgcn_mfma_f32_32x32x16_bf16(ab, bb, c, 0, 0, 0);
+    else return PL == 2 ? __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, c, 0, 0, 0) : __builtin_amdgcn_mfma_f32_16x16x32_bf16(ab, bb, c, 0, 0, 0);
 }
 
 // c[r][t] += a[r] . b[t] for R x TB independent accumulators, both operands in PL parts (largest first): the products are the
 // outer loop, small ones first, so that an accumulator is not needed again right after it was written.
-template <int PL, int R, int TB, class B>
-__device__ __forceinline__ void vs_mfma_parts(const vs_bits (&a)[R][PL], const B& b, vs_f4 (&c)[R][TB]) {
+template <int PL, int M, int R, int TB, class B>
+__device__ __forceinline__ void vs_mfma_parts(const vs_bits (&a)[R][PL], const B& b, typename VsTile<M>::Acc (&c)[R][TB]) {
     constexpr int pa[6] = {1, 2, 0, 1, 0, 0}, pb[6] = {1, 0, 2, 0, 1, 0};
 #pragma unroll
     for (int q = PL == 3 ? 0 : PL == 2 ? 3 : 5; q < 6; ++q)
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int t = 0; t < TB; ++t) c[r][t] = vs_mfma<PL>(a[r][pa[q]], b(t, pb[q]), c[r][t]);
+            for (int t = 0; t < TB; ++t) c[r][t] = vs_mfma<PL, M>(a[r][pa[q]], b(t, pb[q]), c[r][t]);
 }
 
 // v as the sum of PL parts, each rounded to nearest: one bf16 (within 2^-9 |v|), two float16 (within 2^-23 |v| if |v| is between
@@ -106,9 +123,9 @@ __device__ __forceinline__ void vs_split(vs_f8 v, vs_bits* out) {
 }
 
 // ---- fragments ----------------------------------------------------------------------------------------------------
-// S fragments (16 rows x 32 elements): [row / 16][KS][PL][lane] of eight elements, lane l holding row l % 16, elements
-// 8 (l / 16).. .  T fragments (16 elements x 32 rows): [row / 32][2 KS][PL][lane], lane l holding element l % 16 and the rows
-// in the order 16 (j / 4) + 4 (l / 16) + j % 4.  Rows past the end and elements past `dim` are zero.  A fragment is one
+// 2 KS fragments of either kind for 32 rows, each [PL][lane] of eight elements.  S fragments (M rows x K elements): lane l
+// holds row l % M, elements 8 (l / M) .. .  T fragments (M elements x K rows): lane l holds element l % M and eight rows in the
+// order that a lane has values in.  Rows past the end and elements past `dim` are zero.  A fragment is one
 // coalesced 1 KiB load of a wave, whatever the caller's row length, stride and alignment are.  One workgroup packs 32 rows:
 // a lane loads the eight elements that its place in an S fragment asks for; T fragments are read back through LDS.
 // PL = 2: the 32 rows are multiplied by 2^e, e such that the largest finite element comes to just under 2^13.
@@ -139,21 +156,23 @@ struct VsPack {
     float* exps;               // PL = 2: e of group g at exps[g * exps_step]
     int32_t exps_step;
 };
-template <int KS, int PL>
+template <int KS, int PL, int M>
 __global__ __launch_bounds__(256) void k_vs_pack(VsPack a) {
     constexpr int DP = KS * 32, LD = DP + 4, N = (KS + 1) / 2;      // fragments of a wave
     __shared__ float tile[32 * LD];
     __shared__ float wmax[4], wfin[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+    constexpr int K = VsTile<M>::K, STEPS = DP / K;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane % M;
+    auto row_of = [&](int f) { return f / STEPS * M + col; };
+    auto element_of = [&](int f) { return f % STEPS * K + lane / M * 8; };
     const int64_t row0 = (int64_t)blockIdx.x * 32;
     vs_f8 v[N];
     float big = 0.0f, fin = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int f = i * 4 + wave, rb = f / KS, ks = f % KS;
-        const int64_t row = row0 + rb * 16 + col;
+        const int f = i * 4 + wave;
         v[i] = vs_f8(0.0f);
-        if (f < 2 * KS && row < a.src.rows && ks * 32 + quad * 8 < a.src.dim) v[i] = vs_eight<PL>(a.src, row, ks * 32 + quad * 8);
+        if (f < 2 * KS && row0 + row_of(f) < a.src.rows && element_of(f) < a.src.dim) v[i] = vs_eight<PL>(a.src, row0 + row_of(f), element_of(f));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float q = fabsf(v[i][j]);
@@ -174,31 +193,31 @@ __global__ __launch_bounds__(256) void k_vs_pack(VsPack a) {
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int f = i * 4 + wave, rb = f / KS, ks = f % KS;
+        const int f = i * 4 + wave;
         if (f >= 2 * KS) continue;
         if (PL == 2)
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] = ldexpf(v[i][j], e);
         if (a.T) {
-            float* to = tile + (rb * 16 + col) * LD + ks * 32 + quad * 8;
+            float* to = tile + row_of(f) * LD + element_of(f);
             *(vs_f4*)to = vs_f4{v[i][0], v[i][1], v[i][2], v[i][3]};
             *(vs_f4*)(to + 4) = vs_f4{v[i][4], v[i][5], v[i][6], v[i][7]};
         }
         vs_bits part[PL];
         vs_split<PL>(v[i], part);
 #pragma unroll
-        for (int p = 0; p < PL; ++p) *(vs_bits*)&a.S[((((int64_t)blockIdx.x * 2 + rb) * KS + ks) * PL + p) * 64 + lane] = part[p];
+        for (int p = 0; p < PL; ++p) *(vs_bits*)&a.S[(((int64_t)blockIdx.x * 2 * KS + f) * PL + p) * 64 + lane] = part[p];
     }
     if (!a.T) return;
     __syncthreads();
-    for (int db = wave; db < 2 * KS; db += 4) {
+    for (int f = wave; f < 2 * KS; f += 4) {
         vs_f8 q;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] = tile[((j >> 2) * 16 + quad * 4 + (j & 3)) * LD + db * 16 + col];
+        for (int j = 0; j < 8; ++j) q[j] = tile[vs_row<M>(f % VS_HALVES<M> * 8 + j, lane) * LD + f / VS_HALVES<M> * M + col];
         vs_bits part[PL];
         vs_split<PL>(q, part);
 #pragma unroll
-        for (int p = 0; p < PL; ++p) *(vs_bits*)&a.T[(((int64_t)blockIdx.x * 2 * KS + db) * PL + p) * 64 + lane] = part[p];
+        for (int p = 0; p < PL; ++p) *(vs_bits*)&a.T[(((int64_t)blockIdx.x * 2 * KS + f) * PL + p) * 64 + lane] = part[p];
     }
 }
 
@@ -212,12 +231,20 @@ __global__ __launch_bounds__(256) void k_vs_bias(const float* __restrict__ bias,
     if (v < padded) info[(v >> 5) * VS_INFO + (v & 31)] = v >= vocab ? -INFINITY : !bias ? 0.0f : bias[v] <= VS_NOTHING ? -INFINITY : bias[v] * unit;
 }
 
-// All four are known before any is written back: without this the compiler takes a new register quadruple for what a rarely
-// taken branch changes, and copies the old one into it each time the branch is not taken.
-__device__ __forceinline__ void vs_in_place(vs_f4& v) {
-    float a = v[0], b = v[1], c = v[2], d = v[3];
-    asm volatile("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
-    v = vs_f4{a, b, c, d};
+// All are known before any is written back: without this the compiler takes new registers for what a rarely taken branch
+// changes, and copies the old ones into them each time the branch is not taken.
+template <class V>
+__device__ __forceinline__ void vs_in_place(V& v) {
+    constexpr int N = sizeof(V) / 4;
+    float a[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = v[i];
+    if constexpr (N == 4) asm volatile("" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]));
+    else
+        asm volatile("" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(a[4]), "+v"(a[5]), "+v"(a[6]), "+v"(a[7]), "+v"(a[8]), "+v"(a[9]),
+                     "+v"(a[10]), "+v"(a[11]), "+v"(a[12]), "+v"(a[13]), "+v"(a[14]), "+v"(a[15]));
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = a[i];
 }
 
 // 2^n as a factor of log2(e), kept finite (logits beyond float32 are inf or 0 all the same)
@@ -230,7 +257,7 @@ struct VsFwd {
     const float* x_exp;        // PL = 2: [tokens / 32]
     int32_t has_bias;          // the caller gave one: -inf may stand anywhere (else only past `vocab`)
     int32_t vocab;
-    int32_t n_tiles;           // token tiles of 16 TB rows
+    int32_t n_tiles;           // token tiles of TB M rows
     int32_t splits;            // ranges of the vocabulary
     int32_t blocks;            // blocks of VS_BLOCK ids
     int32_t chunks;            // chunks of VS_CHUNK ids: 16 a block
@@ -263,32 +290,50 @@ struct VsStat {
     }
 };
 
-// 32 streaming rows against the stationary ones: s[rb][t] += w . x
-template <int KS, int PL, int TB>
-__device__ __forceinline__ void vs_product(const uint4* w, const vs_bits (&x)[TB][KS][PL], vs_f4 (&s)[2][TB]) {
+template <int KS, int PL, int M>
+using VsOperand = vs_bits[KS * 32 / VsTile<M>::K][PL];         // the fragments of M stationary rows
+template <int M, int TB>
+using VsLogits = typename VsTile<M>::Acc[VsTile<M>::NB][TB];
+template <int M, int TB>
+__device__ __forceinline__ float vs_value(const VsLogits<M, TB>& s, int t, int j) {
+    constexpr int NI = VS_NJ<M> / VsTile<M>::NB;
+    return s[j / NI][t][j % NI];
+}
+template <int M, int TB>
+__device__ __forceinline__ void vs_set(VsLogits<M, TB>& s, int t, int j, float v) {
+    constexpr int NI = VS_NJ<M> / VsTile<M>::NB;
+    s[j / NI][t][j % NI] = v;
+}
+
+// 32 streaming rows against the stationary ones: s += w . x
+template <int KS, int PL, int M, int TB>
+__device__ __forceinline__ void vs_product(const uint4* w, const VsOperand<KS, PL, M> (&x)[TB], VsLogits<M, TB>& s) {
+    constexpr int STEPS = KS * 32 / VsTile<M>::K, NB = VsTile<M>::NB;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-        vs_bits wf[2][PL];
+    for (int k = 0; k < STEPS; ++k) {
+        vs_bits wf[NB][PL];
 #pragma unroll
-        for (int rb = 0; rb < 2; ++rb)
+        for (int rb = 0; rb < NB; ++rb)
 #pragma unroll
-            for (int p = 0; p < PL; ++p) wf[rb][p] = *(const vs_bits*)&w[((rb * KS + k) * PL + p) * 64];
-        vs_mfma_parts<PL, 2, TB>(wf, [&](int t, int p) { return x[t][k][p]; }, s);
+            for (int p = 0; p < PL; ++p) wf[rb][p] = *(const vs_bits*)&w[((rb * STEPS + k) * PL + p) * 64];
+        vs_mfma_parts<PL, M, NB, TB>(wf, [&](int t, int p) { return x[t][k][p]; }, s);
     }
 }
 
-template <int KS, int PL, int TB>
-__device__ __forceinline__ void vs_stationary(const uint4* S, int64_t tile, int lane, vs_bits (&x)[TB][KS][PL]) {
+template <int KS, int PL, int M, int TB>
+__device__ __forceinline__ void vs_stationary(const uint4* S, int64_t tile, int lane, VsOperand<KS, PL, M> (&x)[TB]) {
+    constexpr int STEPS = KS * 32 / VsTile<M>::K;
 #pragma unroll
     for (int t = 0; t < TB; ++t)
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+        for (int k = 0; k < STEPS; ++k)
 #pragma unroll
-            for (int p = 0; p < PL; ++p) x[t][k][p] = *(const vs_bits*)&S[(((tile * TB + t) * KS + k) * PL + p) * 64 + lane];
+            for (int p = 0; p < PL; ++p) x[t][k][p] = *(const vs_bits*)&S[(((tile * TB + t) * STEPS + k) * PL + p) * 64 + lane];
 }
 
-template <int TB>
+template <int M, int TB>
 struct VsRowsOfTile {
+    static constexpr int NJ = VS_NJ<M>;
     VsStat st[TB];
     float top[TB];
     vs_f4 keep[TB];
@@ -298,15 +343,15 @@ struct VsRowsOfTile {
     }
     // the logits of 32 ids, in powers of two after multiplication by unit[t]; TOP: their largest is kept
     template <bool TOP, bool SCALED>
-    __device__ __forceinline__ void add(const vs_f4 (&s)[2][TB], const float (&unit)[TB]) {
+    __device__ __forceinline__ void add(const VsLogits<M, TB>& s, const float (&unit)[TB]) {
         float ls[TB], le[TB];
         auto sums = [&]() {
             float most = 0.0f;
 #pragma unroll
             for (int t = 0; t < TB; ++t) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float e = fmaf(s[j >> 2][t][j & 3], SCALED ? unit[t] : VS_LOG2E, -st[t].ref), p = __builtin_amdgcn_exp2f(e);
+                for (int j = 0; j < NJ; ++j) {
+                    const float e = fmaf(vs_value<M, TB>(s, t, j), SCALED ? unit[t] : VS_LOG2E, -st[t].ref), p = __builtin_amdgcn_exp2f(e);
                     ls[t] = j ? ls[t] + p : p;
                     le[t] = j ? fmaf(p, e, le[t]) : p * e;
                 }
@@ -323,29 +368,35 @@ struct VsRowsOfTile {
         for (int t = 0; t < TB; ++t) {
             st[t].s += ls[t];
             st[t].e += le[t];
-            if (TOP) top[t] = vs_max(top[t], SCALED ? largest(s, t) * (unit[t] * VS_LN2) : largest(s, t));
+            if (TOP) top[t] = SCALED ? largest(s, t) * (unit[t] * VS_LN2) : largest(s, t);
         }
     }
-    static __device__ __forceinline__ float largest(const vs_f4 (&s)[2][TB], int t) {
-        const float m = vs_max(vs_max(vs_max(s[0][t][0], s[0][t][1]), s[0][t][2]), vs_max(vs_max(s[0][t][3], s[1][t][0]), s[1][t][1]));
-        return vs_max(vs_max(m, s[1][t][2]), s[1][t][3]);
+    static __device__ __forceinline__ float largest(const VsLogits<M, TB>& s, int t) {
+        auto v = [&](int j) { return vs_value<M, TB>(s, t, j); };
+        float m = vs_max(vs_max(v(0), v(1)), v(2)), n = vs_max(vs_max(v(3), v(4)), v(5));
+#pragma unroll
+        for (int j = 6; j < NJ; j += 4) {
+            m = vs_max(vs_max(m, v(j)), v(j + 1));
+            if (j + 3 < NJ) n = vs_max(vs_max(n, v(j + 2)), v(j + 3));
+        }
+        return vs_max(m, n);
     }
-    // 64 ids are done, the h-th of their block: their largest logits are stored with those of the rest of the block, sixteen
-    // bytes a lane (WHOLE: the wave sees whole blocks), or at once
+    // step h of a block (32 ids) is done: the largest logits of four steps are stored together (WHOLE: the wave sees whole
+    // blocks), or at once.  Two lanes of a 16-column tile share a chunk.
     template <bool WHOLE>
     __device__ __forceinline__ void chunk(const VsFwd& a, int64_t tile, int block, int h, int lane, bool live) {
-        {
+        const int part = lane / M;
 #pragma unroll
-            for (int t = 0; t < TB; ++t) {
-                float* to = a.chunk_max + ((tile * TB + t) * 16 + (lane & 15)) * a.chunks + block * 16 + (lane >> 4) * 4;
-                if (WHOLE) {
-                    if (h == 0) keep[t][0] = top[t];
-                    else if (h == 1) keep[t][1] = top[t];
-                    else if (h == 2) keep[t][2] = top[t];
-                    else if (live) *(vs_f4*)to = vs_f4{keep[t][0], keep[t][1], keep[t][2], top[t]};
-                } else if (live) to[h] = top[t];
-                top[t] = -INFINITY;
-            }
+        for (int t = 0; t < TB; ++t) {
+            const float m = M == 32 ? top[t] : vs_max(top[t], __shfl_xor(top[t], 32));
+            float* to = a.chunk_max + ((tile * TB + t) * M + lane % M) * a.chunks + block * 16 + (part & 1) * 8;
+            const bool mine = live && part < 2;
+            if (WHOLE) {
+                if ((h & 3) == 0) keep[t][0] = m;
+                else if ((h & 3) == 1) keep[t][1] = m;
+                else if ((h & 3) == 2) keep[t][2] = m;
+                else if (mine) *(vs_f4*)(to + (h & ~3)) = vs_f4{keep[t][0], keep[t][1], keep[t][2], m};
+            } else if (mine) to[h] = m;
         }
     }
     __device__ __forceinline__ void flush() {
@@ -357,7 +408,7 @@ struct VsRowsOfTile {
         for (int t = 0; t < TB; ++t) {
             st[t].flush();
 #pragma unroll
-            for (int o = 16; o <= 32; o <<= 1) {
+            for (int o = M; o <= 32; o <<= 1) {
                 const float r2 = __shfl_xor(st[t].ref, o), s2 = __shfl_xor(st[t].S, o), e2 = __shfl_xor(st[t].E, o);
                 st[t].join(r2, s2, e2);
             }
@@ -366,45 +417,50 @@ struct VsRowsOfTile {
     __device__ __forceinline__ void store(const VsFwd& a, int64_t tile, int split, int lane) {
         join_lanes();
 #pragma unroll
-        for (int t = 0; t < TB; ++t) {
-            if (lane < 16) a.part[(int64_t)split * a.n_pad + (tile * TB + t) * 16 + lane] = make_float4(st[t].ref, st[t].S, st[t].E, 0.0f);
-        }
+        for (int t = 0; t < TB; ++t)
+            if (lane < M) a.part[(int64_t)split * a.n_pad + (tile * TB + t) * M + lane] = make_float4(st[t].ref, st[t].S, st[t].E, 0.0f);
     }
 };
 
 // Adds the biases where the product did not start from them, and raises masked logits.
-template <int TB, bool SCALED>
-__device__ __forceinline__ void vs_mask(vs_f4 (&s)[2][TB], float (&unit)[TB], const vs_f4 (&b)[2]) {
+template <int M, int TB, bool SCALED>
+__device__ __forceinline__ void vs_mask(VsLogits<M, TB>& s, float (&unit)[TB], const vs_f4 (&b)[VS_NJ<M> / 4]) {
 #pragma unroll
     for (int t = 0; t < TB; ++t) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float v = s[j >> 2][t][j & 3];
+        for (int j = 0; j < VS_NJ<M>; ++j) {
+            float v = vs_value<M, TB>(s, t, j);
             if (SCALED) v = fmaf(v, unit[t], b[j >> 2][j & 3]);
-            s[j >> 2][t][j & 3] = vs_max(v, VS_MASKED);
+            vs_set<M, TB>(s, t, j, vs_max(v, VS_MASKED));
         }
         if (SCALED) unit[t] = 1.0f;
     }
 }
 
+// What 32 rows' logits start from: their biases (`of`: by row), or 0 where the product is scaled
+template <int PL, int M, int TB>
+__device__ __forceinline__ void vs_begin(const float* of, int lane, VsLogits<M, TB>& s, vs_f4 (&b)[VS_NJ<M> / 4]) {
+#pragma unroll
+    for (int q = 0; q < VS_NJ<M> / 4; ++q) b[q] = *(const vs_f4*)&of[vs_row<M>(q * 4, lane)];
+#pragma unroll
+    for (int t = 0; t < TB; ++t)
+#pragma unroll
+        for (int j = 0; j < VS_NJ<M>; ++j) vs_set<M, TB>(s, t, j, PL == 1 ? b[j >> 2][j & 3] : 0.0f);
+}
+
 // 32 ids against a tile: their logits are formed and counted
-template <int KS, int PL, int TB, bool TOP>
-__device__ __forceinline__ void vs_forward_step(const VsFwd& a, int row0, const uint4* w, const float* info, const vs_bits (&x)[TB][KS][PL],
-                                                const float (&x_exp)[TB], VsRowsOfTile<TB>& rows) {
-    const int lane = threadIdx.x & 63, quad = lane >> 4;
-    vs_f4 s[2][TB], b[2];
+template <int KS, int PL, int M, int TB, bool TOP>
+__device__ __forceinline__ void vs_forward_step(const VsFwd& a, int row0, const uint4* w, const float* info, const VsOperand<KS, PL, M> (&x)[TB],
+                                                const float (&x_exp)[TB], VsRowsOfTile<M, TB>& rows) {
+    VsLogits<M, TB> s;
+    vs_f4 b[VS_NJ<M> / 4];
     float unit[TB];
-#pragma unroll
-    for (int rb = 0; rb < 2; ++rb) {
-        b[rb] = *(const vs_f4*)&info[rb * 16 + quad * 4];
-#pragma unroll
-        for (int t = 0; t < TB; ++t) s[rb][t] = PL == 1 ? b[rb] : vs_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    vs_begin<PL, M, TB>(info, threadIdx.x & 63, s, b);
     const float e = PL == 2 ? info[VS_INFO_EXP] : 0.0f;
 #pragma unroll
     for (int t = 0; t < TB; ++t) unit[t] = PL == 2 ? vs_unit(-(e + x_exp[t])) : VS_LOG2E;
-    vs_product<KS, PL, TB>(w, x, s);
-    if (a.has_bias || row0 + 32 > a.vocab) vs_mask<TB, PL == 2>(s, unit, b);      // (the same in the whole grid)
+    vs_product<KS, PL, M, TB>(w, x, s);
+    if (a.has_bias || row0 + 32 > a.vocab) vs_mask<M, TB, PL == 2>(s, unit, b);      // (the same in the whole grid)
     rows.template add<TOP, PL == 2>(s, unit);
 }
 
@@ -428,7 +484,7 @@ __device__ __forceinline__ void vs_copies_done() { __builtin_amdgcn_s_waitcnt(0x
 
 // A stage: SR rows of fragments and what goes with them.  `to` and `from` are different stages, and the compiler has to know
 // it (__restrict__ through an inlined function): else it waits for the copy under way before each read of LDS.
-template <int KS, int PL, int SR>
+template <int KS, int PL, int M, int SR>
 struct VsStage {
     static constexpr int N = SR * KS * PL * 4, INFO = SR / 32 * VS_INFO, SIZE = N + INFO / 4;
     static __device__ __forceinline__ void fetch(const uint4* w, const float* info, uint4* to) {
@@ -437,8 +493,8 @@ struct VsStage {
     }
     template <int TB, bool TOP>
     static __device__ __forceinline__ void step(const VsFwd& a, int base, bool more, const uint4* __restrict__ next, const float* __restrict__ next_info,
-                                                uint4* __restrict__ to, const uint4* __restrict__ from, const vs_bits (&x)[TB][KS][PL],
-                                                const float (&x_exp)[TB], VsRowsOfTile<TB>& rows, int64_t tile, bool live) {
+                                                uint4* __restrict__ to, const uint4* __restrict__ from, const VsOperand<KS, PL, M> (&x)[TB],
+                                                const float (&x_exp)[TB], VsRowsOfTile<M, TB>& rows, int64_t tile, bool live) {
         const int lane = threadIdx.x & 63;
         vs_copies_done();                  // (a barrier alone does not wait for them)
         __syncthreads();                   // `from` has arrived, and nobody reads `to` any more
@@ -446,28 +502,28 @@ struct VsStage {
 #pragma unroll 1
         for (int r = 0; r < SR; r += 32) {
             const int row0 = base + r;
-            vs_forward_step<KS, PL, TB, TOP>(a, row0, from + r * KS * PL * 4 + lane, (const float*)(from + N) + r / 32 * VS_INFO, x, x_exp, rows);
-            if (TOP && (row0 & 32)) rows.template chunk<true>(a, tile, row0 / VS_BLOCK, (row0 >> 6) & 3, lane, live);
+            vs_forward_step<KS, PL, M, TB, TOP>(a, row0, from + r * KS * PL * 4 + lane, (const float*)(from + N) + r / 32 * VS_INFO, x, x_exp, rows);
+            if (TOP) rows.template chunk<true>(a, tile, row0 / VS_BLOCK, (row0 >> 5) & 7, lane, live);
         }
         if (((base + SR) & (VS_BLOCK - 1)) == 0) rows.flush();
     }
 };
 
-template <int KS, int PL, int TB, int SR, bool TOP>
+template <int KS, int PL, int M, int TB, int SR, bool TOP>
 __global__ __launch_bounds__(256, 2) void k_vs_forward(VsFwd a) {
-    using Stage = VsStage<KS, PL, SR>;
+    using Stage = VsStage<KS, PL, M, SR>;
     __shared__ uint4 buf0[Stage::SIZE], buf1[Stage::SIZE];
     const int lane = threadIdx.x & 63;
     const int split = blockIdx.x % a.splits;
     const int tile = (blockIdx.x / a.splits) * 4 + (threadIdx.x >> 6);
     const bool live = tile < a.n_tiles;
     const int row_begin = (int)((int64_t)a.blocks * split / a.splits) * VS_BLOCK, row_end = (int)((int64_t)a.blocks * (split + 1) / a.splits) * VS_BLOCK;
-    vs_bits x[TB][KS][PL];
-    vs_stationary<KS, PL, TB>(a.xS, live ? tile : 0, lane, x);
+    VsOperand<KS, PL, M> x[TB];
+    vs_stationary<KS, PL, M, TB>(a.xS, live ? tile : 0, lane, x);
     float x_exp[TB];
 #pragma unroll
-    for (int t = 0; t < TB; ++t) x_exp[t] = PL == 2 ? a.x_exp[((live ? tile : 0) * TB + t) / 2] : 0.0f;
-    VsRowsOfTile<TB> rows;
+    for (int t = 0; t < TB; ++t) x_exp[t] = PL == 2 ? a.x_exp[((live ? tile : 0) * TB + t) * M / 32] : 0.0f;
+    VsRowsOfTile<M, TB> rows;
     rows.clear();
     const uint4* w = a.wS + (int64_t)row_begin * KS * PL * 4;
     const float* info = a.info + row_begin / 32 * VS_INFO;
@@ -563,7 +619,7 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
             vs_split<PL>(v, x[t][k]);
         }
     }
-    VsRowsOfTile<TB> rows;
+    VsRowsOfTile<16, TB> rows;
     rows.clear();
     const float unscaled[TB] = {};
     const int units = gridDim.x * 4, unit = blockIdx.x * 4 + (threadIdx.x >> 6), pieces = a.f.blocks * 4;
@@ -599,7 +655,7 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
                             big.measure(raw[rb][k]);
                             raw[rb][k].parts(wf[rb]);
                         }
-                        vs_mfma_parts<PL, 2, TB>(wf, [&](int t, int p) { return x[t][g + k][p]; }, s);
+                        vs_mfma_parts<PL, 16, 2, TB>(wf, [&](int t, int p) { return x[t][g + k][p]; }, s);
                     }
                 if (KG < KS) __builtin_amdgcn_sched_barrier(0);     // (the loads of all groups at once would spill)
             }
@@ -618,8 +674,8 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
                 if (lane == 0 && tile == 0) a.group_max[row0 / 32] = m;
             }
             rows.template add<true, false>(s, unscaled);
+            if (a.f.chunk_max) rows.template chunk<false>(a.f, tile, row0 / VS_BLOCK, (row0 >> 5) & 7, lane, true);
         }
-        if (a.f.chunk_max) rows.template chunk<false>(a.f, tile, c >> 2, c & 3, lane, true);
         if ((c & 3) == 3) rows.flush();
     }
     rows.join_lanes();
@@ -1000,7 +1056,7 @@ struct VsBwd {
     float* bias_part;          // [splits][stay_pad]
 };
 
-// A wave: a tile of 16 TB stationary rows against one range of the streaming ones.  OF_IDS = false: the stationary rows
+// A wave: a tile of TB M stationary rows against one range of the streaming ones.  OF_IDS = false: the stationary rows
 // are tokens, the result sum_v p' w_v with p' = p (A + B e), or p alone when there is no entropy gradient (A is then a
 // factor of the whole row, applied at the end); the target's own term is added at the end too, so that the largest
 // coefficient is never rounded to bf16.  OF_IDS = true: the stationary rows are ids, the result sum_n G_nv x_n; the targets'
@@ -1008,20 +1064,23 @@ struct VsBwd {
 //
 // Two float16 parts (PL = 2) of a weight: column t is kept multiplied by 2^sg[t], sg as large as the largest weight of the column
 // so far allows (2^15 after the streaming rows' scale), and the sums with it.  It starts high and falls a few times.
-template <int KS, int PL, int TB, bool OF_IDS, bool ENTROPY>
+template <int KS, int PL, int M, int TB, bool OF_IDS, bool ENTROPY>
 struct VsGrad {
     static constexpr float MOST = 15.0f, AIM = 13.0f;
-    vs_bits y[TB][KS][PL];
-    vs_f4 acc[2 * KS][TB];
+    static constexpr int NJ = VS_NJ<M>, HALVES = VS_HALVES<M>, BLOCKS = KS * 32 / M;
+    using Acc = typename VsTile<M>::Acc;
+    using Weights = vs_bits[HALVES][PL];       // of one column, by streaming row
+    VsOperand<KS, PL, M> y[TB];
+    Acc acc[BLOCKS][TB];
     float L[TB], A[TB], B[TB], db[TB], y_exp[TB], sg[TB], norm[TB];   // (of ids, L is the bias)
     int64_t stay0;
 
     __device__ __forceinline__ void start(const VsBwd& a, int64_t tile, int lane) {
-        vs_stationary<KS, PL, TB>(a.stayS, tile, lane, y);
-        stay0 = tile * TB * 16;
+        vs_stationary<KS, PL, M, TB>(a.stayS, tile, lane, y);
+        stay0 = tile * TB * M;
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
-            const int64_t r = stay0 + t * 16 + (lane & 15);
+            const int64_t r = stay0 + t * M + lane % M;
             db[t] = 0.0f; sg[t] = 300.0f; norm[t] = 0.0f;
             if constexpr (OF_IDS) {
                 const float* of = a.info + (r >> 5) * VS_INFO;
@@ -1040,70 +1099,68 @@ struct VsGrad {
             }
         }
 #pragma unroll
-        for (int d = 0; d < 2 * KS; ++d)
+        for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
-            for (int t = 0; t < TB; ++t) acc[d][t] = vs_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int t = 0; t < TB; ++t) acc[d][t] = Acc(0.0f);
     }
 
     // column t gives up the powers of two that its lanes ask for (`ask` <= 0: none)
     __device__ __forceinline__ void lower(int t, float ask) {
-        ask = fmaxf(ask, __shfl_xor(ask, 16));
+        if (M == 16) ask = fmaxf(ask, __shfl_xor(ask, 16));
         ask = fmaxf(ask, __shfl_xor(ask, 32));
         if (!(ask > 0.0f)) ask = 0.0f;
         sg[t] -= ask;
 #pragma unroll
-        for (int d = 0; d < 2 * KS; ++d) {
-            vs_f4 v;
+        for (int d = 0; d < BLOCKS; ++d) {
+            Acc v;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = ldexpf(acc[d][t][i], -(int)ask);
+            for (int i = 0; i < M * M / 64; ++i) v[i] = ldexpf(acc[d][t][i], -(int)ask);
             vs_in_place(v);
             acc[d][t] = v;
         }
     }
 
     // P: the weights of the 32 streaming rows from row0 on, in parts, without the targets' own terms
-    __device__ __forceinline__ void weights(const VsBwd& a, int row0, const uint4* S, const float* of, vs_bits (&P)[TB][PL]) {
-        const int quad = (threadIdx.x & 63) >> 4;
-        vs_f4 s[2][TB], b[2];
+    __device__ __forceinline__ void weights(const VsBwd& a, int row0, const uint4* S, const float* of, Weights (&P)[TB]) {
+        const int lane = threadIdx.x & 63;
+        VsLogits<M, TB> s;
+        vs_f4 b[NJ / 4];
         float unit[TB];
         const float f_exp = PL == 2 ? of[OF_IDS ? VS_TOKEN_EXP : VS_INFO_EXP] : 0.0f;
+        if constexpr (OF_IDS) {
 #pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
-            if constexpr (!OF_IDS) b[rb] = *(const vs_f4*)&of[rb * 16 + quad * 4];
+            for (int t = 0; t < TB; ++t)
 #pragma unroll
-            for (int t = 0; t < TB; ++t) {
-                if constexpr (PL == 2) s[rb][t] = vs_f4{0.0f, 0.0f, 0.0f, 0.0f};
-                else if constexpr (OF_IDS) s[rb][t] = vs_f4{L[t], L[t], L[t], L[t]};
-                else s[rb][t] = b[rb];
-            }
-        }
+                for (int j = 0; j < NJ; ++j) vs_set<M, TB>(s, t, j, PL == 1 ? L[t] : 0.0f);
+        } else vs_begin<PL, M, TB>(of, lane, s, b);
 #pragma unroll
         for (int t = 0; t < TB; ++t) unit[t] = PL == 2 ? vs_unit(-(f_exp + y_exp[t])) : VS_LOG2E;
-        vs_product<KS, PL, TB>(S, y, s);
-        if (a.has_bias || (OF_IDS ? stay0 + TB * 16 > a.vocab : row0 + 32 > a.vocab)) {
+        vs_product<KS, PL, M, TB>(S, y, s);
+        if (a.has_bias || (OF_IDS ? stay0 + TB * M > a.vocab : row0 + 32 > a.vocab)) {
             if constexpr (OF_IDS) {
 #pragma unroll
                 for (int t = 0; t < TB; ++t) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        float v = s[j >> 2][t][j & 3];
+                    for (int j = 0; j < NJ; ++j) {
+                        float v = vs_value<M, TB>(s, t, j);
                         if (PL == 2) v = fmaf(v, unit[t], L[t]);
-                        s[j >> 2][t][j & 3] = vs_max(v, VS_MASKED);
+                        vs_set<M, TB>(s, t, j, vs_max(v, VS_MASKED));
                     }
                     if (PL == 2) unit[t] = 1.0f;
                 }
-            } else vs_mask<TB, PL == 2>(s, unit, b);
+            } else vs_mask<M, TB, PL == 2>(s, unit, b);
         }
-        vs_f8 G[TB];
+        float G[TB][NJ];
         float big[TB];                         // PL = 2: the power of two that a column's largest scaled weight is below
         auto form = [&]() {
-            vs_f4 rl[2], ra[2], rb_[2];
+            vs_f4 rl[NJ / 4], ra[NJ / 4], rb[NJ / 4];
             if constexpr (OF_IDS) {
 #pragma unroll
-                for (int rb = 0; rb < 2; ++rb) {
-                    rl[rb] = *(const vs_f4*)&of[rb * 16 + quad * 4];
-                    ra[rb] = *(const vs_f4*)&of[VS_TOKEN_A + rb * 16 + quad * 4];
-                    if (ENTROPY) rb_[rb] = *(const vs_f4*)&of[VS_TOKEN_B + rb * 16 + quad * 4];
+                for (int q = 0; q < NJ / 4; ++q) {
+                    const float* at = of + vs_row<M>(q * 4, lane);
+                    rl[q] = *(const vs_f4*)at;
+                    ra[q] = *(const vs_f4*)(at + VS_TOKEN_A);
+                    if (ENTROPY) rb[q] = *(const vs_f4*)(at + VS_TOKEN_B);
                 }
             }
             float most = 0.0f;
@@ -1112,13 +1169,13 @@ struct VsGrad {
                 const float shift = PL == 2 ? sg[t] - f_exp : 0.0f;
                 float m = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float v = s[j >> 2][t][j & 3];
+                for (int j = 0; j < NJ; ++j) {
+                    const float v = vs_value<M, TB>(s, t, j);
                     if constexpr (OF_IDS) {
                         float e = fmaf(v, PL == 2 ? unit[t] : VS_LOG2E, -rl[j >> 2][j & 3]);
                         const float p = __builtin_amdgcn_exp2f(e);
                         if (ENTROPY) e = vs_max(e, VS_TMIN);
-                        G[t][j] = p * (ENTROPY ? fmaf(rb_[j >> 2][j & 3], e, ra[j >> 2][j & 3]) : ra[j >> 2][j & 3]);
+                        G[t][j] = p * (ENTROPY ? fmaf(rb[j >> 2][j & 3], e, ra[j >> 2][j & 3]) : ra[j >> 2][j & 3]);
                         if (PL == 2) m = fmaxf(m, fabsf(G[t][j]));
                     } else {
                         float e = fmaf(v, PL == 2 ? unit[t] : VS_LOG2E, shift - L[t]);
@@ -1145,55 +1202,64 @@ struct VsGrad {
             }
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
-            if constexpr (OF_IDS) {
-                if (a.want_db) db[t] += ((G[t][0] + G[t][1]) + (G[t][2] + G[t][3])) + ((G[t][4] + G[t][5]) + (G[t][6] + G[t][7]));
-                if constexpr (PL == 2) {
-                    const int by = (int)(sg[t] - f_exp);
+            if constexpr (OF_IDS)
+                if (a.want_db) {
+                    float v = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) G[t][j] = ldexpf(G[t][j], by);
+                    for (int j = 0; j < NJ; j += 4) v += (G[t][j] + G[t][j + 1]) + (G[t][j + 2] + G[t][j + 3]);
+                    db[t] += v;
                 }
+            const int by = PL == 2 ? (int)(sg[t] - f_exp) : 0;
+#pragma unroll
+            for (int u = 0; u < HALVES; ++u) {
+                vs_f8 v;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = PL == 2 && OF_IDS ? ldexpf(G[t][u * 8 + j], by) : G[t][u * 8 + j];
+                vs_split<PL>(v, P[t][u]);
             }
-            vs_split<PL>(G[t], P[t]);
         }
     }
 
-    __device__ __forceinline__ void products(const uint4* T, const vs_bits (&P)[TB][PL]) {
+    __device__ __forceinline__ void products(const uint4* T, const Weights (&P)[TB]) {
+        constexpr int R = BLOCKS % 2 ? 1 : 2;      // blocks at once: their accumulators are independent
 #pragma unroll
-        for (int d = 0; d < 2 * KS; d += 2) {
-            vs_bits f[2][PL];
+        for (int d = 0; d < BLOCKS; d += R)
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
+            for (int u = 0; u < HALVES; ++u) {
+                vs_bits f[R][PL];
 #pragma unroll
-                for (int p = 0; p < PL; ++p) f[r][p] = *(const vs_bits*)&T[((d + r) * PL + p) * 64];
-            vs_mfma_parts<PL, 2, TB>(f, [&](int t, int p) { return P[t][p]; }, *(vs_f4(*)[2][TB]) & acc[d]);
-        }
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int p = 0; p < PL; ++p) f[r][p] = *(const vs_bits*)&T[(((d + r) * HALVES + u) * PL + p) * 64];
+                vs_mfma_parts<PL, M, R, TB>(f, [&](int t, int p) { return P[t][u][p]; }, *(Acc(*)[R][TB]) & acc[d]);
+            }
     }
 
     // OF_IDS: gl of the tokens whose target lies in the tile, in two parts of either type.  Rare: a token has one target.
     __device__ __forceinline__ void targets(const VsBwd& a, const uint4* T, const float* of) {
-        const int lane = threadIdx.x & 63, quad = lane >> 4;
+        const int lane = threadIdx.x & 63;
         const int target = __float_as_int(of[VS_TOKEN_TARGET + (lane & 31)]);
-        if (!__any(target >= stay0 && target < stay0 + TB * 16)) return;
+        if (!__any(target >= stay0 && target < stay0 + TB * M)) return;
+        const float f_exp = PL == 2 ? of[VS_TOKEN_EXP] : 0.0f;
 #pragma unroll 1
-        for (int t = 0; t < TB; ++t) {
+        for (int q = 0; q < TB * HALVES; ++q) {
+            const int t = q / HALVES, u = q % HALVES;
             vs_f8 G;
+            float m = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int at = (j >> 2) * 16 + quad * 4 + (j & 3);
-                G[j] = __float_as_int(of[VS_TOKEN_TARGET + at]) == (int32_t)(stay0 + t * 16 + (lane & 15)) ? of[VS_TOKEN_GL + at] : 0.0f;
+                const int at = vs_row<M>(u * 8 + j, lane);
+                G[j] = __float_as_int(of[VS_TOKEN_TARGET + at]) == (int32_t)(stay0 + t * M + lane % M) ? of[VS_TOKEN_GL + at] : 0.0f;
+                m = fmaxf(m, fabsf(G[j]));
             }
             vs_bits part[2];
 #pragma unroll
-            for (int u = 0; u < TB; ++u)       // (registers have no index)
-                if (u == t) {
-                    db[u] += ((G[0] + G[1]) + (G[2] + G[3])) + ((G[4] + G[5]) + (G[6] + G[7]));
+            for (int v = 0; v < TB; ++v)       // (registers have no index)
+                if (v == t) {
+                    db[v] += ((G[0] + G[1]) + (G[2] + G[3])) + ((G[4] + G[5]) + (G[6] + G[7]));
                     if constexpr (PL == 2) {
-                        const float f_exp = of[VS_TOKEN_EXP];
-                        float m = 0.0f;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(G[j]));
-                        lower(u, m > 0.0f ? (float)__builtin_amdgcn_frexp_expf(m) + sg[u] - f_exp - AIM : 0.0f);
-                        const int by = (int)(sg[u] - f_exp);
+                        lower(v, m > 0.0f ? (float)__builtin_amdgcn_frexp_expf(m) + sg[v] - f_exp - AIM : 0.0f);
+                        const int by = (int)(sg[v] - f_exp);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) G[j] = ldexpf(G[j], by);
                         vs_split<2>(G, part);
@@ -1203,39 +1269,40 @@ struct VsGrad {
                         vs_split<1>(rest, &part[1]);
                     }
 #pragma unroll
-                    for (int d = 0; d < 2 * KS; ++d) {
-                        vs_f4 v = acc[d][u];
+                    for (int d = 0; d < BLOCKS; ++d) {
+                        Acc c = acc[d][v];
 #pragma unroll
                         for (int p = 0; p < PL; ++p) {
-                            const vs_bits f = *(const vs_bits*)&T[(d * PL + p) * 64];
-                            v = vs_mfma<PL>(f, part[1], v);
-                            v = vs_mfma<PL>(f, part[0], v);
+                            const vs_bits f = *(const vs_bits*)&T[((d * HALVES + u) * PL + p) * 64];
+                            c = vs_mfma<PL, M>(f, part[1], c);
+                            c = vs_mfma<PL, M>(f, part[0], c);
                         }
-                        vs_in_place(v);
-                        acc[d][u] = v;
+                        vs_in_place(c);
+                        acc[d][v] = c;
                     }
                 }
         }
     }
 
     __device__ __forceinline__ void store(const VsBwd& a, int split, int lane) {
-        const int col = lane & 15, quad = lane >> 4;
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
-            const int64_t r = stay0 + t * 16 + col;
+            const int64_t r = stay0 + t * M + lane % M;
             float* out = a.part + ((int64_t)split * a.stay_pad + r) * (KS * 32);
 #pragma unroll
-            for (int d = 0; d < 2 * KS; ++d) {
-                vs_f4 v = acc[d][t];
-                if (PL == 2)
+            for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = ldexpf(v[i], (int)(norm[t] - sg[t]));
-                *(vs_f4*)&out[d * 16 + quad * 4] = v;
-            }
+                for (int q = 0; q < M * M / 256; ++q) {
+                    vs_f4 v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = PL == 2 ? ldexpf(acc[d][t][q * 4 + i], (int)(norm[t] - sg[t])) : acc[d][t][q * 4 + i];
+                    *(vs_f4*)&out[d * M + q * 8 + lane / M * 4] = v;
+                }
             if (OF_IDS && a.want_db) {
-                float v = db[t] + __shfl_xor(db[t], 16);
+                float v = db[t];
+                if (M == 16) v += __shfl_xor(v, 16);
                 v += __shfl_xor(v, 32);
-                if (quad == 0) a.bias_part[(int64_t)split * a.stay_pad + r] = v;
+                if (lane < M) a.bias_part[(int64_t)split * a.stay_pad + r] = v;
             }
         }
     }
@@ -1243,8 +1310,9 @@ struct VsGrad {
 
 // The stages in LDS.  TURNS = false: SR rows with both their fragments at a time, two stages (one worked on, one under way).
 // TURNS = true (wide rows): 32 rows, their S and their T fragments by turns, each under way while the other is worked on.
-template <int KS, int PL, int SR, bool OF_IDS, bool ENTROPY>
+template <int KS, int PL, int M, int TB, int SR, bool OF_IDS, bool ENTROPY>
 struct VsGradStage {
+    using Grad = VsGrad<KS, PL, M, TB, OF_IDS, ENTROPY>;
     static constexpr int HALF = SR * KS * PL * 4, INFO = (OF_IDS ? VS_TOKEN : VS_INFO), INFOS = SR / 32 * INFO;
     static constexpr int SIZE = 2 * HALF + (INFOS + 3) / 4;
     static __device__ __forceinline__ void fetch(const uint4* S, const uint4* T, const float* info, uint4* to) {
@@ -1253,17 +1321,16 @@ struct VsGradStage {
 #pragma unroll
         for (int i = 0; i < SR / 32; ++i) vs_stage_floats<INFO>(info + i * INFO, (float*)(to + 2 * HALF) + i * INFO);
     }
-    template <int TB>
     static __device__ __forceinline__ void step(const VsBwd& a, int base, bool more, const uint4* __restrict__ S, const uint4* __restrict__ T,
                                                 const float* __restrict__ info, uint4* __restrict__ to, const uint4* __restrict__ from,
-                                                VsGrad<KS, PL, TB, OF_IDS, ENTROPY>& g) {
+                                                Grad& g) {
         const int lane = threadIdx.x & 63;
         vs_copies_done();
         __syncthreads();
         if (more) fetch(S, T, info, to);
 #pragma unroll 1
         for (int r = 0; r < SR; r += 32) {
-            vs_bits P[TB][PL];
+            typename Grad::Weights P[TB];
             const float* of = (const float*)(from + 2 * HALF) + r / 32 * INFO;
             g.weights(a, base + r, from + r * KS * PL * 4 + lane, of, P);
             g.products(from + HALF + r * KS * PL * 4 + lane, P);
@@ -1276,17 +1343,15 @@ struct VsGradStage {
         vs_stage<HALF>(half, to);
         vs_stage_floats<INFO>(info, (float*)(to + HALF));
     }
-    template <int TB>
     static __device__ __forceinline__ void turn_s(const VsBwd& a, int base, const uint4* __restrict__ T, const float* __restrict__ info, uint4* __restrict__ to,
-                                                  const uint4* __restrict__ from, VsGrad<KS, PL, TB, OF_IDS, ENTROPY>& g, vs_bits (&P)[TB][PL]) {
+                                                  const uint4* __restrict__ from, Grad& g, typename Grad::Weights (&P)[TB]) {
         vs_copies_done();
         __syncthreads();
         fetch_half(T, info, to);
         g.weights(a, base, from + (threadIdx.x & 63), (const float*)(from + HALF), P);
     }
-    template <int TB>
     static __device__ __forceinline__ void turn_t(const VsBwd& a, bool more, const uint4* __restrict__ S, const float* __restrict__ info, uint4* __restrict__ to,
-                                                  const uint4* __restrict__ from, VsGrad<KS, PL, TB, OF_IDS, ENTROPY>& g, const vs_bits (&P)[TB][PL]) {
+                                                  const uint4* __restrict__ from, Grad& g, const typename Grad::Weights (&P)[TB]) {
         vs_copies_done();
         __syncthreads();
         if (more) fetch_half(S, info, to);
@@ -1295,9 +1360,9 @@ struct VsGradStage {
     }
 };
 
-template <int KS, int PL, int TB, int SR, bool TURNS, bool OF_IDS, bool ENTROPY>
-__global__ __launch_bounds__(256, TB * KS * (4 * PL + 8) > 170 ? 1 : 2) void k_vs_backward(VsBwd a) {
-    using Stage = VsGradStage<KS, PL, SR, OF_IDS, ENTROPY>;
+template <int KS, int PL, int M, int TB, int SR, bool TURNS, bool OF_IDS, bool ENTROPY>
+__global__ __launch_bounds__(256, TB * M * KS * (4 * PL + 8) > 170 * 16 ? 1 : 2) void k_vs_backward(VsBwd a) {
+    using Stage = VsGradStage<KS, PL, M, TB, SR, OF_IDS, ENTROPY>;
     constexpr int SIZE = TURNS ? Stage::TURN : Stage::SIZE;
     __shared__ uint4 buf0[SIZE], buf1[SIZE];
     constexpr int PIECE = KS * PL * 4;         // 16-byte pieces of a row's fragments
@@ -1305,7 +1370,7 @@ __global__ __launch_bounds__(256, TB * KS * (4 * PL + 8) > 170 ? 1 : 2) void k_v
     const int split = blockIdx.x % a.splits;
     const int tile = (blockIdx.x / a.splits) * 4 + (threadIdx.x >> 6);
     const bool live = tile < a.n_tiles;
-    VsGrad<KS, PL, TB, OF_IDS, ENTROPY> g;
+    typename Stage::Grad g;
     g.start(a, live ? tile : 0, lane);
     const float* info = OF_IDS ? a.tokens : a.info;
     if constexpr (TURNS) {
@@ -1314,10 +1379,10 @@ __global__ __launch_bounds__(256, TB * KS * (4 * PL + 8) > 170 ? 1 : 2) void k_v
         info += (int64_t)row_begin / 32 * Stage::INFO;
         Stage::fetch_half(S, info, buf0);
         for (int base = row_begin; base < row_end; base += 32) {
-            vs_bits P[TB][PL];
-            Stage::template turn_s<TB>(a, base, T, info, buf1, buf0, g, P);
+            typename Stage::Grad::Weights P[TB];
+            Stage::turn_s(a, base, T, info, buf1, buf0, g, P);
             S += 32 * PIECE; T += 32 * PIECE; info += Stage::INFO;
-            Stage::template turn_t<TB>(a, base + 32 < row_end, S, info, buf0, buf1, g, P);
+            Stage::turn_t(a, base + 32 < row_end, S, info, buf0, buf1, g, P);
         }
     } else {
         const int units = a.groups / (SR / 32);
@@ -1327,10 +1392,10 @@ __global__ __launch_bounds__(256, TB * KS * (4 * PL + 8) > 170 ? 1 : 2) void k_v
         Stage::fetch(S, T, info, buf0);
         for (int base = row_begin; base < row_end; base += 2 * SR) {
             S += SR * PIECE; T += SR * PIECE; info += Stage::INFOS;
-            Stage::template step<TB>(a, base, base + SR < row_end, S, T, info, buf1, buf0, g);
+            Stage::step(a, base, base + SR < row_end, S, T, info, buf1, buf0, g);
             if (base + SR >= row_end) break;
             S += SR * PIECE; T += SR * PIECE; info += Stage::INFOS;
-            Stage::template step<TB>(a, base + SR, base + 2 * SR < row_end, S, T, info, buf0, buf1, g);
+            Stage::step(a, base + SR, base + 2 * SR < row_end, S, T, info, buf0, buf1, g);
         }
     }
     if (live) g.store(a, split, lane);

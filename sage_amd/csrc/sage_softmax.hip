@@ -60,12 +60,23 @@ int vs_steps(int dim) {
 }
 
 // How each width runs.  ks: 32-element steps of the padded row; pl: parts of a packed element (1 bf16, 2 float32).
-// 16-row blocks of stationary rows a wave holds: as many as leave two waves to a SIMD
-constexpr int vs_fwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 4 ? 4 : 2) : (ks <= 2 ? 4 : ks <= 8 ? 2 : 1); }
-constexpr int vs_bwd_blocks(int ks, int pl) { return pl == 1 ? (ks <= 2 ? 4 : ks <= 8 ? 2 : 1) : (ks <= 2 ? 2 : 1); }
+// Columns of a tile (the matrix instruction's) and tiles of a wave, as measured for each width (ks = 2, 4, 8, 10, 16 at
+// D = 50, 100, 200, 300, 500, 4,096 tokens x 65,536 ids, D = 50 twice that both ways; us, best first, then the other choices in turn):
+//   forward   32x2 32x2 16x2 32x2 32x1   float32   431 [458 489 490]   192 [207 200]   337 [359 688]   476 [531 498]   864 [949 1193]
+//             32x2 32x2 32x2 16x2 16x2   bf16      268 [303 308]       106 [111 113]   156 [168 167]   190 [204 181]   281 [304 656]
+//     (16x2 against 32x2 at ks = 10, bf16: 347 against 385 with alternatives)
+//   dx        16x2 16x2 16x1 16x2 16x1   float32   714 [773 803 908]   351 [378 417]   751 [821 915]   1,259 [1,563]   2,623 [4,732]
+//             16x2 16x2 16x1 16x1 16x1   bf16      286 [279 321 333]   144 [157 164]   300 [305 354]   379 [438 441]   628 [670 682]
+//   dw        16x2 16x2 16x1 16x2 16x1   float32   765 [757 836 896]   379 [409 448]   796 [1,058]     1,540 [1,617]   2,613 [4,576]
+//             16x2 16x2 16x1 16x1 16x2   bf16      350 [350 396 445]   166 [185 216]   364 [438 463]   447 [554 899]   922 [1,385]
+// (Wider than that the sums of a gradient spill; 16-column tiles give an accumulator time to be ready.)
+constexpr int vs_fwd_tile(int ks, int pl) { return pl == 1 ? (ks <= 8 ? 32 : 16) : ks == 8 ? 16 : 32; }
+constexpr int vs_fwd_blocks(int ks, int pl) { return pl == 2 && ks == 16 ? 1 : 2; }
+constexpr int vs_bwd_tile(int, int) { return 16; }
+constexpr int vs_bwd_blocks(int ks, int pl, bool of_ids) { return ks <= 4 || (pl == 2 && ks == 10) || (pl == 1 && ks == 16 && of_ids) ? 2 : 1; }
 // streaming rows of a stage: two stages of 16 to 64 KiB
 constexpr int vs_fwd_rows(int ks, int pl) { return ks * pl <= 2 ? 128 : ks * pl <= 8 ? 64 : 32; }
-constexpr int vs_bwd_rows(int ks, int pl) { return ks * pl <= 4 ? 64 : 32; }
+constexpr int vs_bwd_rows(int, int) { return 32; }
 constexpr bool vs_bwd_turns(int ks, int) { return ks >= 8; }
 // 16-token blocks of a wave that reads the weights as they lie (the three bf16 parts of float32 are formed there)
 constexpr int vs_raw_parts(int pl) { return pl == 1 ? 1 : 3; }
@@ -97,9 +108,9 @@ struct Shape {
     int dim, ks, pl, k, cus;
 };
 
-template <int KS, int PL, bool TOP> constexpr auto vs_fwd_kernel = &k_vs_forward<KS, PL, vs_fwd_blocks(KS, PL), vs_fwd_rows(KS, PL), TOP>;
+template <int KS, int PL, bool TOP> constexpr auto vs_fwd_kernel = &k_vs_forward<KS, PL, vs_fwd_tile(KS, PL), vs_fwd_blocks(KS, PL), vs_fwd_rows(KS, PL), TOP>;
 template <int KS, int PL, bool OF_IDS, bool ENTROPY>
-constexpr auto vs_bwd_kernel = &k_vs_backward<KS, PL, vs_bwd_blocks(KS, PL), vs_bwd_rows(KS, PL), vs_bwd_turns(KS, PL), OF_IDS, ENTROPY>;
+constexpr auto vs_bwd_kernel = &k_vs_backward<KS, PL, vs_bwd_tile(KS, PL), vs_bwd_blocks(KS, PL, OF_IDS), vs_bwd_rows(KS, PL), vs_bwd_turns(KS, PL), OF_IDS, ENTROPY>;
 
 // workgroups of a kernel that a CU holds at once (the same on every gfx950)
 template <auto KERNEL>
@@ -161,7 +172,7 @@ FwdPlan plan_fwd(const Shape& s, void* ws) {
         p.rows = std::min(s.n, VS_ROWS_MAX);
         p.n_pad = up(p.rows, VS_PAD);
         int64_t resident = s.cus;
-#define VS_F(KS, PL) p.tiles = cdiv(p.rows, vs_fwd_blocks(KS, PL) * 16); resident *= per_cu<vs_fwd_kernel<KS, PL, false>>()
+#define VS_F(KS, PL) p.tiles = cdiv(p.rows, vs_fwd_blocks(KS, PL) * vs_fwd_tile(KS, PL)); resident *= per_cu<vs_fwd_kernel<KS, PL, false>>()
         VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
         p.splits = vs_splits(resident, cdiv(p.tiles, 4), blocks, 1.0);
@@ -190,7 +201,7 @@ BwdPlan plan_bwd(const Shape& s, void* ws) {
     p.np = up(s.n, VS_PAD);
     int64_t units_w = 1, units_x = 1, resident_x = s.cus, resident_w = s.cus;
 #define VS_F(KS, PL)                                                                            \
-    p.tiles_x = cdiv(s.n, vs_bwd_blocks(KS, PL) * 16); p.tiles_w = cdiv(s.vocab, vs_bwd_blocks(KS, PL) * 16); \
+    p.tiles_x = cdiv(s.n, vs_bwd_blocks(KS, PL, false) * vs_bwd_tile(KS, PL)); p.tiles_w = cdiv(s.vocab, vs_bwd_blocks(KS, PL, true) * vs_bwd_tile(KS, PL)); \
     units_x = s.vp / vs_bwd_rows(KS, PL); units_w = p.np / vs_bwd_rows(KS, PL);                 \
     resident_x *= per_cu<vs_bwd_kernel<KS, PL, false, false>>(); resident_w *= per_cu<vs_bwd_kernel<KS, PL, true, false>>()
     VS_BY_WIDTH(s.ks, s.pl, VS_F);
@@ -240,8 +251,9 @@ int check_workspace(sage_ctx* c, const void* p, int64_t have, int64_t need) {
     return sage_ctx_fail(c, SAGE_E_ARG, msg);
 }
 
+template <bool FORWARD>
 void pack(const Shape& s, const VsPack& p, int64_t padded, hipStream_t st) {
-#define VS_F(KS, PL) k_vs_pack<KS, PL><<<(uint32_t)(padded / 32), 256, 0, st>>>(p)
+#define VS_F(KS, PL) k_vs_pack<KS, PL, FORWARD ? vs_fwd_tile(KS, PL) : vs_bwd_tile(KS, PL)><<<(uint32_t)(padded / 32), 256, 0, st>>>(p)
     VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
 }
@@ -289,7 +301,7 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
     const hipStream_t st = (hipStream_t)stream;
     const VsSrc w{d_weight, ldw, (int32_t)vocab, dim, dtype == SAGE_BF16}, x{d_x, ldx, (int32_t)n, dim, dtype == SAGE_BF16};
     if (!p.raw) {
-        pack(s, VsPack{w, p.wS, nullptr, alternatives ? p.group_max : nullptr, p.info + VS_INFO_EXP, VS_INFO}, s.vp, st);
+        pack<true>(s, VsPack{w, p.wS, nullptr, alternatives ? p.group_max : nullptr, p.info + VS_INFO_EXP, VS_INFO}, s.vp, st);
         pack_info(s, d_bias, p.info, st);
     }
     for (int64_t r0 = 0; r0 < n; r0 += p.rows) {
@@ -307,7 +319,7 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
             VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
         } else {
-            pack(s, VsPack{xr, p.xS, nullptr, nullptr, p.x_exp, 1}, p.n_pad, st);
+            pack<true>(s, VsPack{xr, p.xS, nullptr, nullptr, p.x_exp, 1}, p.n_pad, st);
             const uint32_t grid = cdiv(p.tiles, 4) * p.splits;
 #define VS_F(KS, PL) if (alternatives) vs_fwd_kernel<KS, PL, true><<<grid, 256, 0, st>>>(f); else vs_fwd_kernel<KS, PL, false><<<grid, 256, 0, st>>>(f)
             VS_BY_WIDTH(s.ks, s.pl, VS_F);
@@ -365,8 +377,8 @@ int sage_token_logprobs_backward_device(sage_ctx* c, int32_t dtype, int64_t n, i
     const BwdPlan p = plan_bwd(s, d_workspace);
     if ((rc = check_workspace(c, d_workspace, workspace_bytes, p.bytes))) return rc;
     const VsSrc w{d_weight, ldw, (int32_t)vocab, dim, bf16}, x{d_x, ldx, (int32_t)n, dim, bf16};
-    pack(s, VsPack{w, p.wS, d_dx ? p.wT : nullptr, nullptr, p.info + VS_INFO_EXP, VS_INFO}, s.vp, st);
-    pack(s, VsPack{x, p.xS, d_dweight ? p.xT : nullptr, nullptr, p.tokens + VS_TOKEN_EXP, VS_TOKEN}, p.np, st);
+    pack<false>(s, VsPack{w, p.wS, d_dx ? p.wT : nullptr, nullptr, p.info + VS_INFO_EXP, VS_INFO}, s.vp, st);
+    pack<false>(s, VsPack{x, p.xS, d_dweight ? p.xT : nullptr, nullptr, p.tokens + VS_TOKEN_EXP, VS_TOKEN}, p.np, st);
     pack_info(s, d_bias, p.info, st);
     k_vs_rows<<<cdiv(p.np, 256), 256, 0, st>>>(d_lse, d_entropy, d_targets, d_grad_logprob, d_grad_entropy, (int32_t)n, p.np, (int32_t)vocab, p.tokens);
     const bool entropy = d_grad_entropy != nullptr;
