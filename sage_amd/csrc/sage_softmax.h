@@ -705,27 +705,33 @@ struct VsJoin {
 template <int WAVES>
 __device__ __forceinline__ float vs_join_row(const VsJoin& a, int64_t row, int tid, float4* red, double* dred) {
     const int lane = tid & 63, wave = tid >> 6;
-    VsStat st;
-    st.clear();
-    for (int i = tid; i < a.splits; i += 64 * WAVES) {
-        const float4 q = a.part[(int64_t)i * a.n_pad + row];
-        st.join(q.x, q.y, q.z);
-    }
+    const bool alone = WAVES == 1 || a.splits <= 64;       // few ranges: the first wave joins them, the others are told
     const int64_t t = a.targets ? a.targets[row] : -1;
+    VsStat st;
     double dot = 0.0;
-    if (t >= 0 && t < a.w.rows)
-        for (int d = tid; d < a.w.dim; d += 64 * WAVES) dot += (double)vs_load(a.x, row, d) * (double)vs_load(a.w, t, d);
-    for (int o = 1; o < 64; o <<= 1) {
-        const float r2 = __shfl_xor(st.ref, o), s2 = __shfl_xor(st.S, o), e2 = __shfl_xor(st.E, o);
-        st.join(r2, s2, e2);
-        dot += __shfl_xor(dot, o);
+    st.clear();
+    if (!alone || wave == 0) {
+        const int step = alone ? 64 : 64 * WAVES;
+        for (int i = tid; i < a.splits; i += step) {
+            const float4 q = a.part[(int64_t)i * a.n_pad + row];
+            st.join(q.x, q.y, q.z);
+        }
+        if (t >= 0 && t < a.w.rows)
+            for (int d = tid; d < a.w.dim; d += step) dot += (double)vs_load(a.x, row, d) * (double)vs_load(a.w, t, d);
+        for (int o = 1; o < 64; o <<= 1) {
+            if (o < a.splits) {                // (the first lane has them all)
+                const float r2 = __shfl_xor(st.ref, o), s2 = __shfl_xor(st.S, o), e2 = __shfl_xor(st.E, o);
+                st.join(r2, s2, e2);
+            }
+            dot += __shfl_xor(dot, o);
+        }
+        if (WAVES > 1 && lane == 0) { red[wave] = make_float4(st.ref, st.S, st.E, 0.0f); dred[wave] = dot; }
     }
     if constexpr (WAVES > 1) {
-        if (lane == 0) { red[wave] = make_float4(st.ref, st.S, st.E, 0.0f); dred[wave] = dot; }
         __syncthreads();
         st.clear();
         dot = 0.0;
-        for (int i = 0; i < WAVES; ++i) { st.join(red[i].x, red[i].y, red[i].z); dot += dred[i]; }
+        for (int i = 0; i < (alone ? 1 : WAVES); ++i) { st.join(red[i].x, red[i].y, red[i].z); dot += dred[i]; }
     }
     const bool empty = st.S == 0.0f;                // nothing but -inf
     const double lse = empty ? -INFINITY : ((double)st.ref + (double)log2f(st.S)) * 0.6931471805599453;
@@ -808,34 +814,49 @@ __device__ __forceinline__ float vs_row_sum(float v) {
     return v;
 }
 
-// x . row over 16 lanes (xs: x in LDS); the result is in all of them.  The last piece of a row that is no whole number of
-// pieces long is taken back from the row's end, with the elements before it weighted 0 -- no read leaves the row.
-template <bool BF16>
-__device__ __forceinline__ float vs_dot16(const VsSrc& w, int64_t row, const float* xs, int l16) {
+// x . row over LANES lanes, each its part (xs: x in LDS, and behind it, from xs[dim up to a whole piece], the last piece again as
+// it is multiplied: a row that is no whole number of pieces long has it taken back from the row's end, with the elements
+// before it weighted 0 -- no read leaves the row).
+template <bool BF16, int LANES, class T>
+__device__ __forceinline__ T vs_dot(const VsSrc& w, int64_t row, const float* xs, int lane) {
     constexpr int E = VsVec<BF16>::E;
-    float s = 0.0f;
+    T s = 0;
     if (w.dim < E) {
-        if (l16 < w.dim) s = xs[l16] * vs_load(w, row, l16);
+        if (lane < w.dim) s = (T)xs[lane] * (T)vs_load(w, row, lane);
     } else {
-        for (int d = l16 * E; d < w.dim; d += 16 * E) {
-            const int at = min(d, w.dim - E);
+        const int whole = w.dim / E * E;
+        for (int d = lane * E; d < w.dim; d += LANES * E) {
             VsVec<BF16> v;
-            v.load(w.p, row * w.ld + at);
+            v.load(w.p, row * w.ld + min(d, w.dim - E));
+            const float* x = xs + (d < whole ? d : whole + E);
 #pragma unroll
-            for (int i = 0; i < E; ++i) s = at + i >= d ? fmaf(xs[at + i], v.f[i], s) : s;
+            for (int i = 0; i < E; ++i) s = fma((T)x[i], (T)v.f[i], s);
         }
     }
-    return vs_row_sum(s);
+    return s;
+}
+// x into LDS in that form, by all threads
+template <bool BF16>
+__device__ __forceinline__ float vs_put_x(const VsSrc& x, int64_t row, float* xs, int tid, int threads) {      // -> this thread's sum of sizes
+    constexpr int E = VsVec<BF16>::E;
+    const int whole = x.dim / E * E;
+    float l1 = 0.0f;
+    for (int d = tid; d < x.dim; d += threads) {
+        const float v = vs_load(x, row, d);
+        xs[d] = v;
+        l1 += fabsf(v);
+    }
+    if (x.dim > E && tid < E) xs[whole + E + tid] = x.dim - E + tid >= whole ? vs_load(x, row, x.dim - E + tid) : 0.0f;
+    return l1;
 }
 
 template <bool BF16, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
     const VsSrc &x = a.join.x, &w = a.join.w;
-    __shared__ float xs[512];
-    __shared__ float best[256];
+    __shared__ __align__(16) float xs[512 + 16], best[256];
     __shared__ double cv[VS_CAND], cw[VS_MAX_K];
     __shared__ int ci[VS_CAND], cj[VS_MAX_K];
-    __shared__ float red[THREADS / 64];
+    __shared__ float red[THREADS / 64], red2[THREADS / 64];
     __shared__ uint32_t found[4];
     __shared__ uint16_t list[VS_LIST], rows[VS_CAND];
     __shared__ int n_cand, n_rows, n_list;
@@ -848,32 +869,34 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
         if (tid < a.k) { a.ids[row * a.k + tid] = -1; a.logprobs[row * a.k + tid] = NAN; }
         return;
     }
-    float l1 = 0.0f;
-    for (int d = tid; d < x.dim; d += THREADS) { const float v = vs_load(x, row, d); xs[d] = v; l1 += fabsf(v); }
-    for (int o = 1; o < 64; o <<= 1) l1 += __shfl_xor(l1, o);
-    if (lane == 0) red[wave] = l1;
+    float l1 = vs_put_x<BF16>(x, row, xs, tid, THREADS), widest = 0.0f;
+#pragma unroll 4
+    for (int g = tid * 4; g < a.chunks / 2; g += THREADS * 4) {
+        const float4 q = *(const float4*)&a.group_max[g];
+        widest = fmaxf(widest, fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)));
+    }
+    for (int o = 1; o < 64; o <<= 1) { l1 += __shfl_xor(l1, o); widest = fmaxf(widest, __shfl_xor(widest, o)); }
+    if (lane == 0) { red[wave] = l1; red2[wave] = widest; }
     if (tid == 0) n_cand = n_rows = n_list = 0;
     __syncthreads();
     l1 = 0.0f;
-    for (int i = 0; i < THREADS / 64; ++i) l1 += red[i];
+    for (int i = 0; i < THREADS / 64; ++i) { l1 += red[i]; widest = fmaxf(widest, red2[i]); }
     __syncthreads();
     const float eps = 4.0f * (float)(x.dim + 16) * 5.9604645e-8f;
-    auto widest = [&](int block) {          // eps 2 |x|_1 max |w| of the block
-        const float4 p = *(const float4*)&a.group_max[block * 8], q = *(const float4*)&a.group_max[block * 8 + 4];
-        return eps * 2.0f * l1 * fmaxf(fmaxf(fmaxf(p.x, p.y), fmaxf(p.z, p.w)), fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)));
-    };
-    auto off = [&](int c, float m) { return fmaf(eps, fabsf(m), widest(c >> 4)); };
-    float low = -INFINITY;
+    const float slack = eps * 2.0f * l1 * widest;
+    auto off = [&](float m) { return fmaf(eps, fabsf(m), slack); };       // d
+    // (m - d and m + d are increasing in m; a chunk that is masked holds VS_MASKED or less)
+    float mine = VS_MASKED;                 // this thread's largest
     if (a.chunks <= 256) {
-        if (tid < a.chunks && cm[tid] > VS_NOTHING) low = cm[tid] - off(tid, cm[tid]);
-    } else
-#pragma unroll 2
-    for (int c = tid * 4; c < a.chunks; c += THREADS * 4) {
-        const float4 m = *(const float4*)&cm[c];
-        const float g = widest(c >> 4);
-        const float top = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));      // (m - d is increasing in m)
-        if (top > VS_NOTHING) low = fmaxf(low, top - fmaf(eps, fabsf(top), g));
+        if (tid < a.chunks) mine = cm[tid];
+    } else {
+#pragma unroll 4
+        for (int c = tid * 4; c < a.chunks; c += THREADS * 4) {
+            const float4 m = *(const float4*)&cm[c];
+            mine = fmaxf(mine, fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w)));
+        }
     }
+    float low = mine > VS_NOTHING ? mine - off(mine) : -INFINITY;
     if (a.chunks <= 256) {
         if (tid < 256) best[tid] = low;
     } else {
@@ -881,22 +904,28 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
         if (tid % (THREADS / 256) == 0) best[tid / (THREADS / 256)] = low;
     }
     __syncthreads();
-    {                                       // the k-th largest of the 256: the largest value with at least k not below it
-        float t = -INFINITY;
-        if (tid < 256) {
-            const float mine = best[tid];
-            int above = 0;
-            for (int j = 0; j < 256; j += 4) {
-                const float4 q = *(const float4*)&best[j];
-                above += (q.x >= mine) + (q.y >= mine) + (q.z >= mine) + (q.w >= mine);
-            }
-            t = above >= a.k ? mine : -INFINITY;
-            for (int o = 1; o < 64; o <<= 1) t = fmaxf(t, __shfl_xor(t, o));
-            if (lane == 0) red[wave] = t;
+    if (wave == 0) {
+        // the k-th largest of the 256 by halving, over the upper 23 bits of a key in the floats' order (a lower bound will do)
+        uint32_t key[4];
+        const float4 q = *(const float4*)&best[lane * 4];
+        const float v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t u = __float_as_uint(v[i]);
+            key[i] = (u & 0x80000000u) ? ~u : u | 0x80000000u;
         }
+        uint32_t at = 0;
+        for (int bit = 31; bit > 8; --bit) {
+            const uint32_t next = at | (1u << bit);
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) n += __popcll(__ballot(key[i] >= next));
+            if (n >= a.k) at = next;
+        }
+        if (lane == 0) red[0] = at <= 0x007FFFFFu ? -INFINITY : __uint_as_float((at & 0x80000000u) ? at & 0x7FFFFFFFu : ~at);
     }
     __syncthreads();
-    const float bound = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float bound = red[0];
     double least = -INFINITY;               // the k-th best so far once k are known: what comes later must beat it
     bool full = false;
     auto compact = [&]() {                  // keeps the best k of the candidates, in order
@@ -916,11 +945,11 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
     };
     // the ids of a chunk that reach the bound, four at a time; the float64 logit of an id
     auto look = [&](int c, int i0, int i1, int tag) {
-        const float d = off(c, cm[c]);
+        const float d = off(cm[c]);
 #pragma unroll 4
         for (int i = i0; i < i1; i += 4) {
             const int v = vs_chunk_row(c, i + quarter), u = min(v, w.rows - 1);
-            const float s = vs_dot16<BF16>(w, u, xs, l16) + vs_bias_of(a.join.bias, u);
+            const float s = vs_row_sum(vs_dot<BF16, 16, float>(w, u, xs, l16)) + vs_bias_of(a.join.bias, u);
             if (l16 == 0 && v == u && s > -INFINITY && s + d >= bound) {
                 const int at = atomicAdd(&n_rows, 1);
                 if (at < VS_CAND) rows[at] = (uint16_t)(tag * VS_CHUNK + i + quarter);
@@ -930,8 +959,7 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
     int least_end = 0;                      // ids from here on had no part in `least`: equal ones come after it
     auto beaten = [&](double s, int v) { return full && (s < least || (s == least && v >= least_end)); };
     auto exact = [&](int v) {
-        double s = 0.0;
-        for (int q = lane; q < w.dim; q += 64) s = fma((double)xs[q], (double)vs_load(w, v, q), s);
+        double s = vs_dot<BF16, 64, double>(w, v, xs, lane);
         for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
         s += (double)vs_bias_of(a.join.bias, v);
         if (lane == 0 && !beaten(s, v)) {
@@ -940,21 +968,25 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
         }
     };
     auto may = [&](int c, float m) {
-        const float up = m + off(c, m);
+        const float up = m + off(m);
         return m > VS_NOTHING && up >= bound && !beaten((double)up, (c >> 4) * VS_BLOCK);
     };
-    // every chunk that may hold one of the k: usually a few more than k
-#pragma unroll 2
-    for (int c = tid * 4; c < a.chunks; c += THREADS * 4) {
-        const float4 m = *(const float4*)&cm[c];
-        const float g = widest(c >> 4);
-        const float v[4] = {m.x, m.y, m.z, m.w};
+    // every chunk that may hold one of the k, usually a few more than k: only threads whose best may looks again
+    const bool may_be = mine > VS_NOTHING && mine + off(mine) >= bound;
+    if (a.chunks <= 256) {
+        if (may_be && tid < a.chunks) list[atomicAdd(&n_list, 1)] = (uint16_t)tid;
+    } else if (may_be) {
+#pragma unroll 4
+        for (int c = tid * 4; c < a.chunks; c += THREADS * 4) {
+            const float4 m = *(const float4*)&cm[c];
+            const float v[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (v[i] > VS_NOTHING && v[i] + fmaf(eps, fabsf(v[i]), g) >= bound) {
-                const int at = atomicAdd(&n_list, 1);
-                if (at < VS_LIST) list[at] = (uint16_t)(c + i);
-            }
+            for (int i = 0; i < 4; ++i)
+                if (v[i] > VS_NOTHING && v[i] + off(v[i]) >= bound) {
+                    const int at = atomicAdd(&n_list, 1);
+                    if (at < VS_LIST) list[at] = (uint16_t)(c + i);
+                }
+        }
     }
     __syncthreads();
     bool done = n_list <= VS_LIST;
