@@ -149,15 +149,68 @@ __device__ __forceinline__ vs_f8 vs_eight(const VsSrc& s, int64_t row, int d) {
     return v;
 }
 
+// What goes with the fragments of 32 ids: their biases (0 where the caller gives none, -inf past the end: p = 0 there), then
+// the exponent of their scale.  A mask of the type's lowest value becomes -inf too: next to it no logit keeps a bit, and
+// float32 could not hold it in powers of two.  PL = 2 keeps the biases in powers of two.
+#define VS_INFO 36
+#define VS_INFO_EXP 32
+// What goes with those of 32 tokens in the gradient: lse in powers of two (L), and A, B, gl of G = p (A + B e) + gl [v = target],
+// e = log2 p; the target; the exponent of their scale last.
+#define VS_TOKEN 164
+#define VS_TOKEN_A 32
+#define VS_TOKEN_B 64
+#define VS_TOKEN_GL 96
+#define VS_TOKEN_TARGET 128
+#define VS_TOKEN_EXP 160
+
 struct VsPack {
     VsSrc src;
     uint4 *S, *T;              // T may be null
     float* group_max;          // [rows / 32] largest size, or null
     float* exps;               // PL = 2: e of group g at exps[g * exps_step]
     int32_t exps_step;
+    int32_t groups;            // of 32 rows
+    // ids: their biases (`bias` or null)
+    float* info;               // null: not of ids
+    const float* bias;
+    // tokens of a gradient
+    float* tokens;             // null: not of those
+    const float *lse, *entropy, *g, *h;
+    const int64_t* targets;
+    int32_t vocab;
 };
+
+__device__ __forceinline__ void vs_put_token(const VsPack& a, int64_t i) {
+    // rows past the end and rows whose every id is masked: an lse that makes every p 0, whatever the bias is
+    float l2 = -VS_NOTHING, A = 0.0f, B = 0.0f, gl = 0.0f;
+    int32_t t = -1;
+    if (i < a.src.rows) {
+        const float l = a.lse[i];
+        const int64_t tt = a.targets ? a.targets[i] : -1;
+        const bool empty = l == -INFINITY;
+        float fix = 1.0f;                         // p is short of 2^-(rounding of l2); A and B make up for it
+        if (!empty) {
+            const double exact = (double)l * 1.4426950408889634;
+            l2 = (float)exact;
+            fix = exp2f((float)((double)l2 - exact));
+        }
+        if (tt >= 0 && a.g) gl = a.g[i];
+        if (tt >= a.vocab) gl = NAN;
+        t = tt >= 0 && tt < a.vocab ? (int32_t)tt : -1;
+        A = -gl;
+        if (a.h && !empty) { A -= a.h[i] * a.entropy[i]; B = -a.h[i] * VS_LN2; }
+        A *= fix; B *= fix;
+    }
+    float* to = a.tokens + (i >> 5) * VS_TOKEN + (i & 31);
+    to[0] = l2; to[VS_TOKEN_A] = A; to[VS_TOKEN_B] = B; to[VS_TOKEN_GL] = gl; to[VS_TOKEN_TARGET] = __int_as_float(t);
+}
+
+// Two matrices in one launch: the first workgroups pack `a`, the others `b`.
 template <int KS, int PL, int M>
-__global__ __launch_bounds__(256) void k_vs_pack(VsPack a) {
+__global__ __launch_bounds__(256) void k_vs_pack(VsPack pa, VsPack pb) {
+    const bool second = (int)blockIdx.x >= pa.groups;
+    const VsPack& a = second ? pb : pa;
+    const int64_t group = second ? (int64_t)blockIdx.x - pa.groups : blockIdx.x;
     constexpr int DP = KS * 32, LD = DP + 4, N = (KS + 1) / 2;      // fragments of a wave
     __shared__ float tile[32 * LD];
     __shared__ float wmax[4], wfin[4];
@@ -165,7 +218,7 @@ __global__ __launch_bounds__(256) void k_vs_pack(VsPack a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane % M;
     auto row_of = [&](int f) { return f / STEPS * M + col; };
     auto element_of = [&](int f) { return f % STEPS * K + lane / M * 8; };
-    const int64_t row0 = (int64_t)blockIdx.x * 32;
+    const int64_t row0 = group * 32;
     vs_f8 v[N];
     float big = 0.0f, fin = 0.0f;
 #pragma unroll
@@ -188,8 +241,16 @@ __global__ __launch_bounds__(256) void k_vs_pack(VsPack a) {
     int e = 0;
     if (PL == 2 && fin > 0.0f) e = 13 - __builtin_amdgcn_frexp_expf(fin);
     if (threadIdx.x == 0) {
-        if (a.group_max) a.group_max[blockIdx.x] = big;
-        if (PL == 2) a.exps[(int64_t)blockIdx.x * a.exps_step] = (float)e;
+        if (a.group_max) a.group_max[group] = big;
+        if (PL == 2) a.exps[group * a.exps_step] = (float)e;
+    }
+    if (threadIdx.x < 32) {
+        const int64_t row = row0 + threadIdx.x;
+        if (a.info) {
+            const float b = row >= a.src.rows ? -INFINITY : a.bias ? a.bias[row] : 0.0f;
+            a.info[group * VS_INFO + threadIdx.x] = b <= VS_NOTHING ? -INFINITY : PL == 2 ? b * VS_LOG2E : b;
+        }
+        if (a.tokens) vs_put_token(a, row);
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -206,7 +267,7 @@ __global__ __launch_bounds__(256) void k_vs_pack(VsPack a) {
         vs_bits part[PL];
         vs_split<PL>(v[i], part);
 #pragma unroll
-        for (int p = 0; p < PL; ++p) *(vs_bits*)&a.S[(((int64_t)blockIdx.x * 2 * KS + f) * PL + p) * 64 + lane] = part[p];
+        for (int p = 0; p < PL; ++p) *(vs_bits*)&a.S[((group * 2 * KS + f) * PL + p) * 64 + lane] = part[p];
     }
     if (!a.T) return;
     __syncthreads();
@@ -217,18 +278,8 @@ __global__ __launch_bounds__(256) void k_vs_pack(VsPack a) {
         vs_bits part[PL];
         vs_split<PL>(q, part);
 #pragma unroll
-        for (int p = 0; p < PL; ++p) *(vs_bits*)&a.T[(((int64_t)blockIdx.x * 2 * KS + f) * PL + p) * 64 + lane] = part[p];
+        for (int p = 0; p < PL; ++p) *(vs_bits*)&a.T[((group * 2 * KS + f) * PL + p) * 64 + lane] = part[p];
     }
-}
-
-// What goes with the fragments of 32 ids: their biases (0 where the caller gives none, -inf past the end: p = 0 there), then
-// the exponent of their scale.  A mask of the type's lowest value becomes -inf too: next to it no logit keeps a bit, and
-// float32 could not hold it in powers of two.  PL = 2 keeps the biases in powers of two.
-#define VS_INFO 36
-#define VS_INFO_EXP 32
-__global__ __launch_bounds__(256) void k_vs_bias(const float* __restrict__ bias, float unit, int32_t vocab, int32_t padded, float* __restrict__ info) {
-    const int v = blockIdx.x * 256 + threadIdx.x;
-    if (v < padded) info[(v >> 5) * VS_INFO + (v & 31)] = v >= vocab ? -INFINITY : !bias ? 0.0f : bias[v] <= VS_NOTHING ? -INFINITY : bias[v] * unit;
 }
 
 // All are known before any is written back: without this the compiler takes new registers for what a rarely taken branch
@@ -1038,41 +1089,9 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
-// What the gradient kernels read of 32 tokens: lse in powers of two (L), and G = p (A + B e) + gl [v = target], e = log2 p;
-// the exponent of their scale last.
-#define VS_TOKEN 164
-#define VS_TOKEN_A 32
-#define VS_TOKEN_B 64
-#define VS_TOKEN_GL 96
-#define VS_TOKEN_TARGET 128
-#define VS_TOKEN_EXP 160
-__global__ __launch_bounds__(256) void k_vs_rows(const float* __restrict__ lse, const float* __restrict__ entropy, const int64_t* __restrict__ targets,
-                                                 const float* __restrict__ g, const float* __restrict__ h, int32_t n, int64_t n_pad, int32_t vocab,
-                                                 float* __restrict__ tokens) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n_pad) return;
-    // rows past the end and rows whose every id is masked: an lse that makes every p 0, whatever the bias is
-    float l2 = -VS_NOTHING, A = 0.0f, B = 0.0f, gl = 0.0f;
-    int32_t t = -1;
-    if (i < n) {
-        const float l = lse[i];
-        const int64_t tt = targets ? targets[i] : -1;
-        const bool empty = l == -INFINITY;
-        float fix = 1.0f;                         // p is short of 2^-(rounding of l2); A and B make up for it
-        if (!empty) {
-            const double exact = (double)l * 1.4426950408889634;
-            l2 = (float)exact;
-            fix = exp2f((float)((double)l2 - exact));
-        }
-        if (tt >= 0 && g) gl = g[i];
-        if (tt >= vocab) gl = NAN;
-        t = tt >= 0 && tt < vocab ? (int32_t)tt : -1;
-        A = -gl;
-        if (h && !empty) { A -= h[i] * entropy[i]; B = -h[i] * VS_LN2; }
-        A *= fix; B *= fix;
-    }
-    float* to = tokens + (i >> 5) * VS_TOKEN + (i & 31);
-    to[0] = l2; to[VS_TOKEN_A] = A; to[VS_TOKEN_B] = B; to[VS_TOKEN_GL] = gl; to[VS_TOKEN_TARGET] = __int_as_float(t);
+__device__ __forceinline__ void vs_store(void* p, int64_t at, float v, int bf16) {
+    if (bf16) ((__bf16*)p)[at] = (__bf16)v;
+    else ((float*)p)[at] = v;
 }
 
 struct VsBwd {
@@ -1086,6 +1105,11 @@ struct VsBwd {
     int64_t stay_pad;          // rows of a partial
     float* part;               // [splits][stay_pad][32 KS]
     float* bias_part;          // [splits][stay_pad]
+    // of ids, one range: the result itself
+    void* out;                 // null: partials
+    int64_t ldo;
+    int32_t rows, dim;
+    float* db;
 };
 
 // A wave: a tile of TB M stationary rows against one range of the streaming ones.  OF_IDS = false: the stationary rows
@@ -1320,6 +1344,8 @@ struct VsGrad {
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
             const int64_t r = stay0 + t * M + lane % M;
+            const bool final = OF_IDS && a.out;
+            if (final && r >= a.rows) continue;
             float* out = a.part + ((int64_t)split * a.stay_pad + r) * (KS * 32);
 #pragma unroll
             for (int d = 0; d < BLOCKS; ++d)
@@ -1328,13 +1354,18 @@ struct VsGrad {
                     vs_f4 v;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[i] = PL == 2 ? ldexpf(acc[d][t][q * 4 + i], (int)(norm[t] - sg[t])) : acc[d][t][q * 4 + i];
-                    *(vs_f4*)&out[d * M + q * 8 + lane / M * 4] = v;
+                    const int e = d * M + q * 8 + lane / M * 4;
+                    if (!final) *(vs_f4*)&out[e] = v;
+                    else
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (e + i < a.dim) vs_store(a.out, r * a.ldo + e + i, v[i], PL == 1);
                 }
             if (OF_IDS && a.want_db) {
                 float v = db[t];
                 if (M == 16) v += __shfl_xor(v, 16);
                 v += __shfl_xor(v, 32);
-                if (lane < M) a.bias_part[(int64_t)split * a.stay_pad + r] = v;
+                if (lane < M) *(final ? &a.db[r] : &a.bias_part[(int64_t)split * a.stay_pad + r]) = v;
             }
         }
     }
@@ -1448,12 +1479,10 @@ struct VsSum {
     int32_t out_bf16;
     float* db;
 };
-__device__ __forceinline__ void vs_store(void* p, int64_t at, float v, int bf16) {
-    if (bf16) ((__bf16*)p)[at] = (__bf16)v;
-    else ((float*)p)[at] = v;
-}
-__global__ __launch_bounds__(256) void k_vs_sum(VsSum a) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// Two results in one launch: the first `first` workgroups sum pa, the others pb.
+__global__ __launch_bounds__(256) void k_vs_sum(VsSum pa, VsSum pb, uint32_t first) {
+    const VsSum& a = blockIdx.x < first ? pa : pb;
+    const int64_t i = (int64_t)(blockIdx.x < first ? blockIdx.x : blockIdx.x - first) * 256 + threadIdx.x;
     if (a.db && i < a.rows) {
         float v = 0.0f;
         for (int s = 0; s < a.splits; ++s) v += a.bias_part[(int64_t)s * a.pad + i];

@@ -192,7 +192,7 @@ struct BwdPlan {
     int64_t np, tiles_x, tiles_w;
     int splits_x, splits_w;
     uint4 *xS, *xT, *wS, *wT;
-    float *info, *tokens, *part, *bias_part;
+    float *info, *tokens, *part_x, *part_w, *bias_part;
     int64_t bytes;
 };
 BwdPlan plan_bwd(const Shape& s, void* ws) {
@@ -215,9 +215,9 @@ BwdPlan plan_bwd(const Shape& s, void* ws) {
     p.xT = a.take<uint4>(p.np / 16 * frag);
     p.info = a.take<float>(s.vp / 32 * VS_INFO);
     p.tokens = a.take<float>(p.np / 32 * VS_TOKEN);
-    // dx and dw are formed one after the other: their partials share the space
-    p.part = a.take<float>(std::max(p.splits_x * p.np, p.splits_w * s.vp) * s.ks * 32);
-    p.bias_part = a.take<float>(p.splits_w * s.vp);
+    p.part_x = a.take<float>(p.splits_x * p.np * s.ks * 32);
+    p.part_w = a.take<float>(p.splits_w > 1 ? p.splits_w * s.vp * s.ks * 32 : 0);
+    p.bias_part = a.take<float>(p.splits_w > 1 ? p.splits_w * s.vp : 0);
     p.bytes = a.used;
     return p;
 }
@@ -252,13 +252,15 @@ int check_workspace(sage_ctx* c, const void* p, int64_t have, int64_t need) {
 }
 
 template <bool FORWARD>
-void pack(const Shape& s, const VsPack& p, int64_t padded, hipStream_t st) {
-#define VS_F(KS, PL) k_vs_pack<KS, PL, FORWARD ? vs_fwd_tile(KS, PL) : vs_bwd_tile(KS, PL)><<<(uint32_t)(padded / 32), 256, 0, st>>>(p)
+void pack(const Shape& s, const VsPack& a, const VsPack& b, hipStream_t st) {
+#define VS_F(KS, PL) k_vs_pack<KS, PL, FORWARD ? vs_fwd_tile(KS, PL) : vs_bwd_tile(KS, PL)><<<(uint32_t)(a.groups + b.groups), 256, 0, st>>>(a, b)
     VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
 }
-void pack_info(const Shape& s, const float* bias, float* info, hipStream_t st) {
-    k_vs_bias<<<cdiv(s.vp, 256), 256, 0, st>>>(bias, s.pl == 2 ? VS_LOG2E : 1.0f, (int32_t)s.vocab, (int32_t)s.vp, info);
+VsPack pack_of(const VsSrc& src, uint4* S, uint4* T, float* exps, int32_t exps_step, int64_t padded) {
+    VsPack p{};
+    p.src = src; p.S = S; p.T = T; p.exps = exps; p.exps_step = exps_step; p.groups = (int32_t)(padded / 32);
+    return p;
 }
 
 VsSrc rows_from(const VsSrc& m, int64_t row, int64_t rows) {
@@ -300,10 +302,8 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
     if (!dev.ok) return sage_ctx_fail(c, SAGE_E_HIP, "the context's device cannot be made current");
     const hipStream_t st = (hipStream_t)stream;
     const VsSrc w{d_weight, ldw, (int32_t)vocab, dim, dtype == SAGE_BF16}, x{d_x, ldx, (int32_t)n, dim, dtype == SAGE_BF16};
-    if (!p.raw) {
-        pack<true>(s, VsPack{w, p.wS, nullptr, alternatives ? p.group_max : nullptr, p.info + VS_INFO_EXP, VS_INFO}, s.vp, st);
-        pack_info(s, d_bias, p.info, st);
-    }
+    VsPack of_w = pack_of(w, p.wS, nullptr, p.info + VS_INFO_EXP, VS_INFO, s.vp);
+    of_w.info = p.info; of_w.bias = d_bias; of_w.group_max = alternatives ? p.group_max : nullptr;
     for (int64_t r0 = 0; r0 < n; r0 += p.rows) {
         const int64_t rows = std::min(p.rows, n - r0);
         const VsSrc xr = rows_from(x, r0, rows);
@@ -319,7 +319,8 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
             VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
         } else {
-            pack<true>(s, VsPack{xr, p.xS, nullptr, nullptr, p.x_exp, 1}, p.n_pad, st);
+            if (r0) of_w.groups = 0;               // packed with the first rows
+            pack<true>(s, of_w, pack_of(xr, p.xS, nullptr, p.x_exp, 1, p.n_pad), st);
             const uint32_t grid = cdiv(p.tiles, 4) * p.splits;
 #define VS_F(KS, PL) if (alternatives) vs_fwd_kernel<KS, PL, true><<<grid, 256, 0, st>>>(f); else vs_fwd_kernel<KS, PL, false><<<grid, 256, 0, st>>>(f)
             VS_BY_WIDTH(s.ks, s.pl, VS_F);
@@ -377,35 +378,42 @@ int sage_token_logprobs_backward_device(sage_ctx* c, int32_t dtype, int64_t n, i
     const BwdPlan p = plan_bwd(s, d_workspace);
     if ((rc = check_workspace(c, d_workspace, workspace_bytes, p.bytes))) return rc;
     const VsSrc w{d_weight, ldw, (int32_t)vocab, dim, bf16}, x{d_x, ldx, (int32_t)n, dim, bf16};
-    pack<false>(s, VsPack{w, p.wS, d_dx ? p.wT : nullptr, nullptr, p.info + VS_INFO_EXP, VS_INFO}, s.vp, st);
-    pack<false>(s, VsPack{x, p.xS, d_dweight ? p.xT : nullptr, nullptr, p.tokens + VS_TOKEN_EXP, VS_TOKEN}, p.np, st);
-    pack_info(s, d_bias, p.info, st);
-    k_vs_rows<<<cdiv(p.np, 256), 256, 0, st>>>(d_lse, d_entropy, d_targets, d_grad_logprob, d_grad_entropy, (int32_t)n, p.np, (int32_t)vocab, p.tokens);
+    VsPack of_w = pack_of(w, p.wS, d_dx ? p.wT : nullptr, p.info + VS_INFO_EXP, VS_INFO, s.vp);
+    of_w.info = p.info; of_w.bias = d_bias;
+    VsPack of_x = pack_of(x, p.xS, d_dweight ? p.xT : nullptr, p.tokens + VS_TOKEN_EXP, VS_TOKEN, p.np);
+    of_x.tokens = p.tokens; of_x.lse = d_lse; of_x.entropy = d_entropy; of_x.g = d_grad_logprob; of_x.h = d_grad_entropy; of_x.targets = d_targets;
+    of_x.vocab = (int32_t)vocab;
+    pack<false>(s, of_w, of_x, st);
     const bool entropy = d_grad_entropy != nullptr;
     VsBwd b{};
     b.info = p.info; b.tokens = p.tokens; b.has_bias = d_bias != nullptr; b.vocab = (int32_t)vocab;
-    b.part = p.part;
+    VsSum sum_x{}, sum_w{};
+    uint32_t groups_x = 0, groups_w = 0;
     if (d_dx) {
         b.stayS = p.xS; b.flowS = p.wS; b.flowT = p.wT;
-        b.n_tiles = (int32_t)p.tiles_x; b.splits = p.splits_x; b.groups = (int32_t)(s.vp / 32); b.stay_pad = p.np;
+        b.n_tiles = (int32_t)p.tiles_x; b.splits = p.splits_x; b.groups = (int32_t)(s.vp / 32); b.stay_pad = p.np; b.part = p.part_x;
         const uint32_t grid = cdiv(p.tiles_x, 4) * p.splits_x;
 #define VS_F(KS, PL) if (entropy) vs_bwd_kernel<KS, PL, false, true><<<grid, 256, 0, st>>>(b); else vs_bwd_kernel<KS, PL, false, false><<<grid, 256, 0, st>>>(b)
         VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
-        const VsSum r{p.part, nullptr, (int32_t)n, dim, s.ks * 32, p.splits_x, p.np, p.tokens, entropy, w, d_dx, lddx, bf16, nullptr};
-        k_vs_sum<<<cdiv(n * dim, 256), 256, 0, st>>>(r);
+        sum_x = VsSum{p.part_x, nullptr, (int32_t)n, dim, s.ks * 32, p.splits_x, p.np, p.tokens, entropy, w, d_dx, lddx, bf16, nullptr};
+        groups_x = cdiv(n * dim, 256);
     }
     if (d_dweight) {
         b.stayS = p.wS; b.flowS = p.xS; b.flowT = p.xT;
         b.n_tiles = (int32_t)p.tiles_w; b.splits = p.splits_w; b.groups = (int32_t)(p.np / 32); b.stay_pad = s.vp;
-        b.want_db = d_dbias != nullptr; b.bias_part = p.bias_part;
+        b.want_db = d_dbias != nullptr; b.bias_part = p.bias_part; b.part = p.part_w;
+        if (p.splits_w == 1) { b.out = d_dweight; b.ldo = lddw; b.rows = (int32_t)vocab; b.dim = dim; b.db = d_dbias; }
         const uint32_t grid = cdiv(p.tiles_w, 4) * p.splits_w;
 #define VS_F(KS, PL) if (entropy) vs_bwd_kernel<KS, PL, true, true><<<grid, 256, 0, st>>>(b); else vs_bwd_kernel<KS, PL, true, false><<<grid, 256, 0, st>>>(b)
         VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
-        const VsSum r{p.part, p.bias_part, (int32_t)vocab, dim, s.ks * 32, p.splits_w, s.vp, nullptr, 0, w, d_dweight, lddw, bf16, d_dbias};
-        k_vs_sum<<<cdiv(vocab * dim, 256), 256, 0, st>>>(r);
+        if (p.splits_w > 1) {
+            sum_w = VsSum{p.part_w, p.bias_part, (int32_t)vocab, dim, s.ks * 32, p.splits_w, s.vp, nullptr, 0, w, d_dweight, lddw, bf16, d_dbias};
+            groups_w = cdiv(vocab * dim, 256);
+        }
     }
+    if (groups_x + groups_w) k_vs_sum<<<groups_x + groups_w, 256, 0, st>>>(sum_x, sum_w, groups_x);
     return launched(c, "sage_token_logprobs_backward_device");
 }
 
