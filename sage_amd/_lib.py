@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from array import array
 from pathlib import Path
 
 import numpy as np
@@ -289,14 +290,15 @@ class HipSage:
                                                                   d_lse, d_entropy, d_grad_logprob, d_grad_entropy, d_dx, lddx, d_dweight,
                                                                   lddw, d_dbias, d_workspace, workspace_bytes, stream))
 
-    def clip_grad_norm_workspace(self, sizes: np.ndarray) -> int:
-        return self._size(self._lib.sage_clip_grad_norm_workspace(self._h, len(sizes), sizes.ctypes.data))
+    def clip_grad_norm_workspace(self, sizes: array) -> int:
+        return self._size(self._lib.sage_clip_grad_norm_workspace(self._h, len(sizes), sizes.buffer_info()[0]))
 
-    def clip_grad_norm_device(self, d_grads: np.ndarray, d_out: np.ndarray, sizes: np.ndarray, dtypes: np.ndarray, max_norm: float,
-                              d_norm: int, d_workspace: int, workspace_bytes: int, stream: int):
-        """sage_clip_grad_norm_device: the four lists are host arrays (uint64 addresses, int64 sizes, int32 types)."""
-        self._check(self._lib.sage_clip_grad_norm_device(self._h, len(sizes), d_grads.ctypes.data, d_out.ctypes.data, sizes.ctypes.data,
-                                                         dtypes.ctypes.data, float(max_norm), d_norm, d_workspace, workspace_bytes, stream))
+    def clip_grad_norm_device(self, d_grads: array, d_out: array, sizes: array, dtypes: array, max_norm: float, d_norm: int,
+                              d_workspace: int, workspace_bytes: int, stream: int):
+        """sage_clip_grad_norm_device: four arrays of one length (addresses "Q", sizes "q", types "i")."""
+        self._check(self._lib.sage_clip_grad_norm_device(self._h, len(sizes), d_grads.buffer_info()[0], d_out.buffer_info()[0],
+                                                         sizes.buffer_info()[0], dtypes.buffer_info()[0], float(max_norm), d_norm,
+                                                         d_workspace, workspace_bytes, stream))
 
     # ---- measurement ------------------------------------------------------------------------------------
     def set_profiling(self, on: bool):

@@ -11,6 +11,8 @@
 
 #define CLIP_TENSORS 128
 #define CLIP_BLOCK 32768
+#define CLIP_ONE 65536      // elements that one workgroup clips in one launch
+#define CLIP_PIECE 1024
 
 struct ClipTable {
     const void* in[CLIP_TENSORS];
@@ -46,16 +48,13 @@ __device__ __forceinline__ double clip_block_sum(double v, double* red) {
     return s;
 }
 
-__global__ __launch_bounds__(256) void k_clip_squares(ClipTable t, double* __restrict__ part) {
-    __shared__ double red[4];
-    const uint32_t i = clip_find(t, blockIdx.x);
-    const bool bf16 = t.size[i] < 0;
-    const int64_t n = bf16 ? -t.size[i] : t.size[i], at = (int64_t)(blockIdx.x - t.first[i]) * CLIP_BLOCK;
-    const int m = (int)min((int64_t)CLIP_BLOCK, n - at);
+// `m` elements of tensor i from `at`, by THREADS threads
+template <int THREADS>
+__device__ __forceinline__ double clip_squares(const ClipTable& t, uint32_t i, int64_t at, int m, int thread) {
     double s0 = 0.0, s1 = 0.0;
-    if (bf16) {
+    if (t.size[i] < 0) {
         const uint16_t* p = (const uint16_t*)t.in[i] + at;
-        for (int j = threadIdx.x * 8; j + 8 <= m; j += 2048) {
+        for (int j = thread * 8; j + 8 <= m; j += THREADS * 8) {
             const clip_u4 q = *(const clip_u4*)(p + j);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -63,11 +62,11 @@ __global__ __launch_bounds__(256) void k_clip_squares(ClipTable t, double* __res
                 s0 = fma(a, a, s0); s1 = fma(b, b, s1);
             }
         }
-        const int j = (m & ~7) + threadIdx.x;
-        if (threadIdx.x < 8 && j < m) { const double a = clip_lo(p[j]); s0 = fma(a, a, s0); }
+        const int j = (m & ~7) + thread;
+        if (thread < 8 && j < m) { const double a = clip_lo(p[j]); s0 = fma(a, a, s0); }
     } else {
         const float* p = (const float*)t.in[i] + at;
-        for (int j = threadIdx.x * 4; j + 4 <= m; j += 1024) {
+        for (int j = thread * 4; j + 4 <= m; j += THREADS * 4) {
             const clip_u4 q = *(const clip_u4*)(p + j);
 #pragma unroll
             for (int k = 0; k < 4; k += 2) {
@@ -75,36 +74,18 @@ __global__ __launch_bounds__(256) void k_clip_squares(ClipTable t, double* __res
                 s0 = fma(a, a, s0); s1 = fma(b, b, s1);
             }
         }
-        const int j = (m & ~3) + threadIdx.x;
-        if (threadIdx.x < 4 && j < m) { const double a = p[j]; s0 = fma(a, a, s0); }
+        const int j = (m & ~3) + thread;
+        if (thread < 4 && j < m) { const double a = p[j]; s0 = fma(a, a, s0); }
     }
-    const double s = clip_block_sum(s0 + s1, red);
-    if (threadIdx.x == 0) part[t.block0 + blockIdx.x] = s;
+    return s0 + s1;
 }
 
-// the norm, and the factor behind it (1 where nothing is to be clipped, or where the norm is not finite)
-__global__ __launch_bounds__(1024) void k_clip_norm(const double* __restrict__ part, uint32_t n, double max_norm, float* __restrict__ norm, float* __restrict__ factor) {
-    __shared__ double red[16];
-    double s = 0.0;
-    for (uint32_t i = threadIdx.x; i < n; i += 1024) s += part[i];
-    s = sqrt(clip_block_sum(s, red));
-    if (threadIdx.x == 0) {
-        *norm = (float)s;
-        *factor = s > max_norm && s < INFINITY ? (float)(max_norm / s) : 1.0f;
-    }
-}
-
-__global__ __launch_bounds__(256) void k_clip_scale(ClipTable t, const float* __restrict__ factor) {
-    const float f = *factor;
-    const uint32_t i = clip_find(t, blockIdx.x);
-    if (f == 1.0f && t.in[i] == t.out[i]) return;
-    const bool bf16 = t.size[i] < 0;
-    const int64_t n = bf16 ? -t.size[i] : t.size[i], at = (int64_t)(blockIdx.x - t.first[i]) * CLIP_BLOCK;
-    const int m = (int)min((int64_t)CLIP_BLOCK, n - at);
-    if (bf16) {
+template <int THREADS>
+__device__ __forceinline__ void clip_scale(const ClipTable& t, uint32_t i, int64_t at, int m, int thread, float f) {
+    if (t.size[i] < 0) {
         const uint16_t* p = (const uint16_t*)t.in[i] + at;
         uint16_t* o = (uint16_t*)t.out[i] + at;
-        for (int j = threadIdx.x * 8; j + 8 <= m; j += 2048) {
+        for (int j = thread * 8; j + 8 <= m; j += THREADS * 8) {
             clip_u4 q = *(const clip_u4*)(p + j);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -113,18 +94,76 @@ __global__ __launch_bounds__(256) void k_clip_scale(ClipTable t, const float* __
             }
             *(clip_u4*)(o + j) = q;
         }
-        const int j = (m & ~7) + threadIdx.x;
-        if (threadIdx.x < 8 && j < m) ((__bf16*)o)[j] = (__bf16)(clip_lo(p[j]) * f);
+        const int j = (m & ~7) + thread;
+        if (thread < 8 && j < m) ((__bf16*)o)[j] = (__bf16)(clip_lo(p[j]) * f);
     } else {
         const float* p = (const float*)t.in[i] + at;
         float* o = (float*)t.out[i] + at;
-        for (int j = threadIdx.x * 4; j + 4 <= m; j += 1024) {
+        for (int j = thread * 4; j + 4 <= m; j += THREADS * 4) {
             clip_u4 q = *(const clip_u4*)(p + j);
 #pragma unroll
             for (int k = 0; k < 4; ++k) q.v[k] = __float_as_uint(__uint_as_float(q.v[k]) * f);
             *(clip_u4*)(o + j) = q;
         }
-        const int j = (m & ~3) + threadIdx.x;
-        if (threadIdx.x < 4 && j < m) o[j] = p[j] * f;
+        const int j = (m & ~3) + thread;
+        if (thread < 4 && j < m) o[j] = p[j] * f;
+    }
+}
+__device__ __forceinline__ int clip_part(const ClipTable& t, uint32_t i, int64_t at, int block) {
+    const int64_t n = t.size[i] < 0 ? -t.size[i] : t.size[i];
+    return (int)min((int64_t)block, n - at);
+}
+// 1 where nothing is to be clipped, or where the norm is not finite
+__device__ __forceinline__ float clip_factor(double norm, double max_norm) {
+    return norm > max_norm && norm < INFINITY ? (float)(max_norm / norm) : 1.0f;
+}
+
+__global__ __launch_bounds__(256) void k_clip_squares(ClipTable t, double* __restrict__ part) {
+    __shared__ double red[4];
+    const uint32_t i = clip_find(t, blockIdx.x);
+    const int64_t at = (int64_t)(blockIdx.x - t.first[i]) * CLIP_BLOCK;
+    const double s = clip_block_sum(clip_squares<256>(t, i, at, clip_part(t, i, at, CLIP_BLOCK), threadIdx.x), red);
+    if (threadIdx.x == 0) part[t.block0 + blockIdx.x] = s;
+}
+
+// the norm, and the factor behind it
+__global__ __launch_bounds__(1024) void k_clip_norm(const double* __restrict__ part, uint32_t n, double max_norm, float* __restrict__ norm, float* __restrict__ factor) {
+    __shared__ double red[16];
+    double s = 0.0;
+    for (uint32_t i = threadIdx.x; i < n; i += 1024) s += part[i];
+    s = sqrt(clip_block_sum(s, red));
+    if (threadIdx.x == 0) {
+        *norm = (float)s;
+        *factor = clip_factor(s, max_norm);
+    }
+}
+
+__global__ __launch_bounds__(256) void k_clip_scale(ClipTable t, const float* __restrict__ factor) {
+    const float f = *factor;
+    const uint32_t i = clip_find(t, blockIdx.x);
+    if (f == 1.0f && t.in[i] == t.out[i]) return;
+    const int64_t at = (int64_t)(blockIdx.x - t.first[i]) * CLIP_BLOCK;
+    clip_scale<256>(t, i, at, clip_part(t, i, at, CLIP_BLOCK), threadIdx.x, f);
+}
+
+// Few gradients: all by one workgroup, a wave per piece of CLIP_PIECE elements.
+__global__ __launch_bounds__(1024) void k_clip_one(ClipTable t, double max_norm, float* __restrict__ norm) {
+    __shared__ double red[16];
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = threadIdx.x >> 6, pieces = t.first[t.n];
+    double s = 0.0;
+    for (uint32_t p = wave; p < pieces; p += 16) {
+        const uint32_t i = clip_find(t, p);
+        const int64_t at = (int64_t)(p - t.first[i]) * CLIP_PIECE;
+        s += clip_squares<64>(t, i, at, clip_part(t, i, at, CLIP_PIECE), lane);
+    }
+    s = sqrt(clip_block_sum(s, red));
+    const float f = clip_factor(s, max_norm);
+    if (threadIdx.x == 0) *norm = (float)s;
+    for (uint32_t p = wave; p < pieces; p += 16) {
+        const uint32_t i = clip_find(t, p);
+        if (f == 1.0f && t.in[i] == t.out[i]) continue;
+        const int64_t at = (int64_t)(p - t.first[i]) * CLIP_PIECE;
+        clip_scale<64>(t, i, at, clip_part(t, i, at, CLIP_PIECE), lane, f);
     }
 }

@@ -165,7 +165,7 @@ __device__ __forceinline__ vs_f8 vs_eight(const VsSrc& s, int64_t row, int d) {
 
 struct VsPack {
     VsSrc src;
-    uint4 *S, *T;              // T may be null
+    uint4 *S, *T;              // T: of a gradient, or null
     float* group_max;          // [rows / 32] largest size, or null
     float* exps;               // PL = 2: e of group g at exps[g * exps_step]
     int32_t exps_step;
@@ -206,13 +206,13 @@ __device__ __forceinline__ void vs_put_token(const VsPack& a, int64_t i) {
 }
 
 // Two matrices in one launch: the first workgroups pack `a`, the others `b`.
-template <int KS, int PL, int M>
+template <int KS, int PL, int M, bool FORWARD>
 __global__ __launch_bounds__(256) void k_vs_pack(VsPack pa, VsPack pb) {
     const bool second = (int)blockIdx.x >= pa.groups;
     const VsPack& a = second ? pb : pa;
     const int64_t group = second ? (int64_t)blockIdx.x - pa.groups : blockIdx.x;
     constexpr int DP = KS * 32, LD = DP + 4, N = (KS + 1) / 2;      // fragments of a wave
-    __shared__ float tile[32 * LD];
+    __shared__ float tile[FORWARD ? 1 : 32 * LD];      // (a forward pass has no use for T, and more workgroups at a time without it)
     __shared__ float wmax[4], wfin[4];
     constexpr int K = VsTile<M>::K, STEPS = DP / K;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane % M;
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(256) void k_vs_pack(VsPack pa, VsPack pb) {
         if (PL == 2)
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] = ldexpf(v[i][j], e);
-        if (a.T) {
+        if (!FORWARD && a.T) {
             float* to = tile + row_of(f) * LD + element_of(f);
             *(vs_f4*)to = vs_f4{v[i][0], v[i][1], v[i][2], v[i][3]};
             *(vs_f4*)(to + 4) = vs_f4{v[i][4], v[i][5], v[i][6], v[i][7]};
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(256) void k_vs_pack(VsPack pa, VsPack pb) {
 #pragma unroll
         for (int p = 0; p < PL; ++p) *(vs_bits*)&a.S[((group * 2 * KS + f) * PL + p) * 64 + lane] = part[p];
     }
-    if (!a.T) return;
+    if (FORWARD || !a.T) return;
     __syncthreads();
     for (int f = wave; f < 2 * KS; f += 4) {
         vs_f8 q;
@@ -1485,6 +1485,7 @@ __global__ __launch_bounds__(256) void k_vs_sum(VsSum pa, VsSum pb, uint32_t fir
     const int64_t i = (int64_t)(blockIdx.x < first ? blockIdx.x : blockIdx.x - first) * 256 + threadIdx.x;
     if (a.db && i < a.rows) {
         float v = 0.0f;
+#pragma unroll 8
         for (int s = 0; s < a.splits; ++s) v += a.bias_part[(int64_t)s * a.pad + i];
         a.db[i] = v;
     }
@@ -1492,6 +1493,7 @@ __global__ __launch_bounds__(256) void k_vs_sum(VsSum pa, VsSum pb, uint32_t fir
     const int64_t r = i / a.dim;
     const int d = (int)(i % a.dim);
     float v = 0.0f;
+#pragma unroll 8
     for (int s = 0; s < a.splits; ++s) v += a.part[((int64_t)s * a.pad + r) * a.dp + d];
     if (a.tokens) {
         const float* of = a.tokens + (r >> 5) * VS_TOKEN + (r & 31);

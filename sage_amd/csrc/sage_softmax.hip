@@ -253,7 +253,7 @@ int check_workspace(sage_ctx* c, const void* p, int64_t have, int64_t need) {
 
 template <bool FORWARD>
 void pack(const Shape& s, const VsPack& a, const VsPack& b, hipStream_t st) {
-#define VS_F(KS, PL) k_vs_pack<KS, PL, FORWARD ? vs_fwd_tile(KS, PL) : vs_bwd_tile(KS, PL)><<<(uint32_t)(a.groups + b.groups), 256, 0, st>>>(a, b)
+#define VS_F(KS, PL) k_vs_pack<KS, PL, FORWARD ? vs_fwd_tile(KS, PL) : vs_bwd_tile(KS, PL), FORWARD><<<(uint32_t)(a.groups + b.groups), 256, 0, st>>>(a, b)
     VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
 }
@@ -417,6 +417,19 @@ int sage_token_logprobs_backward_device(sage_ctx* c, int32_t dtype, int64_t n, i
     return launched(c, "sage_token_logprobs_backward_device");
 }
 
+static int64_t clip_table(ClipTable& t, int64_t n_tensors, const void* const* d_grads, void* const* d_out, const int64_t* sizes,
+                          const int32_t* dtypes, int64_t block, int64_t i) {
+    t.n = 0; t.first[0] = 0;
+    for (; i < n_tensors && t.n < CLIP_TENSORS; ++i) {
+        if (sizes[i] == 0) continue;
+        t.in[t.n] = d_grads[i]; t.out[t.n] = d_out[i];
+        t.size[t.n] = dtypes[i] == SAGE_BF16 ? -sizes[i] : sizes[i];
+        t.first[t.n + 1] = t.first[t.n] + cdiv(sizes[i], block);
+        ++t.n;
+    }
+    return i;
+}
+
 int64_t sage_clip_grad_norm_workspace(sage_ctx* c, int64_t n_tensors, const int64_t* sizes) {
     if (!c) return SAGE_E_ARG;
     if (n_tensors < 0 || (n_tensors && !sizes)) return sage_ctx_fail(c, SAGE_E_ARG, "need n_tensors >= 0 and their sizes");
@@ -474,19 +487,20 @@ int sage_clip_grad_norm_device(sage_ctx* c, int64_t n_tensors, const void* const
     double* part = (double*)d_workspace;
     float* factor = (float*)((char*)d_workspace + need - VS_ALIGN);
     ClipTable t;
+    int64_t elements = 0;
+    for (int64_t i = 0; i < n_tensors; ++i) elements += sizes[i];
+    if (elements <= CLIP_ONE && n_tensors <= CLIP_TENSORS) {
+        clip_table(t, n_tensors, d_grads, d_out, sizes, dtypes, CLIP_PIECE, 0);
+        k_clip_one<<<1, 1024, 0, st>>>(t, max_norm, d_norm);
+        return launched(c, "sage_clip_grad_norm_device");
+    }
     uint32_t total = 0;
     for (int pass = 0; pass < 2; ++pass) {
         uint32_t block0 = 0;
         int64_t i = 0;
         while (i < n_tensors) {
-            t.n = 0; t.block0 = block0; t.first[0] = 0;
-            for (; i < n_tensors && t.n < CLIP_TENSORS; ++i) {
-                if (sizes[i] == 0) continue;
-                t.in[t.n] = d_grads[i]; t.out[t.n] = d_out[i];
-                t.size[t.n] = dtypes[i] == SAGE_BF16 ? -sizes[i] : sizes[i];
-                t.first[t.n + 1] = t.first[t.n] + cdiv(sizes[i], CLIP_BLOCK);
-                ++t.n;
-            }
+            t.block0 = block0;
+            i = clip_table(t, n_tensors, d_grads, d_out, sizes, dtypes, CLIP_BLOCK, i);
             const uint32_t blocks = t.first[t.n];
             if (!blocks) continue;
             if (pass == 0) k_clip_squares<<<blocks, 256, 0, st>>>(t, part);

@@ -7,9 +7,9 @@ log-sigmoids of row products (utils.py:125-138); here the sum over the vocabular
 be captured into a graph, and take their workspace from torch's allocator."""
 from __future__ import annotations
 
+from array import array
 from typing import NamedTuple, Optional, Sequence, Tuple
 
-import numpy as np
 import torch
 
 from .parallel import get_engine
@@ -63,6 +63,10 @@ def _targets(t: Optional[torch.Tensor], n: int, device) -> Optional[torch.Tensor
     return _vector("targets", t, n, torch.int64, device)
 
 
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device.index).cuda_stream
+
+
 def _workspace(nbytes: int, device) -> torch.Tensor:
     return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
 
@@ -88,7 +92,7 @@ def token_logprobs(x: torch.Tensor, weight: torch.Tensor, targets: Optional[torc
     ws = _workspace(need, dev)
     engine.token_logprobs_device(kind, n, vocab, dim, x.data_ptr(), _stride(x), weight.data_ptr(), _stride(weight), _address(bias),
                                  _address(targets), int(alternatives), _address(logprob), out[1].data_ptr(), out[2].data_ptr(),
-                                 _address(alt[0]), _address(alt[1]), ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream)
+                                 _address(alt[0]), _address(alt[1]), ws.data_ptr(), ws.numel(), _stream(dev))
     return TokenLogprobs(logprob, out[1], out[2], *alt)
 
 
@@ -121,7 +125,7 @@ def token_logprobs_backward(x: torch.Tensor, weight: torch.Tensor, targets: Opti
     engine.token_logprobs_backward_device(kind, n, vocab, dim, x.data_ptr(), _stride(x), weight.data_ptr(), _stride(weight),
                                           _address(bias), _address(targets), lse.data_ptr(), entropy.data_ptr(), _address(grad_logprob),
                                           _address(grad_entropy), dx.data_ptr(), dim, dw.data_ptr(), dim, _address(db), ws.data_ptr(),
-                                          ws.numel(), torch.cuda.current_stream(dev).cuda_stream)
+                                          ws.numel(), _stream(dev))
     return dx, dw, db
 
 
@@ -142,13 +146,12 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optio
         if o is not g and (o.dtype != g.dtype or o.device != dev or o.numel() != g.numel() or not o.is_contiguous()):
             raise ValueError("results must be contiguous tensors of the gradients' sizes, types and device")
     engine = get_engine(dev.index)
-    count = len(grads)
-    addresses = np.fromiter((g.data_ptr() for g in grads), dtype=np.uint64, count=count)
-    results = addresses if out is grads else np.fromiter((o.data_ptr() for o in out), dtype=np.uint64, count=count)
-    sizes = np.fromiter((g.numel() for g in grads), dtype=np.int64, count=count)
-    types = np.fromiter((_TYPES[g.dtype] for g in grads), dtype=np.int32, count=count)
+    addresses = array("Q", [g.data_ptr() for g in grads])
+    results = addresses if out is grads else array("Q", [o.data_ptr() for o in out])
+    sizes = array("q", [g.numel() for g in grads])
+    types = array("i", [_TYPES[g.dtype] for g in grads])
     norm = torch.empty((), dtype=torch.float32, device=dev)
     ws = _workspace(engine.clip_grad_norm_workspace(sizes), dev)
     engine.clip_grad_norm_device(addresses, results, sizes, types, max_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(),
-                                 torch.cuda.current_stream(dev).cuda_stream)
+                                 _stream(dev))
     return norm
