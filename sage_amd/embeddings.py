@@ -1,13 +1,15 @@
 """Embedding checkpoints and word2vec retraining (reference: embeddings.py:28-89).
 
 A run whose `embeddings_<label>.npy` files are present never retrains -- that is also the reference's resume
-mechanism (embeddings.py:31-35).  When a retrain is needed there are two back ends:
+mechanism (embeddings.py:31-35).  When a retrain is needed there are three back ends:
   "gensim"  the reference's host call (embeddings.py:68-75); the corpus file handed to gensim is written from GPU
             tokenization (one batched call, model.py:103-107 semantics) instead of a per-line Python loop;
   "hip"     `sage_train_embeddings` (include/sage_hip.h): the same skip-gram / negative-sampling algorithm on the GPU
             over the resident corpus, no corpus file and no gensim needed.
-SAGE_W2V_BACKEND=gensim|hip chooses; the default is gensim when it can be imported (the reference's behaviour), else
-hip.  Neither back end is reproducible bit for bit (lock-free training): parity of the vectors is unpinned."""
+  "softmax" skip-gram with the softmax over the whole vocabulary in place of negative samples, on the GPU (w2v_softmax.py);
+            `negative` has no meaning there.
+SAGE_W2V_BACKEND=gensim|hip|softmax chooses; the default is gensim when it can be imported (the reference's behaviour),
+else hip.  No back end is reproducible bit for bit (lock-free training, sums by atomics): parity of the vectors is unpinned."""
 from __future__ import annotations
 
 import logging
@@ -66,7 +68,7 @@ GENSIM_MIN_ALPHA = 1e-4
 
 def _backend() -> str:
     want = os.environ.get("SAGE_W2V_BACKEND", "").strip().lower()
-    if want in ("gensim", "hip"):
+    if want in ("gensim", "hip", "softmax"):
         return want
     try:
         import gensim.models  # noqa: F401
@@ -106,8 +108,20 @@ def train_embeddings_hip(sage_model, partial_corpus, word2vec_params: Word2VecPa
     return fill_matrix(sage_model, word2vec_params.D, lambda idx, token: vec[idx] if trained[idx] else None)
 
 
+def train_embeddings_softmax(sage_model, partial_corpus, word2vec_params: Word2VecParams, seed: int = 1) -> np.ndarray:
+    """word2vec on the GPU with the full softmax (w2v_softmax.py)."""
+    from . import w2v_softmax
+    model, counts = w2v_softmax.train(sage_model, partial_corpus, word2vec_params, GENSIM_EPOCHS, GENSIM_SAMPLE, GENSIM_MIN_ALPHA, seed)
+    vec, trained = model.w_in.cpu().numpy(), counts >= max(word2vec_params.min_count, 1)
+    return fill_matrix(sage_model, word2vec_params.D, lambda idx, token: vec[idx] if trained[idx] else None)
+
+
 def train_embeddings(sage_model, partial_corpus: List[str], workers: int, word2vec_params: Word2VecParams) -> np.ndarray:
-    if _backend() == "hip":
+    backend = _backend()
+    if backend == "softmax":
+        logging.info("word2vec back end: softmax over the vocabulary (token_logprobs)")
+        return train_embeddings_softmax(sage_model, partial_corpus, word2vec_params)
+    if backend == "hip":
         logging.info("word2vec back end: HIP (sage_train_embeddings)")
         return train_embeddings_hip(sage_model, partial_corpus, word2vec_params)
     return train_embeddings_gensim(sage_model, partial_corpus, workers, word2vec_params)
