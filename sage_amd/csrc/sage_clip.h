@@ -2,7 +2,7 @@
 // max_norm.  Memory-bound: the gradients are read twice and written once (N is not known before the last one is read).
 //
 // Squares are summed in float64 (no float32 square overflows or vanishes, and the sum of 10^9 of them keeps its bits), in an
-// order that depends on the sizes alone: one partial per block of CLIP_BLOCK elements of one tensor, then one workgroup sums
+// order that depends on the sizes alone: one partial per block of `block` elements of one tensor, then one workgroup sums
 // the partials.  The list of tensors travels in the kernel arguments, CLIP_TENSORS at a time, so that a captured call
 // holds it by value.
 #pragma once
@@ -10,8 +10,9 @@
 #include <stdint.h>
 
 #define CLIP_TENSORS 128
-#define CLIP_BLOCK 32768
-#define CLIP_ONE 65536      // elements that one workgroup clips in one launch
+#define CLIP_BLOCK 8192
+#define CLIP_SMALL 2048
+#define CLIP_ONE 32768      // elements that one workgroup clips in one launch
 #define CLIP_PIECE 1024
 
 struct ClipTable {
@@ -21,19 +22,26 @@ struct ClipTable {
     uint32_t first[CLIP_TENSORS + 1];    // block that a tensor starts at
     uint32_t n;
     uint32_t block0;                     // partial of block 0
+    int32_t block;                       // elements of a block
 };
 
 // 16 bytes at the alignment that elements have
 struct __attribute__((packed, aligned(2))) clip_u4 { uint32_t v[4]; };
 
-__device__ __forceinline__ uint32_t clip_find(const ClipTable& t, uint32_t block) {
-    uint32_t lo = 0, hi = t.n;           // the last tensor whose first block is not past this one
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (t.first[mid] <= block) lo = mid; else hi = mid;
+// The tensor that a block lies in: the last whose first block is not past it.  A whole wave asks, and each lane looks at two of
+// the entries.
+struct ClipFind {
+    uint32_t a, b;
+    __device__ __forceinline__ explicit ClipFind(const ClipTable& t) {
+        const uint32_t lane = threadIdx.x & 63;
+        a = lane < t.n ? t.first[lane] : 0xFFFFFFFFu;
+        b = lane + 64 < t.n ? t.first[lane + 64] : 0xFFFFFFFFu;
     }
-    return lo;
-}
+    __device__ __forceinline__ uint32_t operator()(uint32_t block) const {
+        return __popcll(__ballot(a <= block)) + __popcll(__ballot(b <= block)) - 1;
+    }
+};
+static_assert(CLIP_TENSORS == 128, "two entries a lane");
 __device__ __forceinline__ float clip_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float clip_hi(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
 
@@ -49,11 +57,12 @@ __device__ __forceinline__ double clip_block_sum(double v, double* red) {
 }
 
 // `m` elements of tensor i from `at`, by THREADS threads
-template <int THREADS>
+template <int THREADS, int UNROLL>
 __device__ __forceinline__ double clip_squares(const ClipTable& t, uint32_t i, int64_t at, int m, int thread) {
     double s0 = 0.0, s1 = 0.0;
     if (t.size[i] < 0) {
         const uint16_t* p = (const uint16_t*)t.in[i] + at;
+#pragma unroll UNROLL
         for (int j = thread * 8; j + 8 <= m; j += THREADS * 8) {
             const clip_u4 q = *(const clip_u4*)(p + j);
 #pragma unroll
@@ -66,6 +75,7 @@ __device__ __forceinline__ double clip_squares(const ClipTable& t, uint32_t i, i
         if (thread < 8 && j < m) { const double a = clip_lo(p[j]); s0 = fma(a, a, s0); }
     } else {
         const float* p = (const float*)t.in[i] + at;
+#pragma unroll UNROLL
         for (int j = thread * 4; j + 4 <= m; j += THREADS * 4) {
             const clip_u4 q = *(const clip_u4*)(p + j);
 #pragma unroll
@@ -80,11 +90,12 @@ __device__ __forceinline__ double clip_squares(const ClipTable& t, uint32_t i, i
     return s0 + s1;
 }
 
-template <int THREADS>
+template <int THREADS, int UNROLL>
 __device__ __forceinline__ void clip_scale(const ClipTable& t, uint32_t i, int64_t at, int m, int thread, float f) {
     if (t.size[i] < 0) {
         const uint16_t* p = (const uint16_t*)t.in[i] + at;
         uint16_t* o = (uint16_t*)t.out[i] + at;
+#pragma unroll UNROLL
         for (int j = thread * 8; j + 8 <= m; j += THREADS * 8) {
             clip_u4 q = *(const clip_u4*)(p + j);
 #pragma unroll
@@ -99,6 +110,7 @@ __device__ __forceinline__ void clip_scale(const ClipTable& t, uint32_t i, int64
     } else {
         const float* p = (const float*)t.in[i] + at;
         float* o = (float*)t.out[i] + at;
+#pragma unroll UNROLL
         for (int j = thread * 4; j + 4 <= m; j += THREADS * 4) {
             clip_u4 q = *(const clip_u4*)(p + j);
 #pragma unroll
@@ -120,9 +132,9 @@ __device__ __forceinline__ float clip_factor(double norm, double max_norm) {
 
 __global__ __launch_bounds__(256) void k_clip_squares(ClipTable t, double* __restrict__ part) {
     __shared__ double red[4];
-    const uint32_t i = clip_find(t, blockIdx.x);
-    const int64_t at = (int64_t)(blockIdx.x - t.first[i]) * CLIP_BLOCK;
-    const double s = clip_block_sum(clip_squares<256>(t, i, at, clip_part(t, i, at, CLIP_BLOCK), threadIdx.x), red);
+    const uint32_t i = ClipFind(t)(blockIdx.x);
+    const int64_t at = (int64_t)(blockIdx.x - t.first[i]) * t.block;
+    const double s = clip_block_sum(clip_squares<256, 4>(t, i, at, clip_part(t, i, at, t.block), threadIdx.x), red);
     if (threadIdx.x == 0) part[t.block0 + blockIdx.x] = s;
 }
 
@@ -140,30 +152,31 @@ __global__ __launch_bounds__(1024) void k_clip_norm(const double* __restrict__ p
 
 __global__ __launch_bounds__(256) void k_clip_scale(ClipTable t, const float* __restrict__ factor) {
     const float f = *factor;
-    const uint32_t i = clip_find(t, blockIdx.x);
+    const uint32_t i = ClipFind(t)(blockIdx.x);
     if (f == 1.0f && t.in[i] == t.out[i]) return;
-    const int64_t at = (int64_t)(blockIdx.x - t.first[i]) * CLIP_BLOCK;
-    clip_scale<256>(t, i, at, clip_part(t, i, at, CLIP_BLOCK), threadIdx.x, f);
+    const int64_t at = (int64_t)(blockIdx.x - t.first[i]) * t.block;
+    clip_scale<256, 4>(t, i, at, clip_part(t, i, at, t.block), threadIdx.x, f);
 }
 
 // Few gradients: all by one workgroup, a wave per piece of CLIP_PIECE elements.
 __global__ __launch_bounds__(1024) void k_clip_one(ClipTable t, double max_norm, float* __restrict__ norm) {
     __shared__ double red[16];
     const int lane = threadIdx.x & 63;
-    const uint32_t wave = threadIdx.x >> 6, pieces = t.first[t.n];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pieces = t.first[t.n];
+    const ClipFind find(t);
     double s = 0.0;
     for (uint32_t p = wave; p < pieces; p += 16) {
-        const uint32_t i = clip_find(t, p);
+        const uint32_t i = find(p);
         const int64_t at = (int64_t)(p - t.first[i]) * CLIP_PIECE;
-        s += clip_squares<64>(t, i, at, clip_part(t, i, at, CLIP_PIECE), lane);
+        s += clip_squares<64, 4>(t, i, at, clip_part(t, i, at, CLIP_PIECE), lane);
     }
     s = sqrt(clip_block_sum(s, red));
     const float f = clip_factor(s, max_norm);
     if (threadIdx.x == 0) *norm = (float)s;
     for (uint32_t p = wave; p < pieces; p += 16) {
-        const uint32_t i = clip_find(t, p);
+        const uint32_t i = find(p);
         if (f == 1.0f && t.in[i] == t.out[i]) continue;
         const int64_t at = (int64_t)(p - t.first[i]) * CLIP_PIECE;
-        clip_scale<64>(t, i, at, clip_part(t, i, at, CLIP_PIECE), lane, f);
+        clip_scale<64, 4>(t, i, at, clip_part(t, i, at, CLIP_PIECE), lane, f);
     }
 }

@@ -905,7 +905,7 @@ template <bool BF16, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
     const VsSrc &x = a.join.x, &w = a.join.w;
     __shared__ __align__(16) float xs[512 + 16], best[256];
-    __shared__ double cv[VS_CAND], cw[VS_MAX_K];
+    __shared__ __align__(16) double cv[VS_CAND], cw[VS_MAX_K];
     __shared__ int ci[VS_CAND], cj[VS_MAX_K];
     __shared__ float red[THREADS / 64], red2[THREADS / 64];
     __shared__ uint32_t found[4];

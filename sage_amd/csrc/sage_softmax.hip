@@ -16,7 +16,7 @@ namespace {
 
 constexpr int64_t VS_PAD = 128;                 // rows are padded to this (ids to VS_BLOCK)
 constexpr int64_t VS_ROWS_MAX = 16384;          // tokens of one pass of the forward kernels
-constexpr int64_t VS_RAW = 128;                 // at most this many tokens read the weights as they lie
+constexpr int64_t VS_RAW = 512;                 // at most this many tokens read the weights as they lie
 constexpr size_t VS_ALIGN = 256;
 
 inline int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -138,13 +138,16 @@ int vs_splits(int64_t resident, int64_t groups, int64_t units, double cost) {
     return (int)best;
 }
 
-// Token blocks of a wave that reads the weights as they lie: one, or two where registers allow and tokens are there
+// Token blocks (of 16) of a wave that reads the weights as they lie, one, or two where registers allow and tokens are there;
+// 0: the weights are packed first.
 int vs_raw_blocks(const Shape& s) {
     if (s.n > VS_RAW || s.dim < 8) return 0;
     int most = 1;
 #define VS_F(KS, PL) most = vs_raw_most(KS, PL)
     VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
+    const int64_t tiles = cdiv(s.n, most * 16);
+    if ((tiles - most - 1) * s.vp * (s.ks + 8) > (1 << 20)) return 0;
     return s.n <= 16 ? 1 : most;
 }
 
@@ -417,9 +420,11 @@ int sage_token_logprobs_backward_device(sage_ctx* c, int32_t dtype, int64_t n, i
     return launched(c, "sage_token_logprobs_backward_device");
 }
 
+static int64_t clip_block(int64_t elements) { return elements <= (1 << 22) ? CLIP_SMALL : CLIP_BLOCK; }
+
 static int64_t clip_table(ClipTable& t, int64_t n_tensors, const void* const* d_grads, void* const* d_out, const int64_t* sizes,
                           const int32_t* dtypes, int64_t block, int64_t i) {
-    t.n = 0; t.first[0] = 0;
+    t.n = 0; t.first[0] = 0; t.block = (int32_t)block;
     for (; i < n_tensors && t.n < CLIP_TENSORS; ++i) {
         if (sizes[i] == 0) continue;
         t.in[t.n] = d_grads[i]; t.out[t.n] = d_out[i];
@@ -433,13 +438,14 @@ static int64_t clip_table(ClipTable& t, int64_t n_tensors, const void* const* d_
 int64_t sage_clip_grad_norm_workspace(sage_ctx* c, int64_t n_tensors, const int64_t* sizes) {
     if (!c) return SAGE_E_ARG;
     if (n_tensors < 0 || (n_tensors && !sizes)) return sage_ctx_fail(c, SAGE_E_ARG, "need n_tensors >= 0 and their sizes");
-    int64_t blocks = 0;
+    int64_t blocks = 0, elements = 0;
     for (int64_t i = 0; i < n_tensors; ++i) {
         if (sizes[i] < 0) return sage_ctx_fail(c, SAGE_E_ARG, "a tensor has a negative size");
-        if (sizes[i] > (int64_t)1 << 40) return sage_ctx_fail(c, SAGE_E_LIMIT, "a tensor of more than 2^40 elements is not supported");
-        blocks += (sizes[i] + CLIP_BLOCK - 1) / CLIP_BLOCK;
-        if (blocks > 1 << 30) return sage_ctx_fail(c, SAGE_E_LIMIT, "more than 2^45 elements are not supported");
+        if (sizes[i] > (int64_t)1 << 44 || (elements += sizes[i]) > (int64_t)1 << 44) return sage_ctx_fail(c, SAGE_E_LIMIT, "more than 2^44 elements are not supported");
     }
+    const int64_t block = clip_block(elements);
+    for (int64_t i = 0; i < n_tensors; ++i) blocks += (sizes[i] + block - 1) / block;
+    if (blocks > 1 << 30) return sage_ctx_fail(c, SAGE_E_LIMIT, "more than 2^30 tensors and blocks of tensors are not supported");
     return up(blocks * 8, VS_ALIGN) + (int64_t)VS_ALIGN;
 }
 
@@ -494,13 +500,14 @@ int sage_clip_grad_norm_device(sage_ctx* c, int64_t n_tensors, const void* const
         k_clip_one<<<1, 1024, 0, st>>>(t, max_norm, d_norm);
         return launched(c, "sage_clip_grad_norm_device");
     }
+    const int64_t block = clip_block(elements);
     uint32_t total = 0;
     for (int pass = 0; pass < 2; ++pass) {
         uint32_t block0 = 0;
         int64_t i = 0;
         while (i < n_tensors) {
             t.block0 = block0;
-            i = clip_table(t, n_tensors, d_grads, d_out, sizes, dtypes, CLIP_BLOCK, i);
+            i = clip_table(t, n_tensors, d_grads, d_out, sizes, dtypes, block, i);
             const uint32_t blocks = t.first[t.n];
             if (!blocks) continue;
             if (pass == 0) k_clip_squares<<<blocks, 256, 0, st>>>(t, part);

@@ -139,6 +139,8 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optio
         raise ValueError("need at least one gradient")
     if len(out) != len(grads):
         raise ValueError(f"{len(grads)} gradients, but {len(out)} tensors for the result")
+    if not all(isinstance(t, torch.Tensor) for t in (*grads, *out)):
+        raise ValueError("gradients and results must be tensors")
     dev = grads[0].device
     for g, o in zip(grads, out):
         if g.dtype not in _TYPES or not g.is_cuda or g.device != dev or not g.is_contiguous():

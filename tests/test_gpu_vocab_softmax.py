@@ -11,7 +11,7 @@ Tolerances, with u = 2^-24 (half a float32 step) and D, V, n the lengths summed 
   entropy          the derivative of H by the logits is p (log p + H): (1 + H) times twice lse's tolerance
   gradients        |G|'s error as an [n, V] matrix, taken through |w| or |x|, plus the sum's, plus half a step of the result's type;
                    bf16 inputs round G to bf16 before the second product: 2^-8 |G| more.
-                   float32 products (of more than 128 tokens, and all gradients) take an element as two float16 of a value
+                   float32 products (where the weights are packed first, and in all gradients) take an element as two float16 of a value
                    scaled by a power of two, so that the largest of its 32 rows, m, lies in [2^12, 2^13): an element is off by
                    at most 2^-25 of that scale (half a step of the smallest float16), 2^-25 / 2^12 m = 2^-37 m, beside its
                    relative 2^-22; a weight likewise by 2^-25 of a scale in which the largest weight of its column times m

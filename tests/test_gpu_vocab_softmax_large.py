@@ -1,0 +1,156 @@
+"""GPU: the vocabulary softmax where its kernels change: enough tokens for the weights to be packed first, vocabularies whose
+gradient one range of tokens forms (stored without partial sums), row strides of the results, workspaces full of NaN.
+Definition and tolerances are those of test_gpu_vocab_softmax.py."""
+import math
+
+import pytest
+import torch
+
+from .test_gpu_vocab_softmax import BF16, F32, Exact, check_forward, close, grads_of, exact_norm, make
+
+pytestmark = pytest.mark.gpu
+WIDTHS = [1, 7, 8, 31, 50, 64, 65, 128, 129, 200, 256, 257, 300, 320, 321, 511, 512]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", WIDTHS)
+def test_packed_weights(D, dtype):
+    from sage_amd import vocab_softmax as vs
+    for n, V, bias, k in ((513, 700, "none", 0), (600, 257, "mask", 32), (520, 1300, "prior", 5)):
+        x, w, b, t = make(n, V, D, dtype, bias, seed=k)
+        check_forward(vs.token_logprobs(x, w, t, bias=b, alternatives=k), Exact(x, w, b, t, k), k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [17, 33, 48, 49, 64, 96, 97, 192, 321, 512])
+def test_as_many_tokens_as_read_the_weights_as_they_lie(n, dtype):
+    from sage_amd import vocab_softmax as vs
+    for V, D, k in ((33, 50, 3), (9000, 50, 3), (1200, 300, 9), (5000, 511, 2)):
+        x, w, b, t = make(n, V, D, dtype, "prior", seed=k)
+        check_forward(vs.token_logprobs(x, w, t, bias=b, alternatives=k), Exact(x, w, b, t, k), k)
+
+
+@pytest.mark.parametrize("low", [float("-inf"), -1e30])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_packed_masks_and_empty_rows(dtype, low):
+    from sage_amd import vocab_softmax as vs
+    for V in (1, 70, 500):
+        x, w, _, _ = make(530, V, 40, dtype)
+        t = torch.arange(530, device="cuda") % V
+        for m in (torch.ones(V, dtype=torch.bool), torch.arange(V) != V - 1, torch.arange(V) < min(V - 1, 64)):
+            b = torch.where(m, low, 0.5).float().cuda()
+            e = Exact(x, w, b, t, 5)
+            f = vs.token_logprobs(x, w, t, bias=b, alternatives=5)
+            check_forward(f, e, 5)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_packed_ties_and_bad_rows(dtype):
+    from sage_amd import vocab_softmax as vs
+    x, w, _, t = make(540, 3000, 24, dtype)
+    w[1000:2000] = w[:1000]
+    x[3] = x[539] = 0
+    clean = vs.token_logprobs(x, w, t, alternatives=32)
+    check_forward(clean, Exact(x, w, None, t, 32), 32)
+    bad = x.clone()
+    bad[7, 3], bad[500, 20] = float("nan"), float("inf")
+    f = vs.token_logprobs(bad, w, t, alternatives=32)
+    rows = torch.ones(540, dtype=torch.bool, device="cuda")
+    rows[[7, 500]] = False
+    for a, c in zip(f, clean):
+        assert torch.equal(a[rows], c[rows])
+    assert torch.isnan(f.lse[~rows]).all() and (f.alt_ids[~rows] == -1).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,V,D", [(70, 70001, 50), (33, 40003, 100), (129, 40003, 200), (5, 40003, 300), (64, 33001, 511), (1, 100000, 7)])
+def test_gradient_of_a_long_vocabulary(n, V, D, dtype):
+    from sage_amd import vocab_softmax as vs
+    for bias, entropy in (("none", False), ("mask", True)):
+        x, w, b, t = make(n, V, D, dtype, bias, seed=3)
+        t[: n // 2] = V - 1                          # one target many times
+        gl = torch.linspace(-1, 0.5, n).cuda()
+        gh = torch.linspace(0.3, -0.2, n).cuda() if entropy else None
+        f = vs.token_logprobs(x, w, t, bias=b)
+        dx, dw, db = vs.token_logprobs_backward(x, w, t, f, gl, bias=b, grad_entropy=gh)
+        (wx, tx), (ww, tw), (wb, tb) = Exact(x, w, b, t).gradient(gl, gh, dtype)
+        close(dx, wx, tx, "dx"), close(dw, ww, tw, "dw")
+        if db is not None:
+            close(db, wb, tb, "db")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,V,D", [(40, 900, 33), (40, 70001, 33), (530, 257, 130)])
+def test_results_between_other_data(n, V, D, dtype):
+    """The C-ABI with row strides of its own, some results left out, and a workspace that holds NaN."""
+    from sage_amd import vocab_softmax as vs
+    from sage_amd.parallel import get_engine
+    eng, kind = get_engine(), 0 if dtype == F32 else 1
+    x, w, b, t = make(n, V, D, dtype, "prior", seed=1)
+    gl = torch.linspace(-1, 1, n).cuda()
+    f = vs.token_logprobs(x, w, t, bias=b)
+    want = vs.token_logprobs_backward(x, w, t, f, gl, bias=b)
+    st = torch.cuda.current_stream().cuda_stream
+    need = eng.token_logprobs_backward_workspace(kind, n, V, D)
+    for parts in ((1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 1, 1)):
+        ws = torch.full((need // 4 + 64,), float("nan"), device="cuda")
+        dx, dw = torch.full((n + 2, D + 5), 7.0, dtype=dtype, device="cuda"), torch.full((V + 2, D + 3), 7.0, dtype=dtype, device="cuda")
+        db = torch.full((V + 2,), 7.0, device="cuda")
+        eng.token_logprobs_backward_device(kind, n, V, D, x.data_ptr(), D, w.data_ptr(), D, b.data_ptr(), t.data_ptr(), f.lse.data_ptr(), f.entropy.data_ptr(),
+                                           gl.data_ptr(), 0, dx[1:, 1:].data_ptr() if parts[0] else 0, D + 5, dw[1:, 1:].data_ptr() if parts[1] else 0, D + 3,
+                                           db[1:].data_ptr() if parts[2] else 0, ws.data_ptr(), need, st)
+        for got, ref, on in ((dx, want[0], parts[0]), (dw, want[1], parts[1])):
+            keep = torch.full_like(got, 7.0)
+            if on:
+                keep[1:-1, 1:D + 1] = ref
+            assert torch.equal(got, keep)
+        assert torch.equal(db, torch.cat([db[:1] * 0 + 7, want[2], db[:1] * 0 + 7]) if parts[2] else torch.full_like(db, 7.0))
+        assert torch.isnan(ws[(need + 3) // 4:]).all()
+    # the forward call, with neither logprob nor entropy, and with alternatives
+    for k in (0, 4):
+        need = eng.token_logprobs_workspace(kind, n, V, D, k)
+        ws = torch.full((need // 4 + 64,), float("nan"), device="cuda")
+        lse, ids, lp = torch.full((n + 1,), 7.0, device="cuda"), torch.full((n * k + 1,), 7, dtype=torch.int32, device="cuda"), torch.full((n * k + 1,), 7.0, device="cuda")
+        eng.token_logprobs_device(kind, n, V, D, x.data_ptr(), D, w.data_ptr(), D, b.data_ptr(), 0, k, 0, 0, lse.data_ptr(), ids.data_ptr(), lp.data_ptr(),
+                                  ws.data_ptr(), need, st)
+        ref = vs.token_logprobs(x, w, bias=b, alternatives=k)
+        assert torch.equal(lse[:-1], ref.lse) and lse[-1] == 7 and ids[-1] == 7 and lp[-1] == 7
+        if k:
+            assert torch.equal(ids[:-1].view(n, k), ref.alt_ids) and torch.equal(lp[:-1].view(n, k), ref.alt_logprobs)
+        assert torch.isnan(ws[(need + 3) // 4:]).all()
+
+
+def test_the_two_calls_at_once():
+    """Two streams, each with its own tensors and workspace."""
+    from sage_amd import vocab_softmax as vs
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    args = [make(600, 9000, 50, F32, "prior", seed=s) for s in range(2)]
+    gl = torch.ones(600, device="cuda")
+
+    def run(x, w, b, t):
+        f = vs.token_logprobs(x, w, t, bias=b, alternatives=3)
+        return (*f, *vs.token_logprobs_backward(x, w, t, f, gl, bias=b))
+    want = [run(*a) for a in args]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(3):
+        for i, s in enumerate(sides):
+            with torch.cuda.stream(s):
+                got[i].append(run(*args[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, c) for result in got[i] for a, c in zip(result, want[i]))
+
+
+@pytest.mark.parametrize("sizes", [[0], [0, 0], [1] * 128, [1] * 129, [256] * 128, [257] * 128, [32768], [32767, 1], [32767, 2], [1 << 22], [(1 << 22) + 1],
+                                   [8191, 8192, 8193, 1 << 23]])
+def test_clip_where_the_kernels_change(sizes):
+    from sage_amd import vocab_softmax as vs
+    for kinds in ([F32] * len(sizes), [BF16, F32] * len(sizes)):
+        grads = grads_of(sizes, kinds)
+        before, want = [t.clone() for t in grads], exact_norm(grads)
+        limit = want * 0.3
+        assert abs(float(vs.clip_grad_norm(grads, limit)) - want) <= 2.0 ** -23 * want
+        for t, o in zip(before, grads):
+            d = t.double() * (limit / want if want else 1.0)
+            close(o, d, d.abs() * (torch.finfo(t.dtype).eps / 2 + 3 * 2.0 ** -24) + 1e-37, "clipped")

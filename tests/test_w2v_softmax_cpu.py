@@ -30,6 +30,7 @@ def test_refused_inputs(x, weight):
 @pytest.mark.parametrize("grads, out", [
     ([], None), (iter(()), None),
     ([torch.zeros(4)], None),                                       # not on a GPU
+    ([None], None), ([torch.zeros(4), 1.0], None),                  # not tensors
     ([torch.zeros(4, dtype=torch.float16)], None),
     ([torch.zeros(4)], []), ([torch.zeros(4)], [torch.zeros(4), torch.zeros(4)]),
 ])
