@@ -502,22 +502,19 @@ int sage_clip_grad_norm_device(sage_ctx* c, int64_t n_tensors, const void* const
     }
     const int64_t block = clip_block(elements);
     uint32_t total = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        uint32_t block0 = 0;
-        int64_t i = 0;
-        while (i < n_tensors) {
-            t.block0 = block0;
-            i = clip_table(t, n_tensors, d_grads, d_out, sizes, dtypes, block, i);
-            const uint32_t blocks = t.first[t.n];
-            if (!blocks) continue;
-            if (pass == 0) k_clip_squares<<<blocks, 256, 0, st>>>(t, part);
-            else k_clip_scale<<<blocks, 256, 0, st>>>(t, factor);
-            block0 += blocks;
-        }
-        if (pass == 0) {
-            total = block0;
-            k_clip_norm<<<1, 1024, 0, st>>>(part, total, max_norm, d_norm, factor);
-        }
+    for (int64_t i = 0; i < n_tensors;) {
+        i = clip_table(t, n_tensors, d_grads, d_out, sizes, dtypes, block, i);
+        t.block0 = total;
+        if (!t.n) break;
+        k_clip_squares<<<t.first[t.n], 256, 0, st>>>(t, part);
+        total += t.first[t.n];
+    }
+    k_clip_norm<<<1, 1024, 0, st>>>(part, total, max_norm, d_norm, factor);
+    for (int64_t end = n_tensors, i; end > 0; end = i) {         // the last tables first
+        int full = 0;
+        for (i = end; i > 0 && full < CLIP_TENSORS; --i) full += sizes[i - 1] > 0;
+        clip_table(t, end, d_grads, d_out, sizes, dtypes, block, i);
+        if (t.n) k_clip_scale<<<t.first[t.n], 256, 0, st>>>(t, factor);
     }
     return launched(c, "sage_clip_grad_norm_device");
 }
