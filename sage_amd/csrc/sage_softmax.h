@@ -46,12 +46,12 @@ template <int M> __device__ __forceinline__ int vs_row(int j, int lane) { return
 
 #define VS_LOG2E 1.4426950408889634f
 #define VS_LN2 0.6931471805599453f
-#define VS_CHUNK 16            // ids per stored maximum (the unit in which alternatives are looked for)
+#define VS_CHUNK 8             // ids per stored maximum (the unit in which alternatives are looked for)
 #define VS_BLOCK 256           // ids are dealt out in blocks of this many
-// A chunk is what one lane sees of 32 rows in a 32x32 tile: its maximum needs no other lane.  Chunk c: of block c / 16 the lane
-// half c / 8 % 2 of the 32 ids c % 8.
-__device__ __forceinline__ int vs_chunk_row(int c, int i) {      // the i-th of the 16 ids of a chunk
-    return (c >> 4) * VS_BLOCK + (c & 7) * 32 + (i >> 2) * 8 + ((c >> 3) & 1) * 4 + (i & 3);
+// A chunk is eight of 32 ids that one lane sees, of a tile of either width: its maximum needs no other lane.  Chunk c: of block
+// c / 32 the ids 32 (c % 8) .. + 31, of these rows 4 p .. and 16 + 4 p .. with p = c / 8 % 4.
+__device__ __forceinline__ int vs_chunk_row(int c, int i) {      // the i-th of the 8 ids of a chunk
+    return (c >> 5) * VS_BLOCK + (c & 7) * 32 + (i >> 2) * 16 + ((c >> 3) & 3) * 4 + (i & 3);
 }
 #define VS_NOTHING (-1.0e30f)  // reference of a row that has seen no finite logit yet; a bias this low masks its id
 #define VS_MASKED (-3.0e30f)   // what a masked logit is raised to: p is 0 there, and p times the exponent too
@@ -311,10 +311,10 @@ struct VsFwd {
     int32_t n_tiles;           // token tiles of TB M rows
     int32_t splits;            // ranges of the vocabulary
     int32_t blocks;            // blocks of VS_BLOCK ids
-    int32_t chunks;            // chunks of VS_CHUNK ids: 16 a block
+    int32_t chunks;            // chunks of VS_CHUNK ids: 32 a block
     int64_t n_pad;             // row length of the partials
     float4* part;              // [splits][n_pad]: reference (in powers of two), sum of exps, sum of exp * exponent
-    float* chunk_max;          // [n_pad][chunks] or null
+    _Float16* chunk_max;       // [n_pad][chunks] or null: largest logits, -inf where all are masked
 };
 
 // Sums of a row, relative to 2^ref: s of exp, e of exp * exponent (the entropy's).  A softmax in one pass: the reference is
@@ -385,12 +385,13 @@ __device__ __forceinline__ void vs_stationary(const uint4* S, int64_t tile, int 
 template <int M, int TB>
 struct VsRowsOfTile {
     static constexpr int NJ = VS_NJ<M>;
+    static constexpr int C = NJ / VS_CHUNK;    // chunks of a lane in 32 ids
     VsStat st[TB];
-    float top[TB];
-    vs_f4 keep[TB];
+    float top[TB][C], even[TB][C];
+    uint32_t keep[TB][C][3];
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int t = 0; t < TB; ++t) { st[t].clear(); top[t] = -INFINITY; }
+        for (int t = 0; t < TB; ++t) st[t].clear();
     }
     // the logits of 32 ids, in powers of two after multiplication by unit[t]; TOP: their largest is kept
     template <bool TOP, bool SCALED>
@@ -419,36 +420,36 @@ struct VsRowsOfTile {
         for (int t = 0; t < TB; ++t) {
             st[t].s += ls[t];
             st[t].e += le[t];
-            if (TOP) top[t] = SCALED ? largest(s, t) * (unit[t] * VS_LN2) : largest(s, t);
+            if (TOP)
+#pragma unroll
+                for (int c = 0; c < C; ++c) top[t][c] = SCALED ? of_chunk(s, t, c) * (unit[t] * VS_LN2) : of_chunk(s, t, c);
         }
+    }
+    static __device__ __forceinline__ float of_chunk(const VsLogits<M, TB>& s, int t, int c) {
+        auto v = [&](int i) { return vs_value<M, TB>(s, t, C == 1 ? i : (i >> 2) * 8 + c * 4 + (i & 3)); };
+        return vs_max(vs_max(vs_max(vs_max(vs_max(vs_max(vs_max(v(0), v(1)), v(2)), v(3)), v(4)), v(5)), v(6)), v(7));
     }
     static __device__ __forceinline__ float largest(const VsLogits<M, TB>& s, int t) {
-        auto v = [&](int j) { return vs_value<M, TB>(s, t, j); };
-        float m = vs_max(vs_max(v(0), v(1)), v(2)), n = vs_max(vs_max(v(3), v(4)), v(5));
-#pragma unroll
-        for (int j = 6; j < NJ; j += 4) {
-            m = vs_max(vs_max(m, v(j)), v(j + 1));
-            if (j + 3 < NJ) n = vs_max(vs_max(n, v(j + 2)), v(j + 3));
-        }
-        return vs_max(m, n);
+        return C == 1 ? of_chunk(s, t, 0) : vs_max(of_chunk(s, t, 0), of_chunk(s, t, C - 1));
     }
-    // step h of a block (32 ids) is done: the largest logits of four steps are stored together (WHOLE: the wave sees whole
-    // blocks), or at once.  Two lanes of a 16-column tile share a chunk.
+    // Step h of a block (32 ids) is done: its largest logits are kept as float16 (-inf stands for masked ids alone) and those of
+    // eight steps are stored together (WHOLE: the wave sees whole blocks), or of two.
     template <bool WHOLE>
     __device__ __forceinline__ void chunk(const VsFwd& a, int64_t tile, int block, int h, int lane, bool live) {
-        const int part = lane / M;
 #pragma unroll
-        for (int t = 0; t < TB; ++t) {
-            const float m = M == 32 ? top[t] : vs_max(top[t], __shfl_xor(top[t], 32));
-            float* to = a.chunk_max + ((tile * TB + t) * M + lane % M) * a.chunks + block * 16 + (part & 1) * 8;
-            const bool mine = live && part < 2;
-            if (WHOLE) {
-                if ((h & 3) == 0) keep[t][0] = m;
-                else if ((h & 3) == 1) keep[t][1] = m;
-                else if ((h & 3) == 2) keep[t][2] = m;
-                else if (mine) *(vs_f4*)(to + (h & ~3)) = vs_f4{keep[t][0], keep[t][1], keep[t][2], m};
-            } else if (mine) to[h] = m;
-        }
+        for (int t = 0; t < TB; ++t)
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const float m = a.has_bias && top[t][c] < VS_NOTHING ? -INFINITY : top[t][c];
+                if ((h & 1) == 0) { even[t][c] = m; continue; }
+                const uint32_t two = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(even[t][c], m));     // (stays finite)
+                _Float16* to = a.chunk_max + ((tile * TB + t) * M + lane % M) * a.chunks + block * 32 + (lane / M + c * 2) * 8;
+                if (!WHOLE) { if (live) *(uint32_t*)(to + h - 1) = two; }
+                else if (h == 1) keep[t][c][0] = two;
+                else if (h == 3) keep[t][c][1] = two;
+                else if (h == 5) keep[t][c][2] = two;
+                else if (live) *(uint4*)to = make_uint4(keep[t][c][0], keep[t][c][1], keep[t][c][2], two);
+            }
     }
     __device__ __forceinline__ void flush() {
 #pragma unroll
@@ -828,7 +829,7 @@ __global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
 #define VS_LIST 256
 struct VsTop {
     VsJoin join;               // the row's ranges are joined first
-    const float* chunk_max;    // [rows][chunks]
+    const _Float16* chunk_max; // [rows][chunks]
     const float* group_max;    // [8 blocks] largest |w| of 32 ids
     int32_t chunks, k;
     int32_t* ids;              // [n][k]
@@ -909,11 +910,13 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
     __shared__ int ci[VS_CAND], cj[VS_MAX_K];
     __shared__ float red[THREADS / 64], red2[THREADS / 64];
     __shared__ uint32_t found[4];
-    __shared__ uint16_t list[VS_LIST], rows[VS_CAND];
+    __shared__ uint32_t list[VS_LIST];
+    __shared__ uint16_t rows[VS_CAND];
     __shared__ int n_cand, n_rows, n_list;
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = tid & 15, quarter = lane >> 4;
-    const float* cm = a.chunk_max + row * a.chunks;
+    const _Float16* cm = a.chunk_max + row * a.chunks;
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
     const float lse = vs_join_row<THREADS / 64>(a.join, row, tid, (float4*)cv, cw);
     __syncthreads();
     if (lse != lse) {                       // no order among the logits
@@ -922,7 +925,7 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
     }
     float l1 = vs_put_x<BF16>(x, row, xs, tid, THREADS), widest = 0.0f;
 #pragma unroll 4
-    for (int g = tid * 4; g < a.chunks / 2; g += THREADS * 4) {
+    for (int g = tid * 4; g < a.chunks / 4; g += THREADS * 4) {
         const float4 q = *(const float4*)&a.group_max[g];
         widest = fmaxf(widest, fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)));
     }
@@ -935,19 +938,21 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
     __syncthreads();
     const float eps = 4.0f * (float)(x.dim + 16) * 5.9604645e-8f;
     const float slack = eps * 2.0f * l1 * widest;
-    auto off = [&](float m) { return fmaf(eps, fabsf(m), slack); };       // d
-    // (m - d and m + d are increasing in m; a chunk that is masked holds VS_MASKED or less)
-    float mine = VS_MASKED;                 // this thread's largest
+    // a chunk's largest logit lies between these (d, and a step of float16; past its range there is one bound only)
+    auto off = [&](float m) { return fmaf(eps + 0.0009765625f, fabsf(m), slack + 5.9604645e-8f); };
+    auto above = [&](float m) { return m >= 65504.0f ? INFINITY : m + off(m); };
+    auto below = [&](float m) { return m <= -65504.0f ? -INFINITY : fminf(m, 65504.0f) - off(fminf(m, 65504.0f)); };
+    float mine = -INFINITY;                 // this thread's largest (both bounds grow with it)
     if (a.chunks <= 256) {
-        if (tid < a.chunks) mine = cm[tid];
+        if (tid < a.chunks) mine = (float)cm[tid];
     } else {
+        h8 most = h8(-(_Float16)INFINITY);
 #pragma unroll 4
-        for (int c = tid * 4; c < a.chunks; c += THREADS * 4) {
-            const float4 m = *(const float4*)&cm[c];
-            mine = fmaxf(mine, fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w)));
-        }
+        for (int c = tid * 8; c < a.chunks; c += THREADS * 8) most = __builtin_elementwise_max(most, *(const h8*)&cm[c]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine = fmaxf(mine, (float)most[i]);
     }
-    float low = mine > VS_NOTHING ? mine - off(mine) : -INFINITY;
+    float low = below(mine);
     if (a.chunks <= 256) {
         if (tid < 256) best[tid] = low;
     } else {
@@ -995,13 +1000,12 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
         if (m == a.k) { full = true; least = cv[m - 1]; }
     };
     // the ids of a chunk that reach the bound, four at a time; the float64 logit of an id
-    auto look = [&](int c, int i0, int i1, int tag) {
-        const float d = off(cm[c]);
-#pragma unroll 4
-        for (int i = i0; i < i1; i += 4) {
+    auto look = [&](int c, int tag) {
+#pragma unroll
+        for (int i = 0; i < VS_CHUNK; i += 4) {
             const int v = vs_chunk_row(c, i + quarter), u = min(v, w.rows - 1);
             const float s = vs_row_sum(vs_dot<BF16, 16, float>(w, u, xs, l16)) + vs_bias_of(a.join.bias, u);
-            if (l16 == 0 && v == u && s > -INFINITY && s + d >= bound) {
+            if (l16 == 0 && v == u && s > -INFINITY && fmaf(eps, fabsf(s), s + slack) >= bound) {
                 const int at = atomicAdd(&n_rows, 1);
                 if (at < VS_CAND) rows[at] = (uint16_t)(tag * VS_CHUNK + i + quarter);
             }
@@ -1019,23 +1023,22 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
         }
     };
     auto may = [&](int c, float m) {
-        const float up = m + off(m);
-        return m > VS_NOTHING && up >= bound && !beaten((double)up, (c >> 4) * VS_BLOCK);
+        const float up = above(m);
+        return m > -INFINITY && up >= bound && !beaten((double)up, (c >> 5) * VS_BLOCK);
     };
     // every chunk that may hold one of the k, usually a few more than k: only threads whose best may looks again
-    const bool may_be = mine > VS_NOTHING && mine + off(mine) >= bound;
+    const bool may_be = mine > -INFINITY && above(mine) >= bound;
     if (a.chunks <= 256) {
-        if (may_be && tid < a.chunks) list[atomicAdd(&n_list, 1)] = (uint16_t)tid;
+        if (may_be && tid < a.chunks) list[atomicAdd(&n_list, 1)] = tid;
     } else if (may_be) {
 #pragma unroll 4
-        for (int c = tid * 4; c < a.chunks; c += THREADS * 4) {
-            const float4 m = *(const float4*)&cm[c];
-            const float v[4] = {m.x, m.y, m.z, m.w};
+        for (int c = tid * 8; c < a.chunks; c += THREADS * 8) {
+            const h8 m = *(const h8*)&cm[c];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (v[i] > VS_NOTHING && v[i] + off(v[i]) >= bound) {
+            for (int i = 0; i < 8; ++i)
+                if (m[i] > -(_Float16)INFINITY && above((float)m[i]) >= bound) {
                     const int at = atomicAdd(&n_list, 1);
-                    if (at < VS_LIST) list[at] = (uint16_t)(c + i);
+                    if (at < VS_LIST) list[at] = c + i;
                 }
         }
     }
@@ -1043,7 +1046,7 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
     bool done = n_list <= VS_LIST;
     if (done) {                             // all their ids at once, a chunk for each wave
         const int n = n_list;
-        for (int i = wave; i < n; i += THREADS / 64) look(list[i], 0, VS_CHUNK, i);
+        for (int i = wave; i < n; i += THREADS / 64) look(list[i], i);
         __syncthreads();
         done = n_rows <= VS_CAND;
         if (done) {
@@ -1055,26 +1058,26 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
         __syncthreads();
         for (int c0 = 0; c0 < a.chunks; c0 += 256) {
             const int c = c0 + tid;
-            const bool want = tid < 256 && c < a.chunks && may(c, cm[c]);
+            const bool want = tid < 256 && c < a.chunks && may(c, (float)cm[c]);
             const unsigned long long bal = __ballot(want);
             if (lane == 0 && wave < 4) found[wave] = __popcll(bal);
             __syncthreads();
             int before = 0;
             for (int i = 0; i < min(wave, 4); ++i) before += found[i];
             const int nl = found[0] + found[1] + found[2] + found[3];
-            if (want) list[before + __popcll(bal & ((1ull << lane) - 1ull))] = (uint16_t)c;
+            if (want) list[before + __popcll(bal & ((1ull << lane) - 1ull))] = c;
             __syncthreads();
-            for (int i0 = 0; i0 < nl; i0 += 16) {
+            for (int i0 = 0; i0 < nl; i0 += 32) {
                 if (tid == 0) n_rows = 0;
                 __syncthreads();
-                for (int i = i0 + wave; i < min(i0 + 16, nl); i += THREADS / 64)
-                    if (may(list[i], cm[list[i]])) look(list[i], 0, VS_CHUNK, i - i0);
+                for (int i = i0 + wave; i < min(i0 + 32, nl); i += THREADS / 64)
+                    if (may(list[i], (float)cm[list[i]])) look(list[i], i - i0);
                 __syncthreads();
                 const int nr = n_rows;
                 for (int i = wave; i < nr; i += THREADS / 64) exact(vs_chunk_row(list[i0 + rows[i] / VS_CHUNK], rows[i] % VS_CHUNK));
                 __syncthreads();
                 const bool crowded = n_cand > VS_CAND - 256;
-                if (crowded) { compact(); least_end = ((list[min(i0 + 15, nl - 1)] >> 4) + 1) * VS_BLOCK; }
+                if (crowded) { compact(); least_end = ((int)(list[min(i0 + 31, nl - 1)] >> 5) + 1) * VS_BLOCK; }
                 __syncthreads();
             }
         }

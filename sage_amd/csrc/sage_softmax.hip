@@ -156,7 +156,8 @@ struct FwdPlan {
     int splits;
     int raw;                    // 16-token blocks of a tile of k_vs_forward_raw (0: the weights are packed)
     uint4 *xS, *wS;
-    float *info, *x_exp, *group_max, *chunk_max;
+    float *info, *x_exp, *group_max;
+    _Float16* chunk_max;
     float4* part;
     int64_t bytes;
 };
@@ -186,7 +187,7 @@ FwdPlan plan_fwd(const Shape& s, void* ws) {
     }
     p.group_max = a.take<float>(s.vp / 32);
     p.part = a.take<float4>(p.splits * p.n_pad);
-    p.chunk_max = a.take<float>(s.k ? p.n_pad * p.chunks : 0);
+    p.chunk_max = a.take<_Float16>(s.k ? p.n_pad * p.chunks : 0);
     p.bytes = a.used;
     return p;
 }
