@@ -25,6 +25,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 typedef __bf16 vs_bf8 __attribute__((ext_vector_type(8)));
 typedef float vs_f4 __attribute__((ext_vector_type(4)));
@@ -150,10 +151,11 @@ __device__ __forceinline__ vs_f8 vs_eight(const VsSrc& s, int64_t row, int d) {
 }
 
 // What goes with the fragments of 32 ids: their biases (0 where the caller gives none, -inf past the end: p = 0 there), then
-// the exponent of their scale.  A mask of the type's lowest value becomes -inf too: next to it no logit keeps a bit, and
+// the exponent of their scale and their largest size.  A mask of the type's lowest value becomes -inf too: next to it no logit keeps a bit, and
 // float32 could not hold it in powers of two.  PL = 2 keeps the biases in powers of two.
 #define VS_INFO 36
 #define VS_INFO_EXP 32
+#define VS_INFO_WIDE 33
 // What goes with those of 32 tokens in the gradient: lse in powers of two (L), and A, B, gl of G = p (A + B e) + gl [v = target],
 // e = log2 p; the target; the exponent of their scale last.
 #define VS_TOKEN 164
@@ -166,7 +168,6 @@ __device__ __forceinline__ vs_f8 vs_eight(const VsSrc& s, int64_t row, int d) {
 struct VsPack {
     VsSrc src;
     uint4 *S, *T;              // T: of a gradient, or null
-    float* group_max;          // [rows / 32] largest size, or null
     float* exps;               // PL = 2: e of group g at exps[g * exps_step]
     int32_t exps_step;
     int32_t groups;            // of 32 rows
@@ -241,7 +242,7 @@ __global__ __launch_bounds__(256) void k_vs_pack(VsPack pa, VsPack pb) {
     int e = 0;
     if (PL == 2 && fin > 0.0f) e = 13 - __builtin_amdgcn_frexp_expf(fin);
     if (threadIdx.x == 0) {
-        if (a.group_max) a.group_max[group] = big;
+        if (a.info) a.info[group * VS_INFO + VS_INFO_WIDE] = big;
         if (PL == 2) a.exps[group * a.exps_step] = (float)e;
     }
     if (threadIdx.x < 32) {
@@ -313,7 +314,7 @@ struct VsFwd {
     int32_t blocks;            // blocks of VS_BLOCK ids
     int32_t chunks;            // chunks of VS_CHUNK ids: 32 a block
     int64_t n_pad;             // row length of the partials
-    float4* part;              // [splits][n_pad]: reference (in powers of two), sum of exps, sum of exp * exponent
+    float4* part;              // [splits][n_pad]: reference (in powers of two), sum of exps, sum of exp * exponent; largest |weight|
     _Float16* chunk_max;       // [n_pad][chunks] or null: largest logits, -inf where all are masked
 };
 
@@ -387,11 +388,12 @@ struct VsRowsOfTile {
     static constexpr int NJ = VS_NJ<M>;
     static constexpr int C = NJ / VS_CHUNK;    // chunks of a lane in 32 ids
     VsStat st[TB];
-    float top[TB][C], even[TB][C];
+    float top[TB][C], even[TB][C], wide;       // wide: the largest size of a weight
     uint32_t keep[TB][C][3];
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int t = 0; t < TB; ++t) st[t].clear();
+        wide = 0.0f;
     }
     // the logits of 32 ids, in powers of two after multiplication by unit[t]; TOP: their largest is kept
     template <bool TOP, bool SCALED>
@@ -470,7 +472,7 @@ struct VsRowsOfTile {
         join_lanes();
 #pragma unroll
         for (int t = 0; t < TB; ++t)
-            if (lane < M) a.part[(int64_t)split * a.n_pad + (tile * TB + t) * M + lane] = make_float4(st[t].ref, st[t].S, st[t].E, 0.0f);
+            if (lane < M) a.part[(int64_t)split * a.n_pad + (tile * TB + t) * M + lane] = make_float4(st[t].ref, st[t].S, st[t].E, wide);
     }
 };
 
@@ -504,6 +506,7 @@ __device__ __forceinline__ void vs_begin(const float* of, int lane, VsLogits<M, 
 template <int KS, int PL, int M, int TB, bool TOP>
 __device__ __forceinline__ void vs_forward_step(const VsFwd& a, int row0, const uint4* w, const float* info, const VsOperand<KS, PL, M> (&x)[TB],
                                                 const float (&x_exp)[TB], VsRowsOfTile<M, TB>& rows) {
+    if (TOP) rows.wide = fmaxf(rows.wide, info[VS_INFO_WIDE]);
     VsLogits<M, TB> s;
     vs_f4 b[VS_NJ<M> / 4];
     float unit[TB];
@@ -645,7 +648,6 @@ template <> struct VsPiece<3> {            // of float32
 struct VsRaw {
     VsSrc x, w;
     const float* bias;         // as the caller gave it, or null
-    float* group_max;          // [ids / 32] or null
     VsFwd f;                   // chunks, blocks, n_pad, part, chunk_max; splits: workgroups of a tile
 };
 template <int KS, int PL, int TB>
@@ -673,6 +675,7 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
     }
     VsRowsOfTile<16, TB> rows;
     rows.clear();
+    float wide = 0.0f;
     const float unscaled[TB] = {};
     const int units = gridDim.x * 4, unit = blockIdx.x * 4 + (threadIdx.x >> 6), pieces = a.f.blocks * 4;
     const int c0 = (int)((int64_t)pieces * unit / units), c1 = (int)((int64_t)pieces * (unit + 1) / units);
@@ -720,31 +723,31 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
                     for (int t = 0; t < TB; ++t) s[j >> 2][t][j & 3] = gone ? VS_MASKED : s[j >> 2][t][j & 3] + q;
                 }
             }
-            if (a.group_max) {
-                float m = big.largest();
-                for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-                if (lane == 0 && tile == 0) a.group_max[row0 / 32] = m;
-            }
+            wide = fmaxf(wide, big.largest());
+            __builtin_amdgcn_sched_barrier(0);
             rows.template add<true, false>(s, unscaled);
             if (a.f.chunk_max) rows.template chunk<false>(a.f, tile, row0 / VS_BLOCK, (row0 >> 5) & 7, lane, true);
         }
         if ((c & 3) == 3) rows.flush();
     }
     rows.join_lanes();
+    for (int o = 1; o < 64; o <<= 1) wide = fmaxf(wide, __shfl_xor(wide, o));
 #pragma unroll
     for (int t = 0; t < TB; ++t)
-        if (quad == 0) red[threadIdx.x >> 6][t * 16 + col] = make_float4(rows.st[t].ref, rows.st[t].S, rows.st[t].E, 0.0f);
+        if (quad == 0) red[threadIdx.x >> 6][t * 16 + col] = make_float4(rows.st[t].ref, rows.st[t].S, rows.st[t].E, wide);
     __syncthreads();
     if (threadIdx.x < TB * 16) {
         VsStat st;
         st.clear();
-        for (int i = 0; i < 4; ++i) { const float4 q = red[i][threadIdx.x]; st.join(q.x, q.y, q.z); }
-        a.f.part[(int64_t)blockIdx.x * a.f.n_pad + tile * TB * 16 + threadIdx.x] = make_float4(st.ref, st.S, st.E, 0.0f);
+        wide = 0.0f;
+        for (int i = 0; i < 4; ++i) { const float4 q = red[i][threadIdx.x]; st.join(q.x, q.y, q.z); wide = fmaxf(wide, q.w); }
+        a.f.part[(int64_t)blockIdx.x * a.f.n_pad + tile * TB * 16 + threadIdx.x] = make_float4(st.ref, st.S, st.E, wide);
     }
 }
 
 // Joins the ranges of a row and takes the given token's log probability.  The token's own logit is summed in float64 (its
-// rounding would otherwise show where the probability is near 1).  WAVES waves work on a row; returns its lse to them all.
+// rounding would otherwise show where the probability is near 1).  WAVES waves work on a row; returns its lse, and the largest
+// size of a weight if asked, to them all.
 struct VsJoin {
     VsSrc x, w;
     const float* bias;         // as the caller gave it, or null
@@ -755,18 +758,20 @@ struct VsJoin {
     float *logprob, *entropy, *lse;
 };
 template <int WAVES>
-__device__ __forceinline__ float vs_join_row(const VsJoin& a, int64_t row, int tid, float4* red, double* dred) {
+__device__ __forceinline__ float vs_join_row(const VsJoin& a, int64_t row, int tid, float4* red, double* dred, float* widest = nullptr) {
     const int lane = tid & 63, wave = tid >> 6;
     const bool alone = WAVES == 1 || a.splits <= 64;       // few ranges: the first wave joins them, the others are told
     const int64_t t = a.targets ? a.targets[row] : -1;
     VsStat st;
     double dot = 0.0;
+    float wide = 0.0f;
     st.clear();
     if (!alone || wave == 0) {
         const int step = alone ? 64 : 64 * WAVES;
         for (int i = tid; i < a.splits; i += step) {
             const float4 q = a.part[(int64_t)i * a.n_pad + row];
             st.join(q.x, q.y, q.z);
+            wide = fmaxf(wide, q.w);
         }
         if (t >= 0 && t < a.w.rows)
             for (int d = tid; d < a.w.dim; d += step) dot += (double)vs_load(a.x, row, d) * (double)vs_load(a.w, t, d);
@@ -776,15 +781,17 @@ __device__ __forceinline__ float vs_join_row(const VsJoin& a, int64_t row, int t
                 st.join(r2, s2, e2);
             }
             dot += __shfl_xor(dot, o);
+            if (widest) wide = fmaxf(wide, __shfl_xor(wide, o));
         }
-        if (WAVES > 1 && lane == 0) { red[wave] = make_float4(st.ref, st.S, st.E, 0.0f); dred[wave] = dot; }
+        if (WAVES > 1 && lane == 0) { red[wave] = make_float4(st.ref, st.S, st.E, wide); dred[wave] = dot; }
     }
     if constexpr (WAVES > 1) {
         __syncthreads();
         st.clear();
         dot = 0.0;
-        for (int i = 0; i < (alone ? 1 : WAVES); ++i) { st.join(red[i].x, red[i].y, red[i].z); dot += dred[i]; }
+        for (int i = 0; i < (alone ? 1 : WAVES); ++i) { st.join(red[i].x, red[i].y, red[i].z); dot += dred[i]; wide = fmaxf(wide, red[i].w); }
     }
+    if (widest) *widest = wide;
     const bool empty = st.S == 0.0f;                // nothing but -inf
     const double lse = empty ? -INFINITY : ((double)st.ref + (double)log2f(st.S)) * 0.6931471805599453;
     if (tid == 0) {
@@ -830,7 +837,6 @@ __global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
 struct VsTop {
     VsJoin join;               // the row's ranges are joined first
     const _Float16* chunk_max; // [rows][chunks]
-    const float* group_max;    // [8 blocks] largest |w| of 32 ids
     int32_t chunks, k;
     int32_t* ids;              // [n][k]
     float* logprobs;           // [n][k]
@@ -866,26 +872,45 @@ __device__ __forceinline__ float vs_row_sum(float v) {
     return v;
 }
 
-// x . row over LANES lanes, each its part (xs: x in LDS, and behind it, from xs[dim up to a whole piece], the last piece again as
+__device__ __forceinline__ double vs_row_sum(double v) {
+    auto from = [&](auto ctrl) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, decltype(ctrl)::value, 0xF, 0xF, true),
+                       hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), decltype(ctrl)::value, 0xF, 0xF, true);
+        return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    };
+    v += from(std::integral_constant<int, 0xB1>{});
+    v += from(std::integral_constant<int, 0x4E>{});
+    v += from(std::integral_constant<int, 0x141>{});
+    v += from(std::integral_constant<int, 0x140>{});
+    return v;
+}
+
+// x . row for R rows over 16 lanes, each its part (xs: x in LDS, and behind it, from xs[dim up to a whole piece], the last piece again as
 // it is multiplied: a row that is no whole number of pieces long has it taken back from the row's end, with the elements
 // before it weighted 0 -- no read leaves the row).
-template <bool BF16, int LANES, class T>
-__device__ __forceinline__ T vs_dot(const VsSrc& w, int64_t row, const float* xs, int lane) {
+template <bool BF16, int R, class T>
+__device__ __forceinline__ void vs_dots(const VsSrc& w, const int (&row)[R], const float* xs, int lane, T (&s)[R]) {
     constexpr int E = VsVec<BF16>::E;
-    T s = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r] = 0;
     if (w.dim < E) {
-        if (lane < w.dim) s = (T)xs[lane] * (T)vs_load(w, row, lane);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (lane < w.dim) s[r] = (T)xs[lane] * (T)vs_load(w, row[r], lane);
     } else {
         const int whole = w.dim / E * E;
-        for (int d = lane * E; d < w.dim; d += LANES * E) {
-            VsVec<BF16> v;
-            v.load(w.p, row * w.ld + min(d, w.dim - E));
+        for (int d = lane * E; d < w.dim; d += 16 * E) {
+            VsVec<BF16> v[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) v[r].load(w.p, row[r] * w.ld + min(d, w.dim - E));
             const float* x = xs + (d < whole ? d : whole + E);
 #pragma unroll
-            for (int i = 0; i < E; ++i) s = fma((T)x[i], (T)v.f[i], s);
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int i = 0; i < E; ++i) s[r] = fma((T)x[i], (T)v[r].f[i], s[r]);
         }
     }
-    return s;
 }
 // x into LDS in that form, by all threads
 template <bool BF16>
@@ -903,12 +928,12 @@ __device__ __forceinline__ float vs_put_x(const VsSrc& x, int64_t row, float* xs
 }
 
 template <bool BF16, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
+__global__ __launch_bounds__(THREADS, THREADS == 256 ? BF16 ? 5 : 7 : 4) void k_vs_top(VsTop a) {
     const VsSrc &x = a.join.x, &w = a.join.w;
     __shared__ __align__(16) float xs[512 + 16], best[256];
     __shared__ __align__(16) double cv[VS_CAND], cw[VS_MAX_K];
     __shared__ int ci[VS_CAND], cj[VS_MAX_K];
-    __shared__ float red[THREADS / 64], red2[THREADS / 64];
+    __shared__ float red[THREADS / 64];
     __shared__ uint32_t found[4];
     __shared__ uint32_t list[VS_LIST];
     __shared__ uint16_t rows[VS_CAND];
@@ -917,24 +942,20 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = tid & 15, quarter = lane >> 4;
     const _Float16* cm = a.chunk_max + row * a.chunks;
     typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-    const float lse = vs_join_row<THREADS / 64>(a.join, row, tid, (float4*)cv, cw);
+    float widest;
+    const float lse = vs_join_row<THREADS / 64>(a.join, row, tid, (float4*)cv, cw, &widest);
     __syncthreads();
     if (lse != lse) {                       // no order among the logits
         if (tid < a.k) { a.ids[row * a.k + tid] = -1; a.logprobs[row * a.k + tid] = NAN; }
         return;
     }
-    float l1 = vs_put_x<BF16>(x, row, xs, tid, THREADS), widest = 0.0f;
-#pragma unroll 4
-    for (int g = tid * 4; g < a.chunks / 4; g += THREADS * 4) {
-        const float4 q = *(const float4*)&a.group_max[g];
-        widest = fmaxf(widest, fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)));
-    }
-    for (int o = 1; o < 64; o <<= 1) { l1 += __shfl_xor(l1, o); widest = fmaxf(widest, __shfl_xor(widest, o)); }
-    if (lane == 0) { red[wave] = l1; red2[wave] = widest; }
+    float l1 = vs_put_x<BF16>(x, row, xs, tid, THREADS);
+    for (int o = 1; o < 64; o <<= 1) l1 += __shfl_xor(l1, o);
+    if (lane == 0) red[wave] = l1;
     if (tid == 0) n_cand = n_rows = n_list = 0;
     __syncthreads();
     l1 = 0.0f;
-    for (int i = 0; i < THREADS / 64; ++i) { l1 += red[i]; widest = fmaxf(widest, red2[i]); }
+    for (int i = 0; i < THREADS / 64; ++i) l1 += red[i];
     __syncthreads();
     const float eps = 4.0f * (float)(x.dim + 16) * 5.9604645e-8f;
     const float slack = eps * 2.0f * l1 * widest;
@@ -999,27 +1020,38 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
         __syncthreads();
         if (m == a.k) { full = true; least = cv[m - 1]; }
     };
-    // the ids of a chunk that reach the bound, four at a time; the float64 logit of an id
-    auto look = [&](int c, int tag) {
+    // the ids of two chunks of the list (or one) that reach the bound, by a wave
+    auto look = [&](int i, bool first, bool second, int base) {
+        int v[4], u[4];
+        float s[4];
 #pragma unroll
-        for (int i = 0; i < VS_CHUNK; i += 4) {
-            const int v = vs_chunk_row(c, i + quarter), u = min(v, w.rows - 1);
-            const float s = vs_row_sum(vs_dot<BF16, 16, float>(w, u, xs, l16)) + vs_bias_of(a.join.bias, u);
-            if (l16 == 0 && v == u && s > -INFINITY && fmaf(eps, fabsf(s), s + slack) >= bound) {
+        for (int r = 0; r < 4; ++r) {
+            v[r] = vs_chunk_row((int)list[r >= 2 && second ? i + 1 : i], (r & 1) * 4 + quarter);
+            u[r] = min(v[r], w.rows - 1);
+        }
+        vs_dots<BF16, 4, float>(w, u, xs, l16, s);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            s[r] = vs_row_sum(s[r]) + vs_bias_of(a.join.bias, u[r]);
+            if (l16 == 0 && (r < 2 ? first : second) && v[r] == u[r] && s[r] > -INFINITY && fmaf(eps, fabsf(s[r]), s[r] + slack) >= bound) {
                 const int at = atomicAdd(&n_rows, 1);
-                if (at < VS_CAND) rows[at] = (uint16_t)(tag * VS_CHUNK + i + quarter);
+                if (at < VS_CAND) rows[at] = (uint16_t)((i - base + r / 2) * VS_CHUNK + (r & 1) * 4 + quarter);
             }
         }
     };
     int least_end = 0;                      // ids from here on had no part in `least`: equal ones come after it
     auto beaten = [&](double s, int v) { return full && (s < least || (s == least && v >= least_end)); };
-    auto exact = [&](int v) {
-        double s = vs_dot<BF16, 64, double>(w, v, xs, lane);
-        for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
-        s += (double)vs_bias_of(a.join.bias, v);
-        if (lane == 0 && !beaten(s, v)) {
-            const int at = atomicAdd(&n_cand, 1);
-            cv[at] = s; ci[at] = v;
+    // the float64 logits of those ids, four of a wave at a time
+    auto exact = [&](int n, int base) {
+        for (int i0 = wave * 4; i0 < n; i0 += THREADS / 16) {
+            const int i = min(i0 + quarter, n - 1), v[1] = {vs_chunk_row((int)list[base + rows[i] / VS_CHUNK], rows[i] % VS_CHUNK)};
+            double s[1];
+            vs_dots<BF16, 1, double>(w, v, xs, l16, s);
+            s[0] = vs_row_sum(s[0]) + (double)vs_bias_of(a.join.bias, v[0]);
+            if (l16 == 0 && i0 + quarter < n && !beaten(s[0], v[0])) {
+                const int at = atomicAdd(&n_cand, 1);
+                cv[at] = s[0]; ci[at] = v[0];
+            }
         }
     };
     auto may = [&](int c, float m) {
@@ -1044,15 +1076,12 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
     }
     __syncthreads();
     bool done = n_list <= VS_LIST;
-    if (done) {                             // all their ids at once, a chunk for each wave
+    if (done) {                             // all their ids at once
         const int n = n_list;
-        for (int i = wave; i < n; i += THREADS / 64) look(list[i], i);
+        for (int i = wave * 2; i < n; i += THREADS / 32) look(i, true, i + 1 < n, 0);
         __syncthreads();
         done = n_rows <= VS_CAND;
-        if (done) {
-            const int nr = n_rows;
-            for (int i = wave; i < nr; i += THREADS / 64) exact(vs_chunk_row(list[rows[i] / VS_CHUNK], rows[i] % VS_CHUNK));
-        }
+        if (done) exact(n_rows, 0);
     }
     if (!done) {                            // many equal logits: block after block
         __syncthreads();
@@ -1070,11 +1099,12 @@ __global__ __launch_bounds__(THREADS) void k_vs_top(VsTop a) {
             for (int i0 = 0; i0 < nl; i0 += 32) {
                 if (tid == 0) n_rows = 0;
                 __syncthreads();
-                for (int i = i0 + wave; i < min(i0 + 32, nl); i += THREADS / 64)
-                    if (may(list[i], (float)cm[list[i]])) look(list[i], i - i0);
+                for (int i = i0 + wave * 2; i < min(i0 + 32, nl); i += THREADS / 32) {
+                    const bool one = may(list[i], (float)cm[list[i]]), two = i + 1 < nl && may(list[i + 1], (float)cm[list[i + 1]]);
+                    if (one || two) look(i, one, two, i0);
+                }
                 __syncthreads();
-                const int nr = n_rows;
-                for (int i = wave; i < nr; i += THREADS / 64) exact(vs_chunk_row(list[i0 + rows[i] / VS_CHUNK], rows[i] % VS_CHUNK));
+                exact(n_rows, i0);
                 __syncthreads();
                 const bool crowded = n_cand > VS_CAND - 256;
                 if (crowded) { compact(); least_end = ((int)(list[min(i0 + 31, nl - 1)] >> 5) + 1) * VS_BLOCK; }

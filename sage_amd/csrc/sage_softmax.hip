@@ -156,7 +156,7 @@ struct FwdPlan {
     int splits;
     int raw;                    // 16-token blocks of a tile of k_vs_forward_raw (0: the weights are packed)
     uint4 *xS, *wS;
-    float *info, *x_exp, *group_max;
+    float *info, *x_exp;
     _Float16* chunk_max;
     float4* part;
     int64_t bytes;
@@ -185,7 +185,6 @@ FwdPlan plan_fwd(const Shape& s, void* ws) {
         p.info = a.take<float>(s.vp / 32 * VS_INFO);
         p.x_exp = a.take<float>(p.n_pad / 32);
     }
-    p.group_max = a.take<float>(s.vp / 32);
     p.part = a.take<float4>(p.splits * p.n_pad);
     p.chunk_max = a.take<_Float16>(s.k ? p.n_pad * p.chunks : 0);
     p.bytes = a.used;
@@ -307,14 +306,14 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
     const hipStream_t st = (hipStream_t)stream;
     const VsSrc w{d_weight, ldw, (int32_t)vocab, dim, dtype == SAGE_BF16}, x{d_x, ldx, (int32_t)n, dim, dtype == SAGE_BF16};
     VsPack of_w = pack_of(w, p.wS, nullptr, p.info + VS_INFO_EXP, VS_INFO, s.vp);
-    of_w.info = p.info; of_w.bias = d_bias; of_w.group_max = alternatives ? p.group_max : nullptr;
+    of_w.info = p.info; of_w.bias = d_bias;
     for (int64_t r0 = 0; r0 < n; r0 += p.rows) {
         const int64_t rows = std::min(p.rows, n - r0);
         const VsSrc xr = rows_from(x, r0, rows);
         const VsFwd f{p.xS, p.wS, p.info, p.x_exp, d_bias != nullptr, (int32_t)vocab, (int32_t)p.tiles, p.splits, (int32_t)(s.vp / VS_BLOCK), (int32_t)p.chunks,
                       p.n_pad, p.part, alternatives ? p.chunk_max : nullptr};
         if (p.raw) {
-            const VsRaw q{xr, w, d_bias, alternatives ? p.group_max : nullptr, f};
+            const VsRaw q{xr, w, d_bias, f};
             const dim3 grid(p.splits, (uint32_t)p.tiles);
 #define VS_F(KS, PL)                                                                                                            \
     if constexpr (vs_raw_most(KS, PL) > 1)                                                                                      \
@@ -333,7 +332,7 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
         const VsJoin j{xr, w, d_bias, d_targets ? d_targets + r0 : nullptr, p.part, (int32_t)rows, p.splits, p.n_pad,
                        d_logprob ? d_logprob + r0 : nullptr, d_entropy ? d_entropy + r0 : nullptr, d_lse + r0};
         if (alternatives) {
-            const VsTop t{j, p.chunk_max, p.group_max, (int32_t)p.chunks, alternatives, d_alt_ids + r0 * alternatives, d_alt_logprobs + r0 * alternatives};
+            const VsTop t{j, p.chunk_max, (int32_t)p.chunks, alternatives, d_alt_ids + r0 * alternatives, d_alt_logprobs + r0 * alternatives};
             // a row alone on a CU is bound by latency: sixteen waves share its chain of loads
             const bool wide = rows <= s.cus;
             if (dtype == SAGE_BF16) { if (wide) k_vs_top<true, 1024><<<(uint32_t)rows, 1024, 0, st>>>(t); else k_vs_top<true, 256><<<(uint32_t)rows, 256, 0, st>>>(t); }
