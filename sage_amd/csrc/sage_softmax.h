@@ -761,35 +761,49 @@ template <int WAVES>
 __device__ __forceinline__ float vs_join_row(const VsJoin& a, int64_t row, int tid, float4* red, double* dred, float* widest = nullptr) {
     const int lane = tid & 63, wave = tid >> 6;
     const bool alone = WAVES == 1 || a.splits <= 64;       // few ranges: the first wave joins them, the others are told
-    const int64_t t = a.targets ? a.targets[row] : -1;
     VsStat st;
     double dot = 0.0;
     float wide = 0.0f;
     st.clear();
+    // over `n` lanes (a power of two): the largest reference first, then sums relative to it
+    auto over = [&](int n) {
+        float ref = st.ref;
+        for (int o = 1; o < n; o <<= 1) ref = fmaxf(ref, __shfl_xor(ref, o));
+        VsStat q;
+        q.clear();
+        q.ref = ref;
+        q.join(st.ref, st.S, st.E);
+        for (int o = 1; o < n; o <<= 1) {
+            q.S += __shfl_xor(q.S, o);
+            q.E += __shfl_xor(q.E, o);
+            if (widest) wide = fmaxf(wide, __shfl_xor(wide, o));
+        }
+        st = q;
+    };
+    const int64_t t = a.targets ? a.targets[row] : -1;
     if (!alone || wave == 0) {
-        const int step = alone ? 64 : 64 * WAVES;
-        for (int i = tid; i < a.splits; i += step) {
+#pragma unroll 4
+        for (int i = tid; i < a.splits; i += alone ? 64 : 64 * WAVES) {
             const float4 q = a.part[(int64_t)i * a.n_pad + row];
             st.join(q.x, q.y, q.z);
             wide = fmaxf(wide, q.w);
         }
-        if (t >= 0 && t < a.w.rows)
-            for (int d = tid; d < a.w.dim; d += step) dot += (double)vs_load(a.x, row, d) * (double)vs_load(a.w, t, d);
-        for (int o = 1; o < 64; o <<= 1) {
-            if (o < a.splits) {                // (the first lane has them all)
-                const float r2 = __shfl_xor(st.ref, o), s2 = __shfl_xor(st.S, o), e2 = __shfl_xor(st.E, o);
-                st.join(r2, s2, e2);
-            }
-            dot += __shfl_xor(dot, o);
-            if (widest) wide = fmaxf(wide, __shfl_xor(wide, o));
-        }
-        if (WAVES > 1 && lane == 0) { red[wave] = make_float4(st.ref, st.S, st.E, wide); dred[wave] = dot; }
+        over(a.splits > 32 ? 64 : a.splits > 16 ? 32 : a.splits > 8 ? 16 : 8);
+        if (WAVES > 1 && lane == 0) red[wave] = make_float4(st.ref, st.S, st.E, wide);
+    }
+    if (wave == WAVES - 1 && t >= 0 && t < a.w.rows) {
+#pragma unroll 8
+        for (int d = lane; d < a.w.dim; d += 64) dot += (double)vs_load(a.x, row, d) * (double)vs_load(a.w, t, d);
+        for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
+        if (WAVES > 1 && lane == 0) *dred = dot;
     }
     if constexpr (WAVES > 1) {
         __syncthreads();
+        const float4 q = red[alone ? 0 : lane % WAVES];
         st.clear();
-        dot = 0.0;
-        for (int i = 0; i < (alone ? 1 : WAVES); ++i) { st.join(red[i].x, red[i].y, red[i].z); dot += dred[i]; wide = fmaxf(wide, red[i].w); }
+        st.ref = q.x; st.S = q.y; st.E = q.z; wide = q.w;
+        if (!alone) over(WAVES);
+        dot = *dred;
     }
     if (widest) *widest = wide;
     const bool empty = st.S == 0.0f;                // nothing but -inf
@@ -815,10 +829,10 @@ __device__ __forceinline__ float vs_join_row(const VsJoin& a, int64_t row, int t
 template <int WAVES>
 __global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
     __shared__ float4 red[4];
-    __shared__ double dred[4];
+    __shared__ double dred;
     const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
     if (row >= a.n) return;
-    (void)vs_join_row<WAVES>(a, row, WAVES == 1 ? threadIdx.x & 63 : threadIdx.x, red, dred);
+    (void)vs_join_row<WAVES>(a, row, WAVES == 1 ? threadIdx.x & 63 : threadIdx.x, red, &dred);
 }
 
 // ---- alternatives -------------------------------------------------------------------------------------------------
@@ -1010,6 +1024,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? BF16 ? 5 : 7 : 4) void k_
         const int n = n_cand;
         for (int i = tid; i < n; i += THREADS) {
             int rank = 0;
+#pragma unroll 4
             for (int j = 0; j < n; ++j) rank += vs_before(cv[j], ci[j], cv[i], ci[i]);
             if (rank < a.k) { cw[rank] = cv[i]; cj[rank] = ci[i]; }
         }
@@ -1058,21 +1073,30 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? BF16 ? 5 : 7 : 4) void k_
         const float up = above(m);
         return m > -INFINITY && up >= bound && !beaten((double)up, (c >> 5) * VS_BLOCK);
     };
-    // every chunk that may hold one of the k, usually a few more than k: only threads whose best may looks again
+    // every chunk that may hold one of the k, usually a few more than k: the threads whose best may say so, and all of them look
+    // through what these few have seen
     const bool may_be = mine > -INFINITY && above(mine) >= bound;
     if (a.chunks <= 256) {
         if (may_be && tid < a.chunks) list[atomicAdd(&n_list, 1)] = tid;
-    } else if (may_be) {
-#pragma unroll 4
-        for (int c = tid * 8; c < a.chunks; c += THREADS * 8) {
+    } else {
+        if (may_be) rows[atomicAdd(&n_rows, 1)] = (uint16_t)tid;
+        __syncthreads();
+        const uint32_t pieces = (uint32_t)(a.chunks + THREADS * 8 - 1) / (THREADS * 8);        // of 8 chunks, of a thread
+        const uint32_t all = n_rows * pieces;
+#pragma unroll 2
+        for (uint32_t i = tid; i < all; i += THREADS) {
+            const int c = ((int)(i % pieces) * THREADS + rows[i / pieces]) * 8;
+            if (c >= a.chunks) continue;
             const h8 m = *(const h8*)&cm[c];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (m[i] > -(_Float16)INFINITY && above((float)m[i]) >= bound) {
+            for (int j = 0; j < 8; ++j)
+                if (m[j] > -(_Float16)INFINITY && above((float)m[j]) >= bound) {
                     const int at = atomicAdd(&n_list, 1);
-                    if (at < VS_LIST) list[at] = c + i;
+                    if (at < VS_LIST) list[at] = c + j;
                 }
         }
+        __syncthreads();
+        if (tid == 0) n_rows = 0;
     }
     __syncthreads();
     bool done = n_list <= VS_LIST;
