@@ -745,9 +745,8 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
     }
 }
 
-// Joins the ranges of a row and takes the given token's log probability.  The token's own logit is summed in float64 (its
-// rounding would otherwise show where the probability is near 1).  WAVES waves work on a row; returns its lse, and the largest
-// size of a weight if asked, to them all.
+// Joins the ranges of a row, by WAVES waves, and takes the given token's log probability.  The token's own logit is summed in
+// float64 (its rounding would otherwise show where the probability is near 1).
 struct VsJoin {
     VsSrc x, w;
     const float* bias;         // as the caller gave it, or null
@@ -758,81 +757,97 @@ struct VsJoin {
     float *logprob, *entropy, *lse;
 };
 template <int WAVES>
-__device__ __forceinline__ float vs_join_row(const VsJoin& a, int64_t row, int tid, float4* red, double* dred, float* widest = nullptr) {
-    const int lane = tid & 63, wave = tid >> 6;
-    const bool alone = WAVES == 1 || a.splits <= 64;       // few ranges: the first wave joins them, the others are told
+struct VsJoined {
     VsStat st;
-    double dot = 0.0;
-    float wide = 0.0f;
-    st.clear();
+    float wide;                // the largest size of a weight
+    double lse;
+    bool empty;                // nothing but -inf
     // over `n` lanes (a power of two): the largest reference first, then sums relative to it
-    auto over = [&](int n) {
-        float ref = st.ref;
-        for (int o = 1; o < n; o <<= 1) ref = fmaxf(ref, __shfl_xor(ref, o));
+    __device__ __forceinline__ void over(int n) {
         VsStat q;
         q.clear();
-        q.ref = ref;
+        q.ref = st.ref;
+        for (int o = 1; o < n; o <<= 1) q.ref = fmaxf(q.ref, __shfl_xor(q.ref, o));
         q.join(st.ref, st.S, st.E);
         for (int o = 1; o < n; o <<= 1) {
             q.S += __shfl_xor(q.S, o);
             q.E += __shfl_xor(q.E, o);
-            if (widest) wide = fmaxf(wide, __shfl_xor(wide, o));
+            wide = fmaxf(wide, __shfl_xor(wide, o));
         }
         st = q;
-    };
-    const int64_t t = a.targets ? a.targets[row] : -1;
-    if (!alone || wave == 0) {
+    }
+    static __device__ __forceinline__ bool alone(const VsJoin& a) { return WAVES == 1 || a.splits <= 64; }   // few ranges: the first wave joins them
+    __device__ __forceinline__ void gather(const VsJoin& a, int64_t row, int tid, float4* red) {
+        st.clear();
+        wide = 0.0f;
+        if (alone(a) && tid >= 64) return;
 #pragma unroll 4
-        for (int i = tid; i < a.splits; i += alone ? 64 : 64 * WAVES) {
+        for (int i = tid; i < a.splits; i += alone(a) ? 64 : 64 * WAVES) {
             const float4 q = a.part[(int64_t)i * a.n_pad + row];
             st.join(q.x, q.y, q.z);
             wide = fmaxf(wide, q.w);
         }
         over(a.splits > 32 ? 64 : a.splits > 16 ? 32 : a.splits > 8 ? 16 : 8);
-        if (WAVES > 1 && lane == 0) red[wave] = make_float4(st.ref, st.S, st.E, wide);
+        if (WAVES > 1 && (tid & 63) == 0) red[tid >> 6] = make_float4(st.ref, st.S, st.E, wide);
     }
-    if (wave == WAVES - 1 && t >= 0 && t < a.w.rows) {
-#pragma unroll 8
-        for (int d = lane; d < a.w.dim; d += 64) dot += (double)vs_load(a.x, row, d) * (double)vs_load(a.w, t, d);
-        for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
-        if (WAVES > 1 && lane == 0) *dred = dot;
-    }
-    if constexpr (WAVES > 1) {
-        __syncthreads();
-        const float4 q = red[alone ? 0 : lane % WAVES];
-        st.clear();
-        st.ref = q.x; st.S = q.y; st.E = q.z; wide = q.w;
-        if (!alone) over(WAVES);
-        dot = *dred;
-    }
-    if (widest) *widest = wide;
-    const bool empty = st.S == 0.0f;                // nothing but -inf
-    const double lse = empty ? -INFINITY : ((double)st.ref + (double)log2f(st.S)) * 0.6931471805599453;
-    if (tid == 0) {
+    // (with more than one wave all have to have gathered)
+    __device__ __forceinline__ void finish(const VsJoin& a, int64_t row, int tid, const float4* red) {
+        if constexpr (WAVES > 1) {
+            const float4 q = red[alone(a) ? 0 : tid % WAVES];
+            st.clear();
+            st.ref = q.x; st.S = q.y; st.E = q.z; wide = q.w;
+            if (!alone(a)) over(WAVES);
+        }
+        empty = st.S == 0.0f;
+        const float l = log2f(st.S);
+        lse = empty ? -INFINITY : ((double)st.ref + (double)l) * 0.6931471805599453;
+        if (tid != 0) return;
         a.lse[row] = (float)lse;
         if (a.entropy) {
-            const float h = VS_LN2 * (log2f(st.S) - st.E / st.S);
+            const float h = VS_LN2 * (l - st.E / st.S);
             a.entropy[row] = empty || h < 0.0f ? 0.0f : h;
         }
-        if (a.logprob) {
-            float lp = 0.0f;
-            if (t >= a.w.rows) lp = NAN;
-            else if (t >= 0) {
-                lp = empty ? -INFINITY : (float)(dot + (double)vs_bias_of(a.bias, t) - lse);
-                if (lp > 0.0f) lp = 0.0f;
-            }
-            a.logprob[row] = lp;
-        }
     }
-    return (float)lse;
+};
+// the given token's logit, in every lane of the wave that asks, without its bias; and what is made of it
+__device__ __forceinline__ double vs_target_logit(const VsJoin& a, int64_t row, int64_t t, int lane) {
+    double dot = 0.0;
+    if (t >= 0 && t < a.w.rows) {
+        float x[8], w[8];                  // (512 elements at most, all loads under way together)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int d = min(lane + i * 64, a.w.dim - 1);
+            x[i] = vs_load(a.x, row, d); w[i] = vs_load(a.w, t, d);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dot += lane + i * 64 < a.w.dim ? (double)x[i] * (double)w[i] : 0.0;
+        for (int o = 1; o < 64; o <<= 1) dot += __shfl_xor(dot, o);
+    }
+    return dot;
+}
+__device__ __forceinline__ void vs_put_logprob(const VsJoin& a, int64_t row, int64_t t, double dot, double lse, bool empty) {
+    float lp = 0.0f;
+    if (t >= a.w.rows) lp = NAN;
+    else if (t >= 0) {
+        lp = empty ? -INFINITY : (float)(dot + (double)vs_bias_of(a.bias, t) - lse);
+        if (lp > 0.0f) lp = 0.0f;
+    }
+    a.logprob[row] = lp;
 }
 template <int WAVES>
 __global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
     __shared__ float4 red[4];
-    __shared__ double dred;
     const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
     if (row >= a.n) return;
-    (void)vs_join_row<WAVES>(a, row, WAVES == 1 ? threadIdx.x & 63 : threadIdx.x, red, &dred);
+    const int tid = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const bool last = tid >> 6 == WAVES - 1 && a.logprob;      // its wave takes the given token
+    VsJoined<WAVES> j;
+    j.gather(a, row, tid, red);
+    const int64_t t = last ? a.targets[row] : -1;
+    const double dot = vs_target_logit(a, row, t, tid & 63);
+    if (WAVES > 1) __syncthreads();
+    j.finish(a, row, tid, red);
+    if (last && (tid & 63) == 0) vs_put_logprob(a, row, t, dot, j.lse, j.empty);
 }
 
 // ---- alternatives -------------------------------------------------------------------------------------------------
@@ -956,28 +971,18 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? BF16 ? 5 : 7 : 4) void k_
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = tid & 15, quarter = lane >> 4;
     const _Float16* cm = a.chunk_max + row * a.chunks;
     typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-    float widest;
-    const float lse = vs_join_row<THREADS / 64>(a.join, row, tid, (float4*)cv, cw, &widest);
-    __syncthreads();
-    if (lse != lse) {                       // no order among the logits
-        if (tid < a.k) { a.ids[row * a.k + tid] = -1; a.logprobs[row * a.k + tid] = NAN; }
-        return;
+    VsJoined<THREADS / 64> joined;
+    joined.gather(a.join, row, tid, (float4*)cv);
+    // (few ranges are the first wave's: the others have the row ready by then)
+    float l1 = 0.0f;
+    if (wave) {
+        l1 = vs_put_x<BF16>(x, row, xs, tid - 64, THREADS - 64);
+        for (int o = 1; o < 64; o <<= 1) l1 += __shfl_xor(l1, o);
     }
-    float l1 = vs_put_x<BF16>(x, row, xs, tid, THREADS);
-    for (int o = 1; o < 64; o <<= 1) l1 += __shfl_xor(l1, o);
     if (lane == 0) red[wave] = l1;
     if (tid == 0) n_cand = n_rows = n_list = 0;
-    __syncthreads();
-    l1 = 0.0f;
-    for (int i = 0; i < THREADS / 64; ++i) l1 += red[i];
-    __syncthreads();
-    const float eps = 4.0f * (float)(x.dim + 16) * 5.9604645e-8f;
-    const float slack = eps * 2.0f * l1 * widest;
-    // a chunk's largest logit lies between these (d, and a step of float16; past its range there is one bound only)
-    auto off = [&](float m) { return fmaf(eps + 0.0009765625f, fabsf(m), slack + 5.9604645e-8f); };
-    auto above = [&](float m) { return m >= 65504.0f ? INFINITY : m + off(m); };
-    auto below = [&](float m) { return m <= -65504.0f ? -INFINITY : fminf(m, 65504.0f) - off(fminf(m, 65504.0f)); };
-    float mine = -INFINITY;                 // this thread's largest (both bounds grow with it)
+    const int64_t target = a.join.logprob ? a.join.targets[row] : -1;
+    float mine = -INFINITY;                 // this thread's largest
     if (a.chunks <= 256) {
         if (tid < a.chunks) mine = (float)cm[tid];
     } else {
@@ -987,6 +992,26 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? BF16 ? 5 : 7 : 4) void k_
 #pragma unroll
         for (int i = 0; i < 8; ++i) mine = fmaxf(mine, (float)most[i]);
     }
+    __syncthreads();
+    joined.finish(a.join, row, tid, (float4*)cv);
+    const double lse = joined.lse;
+    auto given = [&]() {                    // by one wave
+        const double dot = vs_target_logit(a.join, row, target, lane);
+        if (lane == 0) vs_put_logprob(a.join, row, target, dot, lse, joined.empty);
+    };
+    if (lse != lse) {                       // no order among the logits
+        if (tid < a.k) { a.ids[row * a.k + tid] = -1; a.logprobs[row * a.k + tid] = NAN; }
+        if (wave == 1 && a.join.logprob) given();
+        return;
+    }
+    l1 = 0.0f;
+    for (int i = 0; i < THREADS / 64; ++i) l1 += red[i];
+    const float eps = 4.0f * (float)(x.dim + 16) * 5.9604645e-8f;
+    const float slack = eps * 2.0f * l1 * joined.wide;
+    // a chunk's largest logit lies between these (d, and a step of float16; past its range there is one bound only)
+    auto off = [&](float m) { return fmaf(eps + 0.0009765625f, fabsf(m), slack + 5.9604645e-8f); };
+    auto above = [&](float m) { return m >= 65504.0f ? INFINITY : m + off(m); };
+    auto below = [&](float m) { return m <= -65504.0f ? -INFINITY : fminf(m, 65504.0f) - off(fminf(m, 65504.0f)); };
     float low = below(mine);
     if (a.chunks <= 256) {
         if (tid < 256) best[tid] = low;
@@ -995,8 +1020,9 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? BF16 ? 5 : 7 : 4) void k_
         if (tid % (THREADS / 256) == 0) best[tid / (THREADS / 256)] = low;
     }
     __syncthreads();
+    if (wave == 1 && a.join.logprob) given();
     if (wave == 0) {
-        // the k-th largest of the 256 by halving, over the upper 23 bits of a key in the floats' order (a lower bound will do)
+        // the k-th largest of the 256, two bits at a time, over the upper 20 of a key in the floats' order (a lower bound will do)
         uint32_t key[4];
         const float4 q = *(const float4*)&best[lane * 4];
         const float v[4] = {q.x, q.y, q.z, q.w};
@@ -1006,12 +1032,16 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? BF16 ? 5 : 7 : 4) void k_
             key[i] = (u & 0x80000000u) ? ~u : u | 0x80000000u;
         }
         uint32_t at = 0;
-        for (int bit = 31; bit > 8; --bit) {
-            const uint32_t next = at | (1u << bit);
-            int n = 0;
+        for (int bit = 30; bit >= 12; bit -= 2) {
+            uint32_t next = at;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) n += __popcll(__ballot(key[i] >= next));
-            if (n >= a.k) at = next;
+            for (uint32_t two = 1; two < 4; ++two) {
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) n += __popcll(__ballot(key[i] >= (at | two << bit)));
+                if (n >= a.k) next = at | two << bit;
+            }
+            at = next;
         }
         if (lane == 0) red[0] = at <= 0x007FFFFFu ? -INFINITY : __uint_as_float((at & 0x80000000u) ? at & 0x7FFFFFFFu : ~at);
     }
@@ -1141,7 +1171,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? BF16 ? 5 : 7 : 4) void k_
     if (tid < a.k) {
         const bool have = tid < n_cand;
         a.ids[row * a.k + tid] = have ? ci[tid] : -1;
-        a.logprobs[row * a.k + tid] = have ? fminf((float)(cv[tid] - (double)lse), 0.0f) : -INFINITY;
+        a.logprobs[row * a.k + tid] = have ? fminf((float)(cv[tid] - lse), 0.0f) : -INFINITY;
     }
 }
 
