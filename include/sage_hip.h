@@ -213,8 +213,9 @@ int sage_train_embeddings(sage_ctx* ctx, int32_t dim, int32_t window, int32_t ne
  * The [n][vocab] matrix of logits is never stored.
  *   d_x [n][dim], d_weight [vocab][dim]   both SAGE_F32 or both SAGE_BF16, rows ldx / ldw elements apart (>= dim); any alignment
  *                    of rows.  Products and sums are float32 (float32 inputs at float32 accuracy); the softmax's too.
- *   d_bias [vocab]   float32 or NULL; -inf, or any value of -1e30 or less, takes an id out (so does a logit of -6e29).  A row that has nothing left gets lse -inf, logprob -inf, entropy 0,
- *                    alternatives -1.  x and weight are finite: a logit that is NaN or +inf makes its row NaN, alternatives -1.
+ *   d_bias [vocab]   float32 or NULL; -inf, or any value of -1e30 or less, takes an id out (so does a logit of -6e29).  A row that
+ *                    has nothing left gets lse -inf, logprob -inf, entropy 0, alternatives -1.  x is finite, and so are the weights of ids that
+ *                    are not taken out: a logit that is NaN or +inf makes its row NaN, alternatives -1.
  *   d_targets [n]    int64, or NULL (then no d_logprob).  A negative target means none: logprob 0, no gradient.  The host cannot
  *                    see a target of `vocab` or more: its logprob is NaN, and so are the gradients it reaches.
  *   d_logprob, d_entropy, d_lse [n] float32 (d_logprob and d_entropy may be NULL); d_alt_ids int32 and d_alt_logprobs float32
@@ -239,8 +240,9 @@ int sage_token_logprobs_device(sage_ctx* ctx, int32_t dtype, int64_t n, int64_t 
  * h = d_grad_entropy (float32 [n]; either may be NULL, not both),
  *   d_dx [n][dim] = G weight,   d_dweight [vocab][dim] = G^T x  (the inputs' type, rows lddx / lddw apart),   d_dbias[v] = sum_n G_nv
  * (float32).  d_dx or d_dweight may be NULL; d_dbias needs d_dweight.  d_lse and d_entropy (needed with d_grad_entropy) are
- * what the forward call returned for the same inputs.  The logits are formed again; sums are float32.  With n == 0 the
- * weight's and bias's gradients are zeros.  Results are overwritten, not accumulated.
+ * what the forward call returned for the same inputs.  A token without a target and without an entropy gradient (or with
+ * gradients of 0) has no part in any result, whatever its row of x holds: dx is 0 there.  The logits are formed again; sums are float32.  With n == 0 the
+ * weight's and bias's gradients are zeros.  Results are overwritten, not accumulated, and lie over no input and no other result.
  */
 int64_t sage_token_logprobs_backward_workspace(sage_ctx* ctx, int32_t dtype, int64_t n, int64_t vocab, int32_t dim);
 int sage_token_logprobs_backward_device(sage_ctx* ctx, int32_t dtype, int64_t n, int64_t vocab, int32_t dim, const void* d_x, int64_t ldx,

@@ -129,7 +129,9 @@ __device__ __forceinline__ void vs_split(vs_f8 v, vs_bits* out) {
 // order that a lane has values in.  Rows past the end and elements past `dim` are zero.  A fragment is one
 // coalesced 1 KiB load of a wave, whatever the caller's row length, stride and alignment are.  One workgroup packs 32 rows:
 // a lane loads the eight elements that its place in an S fragment asks for; T fragments are read back through LDS.
-// PL = 2: the 32 rows are multiplied by 2^e, e such that the largest finite element comes to just under 2^13.
+// PL = 2: the 32 rows are multiplied by 2^e, e such that the largest finite element comes to just under 2^13.  Bound by HBM:
+// 131,072 x 300 bf16 for a forward pass, 79 MB read and 84 MB written, 36 us (4.5 TB/s); rows of 511 bf16, that start at any
+// 2-byte boundary, 84 MB in all in 32 us.
 
 // eight elements from `d` on; zeros past the end of the row
 template <int PL>
@@ -181,11 +183,16 @@ struct VsPack {
     int32_t vocab;
 };
 
+// A token that has no part in the gradient, whatever its x, lse and entropy hold
+__device__ __forceinline__ bool vs_idle(const VsPack& a, int64_t i) {
+    const bool of_target = a.g && a.targets && a.targets[i] >= 0 && a.g[i] != 0.0f;
+    return !of_target && !(a.h && a.h[i] != 0.0f);
+}
 __device__ __forceinline__ void vs_put_token(const VsPack& a, int64_t i) {
-    // rows past the end and rows whose every id is masked: an lse that makes every p 0, whatever the bias is
+    // rows past the end, idle ones and rows whose every id is masked: an lse that makes every p 0, whatever the bias is
     float l2 = -VS_NOTHING, A = 0.0f, B = 0.0f, gl = 0.0f;
     int32_t t = -1;
-    if (i < a.src.rows) {
+    if (i < a.src.rows && !vs_idle(a, i)) {
         const float l = a.lse[i];
         const int64_t tt = a.targets ? a.targets[i] : -1;
         const bool empty = l == -INFINITY;
@@ -199,7 +206,7 @@ __device__ __forceinline__ void vs_put_token(const VsPack& a, int64_t i) {
         if (tt >= a.vocab) gl = NAN;
         t = tt >= 0 && tt < a.vocab ? (int32_t)tt : -1;
         A = -gl;
-        if (a.h && !empty) { A -= a.h[i] * a.entropy[i]; B = -a.h[i] * VS_LN2; }
+        if (a.h && a.h[i] != 0.0f && !empty) { A -= a.h[i] * a.entropy[i]; B = -a.h[i] * VS_LN2; }
         A *= fix; B *= fix;
     }
     float* to = a.tokens + (i >> 5) * VS_TOKEN + (i & 31);
@@ -220,13 +227,19 @@ __global__ __launch_bounds__(256) void k_vs_pack(VsPack pa, VsPack pb) {
     auto row_of = [&](int f) { return f / STEPS * M + col; };
     auto element_of = [&](int f) { return f % STEPS * K + lane / M * 8; };
     const int64_t row0 = group * 32;
+    bool there[32 / M];                        // rows past the end, of masked ids and of idle tokens are taken as 0, whatever they hold
+#pragma unroll
+    for (int r = 0; r < 32 / M; ++r) {
+        const int64_t row = row0 + r * M + col;
+        there[r] = row < a.src.rows && !(a.bias && a.bias[row] <= VS_NOTHING) && !(a.tokens && vs_idle(a, row));
+    }
     vs_f8 v[N];
     float big = 0.0f, fin = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int f = i * 4 + wave;
         v[i] = vs_f8(0.0f);
-        if (f < 2 * KS && row0 + row_of(f) < a.src.rows && element_of(f) < a.src.dim) v[i] = vs_eight<PL>(a.src, row0 + row_of(f), element_of(f));
+        if (f < 2 * KS && there[f / STEPS ? 32 / M - 1 : 0] && element_of(f) < a.src.dim) v[i] = vs_eight<PL>(a.src, row0 + row_of(f), element_of(f));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float q = fabsf(v[i][j]);
@@ -519,6 +532,10 @@ __device__ __forceinline__ void vs_forward_step(const VsFwd& a, int row0, const 
     rows.template add<TOP, PL == 2>(s, unit);
 }
 
+// Bound by the matrix units and the power they draw (the clock falls to 1.8 - 2.2 GHz under them), the exponentials beside
+// them second.  8,192 tokens x 262,144 ids, D = 50 float32: 737 us, 0.82 * 10^12 operations of the MFMAs (three products, 64
+// elements for 50) at 1.1 * 10^15 a second, where a large bf16 matrix product of the library reaches 1.38 * 10^15; 4,096 x 65,536,
+// D = 300 bf16: 184 us, 0.93 * 10^15.
 // Four waves, a tile each, share the streaming rows through LDS.  SR rows at a time are copied straight into LDS (they are
 // packed in the order of the copy) while the SR before them are worked on: one barrier a step.
 typedef const __attribute__((address_space(1))) void* vs_global_ptr;
@@ -601,7 +618,9 @@ __device__ __forceinline__ float vs_bias_of(const float* bias, int64_t v) {
 // Few tokens: bound by the one reading of the weights, which are taken as they lie (no packing): a lane loads the eight
 // elements of a row that its place in a fragment asks for, at whatever alignment they have.  The last piece of a row that is
 // no whole number of pieces long is taken back from the row's end, with the elements before it weighted 0 in x: no read
-// leaves the row (so there are eight elements at least).  A wave is a tile of 16 TB tokens against one range of the vocabulary; the four of a workgroup join theirs.
+// leaves the row (so there are eight elements at least).  A wave is a tile of 16 TB tokens against one range of the vocabulary; the
+// four of a workgroup join theirs.  One token, 262,144 x 50 float32: 52 MB in 14.8 us (3.5 TB/s); five, 229,376 x 300 bf16: 138 MB in
+// 31 us (4.4 TB/s; a copy of 4 GB reaches 4.8).
 template <int PL> struct VsPiece;
 template <> struct VsPiece<1> {            // of bf16: a fragment as it is
     vs_bf8 v;
@@ -683,9 +702,10 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
 #pragma unroll 1
         for (int row0 = c * 64; row0 < (c + 1) * 64; row0 += 32) {
             // (loads first and together; the bias is added last, so that no wait for it stands before the products)
-            VsPiece<PL> raw[2][KG], big;
+            VsPiece<PL> raw[2][KG], big[2];
             vs_f4 s[2][TB], b[2];
-            big.clear();
+            float of_row[2] = {0.0f, 0.0f};
+            big[0].clear(); big[1].clear();
 #pragma unroll
             for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
@@ -699,6 +719,8 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
                         if (g + k < KS) raw[rb][k].load(a.w, min(row0 + rb * 16 + col, a.w.rows - 1), at[g + k]);
                 if (g + KG >= KS && a.bias) {
 #pragma unroll
+                    for (int rb = 0; rb < 2; ++rb) of_row[rb] = a.bias[min(row0 + rb * 16 + col, a.w.rows - 1)];
+#pragma unroll
                     for (int j = 0; j < 8; ++j) b[j >> 2][j & 3] = a.bias[min(row0 + (j >> 2) * 16 + quad * 4 + (j & 3), a.w.rows - 1)];
                 }
 #pragma unroll
@@ -707,7 +729,7 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
                         vs_bits wf[2][PL];
 #pragma unroll
                         for (int rb = 0; rb < 2; ++rb) {
-                            big.measure(raw[rb][k]);
+                            big[rb].measure(raw[rb][k]);
                             raw[rb][k].parts(wf[rb]);
                         }
                         vs_mfma_parts<PL, 16, 2, TB>(wf, [&](int t, int p) { return x[t][g + k][p]; }, s);
@@ -723,7 +745,8 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
                     for (int t = 0; t < TB; ++t) s[j >> 2][t][j & 3] = gone ? VS_MASKED : s[j >> 2][t][j & 3] + q;
                 }
             }
-            wide = fmaxf(wide, big.largest());
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb) wide = fmaxf(wide, of_row[rb] <= VS_NOTHING ? 0.0f : big[rb].largest());
             __builtin_amdgcn_sched_barrier(0);
             rows.template add<true, false>(s, unscaled);
             if (a.f.chunk_max) rows.template chunk<false>(a.f, tile, row0 / VS_BLOCK, (row0 >> 5) & 7, lane, true);
@@ -746,7 +769,8 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
 }
 
 // Joins the ranges of a row, by WAVES waves, and takes the given token's log probability.  The token's own logit is summed in
-// float64 (its rounding would otherwise show where the probability is near 1).
+// float64 (its rounding would otherwise show where the probability is near 1).  Bound by latency: 4 us for 87 rows of 64 ranges,
+// 8 us for 8,192 rows of a few.
 struct VsJoin {
     VsSrc x, w;
     const float* bias;         // as the caller gave it, or null
@@ -829,7 +853,8 @@ __device__ __forceinline__ void vs_put_logprob(const VsJoin& a, int64_t row, int
     float lp = 0.0f;
     if (t >= a.w.rows) lp = NAN;
     else if (t >= 0) {
-        lp = empty ? -INFINITY : (float)(dot + (double)vs_bias_of(a.bias, t) - lse);
+        const float b = vs_bias_of(a.bias, t);
+        lp = empty || b == -INFINITY ? -INFINITY : (float)(dot + (double)b - lse);
         if (lp > 0.0f) lp = 0.0f;
     }
     a.logprob[row] = lp;
@@ -852,14 +877,21 @@ __global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
 
 // ---- alternatives -------------------------------------------------------------------------------------------------
 // The k largest logits of a row, ties to the lower id, in the order of the logits as float64 sums them.  The forward pass
-// left each chunk's largest float32 logit m; a float32 sum is within d = 4 (D + 16) 2^-24 (|m| + 2 |x|_1 max |w|) of the true
-// one.  At least k logits are no less than the k-th largest m - d, so only chunks with m + d at or above that can hold one
-// of the k: a few more than k, of 16 ids each.  Their logits are formed again in float32, those that reach the bound once more in float64,
-// and the best k of these few are ranked by counting.  A workgroup per row.
+// left each chunk's largest float32 logit m, rounded towards 0 to float16; a float32 sum is within d = 4 (D + 16) 2^-24 (|m| + 2 |x|_1
+// max |w|) of the true one, the rounding adds 2^-10 |m|.  At least k logits are no less than the k-th largest m - d, so only
+// chunks with m + d at or above that can hold one of the k: a few more than k, of 8 ids each.  Their logits are formed again in
+// float32, those that reach the bound once more in float64, and the best k of these few are ranked by counting.  A workgroup
+// per row.
 //
 // The bound is taken over 256 groups of chunks (the k-th largest of the groups' largest m - d is a bound too, and rarely a
-// lower one): one pass over the maxima.  Where too many chunks reach it (many equal logits, a zero vector), they are visited
-// in ascending order, and once k logits are known a later one that cannot beat the k-th is skipped even when it ties.
+// lower one): one pass over the maxima, after which all threads look through what the few threads have seen whose best may be
+// one.  Where too many chunks reach it (many equal logits, a zero vector), they are visited in ascending order, and once k
+// logits are known a later one that cannot beat the k-th is skipped even when it ties.
+//
+// Bound by latency for a few rows (11.6 us for one row of 262,144 ids, k = 10), by the reading of the maxima for many: 8,192 rows of
+// 262,144 ids 144 us (537 MB of maxima and 0.15 GB of rows looked at again); by those rows where they are wide and k is large: 1,021
+// rows, D = 511, k = 32, 58 us for 0.28 GB.  Chunks of 8 as float16 take the bytes of chunks of 16 as float32 (which that case
+// paid 140 us for).
 #define VS_MAX_K 32
 #define VS_CAND 1024
 #define VS_LIST 256
@@ -1181,6 +1213,10 @@ __device__ __forceinline__ void vs_store(void* p, int64_t at, float v, int bf16)
     else ((float*)p)[at] = v;
 }
 
+// Either gradient forms the logits again: n V D products beside the n V D of its own sums, and neither is stored.  Bound by the
+// matrix units' power (float32, three products each: 8,192 tokens x 262,144 ids, D = 50, dx 1.42 ms and dw 1.52 ms, 1.65 * 10^12 operations
+// of the MFMAs each, 1.1 * 10^15 a second) and, where a wave has registers for 16 columns only (bf16, D = 300), by the LDS reads of
+// the streaming fragments, 16 operations a byte: 4,096 x 65,536, entropy gradient too, dx 361 us (0.95 * 10^15), dw 474 us.
 struct VsBwd {
     const uint4 *stayS;        // stationary rows (columns of the product)
     const uint4 *flowS, *flowT;// streaming rows, and transposed
@@ -1551,7 +1587,7 @@ __global__ __launch_bounds__(256, TB * M * KS * (4 * PL + 8) > 170 * 16 ? 1 : 2)
     if (live) g.store(a, split, lane);
 }
 
-// Sums the partials of a row in a fixed order and writes it: dx = A sum p w + gl w_t (without an entropy gradient; with
+// Sums the partials of a row in a fixed order (eight loads under way: 17 us for 4,096 x 320 of 8 ranges; 4 us for 129 x 64) and writes it: dx = A sum p w + gl w_t (without an entropy gradient; with
 // one the partials hold p (A + B e) already), dw as it is, db beside it.
 struct VsSum {
     const float* part;

@@ -15,7 +15,7 @@
 namespace {
 
 constexpr int64_t VS_PAD = 128;                 // rows are padded to this (ids to VS_BLOCK)
-constexpr int64_t VS_ROWS_MAX = 16384;          // tokens of one pass of the forward kernels
+constexpr int64_t VS_ROWS_MAX = 16384;          // tokens of one pass of the forward kernels (their chunks' maxima: 1 GB for 262,144 ids)
 constexpr int64_t VS_RAW = 512;                 // at most this many tokens read the weights as they lie
 constexpr size_t VS_ALIGN = 256;
 
@@ -126,7 +126,8 @@ int per_cu() {
 
 // Into how many ranges the streaming axis (of `units` pieces) is cut, for `groups` workgroups along the other: the number that
 // ends soonest if the chip works `resident` workgroups off at a time, each as long as its pieces and `cost` more to start
-// and end (the loading of its stationary rows; for the gradients the writing and adding of its sums too).
+// and end (the loading of its stationary rows; for the gradients the writing and adding of its sums too).  No cost at all
+// and three times as much measure within 2 % of these (6 shapes, 129 x 1,200 to 8,192 x 65,536).
 int vs_splits(int64_t resident, int64_t groups, int64_t units, double cost) {
     const int64_t most = std::min(units, std::max<int64_t>(1, 4 * resident / groups));
     int64_t best = 1;
@@ -139,7 +140,12 @@ int vs_splits(int64_t resident, int64_t groups, int64_t units, double cost) {
 }
 
 // Token blocks (of 16) of a wave that reads the weights as they lie, one, or two where registers allow and tokens are there;
-// 0: the weights are packed first.
+// 0: the weights are packed first.  Packing costs a launch and a pass over the weights, reading them as they lie one such pass per
+// tile: worth it for 2 tiles (3 of two blocks), and for more where the vocabulary is short.  Measured, us, as they lie / packed:
+//   D = 50 float32, 262,144 ids   64 tokens 39 / 55   128: 65 / 55      16,384 ids   256: 13 / 19   384: 16 / 19    32,768   512: 34 / 24
+//   D = 300 bf16, 131,072 ids     64: 38 / 53   128: 64 / 53            8,192 ids    256: 13 / 22                  32,768   256: 26 / 28
+//   D = 300 float32, 131,072 ids  32: 119 / 128   64: 227 / 135         8,192 ids    128: 33 / 44   256: 44 / 44
+//   D = 512 bf16, 131,072 ids     32: 63 / 77   64: 112 / 79            1,200 ids    512: 18 / 25                  32,768   96: 45 / 32
 int vs_raw_blocks(const Shape& s) {
     if (s.n > VS_RAW || s.dim < 8) return 0;
     int most = 1;
@@ -333,10 +339,13 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
                        d_logprob ? d_logprob + r0 : nullptr, d_entropy ? d_entropy + r0 : nullptr, d_lse + r0};
         if (alternatives) {
             const VsTop t{j, p.chunk_max, (int32_t)p.chunks, alternatives, d_alt_ids + r0 * alternatives, d_alt_logprobs + r0 * alternatives};
-            // a row alone on a CU is bound by latency: sixteen waves share its chain of loads
+            // a row alone on a CU is bound by latency: sixteen waves share its chain of loads (262,144 ids, D = 50: one row 33 us
+            // with the forward kernel, 39 with four; 256 rows 73 and 79; 320 rows 121 and 113)
             const bool wide = rows <= s.cus;
             if (dtype == SAGE_BF16) { if (wide) k_vs_top<true, 1024><<<(uint32_t)rows, 1024, 0, st>>>(t); else k_vs_top<true, 256><<<(uint32_t)rows, 256, 0, st>>>(t); }
             else { if (wide) k_vs_top<false, 1024><<<(uint32_t)rows, 1024, 0, st>>>(t); else k_vs_top<false, 256><<<(uint32_t)rows, 256, 0, st>>>(t); }
+        // (many ranges: one token of 262,144 ids 19 us with the forward kernel, 23 where one wave joins its 1,024 ranges; of 16,384 ids, 64
+        // ranges, 8.8 and 8.5)
         } else if (p.splits > 64) k_vs_join<4><<<(uint32_t)rows, 256, 0, st>>>(j);
         else k_vs_join<1><<<cdiv(rows, 4), 256, 0, st>>>(j);
     }

@@ -4,7 +4,7 @@ likely alternatives, the gradient of both, and the clipping of gradients by thei
 The reference trains its embeddings with negative samples in place of this softmax (embeddings.py:68-75) and scores with
 log-sigmoids of row products (utils.py:125-138); here the sum over the vocabulary itself is taken, without storing a
 [tokens][vocabulary] matrix.  All calls are enqueued on the current stream of the tensors' device and return at once, may
-be captured into a graph, and take their workspace from torch's allocator."""
+be captured into a graph (once a first call has made the device's engine), and take their workspace from torch's allocator."""
 from __future__ import annotations
 
 from array import array
@@ -76,7 +76,8 @@ def token_logprobs(x: torch.Tensor, weight: torch.Tensor, targets: Optional[torc
     """log p(targets[n] | x[n]) with p = softmax(x weight^T + bias), the entropy of p, and its `alternatives` largest ids.
 
     x [n, D] and weight [V, D] are both float32 or both bfloat16 with any row stride; bias float32 [V] (-inf masks an id);
-    targets int64 or int32 [n] (negative: none).  D <= 512, V <= 2^20, at most 32 alternatives (ties: the lower id)."""
+    targets int64 or int32 [n] (negative: none; such a row of x may hold anything in the gradient).  What rows of masked ids hold
+    does not matter.  D <= 512, V <= 2^20, at most 32 alternatives (ties: the lower id)."""
     _rows("x", x)
     _rows("weight", weight, x)
     (n, dim), vocab, dev = x.shape, weight.shape[0], x.device
@@ -84,16 +85,17 @@ def token_logprobs(x: torch.Tensor, weight: torch.Tensor, targets: Optional[torc
     targets = _targets(targets, n, dev)
     engine, kind = get_engine(dev.index), _TYPES[x.dtype]
     need = engine.token_logprobs_workspace(kind, n, vocab, dim, int(alternatives))
-    out = torch.empty((3, n), dtype=torch.float32, device=dev)
-    logprob = out[0] if targets is not None else None
+    logprob, entropy, lse = torch.empty((3, n), dtype=torch.float32, device=dev).unbind(0)
+    if targets is None:
+        logprob = None
     alt = (None, None)
     if alternatives:
         alt = (torch.empty((n, alternatives), dtype=torch.int32, device=dev), torch.empty((n, alternatives), dtype=torch.float32, device=dev))
     ws = _workspace(need, dev)
     engine.token_logprobs_device(kind, n, vocab, dim, x.data_ptr(), _stride(x), weight.data_ptr(), _stride(weight), _address(bias),
-                                 _address(targets), int(alternatives), _address(logprob), out[1].data_ptr(), out[2].data_ptr(),
+                                 _address(targets), int(alternatives), _address(logprob), entropy.data_ptr(), lse.data_ptr(),
                                  _address(alt[0]), _address(alt[1]), ws.data_ptr(), ws.numel(), _stream(dev))
-    return TokenLogprobs(logprob, out[1], out[2], *alt)
+    return TokenLogprobs(logprob, entropy, lse, *alt)
 
 
 def token_logprobs_backward(x: torch.Tensor, weight: torch.Tensor, targets: Optional[torch.Tensor], forward: TokenLogprobs,

@@ -154,3 +154,72 @@ def test_clip_where_the_kernels_change(sizes):
         for t, o in zip(before, grads):
             d = t.double() * (limit / want if want else 1.0)
             close(o, d, d.abs() * (torch.finfo(t.dtype).eps / 2 + 3 * 2.0 ** -24) + 1e-37, "clipped")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,V,D", [(3, 700, 50), (40, 20000, 50), (3, 700, 511), (530, 900, 50), (530, 900, 300), (530, 900, 512)])
+def test_what_masked_rows_hold_does_not_matter(n, V, D, dtype):
+    """The weights of masked ids: NaN, infinities and the type's largest values; targets among them."""
+    from sage_amd import vocab_softmax as vs
+    for low in (float("-inf"), -1e30):
+        x, w, _, t = make(n, V, D, dtype, seed=4)
+        g = torch.Generator().manual_seed(8)
+        gone = torch.rand(V, generator=g) < 0.3
+        gone[32:96] = True
+        b = torch.where(gone, low, 0.25).float().cuda()
+        clean, dirty = w.clone(), w.clone()
+        clean[gone.cuda()] = 0
+        for i, v in enumerate((float("nan"), float("inf"), float("-inf"), torch.finfo(dtype).max)):
+            dirty[torch.nonzero(gone).view(-1)[i::4].cuda()] = v
+        ref = vs.token_logprobs(x, clean, t, bias=b, alternatives=6)
+        e = Exact(x, clean, b, t, 6)
+        check_forward(ref, e, 6)
+        got = vs.token_logprobs(x, dirty, t, bias=b, alternatives=6)
+        for a, c in zip(got, ref):
+            assert torch.equal(a, c)
+        t2 = torch.where(gone.cuda()[t.clamp(min=0)], -1, t)          # (the gradient of a masked target asks for its row)
+        gl = torch.linspace(-1, 1, n).cuda()
+        for a, c in zip(vs.token_logprobs_backward(x, dirty, t2, got, gl, bias=b, grad_entropy=gl), vs.token_logprobs_backward(x, clean, t2, ref, gl, bias=b, grad_entropy=gl)):
+            assert torch.isfinite(a).all() and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [50, 300])
+def test_what_idle_tokens_hold_does_not_matter(D, dtype):
+    """A padded batch: the rows without a target hold NaN, infinities and large values."""
+    from sage_amd import vocab_softmax as vs
+    n, V = 200, 1500
+    x, w, b, t = make(n, V, D, dtype, "prior", seed=2)
+    idle = torch.arange(n, device="cuda") % 3 == 1
+    t[:] = torch.where(idle, -1, t.clamp(min=0))
+    dirty = x.clone()
+    for i, v in enumerate((float("nan"), float("inf"), torch.finfo(dtype).max)):
+        dirty[torch.nonzero(idle).view(-1)[i::3]] = v
+    clean = x.clone()
+    clean[idle] = 0
+    gl = torch.linspace(-1, 1, n).cuda() + 0.003
+    gh = torch.where(idle, 0.0, gl)
+    f, ref = vs.token_logprobs(dirty, w, t, bias=b), vs.token_logprobs(clean, w, t, bias=b)
+    assert torch.equal(f.logprob, ref.logprob) and torch.equal(f.lse[~idle], ref.lse[~idle])
+    for h in (None, gh):
+        got, want = (vs.token_logprobs_backward(x, w, t, r, gl, bias=b, grad_entropy=h) for x, r in ((dirty, f), (clean, ref)))
+        for a, c in zip(got, want):
+            assert torch.equal(a, c)
+        assert (got[0][idle] == 0).all()
+        (wx, tx), (ww, tw), (wb, tb) = Exact(clean, w, b, t).gradient(gl, h, dtype)
+        close(got[0], wx, tx, "dx"), close(got[1], ww, tw, "dw"), close(got[2], wb, tb, "db")
+
+
+def test_logits_far_from_zero():
+    """Beyond float16, in which the largest logits of a chunk are kept; and so far that all of them look alike there."""
+    from sage_amd import vocab_softmax as vs
+    for n in (5, 530):
+        x, w, _, t = make(n, 4000, 50, F32, seed=6)
+        for shift in (300.0, -5000.0, 2e5, -2e5, 3e6):
+            b = torch.full((4000,), shift, device="cuda")
+            b[::5] = float("-inf")
+            e = Exact(x, w, b, t, 7)
+            f = vs.token_logprobs(x, w, t, bias=b, alternatives=7)
+            check_forward(f, e, 7)
+            b[7:] = float("-inf")                    # six ids are left
+            check_forward(vs.token_logprobs(x, w, t, bias=b, alternatives=7), Exact(x, w, b, t, 7), 7)
