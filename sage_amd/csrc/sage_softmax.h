@@ -669,10 +669,11 @@ struct VsRaw {
     const float* bias;         // as the caller gave it, or null
     VsFwd f;                   // chunks, blocks, n_pad, part, chunk_max; splits: workgroups of a tile
 };
+// (One wave a SIMD where two would spill: D = 300 float32, 16 tokens, 131,072 ids 39 us against 67; D = 512 bf16 35 against 51.)
 template <int KS, int PL, int TB>
-__global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(VsRaw a) {
+__global__ __launch_bounds__(256, KS * PL > 14 ? 1 : 2) void k_vs_forward_raw(VsRaw a) {
     const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-    constexpr int KG = PL == 1 ? (KS < 16 ? KS : 8) : KS <= 4 ? KS : 2;    // 32-element steps whose loads are under way together
+    constexpr int KG = PL == 1 || KS <= 4 ? KS : KS == 8 ? 4 : KS == 10 ? 5 : 2;    // 32-element steps whose loads are under way together
     __shared__ float4 red[4][TB * 16];
     const int tile = blockIdx.y;
     int at[KS];
@@ -745,9 +746,10 @@ __global__ __launch_bounds__(256, KS * PL > 30 ? 1 : 2) void k_vs_forward_raw(Vs
                     for (int t = 0; t < TB; ++t) s[j >> 2][t][j & 3] = gone ? VS_MASKED : s[j >> 2][t][j & 3] + q;
                 }
             }
+            if (a.f.chunk_max) {
 #pragma unroll
-            for (int rb = 0; rb < 2; ++rb) wide = fmaxf(wide, of_row[rb] <= VS_NOTHING ? 0.0f : big[rb].largest());
-            __builtin_amdgcn_sched_barrier(0);
+                for (int rb = 0; rb < 2; ++rb) wide = fmaxf(wide, of_row[rb] <= VS_NOTHING ? 0.0f : big[rb].largest());
+            }
             rows.template add<true, false>(s, unscaled);
             if (a.f.chunk_max) rows.template chunk<false>(a.f, tile, row0 / VS_BLOCK, (row0 >> 5) & 7, lane, true);
         }

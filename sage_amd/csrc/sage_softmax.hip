@@ -143,9 +143,9 @@ int vs_splits(int64_t resident, int64_t groups, int64_t units, double cost) {
 // 0: the weights are packed first.  Packing costs a launch and a pass over the weights, reading them as they lie one such pass per
 // tile: worth it for 2 tiles (3 of two blocks), and for more where the vocabulary is short.  Measured, us, as they lie / packed:
 //   D = 50 float32, 262,144 ids   64 tokens 39 / 55   128: 65 / 55      16,384 ids   256: 13 / 19   384: 16 / 19    32,768   512: 34 / 24
-//   D = 300 bf16, 131,072 ids     64: 38 / 53   128: 64 / 53            8,192 ids    256: 13 / 22                  32,768   256: 26 / 28
-//   D = 300 float32, 131,072 ids  32: 119 / 128   64: 227 / 135         8,192 ids    128: 33 / 44   256: 44 / 44
-//   D = 512 bf16, 131,072 ids     32: 63 / 77   64: 112 / 79            1,200 ids    512: 18 / 25                  32,768   96: 45 / 32
+//   D = 300 bf16, 131,072 ids     64: 37 / 53   128: 64 / 53            8,192 ids    256: 13 / 22                  32,768   256: 26 / 28
+//   D = 300 float32, 131,072 ids  32: 70 / 128   64: 142 / 135          8,192 ids    128: 18 / 44
+//   D = 512 bf16, 131,072 ids     32: 61 / 77   64: 112 / 79            1,200 ids    512: 16 / 25                  32,768   96: 45 / 32
 int vs_raw_blocks(const Shape& s) {
     if (s.n > VS_RAW || s.dim < 8) return 0;
     int most = 1;
