@@ -1217,8 +1217,11 @@ __device__ __forceinline__ void vs_store(void* p, int64_t at, float v, int bf16)
 
 // Either gradient forms the logits again: n V D products beside the n V D of its own sums, and neither is stored.  Bound by the
 // matrix units' power (float32, three products each: 8,192 tokens x 262,144 ids, D = 50, dx 1.42 ms and dw 1.52 ms, 1.65 * 10^12 operations
-// of the MFMAs each, 1.1 * 10^15 a second) and, where a wave has registers for 16 columns only (bf16, D = 300), by the LDS reads of
-// the streaming fragments, 16 operations a byte: 4,096 x 65,536, entropy gradient too, dx 361 us (0.95 * 10^15), dw 474 us.
+// of the MFMAs each, 1.1 * 10^15 a second).  Wide rows leave registers for 16 columns of a wave and two or three waves of a
+// SIMD, which wait for one another twice in 32 streaming rows: bf16, D = 300, 4,096 x 65,536, entropy gradient too, dx 361 us
+// (0.95 * 10^15; MFMAs busy 54 % of a 1.8 GHz clock), dw 474 us (two waves a SIMD: 37 %).  The LDS reads are not what it waits for: with
+// the weights of four waves shared, each reading a quarter of the transposed fragments (29 KB for 40), dx takes as long and dw 3 %
+// longer.
 struct VsBwd {
     const uint4 *stayS;        // stationary rows (columns of the product)
     const uint4 *flowS, *flowT;// streaming rows, and transposed
