@@ -140,7 +140,18 @@ __device__ __forceinline__ vs_f8 vs_eight(const VsSrc& s, int64_t row, int d) {
     if (d + 8 <= s.dim) {
         if constexpr (PL == 1) {
             struct __attribute__((packed, aligned(2))) Raw { uint32_t v[4]; };
-            v = __builtin_convertvector(__builtin_bit_cast(vs_bf8, *(const Raw*)((const uint16_t*)s.p + row * s.ld + d)), vs_f8);
+            const uint16_t* p = (const uint16_t*)s.p + row * s.ld + d;
+            if (((s.ld & 1) || ((uintptr_t)s.p & 2)) && row > 0 && row + 1 < s.rows) {
+                // rows at odd 2-byte boundaries: the five words that the eight elements lie in (between two other rows: in bounds)
+                struct __attribute__((packed, aligned(4))) Words { uint32_t v[4]; };
+                const uint32_t* q = (const uint32_t*)((uintptr_t)p & ~(uintptr_t)3);
+                const Words a = *(const Words*)q;
+                const uint32_t last = q[4], by = ((uint32_t)(uintptr_t)p & 2) * 8;
+                Raw r;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r.v[i] = __builtin_amdgcn_alignbit(i < 3 ? a.v[i + 1] : last, a.v[i], by);
+                v = __builtin_convertvector(__builtin_bit_cast(vs_bf8, r), vs_f8);
+            } else v = __builtin_convertvector(__builtin_bit_cast(vs_bf8, *(const Raw*)p), vs_f8);
         } else {
             struct __attribute__((packed, aligned(4))) Raw { float v[8]; };
             v = __builtin_bit_cast(vs_f8, *(const Raw*)((const float*)s.p + row * s.ld + d));
