@@ -130,8 +130,8 @@ __device__ __forceinline__ void vs_split(vs_f8 v, vs_bits* out) {
 // coalesced 1 KiB load of a wave, whatever the caller's row length, stride and alignment are.  One workgroup packs 32 rows:
 // a lane loads the eight elements that its place in an S fragment asks for; T fragments are read back through LDS.
 // PL = 2: the 32 rows are multiplied by 2^e, e such that the largest finite element comes to just under 2^13.  Bound by HBM:
-// 131,072 x 300 bf16 for a forward pass, 79 MB read and 84 MB written, 36 us (4.5 TB/s); rows of 511 bf16, that start at any
-// 2-byte boundary, 84 MB in all in 32 us.
+// 131,072 x 300 bf16 for a forward pass, 79 MB read and 84 MB written, 37 us (4.4 TB/s); rows of 511 bf16, that start at any
+// 2-byte boundary, 84 MB in all in 23 us (33 with unaligned loads in place of aligned words).
 
 // eight elements from `d` on; zeros past the end of the row
 template <int PL>
