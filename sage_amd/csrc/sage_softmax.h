@@ -308,7 +308,8 @@ __global__ __launch_bounds__(256) void k_vs_pack(VsPack pa, VsPack pb) {
 }
 
 // All are known before any is written back: without this the compiler takes new registers for what a rarely taken branch
-// changes, and copies the old ones into them each time the branch is not taken.
+// changes, and copies the old ones into them each time the branch is not taken.  The values come
+// from vector instructions (the compiler sees to the waits that a matrix instruction's result needs before those read it).
 template <class V>
 __device__ __forceinline__ void vs_in_place(V& v) {
     constexpr int N = sizeof(V) / 4;
@@ -1472,6 +1473,8 @@ struct VsGrad {
                             c = vs_mfma<PL, M>(f, part[1], c);
                             c = vs_mfma<PL, M>(f, part[0], c);
                         }
+#pragma unroll
+                        for (int i = 0; i < M * M / 64; ++i) c[i] += 0.0f;     // (a vector instruction between, for its waits)
                         vs_in_place(c);
                         acc[d][v] = c;
                     }

@@ -1,12 +1,11 @@
 """GPU: the vocabulary softmax where its kernels change: enough tokens for the weights to be packed first, vocabularies whose
 gradient one range of tokens forms (stored without partial sums), row strides of the results, workspaces full of NaN.
 Definition and tolerances are those of test_gpu_vocab_softmax.py."""
-import math
 
 import pytest
 import torch
 
-from .test_gpu_vocab_softmax import BF16, F32, Exact, check_forward, close, grads_of, exact_norm, make
+from .test_gpu_vocab_softmax import BF16, F32, U, Exact, check_forward, close, exact_norm, grads_of, make
 
 pytestmark = pytest.mark.gpu
 WIDTHS = [1, 7, 8, 31, 50, 64, 65, 128, 129, 200, 256, 257, 300, 320, 321, 511, 512]
@@ -223,3 +222,44 @@ def test_logits_far_from_zero():
             check_forward(f, e, 7)
             b[7:] = float("-inf")                    # six ids are left
             check_forward(vs.token_logprobs(x, w, t, bias=b, alternatives=7), Exact(x, w, b, t, 7), 7)
+
+
+@pytest.mark.parametrize("n,D,dtype", [(3, 512, BF16), (530, 300, BF16), (2, 512, F32), (40, 7, F32)])
+def test_the_largest_vocabulary(n, D, dtype):
+    from sage_amd import vocab_softmax as vs
+    V = 1 << 20
+    x, w, b, t = make(n, V, D, dtype, "mask", seed=9)
+    t[0] = V - 1
+    b[V - 1] = 0.0
+    w[V - 1] = x[0] / x[0].float().norm() * 8            # the last id is the first row's most likely one, or nearly so
+    f = vs.token_logprobs(x, w, t, bias=b, alternatives=12)
+    check_forward(f, Exact(x, w, b, t, 12), 12)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradient_of_the_largest_vocabulary(dtype):
+    from sage_amd import vocab_softmax as vs
+    n, V, D = 20, 1 << 20, 65
+    x, w, b, t = make(n, V, D, dtype, "prior", seed=9)
+    t[0] = V - 1
+    gl = torch.linspace(-1, 1, n).cuda()
+    f = vs.token_logprobs(x, w, t, bias=b)
+    dx, dw, db = vs.token_logprobs_backward(x, w, t, f, gl, bias=b)
+    (wx, tx), (ww, tw), (wb, tb) = Exact(x, w, b, t).gradient(gl, None, dtype)
+    close(dx, wx, tx, "dx"), close(dw, ww, tw, "dw"), close(db, wb, tb, "db")
+
+
+def test_the_most_tokens():
+    from sage_amd import vocab_softmax as vs
+    n = 1 << 22
+    x, w, _, t = make(n, 3, 2, F32, seed=1)
+    e = Exact(x, w, None, t, 2)
+    f = vs.token_logprobs(x, w, t, alternatives=2)
+    close(f.lse, e.lse, e.tol_lse, "lse"), close(f.logprob, e.logprob, e.tol_lse + U * e.logprob.abs(), "logprob")
+    assert torch.equal(f.alt_ids.long(), e.alt_ids)
+    gl = torch.full((n,), 1.0 / n, device="cuda")
+    dx, dw, _ = vs.token_logprobs_backward(x, w, t, f, gl)
+    (wx, tx), (ww, tw), _ = e.gradient(gl, None, F32)
+    close(dx, wx, tx, "dx"), close(dw, ww, tw, "dw")
+    with pytest.raises(ValueError, match="2\\^22"):
+        vs.token_logprobs(torch.zeros(n + 1, 2, device="cuda"), w)
