@@ -64,13 +64,17 @@ int vs_steps(int dim) {
 // D = 50, 100, 200, 300, 500, 4,096 tokens x 65,536 ids, D = 50 twice that both ways; us, best first, then the other choices in turn):
 //   forward   32x2 32x2 16x2 32x2 32x1   float32   431 [458 489 490]   192 [207 200]   337 [359 688]   476 [531 498]   864 [949 1193]
 //             32x2 32x2 32x2 16x2 16x2   bf16      268 [303 308]       106 [111 113]   156 [168 167]   190 [204 181]   281 [304 656]
-//     (16x2 against 32x2 at ks = 10, bf16: 347 against 385 with alternatives)
+//     with alternatives the registers of the largest logits decide too: ks = 10, bf16 16x2 264 [344], without 182 [171];
+//     ks = 2, float32 16x2 589 [613], without 492 [426]; the others as without
 //   dx        16x2 16x2 16x1 16x2 16x1   float32   714 [773 803 908]   351 [378 417]   751 [821 915]   1,259 [1,563]   2,623 [4,732]
 //             16x2 16x2 16x1 16x1 16x1   bf16      286 [279 321 333]   144 [157 164]   300 [305 354]   379 [438 441]   628 [670 682]
 //   dw        16x2 16x2 16x1 16x2 16x1   float32   765 [757 836 896]   379 [409 448]   796 [1,058]     1,540 [1,617]   2,613 [4,576]
 //             16x2 16x2 16x1 16x1 16x2   bf16      350 [350 396 445]   166 [185 216]   364 [438 463]   447 [554 899]   922 [1,385]
 // (Wider than that the sums of a gradient spill; 16-column tiles give an accumulator time to be ready.)
-constexpr int vs_fwd_tile(int ks, int pl) { return pl == 1 ? (ks <= 8 ? 32 : 16) : ks == 8 ? 16 : 32; }
+constexpr int vs_fwd_tile(int ks, int pl, bool top) {
+    if (pl == 1 ? ks == 10 : ks == 2) return top ? 16 : 32;
+    return pl == 1 ? (ks <= 8 ? 32 : 16) : ks == 8 ? 16 : 32;
+}
 constexpr int vs_fwd_blocks(int ks, int pl) { return pl == 2 && ks == 16 ? 1 : 2; }
 constexpr int vs_bwd_tile(int, int) { return 16; }
 constexpr int vs_bwd_blocks(int ks, int pl, bool of_ids) { return ks <= 4 || (pl == 2 && ks == 10) || (pl == 1 && ks == 16 && of_ids) ? 2 : 1; }
@@ -108,7 +112,7 @@ struct Shape {
     int dim, ks, pl, k, cus;
 };
 
-template <int KS, int PL, bool TOP> constexpr auto vs_fwd_kernel = &k_vs_forward<KS, PL, vs_fwd_tile(KS, PL), vs_fwd_blocks(KS, PL), vs_fwd_rows(KS, PL), TOP>;
+template <int KS, int PL, bool TOP> constexpr auto vs_fwd_kernel = &k_vs_forward<KS, PL, vs_fwd_tile(KS, PL, TOP), vs_fwd_blocks(KS, PL), vs_fwd_rows(KS, PL), TOP>;
 template <int KS, int PL, bool OF_IDS, bool ENTROPY>
 constexpr auto vs_bwd_kernel = &k_vs_backward<KS, PL, vs_bwd_tile(KS, PL), vs_bwd_blocks(KS, PL, OF_IDS), vs_bwd_rows(KS, PL), vs_bwd_turns(KS, PL), OF_IDS, ENTROPY>;
 
@@ -182,7 +186,9 @@ FwdPlan plan_fwd(const Shape& s, void* ws) {
         p.rows = std::min(s.n, VS_ROWS_MAX);
         p.n_pad = up(p.rows, VS_PAD);
         int64_t resident = s.cus;
-#define VS_F(KS, PL) p.tiles = cdiv(p.rows, vs_fwd_blocks(KS, PL) * vs_fwd_tile(KS, PL)); resident *= per_cu<vs_fwd_kernel<KS, PL, false>>()
+#define VS_F(KS, PL)                                                                        \
+    p.tiles = cdiv(p.rows, vs_fwd_blocks(KS, PL) * vs_fwd_tile(KS, PL, s.k > 0));           \
+    resident *= s.k > 0 ? per_cu<vs_fwd_kernel<KS, PL, true>>() : per_cu<vs_fwd_kernel<KS, PL, false>>()
         VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
         p.splits = vs_splits(resident, cdiv(p.tiles, 4), blocks, 1.0);
@@ -260,9 +266,9 @@ int check_workspace(sage_ctx* c, const void* p, int64_t have, int64_t need) {
     return sage_ctx_fail(c, SAGE_E_ARG, msg);
 }
 
-template <bool FORWARD>
+template <bool FORWARD, bool TOP = false>
 void pack(const Shape& s, const VsPack& a, const VsPack& b, hipStream_t st) {
-#define VS_F(KS, PL) k_vs_pack<KS, PL, FORWARD ? vs_fwd_tile(KS, PL) : vs_bwd_tile(KS, PL), FORWARD><<<(uint32_t)(a.groups + b.groups), 256, 0, st>>>(a, b)
+#define VS_F(KS, PL) k_vs_pack<KS, PL, FORWARD ? vs_fwd_tile(KS, PL, TOP) : vs_bwd_tile(KS, PL), FORWARD><<<(uint32_t)(a.groups + b.groups), 256, 0, st>>>(a, b)
     VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
 }
@@ -329,7 +335,8 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
 #undef VS_F
         } else {
             if (r0) of_w.groups = 0;               // packed with the first rows
-            pack<true>(s, of_w, pack_of(xr, p.xS, nullptr, p.x_exp, 1, p.n_pad), st);
+            const VsPack of_x = pack_of(xr, p.xS, nullptr, p.x_exp, 1, p.n_pad);
+            if (alternatives) pack<true, true>(s, of_w, of_x, st); else pack<true, false>(s, of_w, of_x, st);
             const uint32_t grid = cdiv(p.tiles, 4) * p.splits;
 #define VS_F(KS, PL) if (alternatives) vs_fwd_kernel<KS, PL, true><<<grid, 256, 0, st>>>(f); else vs_fwd_kernel<KS, PL, false><<<grid, 256, 0, st>>>(f)
             VS_BY_WIDTH(s.ks, s.pl, VS_F);
