@@ -547,7 +547,7 @@ __device__ __forceinline__ void vs_forward_step(const VsFwd& a, int row0, const 
 // Bound by the matrix units and the power they draw (the clock falls to 1.8 - 2.2 GHz under them), the exponentials beside
 // them second.  8,192 tokens x 262,144 ids, D = 50 float32: 737 us, 0.82 * 10^12 operations of the MFMAs (three products, 64
 // elements for 50) at 1.1 * 10^15 a second, where a large bf16 matrix product of the library reaches 1.38 * 10^15; 4,096 x 65,536,
-// D = 300 bf16: 184 us, 0.93 * 10^15.
+// D = 300 bf16: 170 us, 1.01 * 10^15.
 // Four waves, a tile each, share the streaming rows through LDS.  SR rows at a time are copied straight into LDS (they are
 // packed in the order of the copy) while the SR before them are worked on: one barrier a step.
 typedef const __attribute__((address_space(1))) void* vs_global_ptr;

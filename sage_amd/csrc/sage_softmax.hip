@@ -346,13 +346,13 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
                        d_logprob ? d_logprob + r0 : nullptr, d_entropy ? d_entropy + r0 : nullptr, d_lse + r0};
         if (alternatives) {
             const VsTop t{j, p.chunk_max, (int32_t)p.chunks, alternatives, d_alt_ids + r0 * alternatives, d_alt_logprobs + r0 * alternatives};
-            // a row alone on a CU is bound by latency: sixteen waves share its chain of loads (262,144 ids, D = 50: one row 33 us
-            // with the forward kernel, 39 with four; 256 rows 73 and 79; 320 rows 121 and 113)
+            // a row alone on a CU is bound by latency: sixteen waves share its chain of loads (262,144 ids, D = 50, with the forward
+            // kernel: one row 26.6 us, 28.3 by four waves; 256 rows 72 and 73; 320 rows 92 and 87)
             const bool wide = rows <= s.cus;
             if (dtype == SAGE_BF16) { if (wide) k_vs_top<true, 1024><<<(uint32_t)rows, 1024, 0, st>>>(t); else k_vs_top<true, 256><<<(uint32_t)rows, 256, 0, st>>>(t); }
             else { if (wide) k_vs_top<false, 1024><<<(uint32_t)rows, 1024, 0, st>>>(t); else k_vs_top<false, 256><<<(uint32_t)rows, 256, 0, st>>>(t); }
-        // (many ranges: one token of 262,144 ids 19 us with the forward kernel, 23 where one wave joins its 1,024 ranges; of 16,384 ids, 64
-        // ranges, 8.8 and 8.5)
+        // (many ranges: one token of 262,144 ids 18 us with the forward kernel, 22 where one wave joins its 1,024 ranges; of 16,384 ids, 64
+        // ranges, 8.6 and 8.4)
         } else if (p.splits > 64) k_vs_join<4><<<(uint32_t)rows, 256, 0, st>>>(j);
         else k_vs_join<1><<<cdiv(rows, 4), 256, 0, st>>>(j);
     }
