@@ -254,10 +254,11 @@ int sage_token_logprobs_backward_device(sage_ctx* ctx, int32_t dtype, int64_t n,
 
 /*
  * Clips gradients by their global norm N = sqrt(sum of all squares): d_out[i] = d_grads[i] * (max_norm / N) where N > max_norm,
- * else d_out[i] = d_grads[i]; *d_norm = N (float32, device).  max_norm is finite and not negative.  d_out[i] may be d_grads[i] itself (in place); no other overlap
- * is allowed.  sizes[i] elements of dtypes[i] (SAGE_F32 / SAGE_BF16), back to back; the four lists are HOST arrays, read
- * during the call only.  Squares are summed in float64.  A norm that is not finite leaves every gradient as it is: the
- * caller sees it in *d_norm.  Enqueues only, as described above.
+ * else d_out[i] = d_grads[i]; *d_norm = N (float32, device).  max_norm is finite and not negative.  d_out[i] may be d_grads[i]
+ * itself (in place); no other overlap is allowed.  sizes[i] elements of dtypes[i] (SAGE_F32 / SAGE_BF16), back to back; the
+ * four lists are HOST arrays, read during the call only.  Squares are summed in float64.  An infinity or a NaN among the gradients leaves every
+ * gradient as it is; the caller sees a *d_norm that is not finite.  Finite gradients are clipped by their N whatever it is: where it passes
+ * float32's range *d_norm is inf, and max_norm / N may be as small as it comes.  Enqueues only, as described above.
  */
 int64_t sage_clip_grad_norm_workspace(sage_ctx* ctx, int64_t n_tensors, const int64_t* sizes);
 int sage_clip_grad_norm_device(sage_ctx* ctx, int64_t n_tensors, const void* const* d_grads, void* const* d_out, const int64_t* sizes,

@@ -98,8 +98,21 @@ __device__ __forceinline__ double clip_squares(const ClipTable& t, uint32_t i, i
     return s0 + s1;
 }
 
+// max_norm / N as part * 2^power, |part| in [1/2, 1]: N may pass float32's range and the factor fall below it where the clipped
+// gradients do neither.  1 where nothing is to be clipped, or where a gradient is not finite.
+struct ClipFactor {
+    float part;
+    int32_t power;
+    __device__ __forceinline__ ClipFactor() {}
+    __device__ __forceinline__ ClipFactor(double norm, double max_norm) : part(1.0f), power(0) {
+        if (norm > max_norm && norm < INFINITY) part = (float)frexp(max_norm / norm, &power);
+    }
+    __device__ __forceinline__ bool one() const { return part == 1.0f && power == 0; }
+    __device__ __forceinline__ float operator*(float g) const { return ldexpf(g * part, power); }
+};
+
 template <int THREADS, int UNROLL>
-__device__ __forceinline__ void clip_scale(const ClipTable& t, uint32_t i, int64_t at, int m, int thread, float f) {
+__device__ __forceinline__ void clip_scale(const ClipTable& t, uint32_t i, int64_t at, int m, int thread, ClipFactor f) {
     if (t.size[i] < 0) {
         const uint16_t* p = (const uint16_t*)t.in[i] + at;
         uint16_t* o = (uint16_t*)t.out[i] + at;
@@ -108,13 +121,13 @@ __device__ __forceinline__ void clip_scale(const ClipTable& t, uint32_t i, int64
             clip_u4 q = *(const clip_u4*)(p + j);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const __bf16 a = (__bf16)(clip_lo(q.v[k]) * f), b = (__bf16)(clip_hi(q.v[k]) * f);
+                const __bf16 a = (__bf16)(f * clip_lo(q.v[k])), b = (__bf16)(f * clip_hi(q.v[k]));
                 q.v[k] = (uint32_t)__builtin_bit_cast(uint16_t, a) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
             }
             clip_put(o + j, q);
         }
         const int j = (m & ~7) + thread;
-        if (thread < 8 && j < m) ((__bf16*)o)[j] = (__bf16)(clip_lo(p[j]) * f);
+        if (thread < 8 && j < m) ((__bf16*)o)[j] = (__bf16)(f * clip_lo(p[j]));
     } else {
         const float* p = (const float*)t.in[i] + at;
         float* o = (float*)t.out[i] + at;
@@ -122,20 +135,16 @@ __device__ __forceinline__ void clip_scale(const ClipTable& t, uint32_t i, int64
         for (int j = thread * 4; j + 4 <= m; j += THREADS * 4) {
             clip_u4 q = *(const clip_u4*)(p + j);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) q.v[k] = __float_as_uint(__uint_as_float(q.v[k]) * f);
+            for (int k = 0; k < 4; ++k) q.v[k] = __float_as_uint(f * __uint_as_float(q.v[k]));
             clip_put(o + j, q);
         }
         const int j = (m & ~3) + thread;
-        if (thread < 4 && j < m) o[j] = p[j] * f;
+        if (thread < 4 && j < m) o[j] = f * p[j];
     }
 }
 __device__ __forceinline__ int clip_part(const ClipTable& t, uint32_t i, int64_t at, int block) {
     const int64_t n = t.size[i] < 0 ? -t.size[i] : t.size[i];
     return (int)min((int64_t)block, n - at);
-}
-// 1 where nothing is to be clipped, or where the norm is not finite
-__device__ __forceinline__ float clip_factor(double norm, double max_norm) {
-    return norm > max_norm && norm < INFINITY ? (float)(max_norm / norm) : 1.0f;
 }
 
 __global__ __launch_bounds__(256) void k_clip_squares(ClipTable t, double* __restrict__ part) {
@@ -147,7 +156,7 @@ __global__ __launch_bounds__(256) void k_clip_squares(ClipTable t, double* __res
 }
 
 // the norm, and the factor behind it
-__global__ __launch_bounds__(1024) void k_clip_norm(const double* __restrict__ part, uint32_t n, double max_norm, float* __restrict__ norm, float* __restrict__ factor) {
+__global__ __launch_bounds__(1024) void k_clip_norm(const double* __restrict__ part, uint32_t n, double max_norm, float* __restrict__ norm, ClipFactor* __restrict__ factor) {
     __shared__ double red[16];
     double s = 0.0;
 #pragma unroll 8
@@ -155,16 +164,16 @@ __global__ __launch_bounds__(1024) void k_clip_norm(const double* __restrict__ p
     s = sqrt(clip_block_sum(s, red));
     if (threadIdx.x == 0) {
         *norm = (float)s;
-        *factor = clip_factor(s, max_norm);
+        *factor = ClipFactor(s, max_norm);
     }
 }
 
 // From the last block to the first, and with stores that leave the caches alone: what k_clip_squares read last is then still
 // there (10^8 float32: both passes 196 us, 214 from the first block on; with ordinary stores 231).
-__global__ __launch_bounds__(256) void k_clip_scale(ClipTable t, const float* __restrict__ factor) {
-    const float f = *factor;
+__global__ __launch_bounds__(256) void k_clip_scale(ClipTable t, const ClipFactor* __restrict__ factor) {
+    const ClipFactor f = *factor;
     const uint32_t block = gridDim.x - 1 - blockIdx.x, i = ClipFind(t)(block);
-    if (f == 1.0f && t.in[i] == t.out[i]) return;
+    if (f.one() && t.in[i] == t.out[i]) return;
     const int64_t at = (int64_t)(block - t.first[i]) * t.block;
     clip_scale<256, 4>(t, i, at, clip_part(t, i, at, t.block), threadIdx.x, f);
 }
@@ -182,11 +191,11 @@ __global__ __launch_bounds__(1024) void k_clip_one(ClipTable t, double max_norm,
         s += clip_squares<64, 4>(t, i, at, clip_part(t, i, at, CLIP_PIECE), lane);
     }
     s = sqrt(clip_block_sum(s, red));
-    const float f = clip_factor(s, max_norm);
+    const ClipFactor f(s, max_norm);
     if (threadIdx.x == 0) *norm = (float)s;
     for (uint32_t p = wave; p < pieces; p += 16) {
         const uint32_t i = find(p);
-        if (f == 1.0f && t.in[i] == t.out[i]) continue;
+        if (f.one() && t.in[i] == t.out[i]) continue;
         const int64_t at = (int64_t)(p - t.first[i]) * CLIP_PIECE;
         clip_scale<64, 4>(t, i, at, clip_part(t, i, at, CLIP_PIECE), lane, f);
     }

@@ -507,7 +507,7 @@ int sage_clip_grad_norm_device(sage_ctx* c, int64_t n_tensors, const void* const
     if (!dev.ok) return sage_ctx_fail(c, SAGE_E_HIP, "the context's device cannot be made current");
     const hipStream_t st = (hipStream_t)stream;
     double* part = (double*)d_workspace;
-    float* factor = (float*)((char*)d_workspace + need - VS_ALIGN);
+    ClipFactor* factor = (ClipFactor*)((char*)d_workspace + need - VS_ALIGN);
     ClipTable t;
     int64_t elements = 0;
     for (int64_t i = 0; i < n_tensors; ++i) elements += sizes[i];

@@ -134,7 +134,8 @@ def token_logprobs_backward(x: torch.Tensor, weight: torch.Tensor, targets: Opti
 def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *, out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Scales `grads` (float32 and bfloat16 tensors, contiguous, all on one GPU) so that their global 2-norm is at most
     `max_norm`: in place, or into `out` (tensors of the same sizes and types).  Returns the norm before clipping, a float32
-    scalar on the GPU.  A norm that is not finite leaves the gradients unchanged."""
+    scalar on the GPU.  An infinity or a NaN among the gradients makes the norm infinite or NaN and leaves them unchanged; finite
+    gradients whose norm passes float32's range are clipped too (the norm returned is then infinite)."""
     grads = list(grads)
     out = grads if out is None else list(out)
     if not grads:
