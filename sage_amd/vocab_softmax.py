@@ -71,13 +71,22 @@ def _workspace(nbytes: int, device) -> torch.Tensor:
     return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
 
 
+def _not_recorded(**tensors) -> None:
+    for name, t in tensors.items():
+        if torch.is_grad_enabled() and isinstance(t, torch.Tensor) and t.requires_grad:
+            raise ValueError(f"{name} requires a gradient, which autograd cannot find through this call: make it under torch.no_grad() and take "
+                             "the gradient from token_logprobs_backward")
+
+
 def token_logprobs(x: torch.Tensor, weight: torch.Tensor, targets: Optional[torch.Tensor] = None, *, bias: Optional[torch.Tensor] = None,
                    alternatives: int = 0) -> TokenLogprobs:
     """log p(targets[n] | x[n]) with p = softmax(x weight^T + bias), the entropy of p, and its `alternatives` largest ids.
 
     x [n, D] and weight [V, D] are both float32 or both bfloat16 with any row stride; bias float32 [V] (-inf masks an id);
     targets int64 or int32 [n] (negative: none; such a row of x may hold anything in the gradient).  What rows of masked ids hold
-    does not matter.  D <= 512, V <= 2^20, at most 32 alternatives (ties: the lower id)."""
+    does not matter.  D <= 512, V <= 2^20, at most 32 alternatives (ties: the lower id).  The results carry no gradient for
+    autograd (token_logprobs_backward has it): tensors that require one are refused unless under torch.no_grad()."""
+    _not_recorded(x=x, weight=weight, bias=bias)
     _rows("x", x)
     _rows("weight", weight, x)
     (n, dim), vocab, dev = x.shape, weight.shape[0], x.device
