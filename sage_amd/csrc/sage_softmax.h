@@ -169,12 +169,12 @@ __device__ __forceinline__ vs_f8 vs_eight(const VsSrc& s, int64_t row, int d) {
 #define VS_INFO 36
 #define VS_INFO_EXP 32
 #define VS_INFO_WIDE 33
-// What goes with those of 32 tokens in the gradient: lse in powers of two (L), and A, B, gl of G = p (A + B e) + gl [v = target],
-// e = log2 p; the target; the exponent of their scale last.
+// What goes with those of 32 tokens in the gradient: lse in powers of two (L), A and B of G = p (A + B e), e = log2 p, for the ids
+// that are not the target; the target, and its own G (gl until k_vs_target has formed it); the exponent of their scale last.
 #define VS_TOKEN 164
 #define VS_TOKEN_A 32
 #define VS_TOKEN_B 64
-#define VS_TOKEN_GL 96
+#define VS_TOKEN_GT 96
 #define VS_TOKEN_TARGET 128
 #define VS_TOKEN_EXP 160
 
@@ -199,6 +199,13 @@ __device__ __forceinline__ bool vs_idle(const VsPack& a, int64_t i) {
     const bool of_target = a.g && a.targets && a.targets[i] >= 0 && a.g[i] != 0.0f;
     return !of_target && !(a.h && a.h[i] != 0.0f);
 }
+// lse in powers of two; what p is to be multiplied by to make up for its rounding
+__device__ __forceinline__ float vs_lse2(float l, float& fix) {
+    const double exact = (double)l * 1.4426950408889634;
+    const float l2 = (float)exact;
+    fix = exp2f((float)((double)l2 - exact));
+    return l2;
+}
 __device__ __forceinline__ void vs_put_token(const VsPack& a, int64_t i) {
     // rows past the end, idle ones and rows whose every id is masked: an lse that makes every p 0, whatever the bias is
     float l2 = -VS_NOTHING, A = 0.0f, B = 0.0f, gl = 0.0f;
@@ -208,11 +215,7 @@ __device__ __forceinline__ void vs_put_token(const VsPack& a, int64_t i) {
         const int64_t tt = a.targets ? a.targets[i] : -1;
         const bool empty = l == -INFINITY;
         float fix = 1.0f;                         // p is short of 2^-(rounding of l2); A and B make up for it
-        if (!empty) {
-            const double exact = (double)l * 1.4426950408889634;
-            l2 = (float)exact;
-            fix = exp2f((float)((double)l2 - exact));
-        }
+        if (!empty) l2 = vs_lse2(l, fix);
         if (tt >= 0 && a.g) gl = a.g[i];
         if (tt >= a.vocab) gl = NAN;
         t = tt >= 0 && tt < a.vocab ? (int32_t)tt : -1;
@@ -221,7 +224,7 @@ __device__ __forceinline__ void vs_put_token(const VsPack& a, int64_t i) {
         A *= fix; B *= fix;
     }
     float* to = a.tokens + (i >> 5) * VS_TOKEN + (i & 31);
-    to[0] = l2; to[VS_TOKEN_A] = A; to[VS_TOKEN_B] = B; to[VS_TOKEN_GL] = gl; to[VS_TOKEN_TARGET] = __int_as_float(t);
+    to[0] = l2; to[VS_TOKEN_A] = A; to[VS_TOKEN_B] = B; to[VS_TOKEN_GT] = gl; to[VS_TOKEN_TARGET] = __int_as_float(t);
 }
 
 // Two matrices in one launch: the first workgroups pack `a`, the others `b`.
@@ -1243,8 +1246,10 @@ struct VsBwd {
     int32_t vocab;
     int32_t n_tiles, splits, groups;   // groups of 32 streaming rows
     int64_t stay_pad;          // rows of a partial
-    float* part;               // [splits][stay_pad][32 KS]
+    float* part;               // [splits][stay_pad][32 KS]; of tokens null where dx is not asked for
     float* bias_part;          // [splits][stay_pad]
+    // of tokens: the sum of p over all ids but the target, [splits][stay_pad], and log2 p of the target, [stay_pad]
+    float *rest, *target_e;
     // of ids, one range: the result itself
     void* out;                 // null: partials
     int64_t ldo;
@@ -1254,30 +1259,37 @@ struct VsBwd {
 
 // A wave: a tile of TB M stationary rows against one range of the streaming ones.  OF_IDS = false: the stationary rows
 // are tokens, the result sum_v p' w_v with p' = p (A + B e), or p alone when there is no entropy gradient (A is then a
-// factor of the whole row, applied at the end); the target's own term is added at the end too, so that the largest
-// coefficient is never rounded to bf16.  OF_IDS = true: the stationary rows are ids, the result sum_n G_nv x_n; the targets'
-// own terms are products of their own (in two parts, for the same reason) in the few steps in which one lies in the tile.
+// factor of the whole row, applied at the end).  OF_IDS = true: the stationary rows are ids, the result sum_n G_nv x_n.
+//
+// The target's coefficient is g (1 - p_t): small where a token is predicted well, and nothing but rounding errors if it were left to
+// g and g p_t, each rounded, to cancel.  So the sums over tokens leave the target out and find 1 - p_t as what the others
+// add up to (k_vs_target, between the two gradients); dx gets the whole coefficient times w_t at the end, in float32, and dw takes it as
+// the weight of that token and id, rounded as any other is (bf16: one of 2^-8, float32: two float16).
 //
 // Two float16 parts (PL = 2) of a weight: column t is kept multiplied by 2^sg[t], sg as large as the largest weight of the column
 // so far allows (2^15 after the streaming rows' scale), and the sums with it.  It starts high and falls a few times.
-template <int KS, int PL, int M, int TB, bool OF_IDS, bool ENTROPY>
+template <int KS, int PL, int M, int TB, bool OF_IDS, bool ENTROPY, bool SUMS>
 struct VsGrad {
     static constexpr float MOST = 15.0f, AIM = 13.0f;
-    static constexpr int NJ = VS_NJ<M>, HALVES = VS_HALVES<M>, BLOCKS = KS * 32 / M;
+    // Where a step's weights are formed again if a target is among them, and where its logits are changed before (4,096 x 65,536, both
+    // gradients: D = 100 bf16 with entropy 350 us, 383 the other way; D = 100 float32 696, 753; D = 300 bf16 813, 824)
+    static constexpr bool AGAIN = PL == 1 && KS <= 4;
+    static constexpr int NJ = VS_NJ<M>, HALVES = VS_HALVES<M>, BLOCKS = SUMS ? KS * 32 / M : 0;     // SUMS = false: of tokens, without dx
     using Acc = typename VsTile<M>::Acc;
     using Weights = vs_bits[HALVES][PL];       // of one column, by streaming row
     VsOperand<KS, PL, M> y[TB];
-    Acc acc[BLOCKS][TB];
-    float L[TB], A[TB], B[TB], db[TB], y_exp[TB], sg[TB], norm[TB];   // (of ids, L is the bias)
+    Acc acc[SUMS ? BLOCKS : 1][TB];
+    float L[TB], A[TB], B[TB], db[TB], y_exp[TB], sg[TB], norm[TB], rest[TB];   // (of ids, L is the bias)
+    int target[TB];
     int64_t stay0;
 
-    __device__ __forceinline__ void start(const VsBwd& a, int64_t tile, int lane) {
+    __device__ __forceinline__ void start(const VsBwd& a, int64_t tile, int lane, bool live) {
         vs_stationary<KS, PL, M, TB>(a.stayS, tile, lane, y);
         stay0 = tile * TB * M;
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
             const int64_t r = stay0 + t * M + lane % M;
-            db[t] = 0.0f; sg[t] = 300.0f; norm[t] = 0.0f;
+            db[t] = 0.0f; sg[t] = 300.0f; norm[t] = 0.0f; rest[t] = 0.0f;
             if constexpr (OF_IDS) {
                 const float* of = a.info + (r >> 5) * VS_INFO;
                 L[t] = of[r & 31];
@@ -1286,6 +1298,7 @@ struct VsGrad {
                 const float* of = a.tokens + (r >> 5) * VS_TOKEN;
                 L[t] = of[r & 31]; A[t] = of[VS_TOKEN_A + (r & 31)]; B[t] = of[VS_TOKEN_B + (r & 31)];
                 y_exp[t] = PL == 2 ? of[VS_TOKEN_EXP] : 0.0f;
+                target[t] = live ? __float_as_int(of[VS_TOKEN_TARGET + (r & 31)]) : -1;
                 if (PL == 2 && ENTROPY) {      // |A + B e| brought below 1
                     const float size = fabsf(A[t]) + fabsf(B[t]) * 256.0f;
                     norm[t] = size > 0.0f && size < INFINITY ? (float)__builtin_amdgcn_frexp_expf(size) : 0.0f;
@@ -1316,7 +1329,44 @@ struct VsGrad {
         }
     }
 
-    // P: the weights of the 32 streaming rows from row0 on, in parts, without the targets' own terms
+    // Of tokens: targets among the 32 ids from row0 on are taken out of the sums.  Rare: a token has one.
+    __device__ __forceinline__ bool any_target(int row0) const {
+        bool here = false;
+#pragma unroll
+        for (int t = 0; t < TB; ++t) here |= (uint32_t)(target[t] - row0) < 32;
+        return __any(here);
+    }
+    __device__ __forceinline__ void leave_targets(const VsBwd& a, int row0, const float (&unit)[TB], VsLogits<M, TB>& s) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const float v = vs_value<M, TB>(s, t, j);
+                const bool it = target[t] == row0 + vs_row<M>(j, lane);
+                if (it) a.target_e[stay0 + t * M + lane % M] = fmaf(v, unit[t], -L[t]);
+                vs_set<M, TB>(s, t, j, it ? -INFINITY : v);
+            }
+            if (!AGAIN)
+#pragma unroll
+                for (int b = 0; b < VsTile<M>::NB; ++b) vs_in_place(s[b][t]);
+        }
+    }
+    // Of ids: the weights of the tokens whose target lies in the tile
+    __device__ __forceinline__ void put_targets(const float* of, float (&G)[TB][NJ]) {
+        const int lane = threadIdx.x & 63;
+        const int64_t in = __float_as_int(of[VS_TOKEN_TARGET + (lane & 31)]) - stay0;
+        if (!__any(in >= 0 && in < TB * M)) return;
+#pragma unroll
+        for (int t = 0; t < TB; ++t)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int at = vs_row<M>(j, lane);
+                if (__float_as_int(of[VS_TOKEN_TARGET + at]) == (int)stay0 + t * M + lane % M) G[t][j] = of[VS_TOKEN_GT + at];
+            }
+    }
+
+    // P: the weights of the 32 streaming rows from row0 on, in parts
     __device__ __forceinline__ void weights(const VsBwd& a, int row0, const uint4* S, const float* of, Weights (&P)[TB]) {
         const int lane = threadIdx.x & 63;
         VsLogits<M, TB> s;
@@ -1346,8 +1396,10 @@ struct VsGrad {
                 }
             } else vs_mask<M, TB, PL == 2>(s, unit, b);
         }
+        if constexpr (!OF_IDS && !AGAIN)
+            if (any_target(row0)) leave_targets(a, row0, unit, s);
         float G[TB][NJ];
-        float big[TB];                         // PL = 2: the power of two that a column's largest scaled weight is below
+        float big[TB], ps[TB];                 // PL = 2: the power of two that a column's largest scaled weight is below; of tokens: the sum of p
         auto form = [&]() {
             vs_f4 rl[NJ / 4], ra[NJ / 4], rb[NJ / 4];
             if constexpr (OF_IDS) {
@@ -1364,6 +1416,7 @@ struct VsGrad {
             for (int t = 0; t < TB; ++t) {
                 const float shift = PL == 2 ? sg[t] - f_exp : 0.0f;
                 float m = 0.0f;
+                ps[t] = 0.0f;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     const float v = vs_value<M, TB>(s, t, j);
@@ -1372,24 +1425,39 @@ struct VsGrad {
                         const float p = __builtin_amdgcn_exp2f(e);
                         if (ENTROPY) e = vs_max(e, VS_TMIN);
                         G[t][j] = p * (ENTROPY ? fmaf(rb[j >> 2][j & 3], e, ra[j >> 2][j & 3]) : ra[j >> 2][j & 3]);
-                        if (PL == 2) m = fmaxf(m, fabsf(G[t][j]));
                     } else {
                         float e = fmaf(v, PL == 2 ? unit[t] : VS_LOG2E, shift - L[t]);
                         if (PL == 2) m = j ? fmaxf(m, e) : e;
                         G[t][j] = __builtin_amdgcn_exp2f(e);
+                        ps[t] = j ? ps[t] + G[t][j] : G[t][j];
                         if (ENTROPY) {
                             e = vs_max(e, VS_TMIN);
                             G[t][j] *= fmaf(B[t], e, PL == 2 ? fmaf(-B[t], shift, A[t]) : A[t]);
                         }
                     }
                 }
-                if (PL == 2 && OF_IDS) m = m > 0.0f ? (float)__builtin_amdgcn_frexp_expf(m) + shift : 0.0f;
-                big[t] = m;
-                most = fmaxf(most, m);
+                if (!OF_IDS) { big[t] = m; most = fmaxf(most, m); }
             }
             return most;
         };
-        const float most = form();
+        float most = form();
+        if constexpr (!OF_IDS && AGAIN)
+            if (any_target(row0)) {
+                leave_targets(a, row0, unit, s);
+                form();
+            }
+        if constexpr (OF_IDS) {
+            put_targets(of, G);
+            if (PL == 2)
+#pragma unroll
+                for (int t = 0; t < TB; ++t) {
+                    float m = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) m = fmaxf(m, fabsf(G[t][j]));
+                    big[t] = m > 0.0f ? (float)__builtin_amdgcn_frexp_expf(m) + (sg[t] - f_exp) : 0.0f;
+                    most = fmaxf(most, big[t]);
+                }
+        }
         if (PL == 2)
             if (__any(most > MOST)) {
 #pragma unroll
@@ -1406,6 +1474,7 @@ struct VsGrad {
                     db[t] += v;
                 }
             const int by = PL == 2 ? (int)(sg[t] - f_exp) : 0;
+            if (!OF_IDS) rest[t] += PL == 2 ? ldexpf(ps[t], -by) : ps[t];
 #pragma unroll
             for (int u = 0; u < HALVES; ++u) {
                 vs_f8 v;
@@ -1431,63 +1500,19 @@ struct VsGrad {
             }
     }
 
-    // OF_IDS: gl of the tokens whose target lies in the tile, in two parts of either type.  Rare: a token has one target.
-    __device__ __forceinline__ void targets(const VsBwd& a, const uint4* T, const float* of) {
-        const int lane = threadIdx.x & 63;
-        const int target = __float_as_int(of[VS_TOKEN_TARGET + (lane & 31)]);
-        if (!__any(target >= stay0 && target < stay0 + TB * M)) return;
-        const float f_exp = PL == 2 ? of[VS_TOKEN_EXP] : 0.0f;
-#pragma unroll 1
-        for (int q = 0; q < TB * HALVES; ++q) {
-            const int t = q / HALVES, u = q % HALVES;
-            vs_f8 G;
-            float m = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int at = vs_row<M>(u * 8 + j, lane);
-                G[j] = __float_as_int(of[VS_TOKEN_TARGET + at]) == (int32_t)(stay0 + t * M + lane % M) ? of[VS_TOKEN_GL + at] : 0.0f;
-                m = fmaxf(m, fabsf(G[j]));
-            }
-            vs_bits part[2];
-#pragma unroll
-            for (int v = 0; v < TB; ++v)       // (registers have no index)
-                if (v == t) {
-                    db[v] += ((G[0] + G[1]) + (G[2] + G[3])) + ((G[4] + G[5]) + (G[6] + G[7]));
-                    if constexpr (PL == 2) {
-                        lower(v, m > 0.0f ? (float)__builtin_amdgcn_frexp_expf(m) + sg[v] - f_exp - AIM : 0.0f);
-                        const int by = (int)(sg[v] - f_exp);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) G[j] = ldexpf(G[j], by);
-                        vs_split<2>(G, part);
-                    } else {
-                        vs_split<1>(G, &part[0]);
-                        const vs_f8 rest = G - __builtin_convertvector(__builtin_bit_cast(vs_bf8, part[0]), vs_f8);
-                        vs_split<1>(rest, &part[1]);
-                    }
-#pragma unroll
-                    for (int d = 0; d < BLOCKS; ++d) {
-                        Acc c = acc[d][v];
-#pragma unroll
-                        for (int p = 0; p < PL; ++p) {
-                            const vs_bits f = *(const vs_bits*)&T[((d * HALVES + u) * PL + p) * 64];
-                            c = vs_mfma<PL, M>(f, part[1], c);
-                            c = vs_mfma<PL, M>(f, part[0], c);
-                        }
-#pragma unroll
-                        for (int i = 0; i < M * M / 64; ++i) c[i] += 0.0f;     // (a vector instruction between, for its waits)
-                        vs_in_place(c);
-                        acc[d][v] = c;
-                    }
-                }
-        }
-    }
-
     __device__ __forceinline__ void store(const VsBwd& a, int split, int lane) {
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
             const int64_t r = stay0 + t * M + lane % M;
             const bool final = OF_IDS && a.out;
             if (final && r >= a.rows) continue;
+            if constexpr (!OF_IDS) {
+                float v = rest[t];
+                if (M == 16) v += __shfl_xor(v, 16);
+                v += __shfl_xor(v, 32);
+                if (lane < M) a.rest[(int64_t)split * a.stay_pad + r] = v;
+                if (!a.part) continue;
+            }
             float* out = a.part + ((int64_t)split * a.stay_pad + r) * (KS * 32);
 #pragma unroll
             for (int d = 0; d < BLOCKS; ++d)
@@ -1513,11 +1538,16 @@ struct VsGrad {
     }
 };
 
+// Without dx the sums over tokens are not formed: by a branch, or, where their registers leave the compiler no room to
+// keep them in place across one, by a kernel of its own.
+constexpr bool vs_bwd_wide(int ks, int tb) { return ks * tb > 10; }
+
 // The stages in LDS.  TURNS = false: SR rows with both their fragments at a time, two stages (one worked on, one under way).
 // TURNS = true (wide rows): 32 rows, their S and their T fragments by turns, each under way while the other is worked on.
-template <int KS, int PL, int M, int TB, int SR, bool OF_IDS, bool ENTROPY>
+template <int KS, int PL, int M, int TB, int SR, bool OF_IDS, bool ENTROPY, bool SUMS>
 struct VsGradStage {
-    using Grad = VsGrad<KS, PL, M, TB, OF_IDS, ENTROPY>;
+    using Grad = VsGrad<KS, PL, M, TB, OF_IDS, ENTROPY, SUMS>;
+    static __device__ __forceinline__ bool sums(const VsBwd& a) { return SUMS && (OF_IDS || vs_bwd_wide(KS, TB) || a.part); }
     static constexpr int HALF = SR * KS * PL * 4, INFO = (OF_IDS ? VS_TOKEN : VS_INFO), INFOS = SR / 32 * INFO;
     static constexpr int SIZE = 2 * HALF + (INFOS + 3) / 4;
     static __device__ __forceinline__ void fetch(const uint4* S, const uint4* T, const float* info, uint4* to) {
@@ -1538,8 +1568,7 @@ struct VsGradStage {
             typename Grad::Weights P[TB];
             const float* of = (const float*)(from + 2 * HALF) + r / 32 * INFO;
             g.weights(a, base + r, from + r * KS * PL * 4 + lane, of, P);
-            g.products(from + HALF + r * KS * PL * 4 + lane, P);
-            if (OF_IDS) g.targets(a, from + HALF + r * KS * PL * 4 + lane, of);
+            if (sums(a)) g.products(from + HALF + r * KS * PL * 4 + lane, P);
         }
     }
     // by turns: each half with its own copy of what goes with it
@@ -1560,14 +1589,18 @@ struct VsGradStage {
         vs_copies_done();
         __syncthreads();
         if (more) fetch_half(S, info, to);
-        g.products(from + (threadIdx.x & 63), P);
-        if (OF_IDS) g.targets(a, from + (threadIdx.x & 63), (const float*)(from + HALF));
+        if (sums(a)) g.products(from + (threadIdx.x & 63), P);
     }
 };
 
-template <int KS, int PL, int M, int TB, int SR, bool TURNS, bool OF_IDS, bool ENTROPY>
-__global__ __launch_bounds__(256, TB * M * KS * (4 * PL + 8) > 170 * 16 ? 1 : 2) void k_vs_backward(VsBwd a) {
-    using Stage = VsGradStage<KS, PL, M, TB, SR, OF_IDS, ENTROPY>;
+// Waves of a SIMD that the registers are shared out for: as many as need no scratch, and one more where the compiler finds room.
+constexpr int vs_bwd_waves(int KS, int PL, int M, int TB, bool OF_IDS) {
+    return PL == 1 && !OF_IDS && KS >= 10 ? (KS == 10 ? 3 : 2) : TB * M * KS * (4 * PL + 8) > 170 * 16 ? 1 : 2;
+}
+
+template <int KS, int PL, int M, int TB, int SR, bool TURNS, bool OF_IDS, bool ENTROPY, bool SUMS>
+__global__ __launch_bounds__(256, vs_bwd_waves(KS, PL, M, TB, OF_IDS)) void k_vs_backward(VsBwd a) {
+    using Stage = VsGradStage<KS, PL, M, TB, SR, OF_IDS, ENTROPY, SUMS>;
     constexpr int SIZE = TURNS ? Stage::TURN : Stage::SIZE;
     __shared__ uint4 buf0[SIZE], buf1[SIZE];
     constexpr int PIECE = KS * PL * 4;         // 16-byte pieces of a row's fragments
@@ -1576,7 +1609,7 @@ __global__ __launch_bounds__(256, TB * M * KS * (4 * PL + 8) > 170 * 16 ? 1 : 2)
     const int tile = (blockIdx.x / a.splits) * 4 + (threadIdx.x >> 6);
     const bool live = tile < a.n_tiles;
     typename Stage::Grad g;
-    g.start(a, live ? tile : 0, lane);
+    g.start(a, live ? tile : 0, lane, live);
     const float* info = OF_IDS ? a.tokens : a.info;
     if constexpr (TURNS) {
         const int row_begin = (int)((int64_t)a.groups * split / a.splits) * 32, row_end = (int)((int64_t)a.groups * (split + 1) / a.splits) * 32;
@@ -1606,7 +1639,29 @@ __global__ __launch_bounds__(256, TB * M * KS * (4 * PL + 8) > 170 * 16 ? 1 : 2)
     if (live) g.store(a, split, lane);
 }
 
-// Sums the partials of a row in a fixed order (eight loads under way: 17 us for 4,096 x 320 of 8 ranges; 4 us for 129 x 64) and writes it: dx = A sum p w + gl w_t (without an entropy gradient; with
+// A token's coefficient of its target, G_t = g (1 - p_t) - h p_t (log p_t + H), from what the sums over tokens left (several times
+// smaller errors than g has steps of 2^-24 of: where p_t is above a half, 1 - p_t is what the other ids add up to).
+__global__ __launch_bounds__(256) void k_vs_target(VsPack a, const float* __restrict__ rest, const float* __restrict__ target_e, int32_t splits, int64_t pad) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.src.rows) return;
+    float* of = a.tokens + (i >> 5) * VS_TOKEN + (i & 31);
+    if (__float_as_int(of[VS_TOKEN_TARGET]) < 0) return;       // (gl stays: 0, or NaN for a target past the vocabulary)
+    float r = 0.0f, fix = 1.0f;
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) r += rest[(int64_t)s * pad + i];
+    const float l = a.lse[i], e = target_e[i];
+    const bool empty = l == -INFINITY;
+    if (!empty) vs_lse2(l, fix);
+    r *= fix;
+    float p = exp2f(e) * fix;
+    const bool near = p > 0.5f;
+    if (near) p = 1.0f - r;
+    float G = of[VS_TOKEN_GT] * (near ? r : 1.0f - p);
+    if (a.h && a.h[i] != 0.0f && !empty && p > 0.0f) G -= a.h[i] * p * ((near ? log1pf(-r) : e * VS_LN2) + a.entropy[i]);
+    of[VS_TOKEN_GT] = G;
+}
+
+// Sums the partials of a row in a fixed order (eight loads under way: 17 us for 4,096 x 320 of 8 ranges; 4 us for 129 x 64) and writes it: dx = A sum p w + G_t w_t (without an entropy gradient; with
 // one the partials hold p (A + B e) already), dw as it is, db beside it.
 struct VsSum {
     const float* part;
@@ -1641,9 +1696,9 @@ __global__ __launch_bounds__(256) void k_vs_sum(VsSum pa, VsSum pb, uint32_t fir
         const float* of = a.tokens + (r >> 5) * VS_TOKEN + (r & 31);
         if (!a.has_entropy) v *= of[VS_TOKEN_A];
         const int32_t t = __float_as_int(of[VS_TOKEN_TARGET]);
-        const float gl = of[VS_TOKEN_GL];
-        if (t >= 0) v = fmaf(gl, vs_load(a.w, t, d), v);
-        else if (gl != gl) v = gl;
+        const float G = of[VS_TOKEN_GT];
+        if (t >= 0) v = fmaf(G, vs_load(a.w, t, d), v);
+        else if (G != G) v = G;
     }
     vs_store(a.out, r * a.ldo + d, v, a.out_bf16);
 }

@@ -113,8 +113,8 @@ struct Shape {
 };
 
 template <int KS, int PL, bool TOP> constexpr auto vs_fwd_kernel = &k_vs_forward<KS, PL, vs_fwd_tile(KS, PL, TOP), vs_fwd_blocks(KS, PL), vs_fwd_rows(KS, PL), TOP>;
-template <int KS, int PL, bool OF_IDS, bool ENTROPY>
-constexpr auto vs_bwd_kernel = &k_vs_backward<KS, PL, vs_bwd_tile(KS, PL), vs_bwd_blocks(KS, PL, OF_IDS), vs_bwd_rows(KS, PL), vs_bwd_turns(KS, PL), OF_IDS, ENTROPY>;
+template <int KS, int PL, bool OF_IDS, bool ENTROPY, bool SUMS = true>
+constexpr auto vs_bwd_kernel = &k_vs_backward<KS, PL, vs_bwd_tile(KS, PL), vs_bwd_blocks(KS, PL, OF_IDS), vs_bwd_rows(KS, PL), vs_bwd_turns(KS, PL), OF_IDS, ENTROPY, SUMS>;
 
 // workgroups of a kernel that a CU holds at once (the same on every gfx950)
 template <auto KERNEL>
@@ -207,7 +207,7 @@ struct BwdPlan {
     int64_t np, tiles_x, tiles_w;
     int splits_x, splits_w;
     uint4 *xS, *xT, *wS, *wT;
-    float *info, *tokens, *part_x, *part_w, *bias_part;
+    float *info, *tokens, *part_x, *part_w, *bias_part, *rest, *target_e;
     int64_t bytes;
 };
 BwdPlan plan_bwd(const Shape& s, void* ws) {
@@ -233,6 +233,8 @@ BwdPlan plan_bwd(const Shape& s, void* ws) {
     p.part_x = a.take<float>(p.splits_x * p.np * s.ks * 32);
     p.part_w = a.take<float>(p.splits_w > 1 ? p.splits_w * s.vp * s.ks * 32 : 0);
     p.bias_part = a.take<float>(p.splits_w > 1 ? p.splits_w * s.vp : 0);
+    p.rest = a.take<float>(p.splits_x * p.np);
+    p.target_e = a.take<float>(p.np);
     p.bytes = a.used;
     return p;
 }
@@ -408,13 +410,20 @@ int sage_token_logprobs_backward_device(sage_ctx* c, int32_t dtype, int64_t n, i
     b.info = p.info; b.tokens = p.tokens; b.has_bias = d_bias != nullptr; b.vocab = (int32_t)vocab;
     VsSum sum_x{}, sum_w{};
     uint32_t groups_x = 0, groups_w = 0;
-    if (d_dx) {
-        b.stayS = p.xS; b.flowS = p.wS; b.flowT = p.wT;
-        b.n_tiles = (int32_t)p.tiles_x; b.splits = p.splits_x; b.groups = (int32_t)(s.vp / 32); b.stay_pad = p.np; b.part = p.part_x;
+    {                                                            // over tokens first: dw takes from it what the targets' own weights are
+        b.stayS = p.xS; b.flowS = p.wS; b.flowT = d_dx ? p.wT : p.wS;            // (without dx the second half of a stage is not looked at)
+        b.n_tiles = (int32_t)p.tiles_x; b.splits = p.splits_x; b.groups = (int32_t)(s.vp / 32); b.stay_pad = p.np;
+        b.part = d_dx ? p.part_x : nullptr; b.rest = p.rest; b.target_e = p.target_e;
         const uint32_t grid = cdiv(p.tiles_x, 4) * p.splits_x;
-#define VS_F(KS, PL) if (entropy) vs_bwd_kernel<KS, PL, false, true><<<grid, 256, 0, st>>>(b); else vs_bwd_kernel<KS, PL, false, false><<<grid, 256, 0, st>>>(b)
+#define VS_F(KS, PL)                                                                            \
+    if constexpr (vs_bwd_wide(KS, vs_bwd_blocks(KS, PL, false)))                                \
+        if (!d_dx) { vs_bwd_kernel<KS, PL, false, false, false><<<grid, 256, 0, st>>>(b); break; } \
+    if (entropy) vs_bwd_kernel<KS, PL, false, true><<<grid, 256, 0, st>>>(b); else vs_bwd_kernel<KS, PL, false, false><<<grid, 256, 0, st>>>(b)
         VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
+        if (d_targets) k_vs_target<<<cdiv(n, 256), 256, 0, st>>>(of_x, p.rest, p.target_e, p.splits_x, p.np);
+    }
+    if (d_dx) {
         sum_x = VsSum{p.part_x, nullptr, (int32_t)n, dim, s.ks * 32, p.splits_x, p.np, p.tokens, entropy, w, d_dx, lddx, bf16, nullptr};
         groups_x = cdiv(n * dim, 256);
     }
