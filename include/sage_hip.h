@@ -212,7 +212,9 @@ int sage_train_embeddings(sage_ctx* ctx, int32_t dim, int32_t window, int32_t ne
  * and the `alternatives` largest logits of a row, as ids in descending order (ties: the lower id) and log probabilities.
  * The [n][vocab] matrix of logits is never stored.
  *   d_x [n][dim], d_weight [vocab][dim]   both SAGE_F32 or both SAGE_BF16, rows ldx / ldw elements apart (>= dim); any alignment
- *                    of rows.  Products and sums are float32 (float32 inputs at float32 accuracy); the softmax's too.
+ *                    of rows.  Products and sums are float32; the softmax's too.  A float32 element is taken to 2^-22 of itself or 2^-29 of its
+ *                    row's largest, whichever is more, whatever other rows hold: logits are float32's to within a few steps of 2^-24 of
+ *                    sum_d |x_d| max_d |w_d|.
  *   d_bias [vocab]   float32 or NULL; -inf, or any value of -1e30 or less, takes an id out (so does a logit of -6e29).  A row that
  *                    has nothing left gets lse -inf, logprob -inf, entropy 0, alternatives -1.  x is finite, and so are the weights of ids that
  *                    are not taken out: a logit that is NaN or +inf makes its row NaN, alternatives -1.

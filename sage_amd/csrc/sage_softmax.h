@@ -19,8 +19,8 @@
 // two float16 (11 + 11 bits) and three of the four products are formed; what is left out is 2^-22 of |x||w|, the size of
 // float32's own rounding in a sum of a few terms, and it costs 3 MFMAs where three bf16 parts cost 6 and the float32 MFMA 16
 // (256 against 4,096 operations per clock and CU).  float16's narrow range is met by powers of two, exact in both
-// directions: 32 rows share one that brings their largest element to 2^13, and the weights of a column share one that
-// follows their largest (both below).  Where the weights are read only once (few tokens), the three bf16 parts are formed on
+// directions: a row has one that brings its largest element to 2^13 (32 rows share one where they differ by no more than 2^8),
+// and the weights of a column share one that follows their largest (both below).  Where the weights are read only once (few tokens), the three bf16 parts are formed on
 // the way instead: they need no scale.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -129,7 +129,9 @@ __device__ __forceinline__ void vs_split(vs_f8 v, vs_bits* out) {
 // order that a lane has values in.  Rows past the end and elements past `dim` are zero.  A fragment is one
 // coalesced 1 KiB load of a wave, whatever the caller's row length, stride and alignment are.  One workgroup packs 32 rows:
 // a lane loads the eight elements that its place in an S fragment asks for; T fragments are read back through LDS.
-// PL = 2: the 32 rows are multiplied by 2^e, e such that the largest finite element comes to just under 2^13.  Bound by HBM:
+// PL = 2: a row is multiplied by 2^e, e such that its largest finite element comes to just under 2^13, or that of the 32 rows, if no row
+// is smaller by more than 2^VS_SPREAD: elements are then off by at most 2^-37 of that largest one, or 2^-29 of their own row's, a 32nd of a
+// float32's step.  (One scale for 32 rows, whatever they hold, would take all bits of rows beside one 10^9 times larger.)  Bound by HBM:
 // 131,072 x 300 bf16 for a forward pass, 79 MB read and 84 MB written, 37 us (4.4 TB/s); rows of 511 bf16, that start at any
 // 2-byte boundary, 84 MB in all in 23 us (33 with unaligned loads in place of aligned words).
 
@@ -164,25 +166,31 @@ __device__ __forceinline__ vs_f8 vs_eight(const VsSrc& s, int64_t row, int d) {
 }
 
 // What goes with the fragments of 32 ids: their biases (0 where the caller gives none, -inf past the end: p = 0 there), then
-// the exponent of their scale and their largest size.  A mask of the type's lowest value becomes -inf too: next to it no logit keeps a bit, and
-// float32 could not hold it in powers of two.  PL = 2 keeps the biases in powers of two.
-#define VS_INFO 36
+// the exponent of their scale, their largest size, whether their scales differ, and by how much each row's exponent
+// exceeds the common one (a byte each; 0 where they share it).  A mask of the type's lowest value becomes -inf too: next to it no logit
+// keeps a bit, and float32 could not hold it in powers of two.  PL = 2 keeps the biases in powers of two.
+#define VS_SPREAD 8
+#define VS_INFO 44
 #define VS_INFO_EXP 32
 #define VS_INFO_WIDE 33
+#define VS_INFO_DIFFER 34
+#define VS_INFO_MORE 36
 // What goes with those of 32 tokens in the gradient: lse in powers of two (L), A and B of G = p (A + B e), e = log2 p, for the ids
-// that are not the target; the target, and its own G (gl until k_vs_target has formed it); the exponent of their scale last.
-#define VS_TOKEN 164
+// that are not the target; the target, and its own G (gl until k_vs_target has formed it); the exponents as above.
+#define VS_TOKEN 172
 #define VS_TOKEN_A 32
 #define VS_TOKEN_B 64
 #define VS_TOKEN_GT 96
 #define VS_TOKEN_TARGET 128
 #define VS_TOKEN_EXP 160
+#define VS_TOKEN_DIFFER 161
+#define VS_TOKEN_MORE 164
+__device__ __forceinline__ float vs_more(const float* more, int row) { return (float)((const uint8_t*)more)[row]; }
 
 struct VsPack {
     VsSrc src;
     uint4 *S, *T;              // T: of a gradient, or null
-    float* exps;               // PL = 2: e of group g at exps[g * exps_step]
-    int32_t exps_step;
+    float* exps;               // PL = 2, of tokens in a forward pass: e of each row, its own whatever the others are; or null
     int32_t groups;            // of 32 rows
     // ids: their biases (`bias` or null)
     float* info;               // null: not of ids
@@ -235,7 +243,7 @@ __global__ __launch_bounds__(256) void k_vs_pack(VsPack pa, VsPack pb) {
     const int64_t group = second ? (int64_t)blockIdx.x - pa.groups : blockIdx.x;
     constexpr int DP = KS * 32, LD = DP + 4, N = (KS + 1) / 2;      // fragments of a wave
     __shared__ float tile[FORWARD ? 1 : 32 * LD];      // (a forward pass has no use for T, and more workgroups at a time without it)
-    __shared__ float wmax[4], wfin[4];
+    __shared__ float wmax[4], rmax[4][32];
     constexpr int K = VsTile<M>::K, STEPS = DP / K;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane % M;
     auto row_of = [&](int f) { return f / STEPS * M + col; };
@@ -248,32 +256,66 @@ __global__ __launch_bounds__(256) void k_vs_pack(VsPack pa, VsPack pb) {
         there[r] = row < a.src.rows && !(a.bias && a.bias[row] <= VS_NOTHING) && !(a.tokens && vs_idle(a, row));
     }
     vs_f8 v[N];
-    float big = 0.0f, fin = 0.0f;
+    float big = 0.0f, fin[32 / M];             // of all, and the largest finite size of each of this lane's rows
+#pragma unroll
+    for (int r = 0; r < 32 / M; ++r) fin[r] = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int f = i * 4 + wave;
         v[i] = vs_f8(0.0f);
         if (f < 2 * KS && there[f / STEPS ? 32 / M - 1 : 0] && element_of(f) < a.src.dim) v[i] = vs_eight<PL>(a.src, row0 + row_of(f), element_of(f));
+        float most = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float q = fabsf(v[i][j]);
             big = fmaxf(big, q);
-            fin = fmaxf(fin, q < INFINITY ? q : 0.0f);
+            most = fmaxf(most, q < INFINITY ? q : 0.0f);
         }
+#pragma unroll
+        for (int r = 0; r < 32 / M; ++r) fin[r] = fmaxf(fin[r], f / STEPS == r ? most : 0.0f);
     }
-    for (int o = 1; o < 64; o <<= 1) { big = fmaxf(big, __shfl_xor(big, o)); fin = fmaxf(fin, __shfl_xor(fin, o)); }
-    if (lane == 0) { wmax[wave] = big; wfin[wave] = fin; }
+    for (int o = 1; o < 64; o <<= 1) big = fmaxf(big, __shfl_xor(big, o));
+    if (lane == 0) wmax[wave] = big;
+    if (PL == 2)
+#pragma unroll
+        for (int r = 0; r < 32 / M; ++r) {
+            for (int o = M; o < 64; o <<= 1) fin[r] = fmaxf(fin[r], __shfl_xor(fin[r], o));
+            if (lane < M) rmax[wave][r * M + col] = fin[r];
+        }
     __syncthreads();
     big = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
-    fin = fmaxf(fmaxf(wfin[0], wfin[1]), fmaxf(wfin[2], wfin[3]));
-    int e = 0;
-    if (PL == 2 && fin > 0.0f) e = 13 - __builtin_amdgcn_frexp_expf(fin);
+    int e = 0, more = 0, exps[32 / M];         // the common exponent, what row `lane` % 32 has beyond it, those of this lane's rows
+    bool differ = false;
+#pragma unroll
+    for (int r = 0; r < 32 / M; ++r) exps[r] = 0;
+    if (PL == 2) {
+        const int i = lane & 31;
+        const float own = fmaxf(fmaxf(rmax[0][i], rmax[1][i]), fmaxf(rmax[2][i], rmax[3][i]));
+        float all = own;
+        for (int o = 1; o < 32; o <<= 1) all = fmaxf(all, __shfl_xor(all, o));
+        if (all > 0.0f) e = 13 - __builtin_amdgcn_frexp_expf(all);
+        if (own > 0.0f) more = min(13 - __builtin_amdgcn_frexp_expf(own) - e, 255);
+        differ = a.exps || __any(more > VS_SPREAD);
+        if (!differ) more = 0;
+#pragma unroll
+        for (int r = 0; r < 32 / M; ++r) exps[r] = e + __shfl(more, r * M + col);
+    }
     if (threadIdx.x == 0) {
-        if (a.info) a.info[group * VS_INFO + VS_INFO_WIDE] = big;
-        if (PL == 2) a.exps[group * a.exps_step] = (float)e;
+        if (a.info) {
+            a.info[group * VS_INFO + VS_INFO_WIDE] = big;
+            a.info[group * VS_INFO + VS_INFO_EXP] = (float)e;
+            a.info[group * VS_INFO + VS_INFO_DIFFER] = differ ? 1.0f : 0.0f;
+        }
+        if (a.tokens) {
+            a.tokens[group * VS_TOKEN + VS_TOKEN_EXP] = (float)e;
+            a.tokens[group * VS_TOKEN + VS_TOKEN_DIFFER] = differ ? 1.0f : 0.0f;
+        }
     }
     if (threadIdx.x < 32) {
         const int64_t row = row0 + threadIdx.x;
+        if (a.exps) a.exps[row] = (float)(e + more);
+        if (a.info) ((uint8_t*)&a.info[group * VS_INFO + VS_INFO_MORE])[threadIdx.x] = (uint8_t)more;
+        if (a.tokens) ((uint8_t*)&a.tokens[group * VS_TOKEN + VS_TOKEN_MORE])[threadIdx.x] = (uint8_t)more;
         if (a.info) {
             const float b = row >= a.src.rows ? -INFINITY : a.bias ? a.bias[row] : 0.0f;
             a.info[group * VS_INFO + threadIdx.x] = b <= VS_NOTHING ? -INFINITY : PL == 2 ? b * VS_LOG2E : b;
@@ -286,7 +328,7 @@ __global__ __launch_bounds__(256) void k_vs_pack(VsPack pa, VsPack pb) {
         if (f >= 2 * KS) continue;
         if (PL == 2)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = ldexpf(v[i][j], e);
+            for (int j = 0; j < 8; ++j) v[i][j] = ldexpf(v[i][j], exps[f / STEPS ? 32 / M - 1 : 0]);
         if (!FORWARD && a.T) {
             float* to = tile + row_of(f) * LD + element_of(f);
             *(vs_f4*)to = vs_f4{v[i][0], v[i][1], v[i][2], v[i][3]};
@@ -334,7 +376,7 @@ __device__ __forceinline__ float vs_unit(float n) { return ldexpf(VS_LOG2E, (int
 struct VsFwd {
     const uint4 *xS, *wS;
     const float* info;         // [ids / 32][VS_INFO]
-    const float* x_exp;        // PL = 2: [tokens / 32]
+    const float* x_exp;        // PL = 2: [tokens]
     int32_t has_bias;          // the caller gave one: -inf may stand anywhere (else only past `vocab`)
     int32_t vocab;
     int32_t n_tiles;           // token tiles of TB M rows
@@ -504,6 +546,28 @@ struct VsRowsOfTile {
     }
 };
 
+// What the rows that a lane has logits of have beyond the common exponent, four bytes a word
+template <int M>
+__device__ __forceinline__ void vs_mores(const float* more, int lane, uint32_t (&to)[VS_NJ<M> / 4]) {
+#pragma unroll
+    for (int q = 0; q < VS_NJ<M> / 4; ++q) to[q] = ((const uint32_t*)more)[vs_row<M>(q * 4, lane) / 4];
+}
+template <int N>
+__device__ __forceinline__ int vs_more_of(const uint32_t (&more)[N], int j) { return (int)(more[j >> 2] >> (j & 3) * 8 & 255); }
+
+// Where the scales of the 32 streaming rows differ, their logits are brought to the common one.
+template <int M, int TB>
+__device__ __forceinline__ void vs_common(const uint32_t (&more)[VS_NJ<M> / 4], VsLogits<M, TB>& s) {
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+#pragma unroll
+        for (int j = 0; j < VS_NJ<M>; ++j) vs_set<M, TB>(s, t, j, ldexpf(vs_value<M, TB>(s, t, j), -vs_more_of(more, j)));
+#pragma unroll
+        for (int b = 0; b < VsTile<M>::NB; ++b) vs_in_place(s[b][t]);
+    }
+}
+__device__ __forceinline__ bool vs_differ(float flag) { return __builtin_amdgcn_readfirstlane(__float_as_int(flag)) != 0; }
+
 // Adds the biases where the product did not start from them, and raises masked logits.
 template <int M, int TB, bool SCALED>
 __device__ __forceinline__ void vs_mask(VsLogits<M, TB>& s, float (&unit)[TB], const vs_f4 (&b)[VS_NJ<M> / 4]) {
@@ -543,6 +607,12 @@ __device__ __forceinline__ void vs_forward_step(const VsFwd& a, int row0, const 
 #pragma unroll
     for (int t = 0; t < TB; ++t) unit[t] = PL == 2 ? vs_unit(-(e + x_exp[t])) : VS_LOG2E;
     vs_product<KS, PL, M, TB>(w, x, s);
+    if (PL == 2)
+        if (vs_differ(info[VS_INFO_DIFFER])) {
+            uint32_t more[VS_NJ<M> / 4];
+            vs_mores<M>(info + VS_INFO_MORE, threadIdx.x & 63, more);
+            vs_common<M, TB>(more, s);
+        }
     if (a.has_bias || row0 + 32 > a.vocab) vs_mask<M, TB, PL == 2>(s, unit, b);      // (the same in the whole grid)
     rows.template add<TOP, PL == 2>(s, unit);
 }
@@ -597,7 +667,7 @@ struct VsStage {
 };
 
 template <int KS, int PL, int M, int TB, int SR, bool TOP>
-__global__ __launch_bounds__(256, 2) void k_vs_forward(VsFwd a) {
+__global__ __launch_bounds__(256, KS == 2 ? 3 : 2) void k_vs_forward(VsFwd a) {
     using Stage = VsStage<KS, PL, M, SR>;
     __shared__ uint4 buf0[Stage::SIZE], buf1[Stage::SIZE];
     const int lane = threadIdx.x & 63;
@@ -609,7 +679,7 @@ __global__ __launch_bounds__(256, 2) void k_vs_forward(VsFwd a) {
     vs_stationary<KS, PL, M, TB>(a.xS, live ? tile : 0, lane, x);
     float x_exp[TB];
 #pragma unroll
-    for (int t = 0; t < TB; ++t) x_exp[t] = PL == 2 ? a.x_exp[((live ? tile : 0) * TB + t) * M / 32] : 0.0f;
+    for (int t = 0; t < TB; ++t) x_exp[t] = PL == 2 ? a.x_exp[((live ? tile : 0) * TB + t) * M + lane % M] : 0.0f;
     VsRowsOfTile<M, TB> rows;
     rows.clear();
     const uint4* w = a.wS + (int64_t)row_begin * KS * PL * 4;
@@ -895,7 +965,8 @@ __global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
 // ---- alternatives -------------------------------------------------------------------------------------------------
 // The k largest logits of a row, ties to the lower id, in the order of the logits as float64 sums them.  The forward pass
 // left each chunk's largest float32 logit m, rounded towards 0 to float16; a float32 sum is within d = 4 (D + 16) 2^-24 (|m| + 2 |x|_1
-// max |w|) of the true one, the rounding adds 2^-10 |m|.  At least k logits are no less than the k-th largest m - d, so only
+// max |w|) of the true one (elements as two float16 of their row's scale add 2^-22 + 2^-29 + 2^-36 D of |x|_1 max |w|, less than a 16th of that),
+// the rounding adds 2^-10 |m|.  At least k logits are no less than the k-th largest m - d, so only
 // chunks with m + d at or above that can hold one of the k: a few more than k, of 8 ids each.  Their logits are formed again in
 // float32, those that reach the bound once more in float64, and the best k of these few are ranked by counting.  A workgroup
 // per row.
@@ -1293,11 +1364,11 @@ struct VsGrad {
             if constexpr (OF_IDS) {
                 const float* of = a.info + (r >> 5) * VS_INFO;
                 L[t] = of[r & 31];
-                y_exp[t] = PL == 2 ? of[VS_INFO_EXP] : 0.0f;
+                y_exp[t] = PL == 2 ? of[VS_INFO_EXP] + vs_more(of + VS_INFO_MORE, r & 31) : 0.0f;
             } else {
                 const float* of = a.tokens + (r >> 5) * VS_TOKEN;
                 L[t] = of[r & 31]; A[t] = of[VS_TOKEN_A + (r & 31)]; B[t] = of[VS_TOKEN_B + (r & 31)];
-                y_exp[t] = PL == 2 ? of[VS_TOKEN_EXP] : 0.0f;
+                y_exp[t] = PL == 2 ? of[VS_TOKEN_EXP] + vs_more(of + VS_TOKEN_MORE, r & 31) : 0.0f;
                 target[t] = live ? __float_as_int(of[VS_TOKEN_TARGET + (r & 31)]) : -1;
                 if (PL == 2 && ENTROPY) {      // |A + B e| brought below 1
                     const float size = fabsf(A[t]) + fabsf(B[t]) * 256.0f;
@@ -1382,6 +1453,12 @@ struct VsGrad {
 #pragma unroll
         for (int t = 0; t < TB; ++t) unit[t] = PL == 2 ? vs_unit(-(f_exp + y_exp[t])) : VS_LOG2E;
         vs_product<KS, PL, M, TB>(S, y, s);
+        uint32_t more[NJ / 4];
+        const bool differ = PL == 2 && vs_differ(of[OF_IDS ? VS_TOKEN_DIFFER : VS_INFO_DIFFER]);
+        if (differ) {
+            vs_mores<M>(of + (OF_IDS ? VS_TOKEN_MORE : VS_INFO_MORE), lane, more);
+            vs_common<M, TB>(more, s);
+        }
         if (a.has_bias || (OF_IDS ? stay0 + TB * M > a.vocab : row0 + 32 > a.vocab)) {
             if constexpr (OF_IDS) {
 #pragma unroll
@@ -1398,6 +1475,16 @@ struct VsGrad {
         }
         if constexpr (!OF_IDS && !AGAIN)
             if (any_target(row0)) leave_targets(a, row0, unit, s);
+        if (PL == 2 && !OF_IDS && differ) {    // (as for ids, in the exponent)
+#pragma unroll
+            for (int t = 0; t < TB; ++t) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) vs_set<M, TB>(s, t, j, fmaf(vs_value<M, TB>(s, t, j), unit[t], -(float)vs_more_of(more, j)));
+                unit[t] = 1.0f;
+#pragma unroll
+                for (int b = 0; b < VsTile<M>::NB; ++b) vs_in_place(s[b][t]);
+            }
+        }
         float G[TB][NJ];
         float big[TB], ps[TB];                 // PL = 2: the power of two that a column's largest scaled weight is below; of tokens: the sum of p
         auto form = [&]() {
@@ -1448,15 +1535,33 @@ struct VsGrad {
             }
         if constexpr (OF_IDS) {
             put_targets(of, G);
-            if (PL == 2)
+            if (a.want_db)
+#pragma unroll
+                for (int t = 0; t < TB; ++t) {
+                    float v = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < NJ; j += 4) v += (G[t][j] + G[t][j + 1]) + (G[t][j + 2] + G[t][j + 3]);
+                    db[t] += v;
+                }
+            if (PL == 2) {
 #pragma unroll
                 for (int t = 0; t < TB; ++t) {
                     float m = 0.0f;
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) m = fmaxf(m, fabsf(G[t][j]));
                     big[t] = m > 0.0f ? (float)__builtin_amdgcn_frexp_expf(m) + (sg[t] - f_exp) : 0.0f;
-                    most = fmaxf(most, big[t]);
                 }
+                if (differ)                    // weights of rows with a smaller scale of their own are as much larger, for their products
+#pragma unroll
+                    for (int t = 0; t < TB; ++t) {
+                        float m = -1000.0f;
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) m = fmaxf(m, G[t][j] != 0.0f ? (float)(__builtin_amdgcn_frexp_expf(G[t][j]) - vs_more_of(more, j)) : m);
+                        big[t] = m + (sg[t] - f_exp);
+                    }
+#pragma unroll
+                for (int t = 0; t < TB; ++t) most = fmaxf(most, big[t]);
+            }
         }
         if (PL == 2)
             if (__any(most > MOST)) {
@@ -1464,22 +1569,37 @@ struct VsGrad {
                 for (int t = 0; t < TB; ++t) lower(t, ceilf(big[t] - AIM));
                 if (!OF_IDS) form();           // (there the scale is in the exponent already)
             }
+        int by[TB];
 #pragma unroll
         for (int t = 0; t < TB; ++t) {
-            if constexpr (OF_IDS)
-                if (a.want_db) {
-                    float v = 0.0f;
+            by[t] = PL == 2 ? (int)(sg[t] - f_exp) : 0;
+            if (!OF_IDS) ps[t] = PL == 2 ? ldexpf(ps[t], -by[t]) : ps[t];
+        }
+        if (differ)
 #pragma unroll
-                    for (int j = 0; j < NJ; j += 4) v += (G[t][j] + G[t][j + 1]) + (G[t][j + 2] + G[t][j + 3]);
-                    db[t] += v;
+            for (int t = 0; t < TB; ++t) {
+                if (OF_IDS) {
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) G[t][j] = ldexpf(G[t][j], by[t] - vs_more_of(more, j));
+                    by[t] = 0;
+                } else {                       // p is 2^(e + more - by) there, with the e that G was formed of
+                    ps[t] = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        const float e = fmaf(vs_value<M, TB>(s, t, j), unit[t], (float)by[t] - L[t]), q = __builtin_amdgcn_exp2f(e);
+                        ps[t] += ldexpf(q, vs_more_of(more, j) - by[t]);
+                        if (ENTROPY) G[t][j] = q * fmaf(B[t], vs_max(e + (float)vs_more_of(more, j), VS_TMIN), fmaf(-B[t], (float)by[t], A[t]));
+                    }
                 }
-            const int by = PL == 2 ? (int)(sg[t] - f_exp) : 0;
-            if (!OF_IDS) rest[t] += PL == 2 ? ldexpf(ps[t], -by) : ps[t];
+            }
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
+            if (!OF_IDS) rest[t] += ps[t];
 #pragma unroll
             for (int u = 0; u < HALVES; ++u) {
                 vs_f8 v;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = PL == 2 && OF_IDS ? ldexpf(G[t][u * 8 + j], by) : G[t][u * 8 + j];
+                for (int j = 0; j < 8; ++j) v[j] = PL == 2 && OF_IDS ? ldexpf(G[t][u * 8 + j], by[t]) : G[t][u * 8 + j];
                 vs_split<PL>(v, P[t][u]);
             }
         }

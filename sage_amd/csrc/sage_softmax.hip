@@ -195,7 +195,7 @@ FwdPlan plan_fwd(const Shape& s, void* ws) {
         p.wS = a.take<uint4>(s.vp / 16 * frag);
         p.xS = a.take<uint4>(p.n_pad / 16 * frag);
         p.info = a.take<float>(s.vp / 32 * VS_INFO);
-        p.x_exp = a.take<float>(p.n_pad / 32);
+        p.x_exp = a.take<float>(p.n_pad);
     }
     p.part = a.take<float4>(p.splits * p.n_pad);
     p.chunk_max = a.take<_Float16>(s.k ? p.n_pad * p.chunks : 0);
@@ -274,9 +274,9 @@ void pack(const Shape& s, const VsPack& a, const VsPack& b, hipStream_t st) {
     VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
 }
-VsPack pack_of(const VsSrc& src, uint4* S, uint4* T, float* exps, int32_t exps_step, int64_t padded) {
+VsPack pack_of(const VsSrc& src, uint4* S, uint4* T, int64_t padded) {
     VsPack p{};
-    p.src = src; p.S = S; p.T = T; p.exps = exps; p.exps_step = exps_step; p.groups = (int32_t)(padded / 32);
+    p.src = src; p.S = S; p.T = T; p.groups = (int32_t)(padded / 32);
     return p;
 }
 
@@ -319,7 +319,7 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
     if (!dev.ok) return sage_ctx_fail(c, SAGE_E_HIP, "the context's device cannot be made current");
     const hipStream_t st = (hipStream_t)stream;
     const VsSrc w{d_weight, ldw, (int32_t)vocab, dim, dtype == SAGE_BF16}, x{d_x, ldx, (int32_t)n, dim, dtype == SAGE_BF16};
-    VsPack of_w = pack_of(w, p.wS, nullptr, p.info + VS_INFO_EXP, VS_INFO, s.vp);
+    VsPack of_w = pack_of(w, p.wS, nullptr, s.vp);
     of_w.info = p.info; of_w.bias = d_bias;
     for (int64_t r0 = 0; r0 < n; r0 += p.rows) {
         const int64_t rows = std::min(p.rows, n - r0);
@@ -337,7 +337,8 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
 #undef VS_F
         } else {
             if (r0) of_w.groups = 0;               // packed with the first rows
-            const VsPack of_x = pack_of(xr, p.xS, nullptr, p.x_exp, 1, p.n_pad);
+            VsPack of_x = pack_of(xr, p.xS, nullptr, p.n_pad);
+            of_x.exps = p.x_exp;
             if (alternatives) pack<true, true>(s, of_w, of_x, st); else pack<true, false>(s, of_w, of_x, st);
             const uint32_t grid = cdiv(p.tiles, 4) * p.splits;
 #define VS_F(KS, PL) if (alternatives) vs_fwd_kernel<KS, PL, true><<<grid, 256, 0, st>>>(f); else vs_fwd_kernel<KS, PL, false><<<grid, 256, 0, st>>>(f)
@@ -399,9 +400,9 @@ int sage_token_logprobs_backward_device(sage_ctx* c, int32_t dtype, int64_t n, i
     const BwdPlan p = plan_bwd(s, d_workspace);
     if ((rc = check_workspace(c, d_workspace, workspace_bytes, p.bytes))) return rc;
     const VsSrc w{d_weight, ldw, (int32_t)vocab, dim, bf16}, x{d_x, ldx, (int32_t)n, dim, bf16};
-    VsPack of_w = pack_of(w, p.wS, d_dx ? p.wT : nullptr, p.info + VS_INFO_EXP, VS_INFO, s.vp);
+    VsPack of_w = pack_of(w, p.wS, d_dx ? p.wT : nullptr, s.vp);
     of_w.info = p.info; of_w.bias = d_bias;
-    VsPack of_x = pack_of(x, p.xS, d_dweight ? p.xT : nullptr, p.tokens + VS_TOKEN_EXP, VS_TOKEN, p.np);
+    VsPack of_x = pack_of(x, p.xS, d_dweight ? p.xT : nullptr, p.np);
     of_x.tokens = p.tokens; of_x.lse = d_lse; of_x.entropy = d_entropy; of_x.g = d_grad_logprob; of_x.h = d_grad_entropy; of_x.targets = d_targets;
     of_x.vocab = (int32_t)vocab;
     pack<false>(s, of_w, of_x, st);
