@@ -215,9 +215,10 @@ int sage_train_embeddings(sage_ctx* ctx, int32_t dim, int32_t window, int32_t ne
  *                    of rows.  Products and sums are float32; the softmax's too.  A float32 element is taken to 2^-22 of itself or 2^-29 of its
  *                    row's largest, whichever is more, whatever other rows hold: logits are float32's to within a few steps of 2^-24 of
  *                    sum_d |x_d| max_d |w_d|.
- *   d_bias [vocab]   float32 or NULL; -inf, or any value of -1e30 or less, takes an id out (so does a logit of -6e29).  A row that
- *                    has nothing left gets lse -inf, logprob -inf, entropy 0, alternatives -1.  x is finite, and so are the weights of ids that
- *                    are not taken out: a logit that is NaN or +inf makes its row NaN, alternatives -1.
+ *   d_bias [vocab]   float32 or NULL; -inf, or any value of -1e30 or less, takes an id out (so does a logit of -1e30 or less, -inf
+ *                    among them).  A row that has nothing left gets lse -inf, logprob -inf, entropy 0, alternatives -1.  x is finite,
+ *                    and so are the weights of ids that are not taken out, and products x_d w_vd lie in float32's range: a logit that is NaN or
+ *                    +inf makes its row NaN, alternatives -1.
  *   d_targets [n]    int64, or NULL (then no d_logprob).  A negative target means none: logprob 0, no gradient.  The host cannot
  *                    see a target of `vocab` or more: its logprob is NaN, and so are the gradients it reaches.
  *   d_logprob, d_entropy, d_lse [n] float32 (d_logprob and d_entropy may be NULL); d_alt_ids int32 and d_alt_logprobs float32
