@@ -210,6 +210,8 @@ int sage_train_embeddings(sage_ctx* ctx, int32_t dim, int32_t window, int32_t ne
  * and whose compute_losses scores with log-sigmoids, utils.py:125-138): with logits s_nv = x_n . weight_v + bias_v,
  *   logprob[n] = s_n,target(n) - lse[n],   lse[n] = log sum_v exp s_nv,   entropy[n] = lse[n] - sum_v p_nv s_nv,
  * and the `alternatives` largest logits of a row, as ids in descending order (ties: the lower id) and log probabilities.
+ * (logprob is log(1 - the other ids' share) where that share is below a half, to float32's relative precision however small it is; the
+ * log probabilities of alternatives are their logits less lse, to its precision.)
  * The [n][vocab] matrix of logits is never stored.
  *   d_x [n][dim], d_weight [vocab][dim]   both SAGE_F32 or both SAGE_BF16, rows ldx / ldw elements apart (>= dim); any alignment
  *                    of rows.  Products and sums are float32; the softmax's too.  A float32 element is taken to 2^-22 of itself or 2^-29 of its

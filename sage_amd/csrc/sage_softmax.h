@@ -379,36 +379,41 @@ struct VsFwd {
     const float* x_exp;        // PL = 2: [tokens]
     int32_t has_bias;          // the caller gave one: -inf may stand anywhere (else only past `vocab`)
     int32_t vocab;
+    const int64_t* targets;    // of `rows` tokens, or null
+    int32_t rows;
     int32_t n_tiles;           // token tiles of TB M rows
     int32_t splits;            // ranges of the vocabulary
     int32_t blocks;            // blocks of VS_BLOCK ids
     int32_t chunks;            // chunks of VS_CHUNK ids: 32 a block
     int64_t n_pad;             // row length of the partials
-    float4* part;              // [splits][n_pad]: reference (in powers of two), sum of exps, sum of exp * exponent; largest |weight|
+    float4* part;              // [splits][n_pad]: reference (in powers of two), sum of exps, sum of exp * exponent, sum of exps without the target's
+    float* wide;               // [splits]: largest |weight|
     _Float16* chunk_max;       // [n_pad][chunks] or null: largest logits, -inf where all are masked
 };
 
-// Sums of a row, relative to 2^ref: s of exp, e of exp * exponent (the entropy's).  A softmax in one pass: the reference is
+// Sums of a row, relative to 2^ref: s of exp, e of exp * exponent (the entropy's), R of exp over all ids but the target (1 - p_t, to its own
+// last bits where p_t is near 1: the log probability is then log(1 - R / S)).  A softmax in one pass: the reference is
 // moved to the running maximum only when a step's terms have outgrown it by VS_SLACK, a few times per row; the common step
 // neither rescales nor looks for a maximum.  Eight terms are summed first, then up to VS_BLOCK / 4 of those, then these: sums of 262,144 terms keep
 // their last bits.
 struct VsStat {
-    float ref, s, e, S, E;
-    __device__ __forceinline__ void clear() { ref = VS_NOTHING; s = e = S = E = 0.0f; }
+    float ref, s, e, S, E, R;
+    __device__ __forceinline__ void clear() { ref = VS_NOTHING; s = e = S = E = R = 0.0f; }
     __device__ __forceinline__ void flush() { S += s; E += e; s = e = 0.0f; }
     __device__ __forceinline__ void move(float now) {      // (a sum that vanishes takes its exponents with it: 0 * inf)
         const float d = ref - now, f = exp2f(d);
         e = f == 0.0f ? 0.0f : f * fmaf(d, s, e);
         E = f == 0.0f ? 0.0f : f * fmaf(d, S, E);
-        s *= f; S *= f;
+        s *= f; S *= f; R *= f;
         ref = now;
     }
-    __device__ __forceinline__ void join(float r2, float s2, float e2) {     // S and E with another range's
+    __device__ __forceinline__ void join(float r2, float s2, float e2, float R2) {     // S, E and R with another range's
         const float now = fmaxf(ref, r2);
         if (now > ref) move(now);
         const float d = r2 - now, f = exp2f(d);
         E += f == 0.0f ? 0.0f : f * fmaf(d, s2, e2);
         S += s2 != s2 ? s2 : f * s2;
+        R += f * R2;
     }
 };
 
@@ -460,15 +465,24 @@ struct VsRowsOfTile {
     VsStat st[TB];
     float top[TB][C], even[TB][C], wide;       // wide: the largest size of a weight
     uint32_t keep[TB][C][3];
-    __device__ __forceinline__ void clear() {
+    int target[TB];                            // -1: none
+    __device__ __forceinline__ void clear(const VsFwd& a, int64_t row0, bool live) {     // of the tile's first row
 #pragma unroll
-        for (int t = 0; t < TB; ++t) st[t].clear();
+        for (int t = 0; t < TB; ++t) {
+            st[t].clear();
+            const int64_t row = row0 + t * M + threadIdx.x % M;
+            const int64_t v = live && a.targets && row < a.rows ? a.targets[row] : -1;
+            target[t] = v >= 0 && v < a.vocab ? (int)v : -1;
+        }
         wide = 0.0f;
     }
     // the logits of 32 ids, in powers of two after multiplication by unit[t]; TOP: their largest is kept
     template <bool TOP, bool SCALED, bool ONCE = false>
-    __device__ __forceinline__ void add(const VsLogits<M, TB>& s, const float (&unit)[TB]) {
-        float ls[TB], le[TB];
+    __device__ __forceinline__ void add(int row0, const VsLogits<M, TB>& s, const float (&unit)[TB]) {
+        float ls[TB], le[TB], lr[TB];
+        bool here = false;
+#pragma unroll
+        for (int t = 0; t < TB; ++t) here |= (uint32_t)(target[t] - row0) < 32;
         // A logit of -inf has p = 0, and an exponent that 0 times is NaN: the second look, rarely taken, stops exponents where p is 0.
         // ONCE: so does the first (kernels bound by memory: 5 tokens x 229,376 ids of bf16 55.3 us, 57.3 with a second look).
         auto sums = [&](auto again) {
@@ -493,9 +507,23 @@ struct VsRowsOfTile {
             sums(std::true_type{});
         }
 #pragma unroll
+        for (int t = 0; t < TB; ++t) lr[t] = ls[t];
+        if (__any(here))                       // (rare: a token has one target)
+#pragma unroll
+            for (int t = 0; t < TB; ++t) {
+                const int at = target[t] - row0 - vs_row<M>(0, threadIdx.x & 63);
+                lr[t] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(vs_value<M, TB>(s, t, j), SCALED ? unit[t] : VS_LOG2E, -st[t].ref));
+                    lr[t] += at == vs_row<M>(j, 0) ? 0.0f : p;
+                }
+            }
+#pragma unroll
         for (int t = 0; t < TB; ++t) {
             st[t].s += ls[t];
             st[t].e += le[t];
+            st[t].R += lr[t];
             if (TOP)
 #pragma unroll
                 for (int c = 0; c < C; ++c) top[t][c] = SCALED ? of_chunk(s, t, c) * (unit[t] * VS_LN2) : of_chunk(s, t, c);
@@ -537,8 +565,8 @@ struct VsRowsOfTile {
             st[t].flush();
 #pragma unroll
             for (int o = M; o <= 32; o <<= 1) {
-                const float r2 = __shfl_xor(st[t].ref, o), s2 = __shfl_xor(st[t].S, o), e2 = __shfl_xor(st[t].E, o);
-                st[t].join(r2, s2, e2);
+                const float r2 = __shfl_xor(st[t].ref, o), s2 = __shfl_xor(st[t].S, o), e2 = __shfl_xor(st[t].E, o), R2 = __shfl_xor(st[t].R, o);
+                st[t].join(r2, s2, e2, R2);
             }
         }
     }
@@ -546,7 +574,8 @@ struct VsRowsOfTile {
         join_lanes();
 #pragma unroll
         for (int t = 0; t < TB; ++t)
-            if (lane < M) a.part[(int64_t)split * a.n_pad + (tile * TB + t) * M + lane] = make_float4(st[t].ref, st[t].S, st[t].E, wide);
+            if (lane < M) a.part[(int64_t)split * a.n_pad + (tile * TB + t) * M + lane] = make_float4(st[t].ref, st[t].S, st[t].E, st[t].R);
+        if (tile == 0 && lane == 0) a.wide[split] = wide;
     }
 };
 
@@ -618,7 +647,7 @@ __device__ __forceinline__ void vs_forward_step(const VsFwd& a, int row0, const 
             vs_common<M, TB>(more, s);
         }
     if (a.has_bias || row0 + 32 > a.vocab) vs_mask<M, TB, PL == 2>(s, unit, b);      // (the same in the whole grid)
-    rows.template add<TOP, PL == 2>(s, unit);
+    rows.template add<TOP, PL == 2>(row0, s, unit);
 }
 
 // Bound by the matrix units and the power they draw (the clock falls to 1.8 - 2.2 GHz under them), the exponentials beside
@@ -670,8 +699,10 @@ struct VsStage {
     }
 };
 
+// Waves of a SIMD that the registers are shared out for (D = 50, 4,096 x 65,536 bf16: four 90 us, three 97; 8,192 x 262,144 float32: three 765, two 805)
+constexpr int vs_fwd_waves(int KS, int PL, bool TOP) { return KS > 2 ? 2 : PL == 2 ? 3 : TOP ? 2 : 4; }
 template <int KS, int PL, int M, int TB, int SR, bool TOP>
-__global__ __launch_bounds__(256, KS == 2 ? 3 : 2) void k_vs_forward(VsFwd a) {
+__global__ __launch_bounds__(256, vs_fwd_waves(KS, PL, TOP)) void k_vs_forward(VsFwd a) {
     using Stage = VsStage<KS, PL, M, SR>;
     __shared__ uint4 buf0[Stage::SIZE], buf1[Stage::SIZE];
     const int lane = threadIdx.x & 63;
@@ -685,7 +716,7 @@ __global__ __launch_bounds__(256, KS == 2 ? 3 : 2) void k_vs_forward(VsFwd a) {
 #pragma unroll
     for (int t = 0; t < TB; ++t) x_exp[t] = PL == 2 ? a.x_exp[((live ? tile : 0) * TB + t) * M + lane % M] : 0.0f;
     VsRowsOfTile<M, TB> rows;
-    rows.clear();
+    rows.clear(a, (int64_t)tile * TB * M, live);
     const uint4* w = a.wS + (int64_t)row_begin * KS * PL * 4;
     const float* info = a.info + row_begin / 32 * VS_INFO;
     Stage::fetch(w, info, buf0);
@@ -764,6 +795,7 @@ __global__ __launch_bounds__(256, KS * PL > 14 ? 1 : 2) void k_vs_forward_raw(Vs
     const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
     constexpr int KG = PL == 1 || KS <= 4 ? KS : KS == 8 ? 4 : KS == 10 ? 5 : 2;    // 32-element steps whose loads are under way together
     __shared__ float4 red[4][TB * 16];
+    __shared__ float widest[4];
     const int tile = blockIdx.y;
     int at[KS];
     vs_bits x[TB][KS][PL];
@@ -783,7 +815,7 @@ __global__ __launch_bounds__(256, KS * PL > 14 ? 1 : 2) void k_vs_forward_raw(Vs
         }
     }
     VsRowsOfTile<16, TB> rows;
-    rows.clear();
+    rows.clear(a.f, (int64_t)tile * TB * 16, true);
     float wide = 0.0f;
     const float unscaled[TB] = {};
     const int units = gridDim.x * 4, unit = blockIdx.x * 4 + (threadIdx.x >> 6), pieces = a.f.blocks * 4;
@@ -839,7 +871,7 @@ __global__ __launch_bounds__(256, KS * PL > 14 ? 1 : 2) void k_vs_forward_raw(Vs
 #pragma unroll
                 for (int rb = 0; rb < 2; ++rb) wide = fmaxf(wide, of_row[rb] <= VS_NOTHING ? 0.0f : big[rb].largest());
             }
-            rows.template add<true, false, true>(s, unscaled);
+            rows.template add<true, false, true>(row0, s, unscaled);
             if (a.f.chunk_max) rows.template chunk<false>(a.f, tile, row0 / VS_BLOCK, (row0 >> 5) & 7, lane, true);
         }
         if ((c & 3) == 3) rows.flush();
@@ -848,25 +880,27 @@ __global__ __launch_bounds__(256, KS * PL > 14 ? 1 : 2) void k_vs_forward_raw(Vs
     for (int o = 1; o < 64; o <<= 1) wide = fmaxf(wide, __shfl_xor(wide, o));
 #pragma unroll
     for (int t = 0; t < TB; ++t)
-        if (quad == 0) red[threadIdx.x >> 6][t * 16 + col] = make_float4(rows.st[t].ref, rows.st[t].S, rows.st[t].E, wide);
+        if (quad == 0) red[threadIdx.x >> 6][t * 16 + col] = make_float4(rows.st[t].ref, rows.st[t].S, rows.st[t].E, rows.st[t].R);
+    if (lane == 0) widest[threadIdx.x >> 6] = wide;
     __syncthreads();
     if (threadIdx.x < TB * 16) {
         VsStat st;
         st.clear();
-        wide = 0.0f;
-        for (int i = 0; i < 4; ++i) { const float4 q = red[i][threadIdx.x]; st.join(q.x, q.y, q.z); wide = fmaxf(wide, q.w); }
-        a.f.part[(int64_t)blockIdx.x * a.f.n_pad + tile * TB * 16 + threadIdx.x] = make_float4(st.ref, st.S, st.E, wide);
+        for (int i = 0; i < 4; ++i) { const float4 q = red[i][threadIdx.x]; st.join(q.x, q.y, q.z, q.w); }
+        a.f.part[(int64_t)blockIdx.x * a.f.n_pad + tile * TB * 16 + threadIdx.x] = make_float4(st.ref, st.S, st.E, st.R);
+        if (tile == 0 && threadIdx.x == 0) a.f.wide[blockIdx.x] = fmaxf(fmaxf(widest[0], widest[1]), fmaxf(widest[2], widest[3]));
     }
 }
 
-// Joins the ranges of a row, by WAVES waves, and takes the given token's log probability.  The token's own logit is summed in
-// float64 (its rounding would otherwise show where the probability is near 1).  Bound by latency: 4 us for 87 rows of 64 ranges,
+// Joins the ranges of a row, by WAVES waves, and takes the given token's log probability: its logit, summed in float64, less
+// lse; where the others' sum is less than half of all log(1 - that share), since lse has the rounding of the logits it is made of.  Bound by latency: 4 us for 87 rows of 64 ranges,
 // 8 us for 8,192 rows of a few.
 struct VsJoin {
     VsSrc x, w;
     const float* bias;         // as the caller gave it, or null
     const int64_t* targets;    // or null
     const float4* part;
+    const float* wide;         // null where alternatives are not asked for
     int32_t n, splits;
     int64_t n_pad;
     float *logprob, *entropy, *lse;
@@ -876,6 +910,7 @@ struct VsJoined {
     VsStat st;
     float wide;                // the largest size of a weight
     double lse;
+    float rest;                // the share of the ids that are not the target
     bool empty;                // nothing but -inf
     // over `n` lanes (a power of two): the largest reference first, then sums relative to it
     __device__ __forceinline__ void over(int n) {
@@ -883,10 +918,11 @@ struct VsJoined {
         q.clear();
         q.ref = st.ref;
         for (int o = 1; o < n; o <<= 1) q.ref = fmaxf(q.ref, __shfl_xor(q.ref, o));
-        q.join(st.ref, st.S, st.E);
+        q.join(st.ref, st.S, st.E, st.R);
         for (int o = 1; o < n; o <<= 1) {
             q.S += __shfl_xor(q.S, o);
             q.E += __shfl_xor(q.E, o);
+            q.R += __shfl_xor(q.R, o);
             wide = fmaxf(wide, __shfl_xor(wide, o));
         }
         st = q;
@@ -899,21 +935,26 @@ struct VsJoined {
 #pragma unroll 4
         for (int i = tid; i < a.splits; i += alone(a) ? 64 : 64 * WAVES) {
             const float4 q = a.part[(int64_t)i * a.n_pad + row];
-            st.join(q.x, q.y, q.z);
-            wide = fmaxf(wide, q.w);
+            if (a.wide) wide = fmaxf(wide, a.wide[i]);
+            st.join(q.x, q.y, q.z, q.w);
         }
         over(a.splits > 32 ? 64 : a.splits > 16 ? 32 : a.splits > 8 ? 16 : 8);
-        if (WAVES > 1 && (tid & 63) == 0) red[tid >> 6] = make_float4(st.ref, st.S, st.E, wide);
+        if (WAVES > 1 && (tid & 63) == 0) {
+            red[tid >> 6 << 1] = make_float4(st.ref, st.S, st.E, st.R);
+            red[(tid >> 6 << 1) + 1].x = wide;
+        }
     }
     // (with more than one wave all have to have gathered)
     __device__ __forceinline__ void finish(const VsJoin& a, int64_t row, int tid, const float4* red) {
         if constexpr (WAVES > 1) {
-            const float4 q = red[alone(a) ? 0 : tid % WAVES];
+            const int i = alone(a) ? 0 : tid % WAVES * 2;
+            const float4 q = red[i];
             st.clear();
-            st.ref = q.x; st.S = q.y; st.E = q.z; wide = q.w;
+            st.ref = q.x; st.S = q.y; st.E = q.z; st.R = q.w; wide = red[i + 1].x;
             if (!alone(a)) over(WAVES);
         }
         empty = st.S == 0.0f;
+        rest = st.R / st.S;
         const float l = log2f(st.S);
         lse = empty ? -INFINITY : ((double)st.ref + (double)l) * 0.6931471805599453;
         if (tid != 0) return;
@@ -940,19 +981,19 @@ __device__ __forceinline__ double vs_target_logit(const VsJoin& a, int64_t row, 
     }
     return dot;
 }
-__device__ __forceinline__ void vs_put_logprob(const VsJoin& a, int64_t row, int64_t t, double dot, double lse, bool empty) {
+__device__ __forceinline__ void vs_put_logprob(const VsJoin& a, int64_t row, int64_t t, double dot, double lse, float rest, bool empty) {
     float lp = 0.0f;
     if (t >= a.w.rows) lp = NAN;
     else if (t >= 0) {
         const float b = vs_bias_of(a.bias, t);
-        lp = empty || b == -INFINITY ? -INFINITY : (float)(dot + (double)b - lse);
+        lp = empty || b == -INFINITY ? -INFINITY : rest < 0.5f ? log1pf(-rest) : (float)(dot + (double)b - lse);
         if (lp > 0.0f) lp = 0.0f;
     }
     a.logprob[row] = lp;
 }
 template <int WAVES>
 __global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
-    __shared__ float4 red[4];
+    __shared__ float4 red[8];
     const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
     if (row >= a.n) return;
     const int tid = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
@@ -963,7 +1004,7 @@ __global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
     const double dot = vs_target_logit(a, row, t, tid & 63);
     if (WAVES > 1) __syncthreads();
     j.finish(a, row, tid, red);
-    if (last && (tid & 63) == 0) vs_put_logprob(a, row, t, dot, j.lse, j.empty);
+    if (last && (tid & 63) == 0) vs_put_logprob(a, row, t, dot, j.lse, j.rest, j.empty);
 }
 
 // ---- alternatives -------------------------------------------------------------------------------------------------
@@ -1121,7 +1162,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? BF16 ? 5 : 7 : 4) void k_
     const double lse = joined.lse;
     auto given = [&]() {                    // by one wave
         const double dot = vs_target_logit(a.join, row, target, lane);
-        if (lane == 0) vs_put_logprob(a.join, row, target, dot, lse, joined.empty);
+        if (lane == 0) vs_put_logprob(a.join, row, target, dot, lse, joined.rest, joined.empty);
     };
     if (lse != lse) {                       // no order among the logits
         if (tid < a.k) { a.ids[row * a.k + tid] = -1; a.logprobs[row * a.k + tid] = NAN; }

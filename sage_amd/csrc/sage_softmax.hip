@@ -166,7 +166,7 @@ struct FwdPlan {
     int splits;
     int raw;                    // 16-token blocks of a tile of k_vs_forward_raw (0: the weights are packed)
     uint4 *xS, *wS;
-    float *info, *x_exp;
+    float *info, *x_exp, *wide;
     _Float16* chunk_max;
     float4* part;
     int64_t bytes;
@@ -198,6 +198,7 @@ FwdPlan plan_fwd(const Shape& s, void* ws) {
         p.x_exp = a.take<float>(p.n_pad);
     }
     p.part = a.take<float4>(p.splits * p.n_pad);
+    p.wide = a.take<float>(p.splits);
     p.chunk_max = a.take<_Float16>(s.k ? p.n_pad * p.chunks : 0);
     p.bytes = a.used;
     return p;
@@ -324,8 +325,9 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
     for (int64_t r0 = 0; r0 < n; r0 += p.rows) {
         const int64_t rows = std::min(p.rows, n - r0);
         const VsSrc xr = rows_from(x, r0, rows);
-        const VsFwd f{p.xS, p.wS, p.info, p.x_exp, d_bias != nullptr, (int32_t)vocab, (int32_t)p.tiles, p.splits, (int32_t)(s.vp / VS_BLOCK), (int32_t)p.chunks,
-                      p.n_pad, p.part, alternatives ? p.chunk_max : nullptr};
+        const int64_t* targets = d_targets ? d_targets + r0 : nullptr;
+        const VsFwd f{p.xS, p.wS, p.info, p.x_exp, d_bias != nullptr, (int32_t)vocab, targets, (int32_t)rows, (int32_t)p.tiles, p.splits, (int32_t)(s.vp / VS_BLOCK), (int32_t)p.chunks,
+                      p.n_pad, p.part, p.wide, alternatives ? p.chunk_max : nullptr};
         if (p.raw) {
             const VsRaw q{xr, w, d_bias, f};
             const dim3 grid(p.splits, (uint32_t)p.tiles);
@@ -345,7 +347,7 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
             VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
         }
-        const VsJoin j{xr, w, d_bias, d_targets ? d_targets + r0 : nullptr, p.part, (int32_t)rows, p.splits, p.n_pad,
+        const VsJoin j{xr, w, d_bias, targets, p.part, alternatives ? p.wide : nullptr, (int32_t)rows, p.splits, p.n_pad,
                        d_logprob ? d_logprob + r0 : nullptr, d_entropy ? d_entropy + r0 : nullptr, d_lse + r0};
         if (alternatives) {
             const VsTop t{j, p.chunk_max, (int32_t)p.chunks, alternatives, d_alt_ids + r0 * alternatives, d_alt_logprobs + r0 * alternatives};
