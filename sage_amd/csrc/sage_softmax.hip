@@ -356,9 +356,9 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
             const bool wide = rows <= s.cus;
             if (dtype == SAGE_BF16) { if (wide) k_vs_top<true, 1024><<<(uint32_t)rows, 1024, 0, st>>>(t); else k_vs_top<true, 256><<<(uint32_t)rows, 256, 0, st>>>(t); }
             else { if (wide) k_vs_top<false, 1024><<<(uint32_t)rows, 1024, 0, st>>>(t); else k_vs_top<false, 256><<<(uint32_t)rows, 256, 0, st>>>(t); }
-        // (many ranges: one token of 262,144 ids 18 us with the forward kernel, 22 where one wave joins its 1,024 ranges; of 16,384 ids, 64
-        // ranges, 8.6 and 8.4)
-        } else if (p.splits > 64) k_vs_join<4><<<(uint32_t)rows, 256, 0, st>>>(j);
+        // few rows, or many ranges: four waves share a row's ranges, or one joins them while another takes the target's logit (with the
+        // forward kernel: one token, 1,024 ranges 19.1 us, 23.1 by one wave; 87 tokens, 64 ranges 10.7 and 11.7; 8,192 of a few 221 and 217)
+        } else if (rows <= s.cus || p.splits > 64) k_vs_join<4><<<(uint32_t)rows, 256, 0, st>>>(j);
         else k_vs_join<1><<<cdiv(rows, 4), 256, 0, st>>>(j);
     }
     return launched(c, "sage_token_logprobs_device");
