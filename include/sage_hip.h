@@ -249,8 +249,8 @@ int sage_token_logprobs_device(sage_ctx* ctx, int32_t dtype, int64_t n, int64_t 
  * gradients of 0) has no part in any result, whatever its row of x holds: dx is 0 there.  A target that the bias
  * takes out keeps its g (weight_target in dx, x in d_dweight), as if its p were 0.  The logits are formed again; sums are float32.  The
  * coefficient g (1 - p) of a target is the sum of the other ids' p times g where p is near 1, so that a token predicted well keeps its (small) gradient's bits.
- * With SAGE_BF16 a G_nv is rounded to bf16 (2^-8 of itself) before it is multiplied with a row; d_dbias and the target's share of dx have it in
- * float32.  Without d_dx the pass over the tokens runs nevertheless, short of its products.  With n == 0 the
+ * With SAGE_BF16 a G_nv is rounded to bf16 (2^-8 of itself) before it is multiplied with a row, a target's to 2^-16; d_dbias and the target's share
+ * of dx have it in float32.  Without d_dx the pass over the tokens runs nevertheless, short of its products.  With n == 0 the
  * weight's and bias's gradients are zeros.  Results are overwritten, not accumulated, and lie over no input and no other result.
  */
 int64_t sage_token_logprobs_backward_workspace(sage_ctx* ctx, int32_t dtype, int64_t n, int64_t vocab, int32_t dim);

@@ -1380,7 +1380,8 @@ struct VsBwd {
 // The target's coefficient is g (1 - p_t): small where a token is predicted well, and nothing but rounding errors if it were left to
 // g and g p_t, each rounded, to cancel.  So the sums over tokens leave the target out and find 1 - p_t as what the others
 // add up to (k_vs_target, between the two gradients); dx gets the whole coefficient times w_t at the end, in float32, and dw takes it as
-// the weight of that token and id, rounded as any other is (bf16: one of 2^-8, float32: two float16).
+// the weight of that token and id.  In bf16 it is by far the largest of most tokens: dw adds what its rounding left over in the few
+// steps in which one lies in the tile.
 //
 // Two float16 parts (PL = 2) of a weight: column t is kept multiplied by 2^sg[t], sg as large as the largest weight of the column
 // so far allows (2^15 after the streaming rows' scale), and the sums with it.  It starts high and falls a few times.
@@ -1468,11 +1469,12 @@ struct VsGrad {
                 for (int b = 0; b < VsTile<M>::NB; ++b) vs_in_place(s[b][t]);
         }
     }
-    // Of ids: the weights of the tokens whose target lies in the tile
+    // Of ids: whether a target lies in the tile, of 32 tokens, and the weights of those tokens
+    __device__ __forceinline__ bool targets_here(const float* of) const {
+        return __any((uint32_t)(__float_as_int(of[VS_TOKEN_TARGET + (threadIdx.x & 31)]) - (int)stay0) < TB * M);
+    }
     __device__ __forceinline__ void put_targets(const float* of, float (&G)[TB][NJ]) {
         const int lane = threadIdx.x & 63;
-        const int64_t in = __float_as_int(of[VS_TOKEN_TARGET + (lane & 31)]) - stay0;
-        if (!__any(in >= 0 && in < TB * M)) return;
 #pragma unroll
         for (int t = 0; t < TB; ++t)
 #pragma unroll
@@ -1482,8 +1484,8 @@ struct VsGrad {
             }
     }
 
-    // P: the weights of the 32 streaming rows from row0 on, in parts
-    __device__ __forceinline__ void weights(const VsBwd& a, int row0, const uint4* S, const float* of, Weights (&P)[TB]) {
+    // P: the weights of the 32 streaming rows from row0 on, in parts.  -> of ids: is a target among them?
+    __device__ __forceinline__ bool weights(const VsBwd& a, int row0, const uint4* S, const float* of, Weights (&P)[TB]) {
         const int lane = threadIdx.x & 63;
         VsLogits<M, TB> s;
         vs_f4 b[NJ / 4];
@@ -1578,8 +1580,9 @@ struct VsGrad {
                 leave_targets(a, row0, unit, s);
                 form();
             }
+        const bool of_target = OF_IDS && targets_here(of);
         if constexpr (OF_IDS) {
-            put_targets(of, G);
+            if (of_target) put_targets(of, G);
             if (a.want_db)
 #pragma unroll
                 for (int t = 0; t < TB; ++t) {
@@ -1648,6 +1651,7 @@ struct VsGrad {
                 vs_split<PL>(v, P[t][u]);
             }
         }
+        return of_target;
     }
 
     __device__ __forceinline__ void products(const uint4* T, const Weights (&P)[TB]) {
@@ -1663,6 +1667,35 @@ struct VsGrad {
                     for (int p = 0; p < PL; ++p) f[r][p] = *(const vs_bits*)&T[(((d + r) * HALVES + u) * PL + p) * 64];
                 vs_mfma_parts<PL, M, R, TB>(f, [&](int t, int p) { return P[t][u][p]; }, *(Acc(*)[R][TB]) & acc[d]);
             }
+    }
+
+    // Of ids, bf16: what the rounding of the targets' weights left over.  Rare: a token has one target.
+    __device__ __forceinline__ void left_over(const uint4* T, const float* of) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll 1
+        for (int q = 0; q < TB * HALVES; ++q) {
+            const int t = q / HALVES, u = q % HALVES;
+            vs_f8 G;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int at = vs_row<M>(u * 8 + j, lane);
+                G[j] = __float_as_int(of[VS_TOKEN_TARGET + at]) == (int)stay0 + t * M + lane % M ? of[VS_TOKEN_GT + at] : 0.0f;
+            }
+            vs_bits part[2];
+            vs_split<1>(G, &part[0]);
+            vs_split<1>(G - __builtin_convertvector(__builtin_bit_cast(vs_bf8, part[0]), vs_f8), &part[1]);
+#pragma unroll
+            for (int v = 0; v < TB; ++v)       // (registers have no index)
+                if (v == t)
+#pragma unroll
+                    for (int d = 0; d < BLOCKS; ++d) {
+                        Acc c = vs_mfma<PL, M>(*(const vs_bits*)&T[(d * HALVES + u) * 64], part[1], acc[d][v]);
+#pragma unroll
+                        for (int i = 0; i < M * M / 64; ++i) c[i] += 0.0f;     // (a vector instruction between, for its waits)
+                        vs_in_place(c);
+                        acc[d][v] = c;
+                    }
+        }
     }
 
     __device__ __forceinline__ void store(const VsBwd& a, int split, int lane) {
@@ -1732,8 +1765,9 @@ struct VsGradStage {
         for (int r = 0; r < SR; r += 32) {
             typename Grad::Weights P[TB];
             const float* of = (const float*)(from + 2 * HALF) + r / 32 * INFO;
-            g.weights(a, base + r, from + r * KS * PL * 4 + lane, of, P);
+            const bool of_target = g.weights(a, base + r, from + r * KS * PL * 4 + lane, of, P);
             if (sums(a)) g.products(from + HALF + r * KS * PL * 4 + lane, P);
+            if (PL == 1 && of_target) g.left_over(from + HALF + r * KS * PL * 4 + lane, of);
         }
     }
     // by turns: each half with its own copy of what goes with it
@@ -1742,19 +1776,20 @@ struct VsGradStage {
         vs_stage<HALF>(half, to);
         vs_stage_floats<INFO>(info, (float*)(to + HALF));
     }
-    static __device__ __forceinline__ void turn_s(const VsBwd& a, int base, const uint4* __restrict__ T, const float* __restrict__ info, uint4* __restrict__ to,
+    static __device__ __forceinline__ bool turn_s(const VsBwd& a, int base, const uint4* __restrict__ T, const float* __restrict__ info, uint4* __restrict__ to,
                                                   const uint4* __restrict__ from, Grad& g, typename Grad::Weights (&P)[TB]) {
         vs_copies_done();
         __syncthreads();
         fetch_half(T, info, to);
-        g.weights(a, base, from + (threadIdx.x & 63), (const float*)(from + HALF), P);
+        return g.weights(a, base, from + (threadIdx.x & 63), (const float*)(from + HALF), P);
     }
     static __device__ __forceinline__ void turn_t(const VsBwd& a, bool more, const uint4* __restrict__ S, const float* __restrict__ info, uint4* __restrict__ to,
-                                                  const uint4* __restrict__ from, Grad& g, const typename Grad::Weights (&P)[TB]) {
+                                                  const uint4* __restrict__ from, Grad& g, const typename Grad::Weights (&P)[TB], bool of_target) {
         vs_copies_done();
         __syncthreads();
         if (more) fetch_half(S, info, to);
         if (sums(a)) g.products(from + (threadIdx.x & 63), P);
+        if (PL == 1 && of_target) g.left_over(from + (threadIdx.x & 63), (const float*)(from + HALF));
     }
 };
 
@@ -1783,9 +1818,9 @@ __global__ __launch_bounds__(256, vs_bwd_waves(KS, PL, M, TB, OF_IDS)) void k_vs
         Stage::fetch_half(S, info, buf0);
         for (int base = row_begin; base < row_end; base += 32) {
             typename Stage::Grad::Weights P[TB];
-            Stage::turn_s(a, base, T, info, buf1, buf0, g, P);
+            const bool of_target = Stage::turn_s(a, base, T, info, buf1, buf0, g, P);
             S += 32 * PIECE; T += 32 * PIECE; info += Stage::INFO;
-            Stage::turn_t(a, base + 32 < row_end, S, info, buf0, buf1, g, P);
+            Stage::turn_t(a, base + 32 < row_end, S, info, buf0, buf1, g, P, of_target);
         }
     } else {
         const int units = a.groups / (SR / 32);

@@ -211,6 +211,7 @@ struct BwdPlan {
     float *info, *tokens, *part_x, *part_w, *bias_part, *rest, *target_e;
     int64_t bytes;
 };
+// (one plan, with and without an entropy gradient)
 BwdPlan plan_bwd(const Shape& s, void* ws) {
     BwdPlan p{};
     Arena a{(char*)ws};
@@ -219,7 +220,8 @@ BwdPlan plan_bwd(const Shape& s, void* ws) {
 #define VS_F(KS, PL)                                                                            \
     p.tiles_x = cdiv(s.n, vs_bwd_blocks(KS, PL, false) * vs_bwd_tile(KS, PL)); p.tiles_w = cdiv(s.vocab, vs_bwd_blocks(KS, PL, true) * vs_bwd_tile(KS, PL)); \
     units_x = s.vp / vs_bwd_rows(KS, PL); units_w = p.np / vs_bwd_rows(KS, PL);                 \
-    resident_x *= per_cu<vs_bwd_kernel<KS, PL, false, false>>(); resident_w *= per_cu<vs_bwd_kernel<KS, PL, true, false>>()
+    resident_x *= std::min(per_cu<vs_bwd_kernel<KS, PL, false, false>>(), per_cu<vs_bwd_kernel<KS, PL, false, true>>());        \
+    resident_w *= std::min(per_cu<vs_bwd_kernel<KS, PL, true, false>>(), per_cu<vs_bwd_kernel<KS, PL, true, true>>())
     VS_BY_WIDTH(s.ks, s.pl, VS_F);
 #undef VS_F
     p.splits_x = vs_splits(resident_x, cdiv(p.tiles_x, 4), units_x, 8.0);

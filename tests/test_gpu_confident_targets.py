@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from .softmax_tight import Tight
-from .test_gpu_vocab_softmax import BF16, F32, close
+from .test_gpu_vocab_softmax import BF16, F32, close, make
 
 pytestmark = pytest.mark.gpu
 LEFT = [0.5, 0.1, 0.03, 1e-2, 3e-3, 1e-3, 1e-4, 1e-5, 1e-7, 0.9, 0.999]        # 1 - p_t
@@ -87,3 +87,25 @@ def test_certain_and_impossible_targets(dtype):
     dx, dw, db = vs.token_logprobs_backward(x, w, t, f, gl, bias=b)
     (wx, tx), (ww, tw), (wb, tb) = e.gradient(gl, None, dtype)
     close(dx, wx, tx, "dx"), close(dw, ww, tw, "dw"), close(db, wb, tb, "db")
+
+
+@pytest.mark.parametrize("n,V,D", [(300, 5000, 50), (64, 1000, 128), (128, 3000, 200), (257, 9000, 300), (100, 700, 512)])
+def test_unlikely_targets_of_bf16_are_not_rounded_twice(n, V, D):
+    """Tokens with targets of their own that are unlikely: a row of dw is g (1 - p_t) x, to half a step of its type (2^-8), and the other tokens' share, of which
+    each weight is rounded once (2^-8).  Of the target's own weight no more than 2^-16 may be lost beside that."""
+    from sage_amd import vocab_softmax as vs
+    x, w, _, _ = make(n, V, D, BF16, seed=21, scale=0.3)
+    t = torch.randperm(V, generator=torch.Generator().manual_seed(n))[:n].cuda()
+    e = Tight(x, w, None, t)
+    gl = -torch.linspace(0.5, 1.5, n).cuda() / n
+    f = vs.token_logprobs(x, w, t)
+    _, dw, _ = vs.token_logprobs_backward(x, w, t, f, gl)
+    (_, _), (want, _), _ = e.gradient(gl, None, BF16)
+    G = e.G.clone()
+    own = G[torch.arange(n), t].abs()
+    G[torch.arange(n), t] = 0.0
+    others = G.abs().t().contiguous() @ e.x.abs()
+    inner = torch.zeros_like(want)
+    inner[t] = (own * (2.0 ** -16 + e.tol_p.amax(1)))[:, None] * e.x.abs()
+    inner = inner + others * (2.0 ** -8 + e.tol_p.max()) + 64 * 2.0 ** -24 * (others + want.abs())
+    close(dw, want, inner + 2.0 ** -8 * (want.abs() + inner) + 1e-37, "dw")
