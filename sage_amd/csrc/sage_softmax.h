@@ -651,9 +651,9 @@ __device__ __forceinline__ void vs_forward_step(const VsFwd& a, int row0, const 
 }
 
 // Bound by the matrix units and the power they draw (the clock falls to 1.8 - 2.2 GHz under them), the exponentials beside
-// them second.  8,192 tokens x 262,144 ids, D = 50 float32: 737 us, 0.82 * 10^12 operations of the MFMAs (three products, 64
-// elements for 50) at 1.1 * 10^15 a second, where a large bf16 matrix product of the library reaches 1.38 * 10^15; 4,096 x 65,536,
-// D = 300 bf16: 170 us, 1.01 * 10^15.
+// them second.  8,192 tokens x 262,144 ids, D = 50 float32: 764 us (mean of 10, as all below), 0.82 * 10^12 operations of the MFMAs (three
+// products, 64 elements for 50) at 1.08 * 10^15 a second, where a large bf16 matrix product of the library reaches 1.37 * 10^15; 4,096 x
+// 65,536, D = 300 bf16: 175 us, 0.98 * 10^15.  The MFMAs are busy 55 % of a 1.95 GHz clock in both.
 // Four waves, a tile each, share the streaming rows through LDS.  SR rows at a time are copied straight into LDS (they are
 // packed in the order of the copy) while the SR before them are worked on: one barrier a step.
 typedef const __attribute__((address_space(1))) void* vs_global_ptr;
@@ -739,8 +739,8 @@ __device__ __forceinline__ float vs_bias_of(const float* bias, int64_t v) {
 // elements of a row that its place in a fragment asks for, at whatever alignment they have.  The last piece of a row that is
 // no whole number of pieces long is taken back from the row's end, with the elements before it weighted 0 in x: no read
 // leaves the row (so there are eight elements at least).  A wave is a tile of 16 TB tokens against one range of the vocabulary; the
-// four of a workgroup join theirs.  One token, 262,144 x 50 float32: 52 MB in 14.8 us (3.5 TB/s); five, 229,376 x 300 bf16: 138 MB in
-// 31 us (4.4 TB/s; a copy of 4 GB reaches 4.8).
+// four of a workgroup join theirs.  One token, 262,144 x 50 float32: 52 MB in 15.2 us (3.4 TB/s); five, 229,376 x 300 bf16: 138 MB in
+// 32 us (4.3 TB/s; a copy of 4 GB reaches 4.8).
 template <int PL> struct VsPiece;
 template <> struct VsPiece<1> {            // of bf16: a fragment as it is
     vs_bf8 v;
@@ -1021,9 +1021,9 @@ __global__ __launch_bounds__(256) void k_vs_join(VsJoin a) {
 // one.  Where too many chunks reach it (many equal logits, a zero vector), they are visited in ascending order, and once k
 // logits are known a later one that cannot beat the k-th is skipped even when it ties.
 //
-// Bound by latency for a few rows (11.6 us for one row of 262,144 ids, k = 10), by the reading of the maxima for many: 8,192 rows of
+// Bound by latency for a few rows (12.5 us for one row of 262,144 ids, k = 10), by the reading of the maxima for many: 8,192 rows of
 // 262,144 ids 144 us (537 MB of maxima and 0.15 GB of rows looked at again); by those rows where they are wide and k is large: 1,021
-// rows, D = 511, k = 32, 58 us for 0.28 GB.  Chunks of 8 as float16 take the bytes of chunks of 16 as float32 (which that case
+// rows, D = 511, k = 32, 60 us for 0.28 GB.  Chunks of 8 as float16 take the bytes of chunks of 16 as float32 (which that case
 // paid 140 us for).
 #define VS_MAX_K 32
 #define VS_CAND 1024
@@ -1347,12 +1347,14 @@ __device__ __forceinline__ void vs_store(void* p, int64_t at, float v, int bf16)
 }
 
 // Either gradient forms the logits again: n V D products beside the n V D of its own sums, and neither is stored.  Bound by the
-// matrix units' power (float32, three products each: 8,192 tokens x 262,144 ids, D = 50, dx 1.42 ms and dw 1.52 ms, 1.65 * 10^12 operations
+// matrix units' power (float32, three products each: 8,192 tokens x 262,144 ids, D = 50, dx 1.45 ms and dw 1.50 ms, 1.65 * 10^12 operations
 // of the MFMAs each, 1.1 * 10^15 a second).  Wide rows leave registers for 16 columns of a wave and two or three waves of a
-// SIMD, which wait for one another twice in 32 streaming rows: bf16, D = 300, 4,096 x 65,536, entropy gradient too, dx 361 us
-// (0.95 * 10^15; MFMAs busy 54 % of a 1.8 GHz clock), dw 474 us (two waves a SIMD: 37 %).  The LDS reads are not what it waits for: with
-// the weights of four waves shared, each reading a quarter of the transposed fragments (29 KB for 40), dx takes as long and dw 3 %
-// longer.
+// SIMD, which wait for one another twice in 32 streaming rows: bf16, D = 300, 4,096 x 65,536, entropy gradient too, dx 380 us
+// (0.90 * 10^15; MFMAs busy 51 % of a 1.8 GHz clock), dw 499 us (two waves a SIMD: 37 % of 1.9 GHz).  The LDS reads are not what it waits for:
+// with the weights of four waves shared, each reading a quarter of the transposed fragments (29 KB for 40), dx took as long and
+// dw 3 % longer.  What spills, in registers of a lane: float32 of 257 to 320 elements 47 to 70 (dx 1.31 ms, dw 1.39 ms at 4,096 x 65,536),
+// bf16 above 320 21 in dw; in forward passes bf16 of up to 64 4, float32 of 257 to 320 with alternatives 6, and of the kernels that read the
+// weights as they lie bf16 of 257 to 320 with two blocks 11, float32 above 320 67.
 struct VsBwd {
     const uint4 *stayS;        // stationary rows (columns of the product)
     const uint4 *flowS, *flowT;// streaming rows, and transposed
@@ -1839,8 +1841,8 @@ __global__ __launch_bounds__(256, vs_bwd_waves(KS, PL, M, TB, OF_IDS)) void k_vs
     if (live) g.store(a, split, lane);
 }
 
-// A token's coefficient of its target, G_t = g (1 - p_t) - h p_t (log p_t + H), from what the sums over tokens left (several times
-// smaller errors than g has steps of 2^-24 of: where p_t is above a half, 1 - p_t is what the other ids add up to).
+// A token's coefficient of its target, G_t = g (1 - p_t) - h p_t (log p_t + H), from what the sums over tokens left (5 us for
+// 4,096 tokens): where p_t is above a half, 1 - p_t is what the other ids add up to, else it is formed from p_t, which is smaller.
 __global__ __launch_bounds__(256) void k_vs_target(VsPack a, const float* __restrict__ rest, const float* __restrict__ target_e, int32_t splits, int64_t pad) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= a.src.rows) return;

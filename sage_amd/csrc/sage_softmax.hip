@@ -61,16 +61,18 @@ int vs_steps(int dim) {
 
 // How each width runs.  ks: 32-element steps of the padded row; pl: parts of a packed element (1 bf16, 2 float32).
 // Columns of a tile (the matrix instruction's) and tiles of a wave, as measured for each width (ks = 2, 4, 8, 10, 16 at
-// D = 50, 100, 200, 300, 500, 4,096 tokens x 65,536 ids, D = 50 twice that both ways; us, best first, then the other choices in turn):
-//   forward   32x2 32x2 16x2 32x2 32x1   float32   431 [458 489 490]   192 [207 200]   337 [359 688]   476 [531 498]   864 [949 1193]
-//             32x2 32x2 32x2 16x2 16x2   bf16      268 [303 308]       106 [111 113]   156 [168 167]   190 [204 181]   281 [304 656]
-//     with alternatives the registers of the largest logits decide too: ks = 10, bf16 16x2 264 [344], without 182 [171];
-//     ks = 2, float32 16x2 589 [613], without 492 [426]; the others as without
-//   dx        16x2 16x2 16x1 16x2 16x1   float32   714 [773 803 908]   351 [378 417]   751 [821 915]   1,259 [1,563]   2,623 [4,732]
-//             16x2 16x2 16x1 16x1 16x1   bf16      286 [279 321 333]   144 [157 164]   300 [305 354]   379 [438 441]   628 [670 682]
-//   dw        16x2 16x2 16x1 16x2 16x1   float32   765 [757 836 896]   379 [409 448]   796 [1,058]     1,540 [1,617]   2,613 [4,576]
-//             16x2 16x2 16x1 16x1 16x2   bf16      350 [350 396 445]   166 [185 216]   364 [438 463]   447 [554 899]   922 [1,385]
-// (Wider than that the sums of a gradient spill; 16-column tiles give an accumulator time to be ready.)
+// D = 50, 100, 200, 300, 500, 4,096 tokens x 65,536 ids, D = 50 twice that both ways; us, the choice taken first, then the others of 16 and 32
+// columns, one and two tiles, fastest first; without an entropy gradient, dw with its launches):
+//   forward   32x2 32x2 16x2 32x2 32x1   float32   436 [460 461 518]   189 [198 205 234]   337 [358 399 700]     474 [508 552 781]     820 [953 1144 1388]
+//             32x2 32x2 32x2 32x2 16x2   bf16      281 [288 309 334]   106 [105 108 120]   148 [158 164 198]     177 [182 193 217]     269 [286 337 613]
+//   with alternatives the registers of the largest logits decide too
+//             16x2 32x2 16x2 32x2 32x1   float32   548 [551 585 610]   238 [248 256 287]   410 [429 472 1027]    588 [648 669 908]     1063 [1213 1515 2118]
+//             32x2 32x2 32x2 16x2 16x2   bf16      448 [407 426 441]   161 [156 159 171]   217 [231 232 272]     266 [274 295 408]     372 [390 440 988]
+//   dx        16x2 16x2 16x1 16x2 16x1   float32   743 [727 768 828]   363 [377 418 477]   758 [911 1310 3436]   1310 [1686 2945 ..]  2677 [4810 7132 ..]
+//             16x2 16x2 16x1 16x1 16x1   bf16      308 [311 326 358]   150 [160 168 202]   299 [311 359 447]     393 [1575 2526 ..]   620 [2428 2790 ..]
+//   dw        16x2 16x2 16x1 16x2 16x1   float32   759 [740 801 853]   342 [370 423 508]   763 [923 954 3506]    1385 [1553 1768 ..]  2561 [4876 7436 ..]
+//             16x2 16x2 16x1 16x1 16x2   bf16      311 [328 367 377]   134 [163 186 534]   359 [370 387 434]     392 [485 494 1834]    684 [744 935 5282]
+// (The gradients take 16 columns throughout: 32 gain 2 % at the narrowest width alone, and wider ones than that spill their sums.)
 constexpr int vs_fwd_tile(int ks, int pl, bool top) {
     if (pl == 1 ? ks == 10 : ks == 2) return top ? 16 : 32;
     return pl == 1 ? (ks <= 8 ? 32 : 16) : ks == 8 ? 16 : 32;
@@ -146,10 +148,10 @@ int vs_splits(int64_t resident, int64_t groups, int64_t units, double cost) {
 // Token blocks (of 16) of a wave that reads the weights as they lie, one, or two where registers allow and tokens are there;
 // 0: the weights are packed first.  Packing costs a launch and a pass over the weights, reading them as they lie one such pass per
 // tile: worth it for 2 tiles (3 of two blocks), and for more where the vocabulary is short.  Measured, us, as they lie / packed:
-//   D = 50 float32, 262,144 ids   64 tokens 39 / 55   128: 65 / 55      16,384 ids   256: 13 / 19   384: 16 / 19    32,768   512: 34 / 24
-//   D = 300 bf16, 131,072 ids     64: 37 / 53   128: 64 / 53            8,192 ids    256: 13 / 22                  32,768   256: 26 / 28
-//   D = 300 float32, 131,072 ids  32: 70 / 128   64: 142 / 135          8,192 ids    128: 18 / 44
-//   D = 512 bf16, 131,072 ids     32: 61 / 77   64: 112 / 79            1,200 ids    512: 16 / 25                  32,768   96: 45 / 32
+//   D = 50 float32, 262,144 ids   64 tokens 39 / 57   128: 67 / 57      16,384 ids   256: 14 / 22   384: 18 / 22    32,768   512: 35 / 25
+//   D = 300 bf16, 131,072 ids     64: 46 / 65   128: 74 / 65            8,192 ids    256: 15 / 28                  32,768   256: 32 / 34
+//   D = 300 float32, 131,072 ids  32: 75 / 128   64: 139 / 138          8,192 ids    128: 19 / 45
+//   D = 512 bf16, 131,072 ids     32: 71 / 80   64: 127 / 81            1,200 ids    512: 20 / 27                  32,768   96: 51 / 36
 int vs_raw_blocks(const Shape& s) {
     if (s.n > VS_RAW || s.dim < 8) return 0;
     int most = 1;
@@ -354,7 +356,7 @@ int sage_token_logprobs_device(sage_ctx* c, int32_t dtype, int64_t n, int64_t vo
         if (alternatives) {
             const VsTop t{j, p.chunk_max, (int32_t)p.chunks, alternatives, d_alt_ids + r0 * alternatives, d_alt_logprobs + r0 * alternatives};
             // a row alone on a CU is bound by latency: sixteen waves share its chain of loads (262,144 ids, D = 50, with the forward
-            // kernel: one row 26.6 us, 28.3 by four waves; 256 rows 72 and 73; 320 rows 92 and 87)
+            // kernel: one row 26.7 us, 28.7 by four waves; 256 rows 75 and 76; 320 rows 96 and 88)
             const bool wide = rows <= s.cus;
             if (dtype == SAGE_BF16) { if (wide) k_vs_top<true, 1024><<<(uint32_t)rows, 1024, 0, st>>>(t); else k_vs_top<true, 256><<<(uint32_t)rows, 256, 0, st>>>(t); }
             else { if (wide) k_vs_top<false, 1024><<<(uint32_t)rows, 1024, 0, st>>>(t); else k_vs_top<false, 256><<<(uint32_t)rows, 256, 0, st>>>(t); }
