@@ -210,17 +210,17 @@ int sage_train_embeddings(sage_ctx* ctx, int32_t dim, int32_t window, int32_t ne
  * and whose compute_losses scores with log-sigmoids, utils.py:125-138): with logits s_nv = x_n . weight_v + bias_v,
  *   logprob[n] = s_n,target(n) - lse[n],   lse[n] = log sum_v exp s_nv,   entropy[n] = lse[n] - sum_v p_nv s_nv,
  * and the `alternatives` largest logits of a row, as ids in descending order (ties: the lower id) and log probabilities.
- * (logprob is log(1 - the other ids' share) where that share is below a half, to float32's relative precision however small it is; the
- * log probabilities of alternatives are their logits less lse, to its precision.)
+ * (logprob is log(1 - the other ids' share) where that share is below a half, to float32's relative precision however small
+ * it is; the log probabilities of alternatives are their logits less lse, to its precision.)
  * The [n][vocab] matrix of logits is never stored.
  *   d_x [n][dim], d_weight [vocab][dim]   both SAGE_F32 or both SAGE_BF16, rows ldx / ldw elements apart (>= dim); any alignment
- *                    of rows.  Products and sums are float32; the softmax's too.  A float32 element is taken to 2^-22 of itself or 2^-29 of its
- *                    row's largest, whichever is more, whatever other rows hold: logits are float32's to within a few steps of 2^-24 of
- *                    sum_d |x_d| max_d |w_d|.
- *   d_bias [vocab]   float32 or NULL; -inf, or any value of -1e30 or less, takes an id out (so does a logit of -1e30 or less, -inf
- *                    among them).  A row that has nothing left gets lse -inf, logprob -inf, entropy 0, alternatives -1.  x is finite,
- *                    and so are the weights of ids that are not taken out, and products x_d w_vd lie in float32's range: a logit that is NaN or
- *                    +inf makes its row NaN, alternatives -1.
+ *                    of rows.  Products and sums are float32; the softmax's too.  A float32 element is taken to 2^-22 of itself or
+ *                    2^-29 of its row's largest, whichever is more, whatever other rows hold: logits are float32's to within a
+ *                    few steps of 2^-24 of sum_d |x_d| max_d |w_d|.
+ *   d_bias [vocab]   float32 or NULL; -inf, or any value of -1e30 or less, takes an id out (so does a logit below about -7e29,
+ *                    -inf among them).  A row that has nothing left gets lse -inf, logprob -inf, entropy 0, alternatives -1.
+ *                    x is finite, and so are the weights of ids that are not taken out, and products x_d w_vd lie in float32's
+ *                    range: a logit that is NaN or +inf makes its row NaN, alternatives -1.
  *   d_targets [n]    int64, or NULL (then no d_logprob).  A negative target means none: logprob 0, no gradient.  The host cannot
  *                    see a target of `vocab` or more: its logprob is NaN, and so are the gradients it reaches.
  *   d_logprob, d_entropy, d_lse [n] float32 (d_logprob and d_entropy may be NULL); d_alt_ids int32 and d_alt_logprobs float32
@@ -247,11 +247,12 @@ int sage_token_logprobs_device(sage_ctx* ctx, int32_t dtype, int64_t n, int64_t 
  * (float32).  d_dx or d_dweight may be NULL; d_dbias needs d_dweight.  d_lse and d_entropy (needed with d_grad_entropy) are
  * what the forward call returned for the same inputs.  A token without a target and without an entropy gradient (or with
  * gradients of 0) has no part in any result, whatever its row of x holds: dx is 0 there.  A target that the bias
- * takes out keeps its g (weight_target in dx, x in d_dweight), as if its p were 0.  The logits are formed again; sums are float32.  The
- * coefficient g (1 - p) of a target is the sum of the other ids' p times g where p is near 1, so that a token predicted well keeps its (small) gradient's bits.
- * With SAGE_BF16 a G_nv is rounded to bf16 (2^-8 of itself) before it is multiplied with a row, a target's to 2^-16; d_dbias and the target's share
- * of dx have it in float32.  Without d_dx the pass over the tokens runs nevertheless, short of its products.  With n == 0 the
- * weight's and bias's gradients are zeros.  Results are overwritten, not accumulated, and lie over no input and no other result.
+ * takes out keeps its g (weight_target in dx, x in d_dweight), as if its p were 0.  The logits are formed again; sums are float32.
+ * The coefficient g (1 - p) of a target is g times the sum of the other ids' p where p is near 1, so that a token predicted well
+ * keeps its (small) gradient's bits.  With SAGE_BF16 a G_nv is rounded to bf16 (2^-8 of itself) before it is multiplied with a
+ * row, a target's to 2^-16; d_dbias and the target's share of dx have it in float32.  Without d_dx the pass over the tokens
+ * runs nevertheless, short of its products.  With n == 0 the weight's and bias's gradients are zeros.  Results are
+ * overwritten, not accumulated, and lie over no input and no other result.
  */
 int64_t sage_token_logprobs_backward_workspace(sage_ctx* ctx, int32_t dtype, int64_t n, int64_t vocab, int32_t dim);
 int sage_token_logprobs_backward_device(sage_ctx* ctx, int32_t dtype, int64_t n, int64_t vocab, int32_t dim, const void* d_x, int64_t ldx,
@@ -264,9 +265,10 @@ int sage_token_logprobs_backward_device(sage_ctx* ctx, int32_t dtype, int64_t n,
  * Clips gradients by their global norm N = sqrt(sum of all squares): d_out[i] = d_grads[i] * (max_norm / N) where N > max_norm,
  * else d_out[i] = d_grads[i]; *d_norm = N (float32, device).  max_norm is finite and not negative.  d_out[i] may be d_grads[i]
  * itself (in place); no other overlap is allowed.  sizes[i] elements of dtypes[i] (SAGE_F32 / SAGE_BF16), back to back; the
- * four lists are HOST arrays, read during the call only.  Squares are summed in float64.  An infinity or a NaN among the gradients leaves every
- * gradient as it is; the caller sees a *d_norm that is not finite.  Finite gradients are clipped by their N whatever it is: where it passes
- * float32's range *d_norm is inf, and max_norm / N may be as small as it comes.  Enqueues only, as described above.
+ * four lists are HOST arrays, read during the call only.  Squares are summed in float64.  An infinity or a NaN among the
+ * gradients leaves every gradient as it is; the caller sees a *d_norm that is not finite.  Finite gradients are clipped by their
+ * N whatever it is: where it passes float32's range *d_norm is inf, and max_norm / N may be as small as it comes.  Enqueues
+ * only, as described above.
  */
 int64_t sage_clip_grad_norm_workspace(sage_ctx* ctx, int64_t n_tensors, const int64_t* sizes);
 int sage_clip_grad_norm_device(sage_ctx* ctx, int64_t n_tensors, const void* const* d_grads, void* const* d_out, const int64_t* sizes,
